@@ -121,6 +121,17 @@ _SIGS = {
     "snhip_abi_rwkv7_reset": (I32, [V]),
     "snhip_abi_rwkv7_free": (None, [V]),
     "snhip_abi_rwkv7_vocab": (I32, [V]),
+    # include/snhip_ops.h
+    "snhip_op_delta_chunk_floats": (ctypes.c_int64, [CP]),
+    "snhip_op_delta_state_floats": (ctypes.c_int64, [CP]),
+    "snhip_op_delta_bwd_floats": (ctypes.c_int64, [CP]),
+    "snhip_op_delta_fwd_dev": (I32, [CP, V, V, V]),
+    "snhip_op_delta_step_dev": (I32, [CP, V, V, V]),
+    "snhip_op_delta_bwd_dev": (I32, [CP, CP, V]),
+    "snhip_op_norm_fwd_dev": (I32, [V, V, V, V, V, V, ctypes.c_int64, ctypes.c_int64, ctypes.c_float, I32, V]),
+    "snhip_op_norm_bwd_floats": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
+    "snhip_op_norm_bwd_dev": (I32, [V, V, V, V, V, V, V, V, V, ctypes.c_int64, ctypes.c_int64, I32, V]),
+    "snhip_op_sample_dev": (I32, [CP, V, V]),
     "snhip_refmath_host": (I32, [V, V, V, I32]),
     "snhip_refmath_dev": (I32, [V, V, V, I32, V]),
 }
@@ -175,6 +186,25 @@ def check(rc: int, what: str) -> None:
 def stream_handle(device=None) -> int:
     """The raw hipStream_t of torch's current stream."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """Makes a tensor's device the current one for a launch, as the library's
+    operators expect; nothing if it is already."""
+
+    def __init__(self, device):
+        self.at = device.index
+        self.was = -1
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if now != self.at:
+            self.was = now
+            torch.cuda.set_device(self.at)
+
+    def __exit__(self, *exc):
+        if self.was >= 0:
+            torch.cuda.set_device(self.was)
 
 
 def ptr(t) -> int:

@@ -1,0 +1,136 @@
+// Shared pieces of the gated delta rule's kernels (delta.hip, deltabwd.hip).
+//
+// Mathematics, per sequence and value head, in chunks of C = 32 tokens. With c the
+// running sum of g inside the chunk, G_i = exp(c_i), D_ij = exp(c_i - c_j) for j <= i
+// (0 above), S the state before the chunk and everything row by token:
+//   A_ij = beta_i D_ij k_i.k_j (j < i)      M = (I + A)^-1
+//   R = beta (V - G (K S))                   U = M R         (the writes)
+//   P_ij = scale D_ij q_i.k_j (j <= i)       O = scale G (Q S) + P U
+//   S' = G_C S + K^T (L U)                   L_j = exp(c_C - c_j)
+// All exponents are differences of running sums, held in 64 bits: their difference
+// keeps its digits after a strong decay. They are never positive for g <= 0.
+//
+// M, P, G, L and beta depend on no state: k_delta_prep makes them for all chunks at
+// once. What is left is sequential over chunks but independent over the columns of V:
+// a wave owns 16 of them and keeps its (K, 16) of the state in registers, where the
+// results of one product are the operand of the next (planes.h); LDS only holds the
+// tiles that all columns share.
+#pragma once
+
+#include "common.h"
+#include "planes.h"
+#include "snhip_ops.h"
+
+namespace snhip {
+
+constexpr int kDC = 32;                            // tokens per chunk
+// Per chunk and head: M, P (32 x 32 each), then G, L, beta (32 each).
+constexpr int kDeltaP = 1024, kDeltaG = 2048, kDeltaL = 2080, kDeltaB = 2112, kDeltaChunk = 2144;
+
+struct DeltaP {
+    SnHipDelta d;
+    int64_t slots;          // chunk slots of all sequences
+    int KP, VP;             // K and V padded: state slabs are (VP, KP), k contiguous
+    int rep;                // value heads per query and key head
+    bool vec_q, vec_k, vec_v;   // 16-byte loads reach
+};
+
+__host__ __device__ inline int64_t delta_slots(const SnHipDelta& d) {
+    return d.cu ? d.T / kDC + d.N : d.B * ((d.T + kDC - 1) / kDC);
+}
+__host__ __device__ inline int delta_kp(int64_t K) { return K <= 64 ? 64 : 128; }
+__host__ __device__ inline int delta_vp(int64_t V) { return (int)((V + 15) / 16 * 16); }
+
+// A sequence: its first token as a row of the contiguous arrays, its batch entry and
+// first token there, its length, and the slot of its first chunk. With cu the slots of
+// a sequence begin at cu[n] / 32 + n, which leaves every sequence enough of them.
+struct DeltaSeq {
+    int64_t row, b, t0, slot;
+    int len;
+};
+__device__ __forceinline__ int64_t delta_edge(const SnHipDelta& d, int64_t n) {
+    const int64_t e = d.cu[n];
+    return e < 0 ? 0 : e > d.T ? d.T : e;
+}
+__device__ __forceinline__ DeltaSeq delta_seq(const SnHipDelta& d, int64_t n) {
+    DeltaSeq s;
+    if (d.cu) {
+        const int64_t a = delta_edge(d, n), e = delta_edge(d, n + 1);
+        s.row = s.t0 = a;
+        s.b = 0;
+        s.len = (int)(e > a ? e - a : 0);
+        s.slot = a / kDC + n;
+    } else {
+        s.row = n * d.T;
+        s.t0 = 0;
+        s.b = n;
+        s.len = (int)d.T;
+        s.slot = n * ((d.T + kDC - 1) / kDC);
+    }
+    return s;
+}
+// The sequence and chunk of a slot; false for a slot that no chunk uses.
+__device__ __forceinline__ bool delta_chunk_of(const SnHipDelta& d, int64_t slot, DeltaSeq* s, int* chunk) {
+    int64_t n;
+    if (d.cu) {
+        int64_t lo = 0, hi = d.N - 1;          // the last sequence that begins at or before the slot
+        while (lo < hi) {
+            const int64_t mid = (lo + hi + 1) / 2;
+            if (delta_edge(d, mid) / kDC + mid <= slot) lo = mid;
+            else hi = mid - 1;
+        }
+        n = lo;
+    } else {
+        n = slot / ((d.T + kDC - 1) / kDC);
+    }
+    *s = delta_seq(d, n);
+    const int64_t c = slot - s->slot;
+    *chunk = (int)c;
+    return c >= 0 && c * kDC < s->len;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* delta_at(const void* p, const int64_t* st, int64_t b, int64_t t, int64_t h) {
+    return static_cast<const T*>(p) + b * st[0] + t * st[1] + h * st[2];
+}
+
+// Rows [0, 32) of a (tokens, K) tile into LDS, rows from n on and columns from K on 0:
+// rows by token (`rows`) and / or rows by column (`cols`).
+template <typename T, int P, int KP, bool ROWS, bool COLS>
+__device__ __forceinline__ void stage_tile(const T* src, int64_t stride, int n, int K, bool vec,
+                                           Tile<P, kDC, KP> rows, Tile<P, KP, kDC> cols, int tid, int nth) {
+    for (int i = tid; i < kDC * KP / 8; i += nth) {
+        const int t = i / (KP / 8), c = i % (KP / 8) * 8;
+        float x[8];
+        load8(src + t * stride + c, t < n ? K - c : 0, vec, x);
+        if (ROWS) {
+            rows.put4(t, c, x);
+            rows.put4(t, c + 4, x + 4);
+        }
+        if (COLS) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) cols.put(c + j, t, x[j]);
+        }
+    }
+}
+
+// A (32, 32) fp32 matrix into LDS, as stored or transposed.
+template <int P, bool TR>
+__device__ __forceinline__ void stage_mat(const float* src, Tile<P, kDC, kDC> m, int tid, int nth) {
+    for (int i = tid; i < kDC * kDC / 4; i += nth) {
+        const int r = i / 8, c = i % 8 * 4;
+        const f32x4 x = *reinterpret_cast<const f32x4*>(src + r * kDC + c);
+        if (TR) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) m.put(c + j, r, x[j]);
+        } else {
+            const float t[4] = {x[0], x[1], x[2], x[3]};
+            m.put4(r, c, t);
+        }
+    }
+}
+
+// g as the kernels use it: exp(-200) is 0 in fp32, and a sum of 32 such stays finite.
+__device__ __forceinline__ float delta_decay(float g) { return g < -200.f ? -200.f : g; }
+
+}  // namespace snhip

@@ -1,0 +1,388 @@
+// Gated delta rule, forward: the per-chunk matrices, the chunked scan and the
+// token-by-token form. Mathematics and layout: delta.h.
+#include "delta.h"
+
+namespace snhip {
+namespace {
+
+// M, P, G, L, beta of one chunk and value head: a block of four waves, one 16x16 tile
+// of the 32x32 matrices each. The inverse of the unit lower triangular I + A goes by
+// halves: its two diagonal 16x16 blocks by forward substitution, a column per lane,
+// then M10 = -M11 A10 M00.
+template <typename T, int KP>
+__global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
+    constexpr int P = ElemPlanes<T>::n;
+    __shared__ alignas(16) __bf16 sk[Tile<P, kDC, KP>::elems], sq[Tile<P, kDC, KP>::elems];
+    __shared__ double sc[kDC];
+    __shared__ float sb[kDC], sA[kDC][kDC + 1], sM[kDC][kDC + 1], sT[16][17];
+    const SnHipDelta& d = a.d;
+    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    DeltaSeq s;
+    int chunk;
+    if (!delta_chunk_of(d, blockIdx.x, &s, &chunk)) return;
+    const int64_t t0 = (int64_t)chunk * kDC;
+    const int n = (int)(s.len - t0 < kDC ? s.len - t0 : kDC);
+    const Tile<P, kDC, KP> K{sk}, Q{sq};
+    const Tile<P, KP, kDC> none{nullptr};
+    stage_tile<T, P, KP, true, false>(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n,
+                                      (int)d.K, a.vec_k, K, none, tid, 256);
+    stage_tile<T, P, KP, true, false>(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1], n,
+                                      (int)d.K, a.vec_q, Q, none, tid, 256);
+    if (wave == 0) {
+        const int64_t at = (s.row + t0 + lane) * d.H + h;
+        double c = lane < n ? (double)delta_decay(d.g[at]) : 0.0;
+#pragma unroll
+        for (int o = 1; o < kDC; o <<= 1) {
+            const double y = __shfl_up(c, o, kDC);
+            if ((lane & 31) >= o) c += y;
+        }
+        if (lane < kDC) {
+            sc[lane] = c;
+            sb[lane] = lane < n ? d.beta[at] : 0.f;
+        }
+    }
+    __syncthreads();
+    float* out = d.chunks + ((int64_t)blockIdx.x * d.H + h) * kDeltaChunk;
+    const int ti = wave >> 1, tj = wave & 1, col = tj * 16 + (lane & 15);
+    f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
+    if (tj <= ti) {
+#pragma unroll
+        for (int ks = 0; ks < KP / 32; ks++) {
+            const Frag<P> b = K.frag(16 * tj, ks, lane);
+            kk = mma<3>(K.frag(16 * ti, ks, lane), b, kk);
+            qk = mma<3>(Q.frag(16 * ti, ks, lane), b, qk);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int row = ti * 16 + (lane >> 4) * 4 + r;
+        const float D = col <= row ? expf((float)(sc[row] - sc[col])) : 0.f;
+        sA[row][col] = col < row ? sb[row] * D * kk[r] : 0.f;
+        out[kDeltaP + row * kDC + col] = col <= row ? (float)d.scale * D * qk[r] : 0.f;
+    }
+    if (tid < kDC) {
+        out[kDeltaG + tid] = expf((float)sc[tid]);
+        out[kDeltaL + tid] = expf((float)(sc[kDC - 1] - sc[tid]));
+        out[kDeltaB + tid] = sb[tid];
+    }
+    __syncthreads();
+    if (tid < 32) {
+        const int o = tid & 16, c = tid & 15;
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float v = i == c ? 1.f : 0.f;
+#pragma unroll
+            for (int j = 0; j < i; j++) v = fmaf(-sA[o + i][o + j], x[j], v);
+            x[i] = v;
+            sM[o + i][o + c] = v;
+        }
+    }
+    __syncthreads();
+    {
+        const int i = tid >> 4, j = tid & 15;
+        float v = 0.f;
+#pragma unroll
+        for (int l = 0; l < 16; l++) v = fmaf(sA[16 + i][l], sM[l][j], v);
+        sT[i][j] = v;
+        sM[i][16 + j] = 0.f;
+    }
+    __syncthreads();
+    {
+        const int i = tid >> 4, j = tid & 15;
+        float v = 0.f;
+#pragma unroll
+        for (int l = 0; l < 16; l++) v = fmaf(-sM[16 + i][16 + l], sT[l][j], v);
+        sM[16 + i][j] = v;
+    }
+    __syncthreads();
+    for (int i = tid; i < kDC * kDC; i += 256) out[i] = sM[i / kDC][i % kDC];
+}
+
+// The scan over chunks: W waves, 16 columns of V each. Half types read the state by
+// two planes where only out (of that type) depends on it.
+template <typename T, int KP, int W>
+__global__ __launch_bounds__(64 * W) void k_delta_scan(DeltaP a, T* out, float* send) {
+    constexpr int P = ElemPlanes<T>::n, NK = KP / 16;
+    constexpr int LO = sizeof(T) == 4 ? 3 : 2;      // planes of the products that only reach out
+    __shared__ alignas(16) __bf16 sk[Tile<P, kDC, KP>::elems], sq[Tile<P, kDC, KP>::elems],
+        skt[Tile<P, KP, kDC>::elems], sm[Tile<3, kDC, kDC>::elems], sp[Tile<LO, kDC, kDC>::elems];
+    __shared__ alignas(16) float sv[3 * kDC];
+    const SnHipDelta& d = a.d;
+    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4;
+    const DeltaSeq s = delta_seq(d, blockIdx.z);
+    const int v = (blockIdx.x * W + wave) * 16 + (lane & 15), V = (int)d.V, Kd = (int)d.K;
+    const Tile<P, kDC, KP> K{sk}, Q{sq};
+    const Tile<P, KP, kDC> KT{skt}, none{nullptr};
+    const Tile<3, kDC, kDC> M{sm};
+    const Tile<LO, kDC, kDC> PM{sp};
+    const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
+
+    f32x4 S[NK];
+#pragma unroll
+    for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int k = kt * 16 + g4 + r;
+            S[kt][r] = d.s0 && k < Kd && v < V ? d.s0[sbase + (int64_t)k * V + v] : 0.f;
+        }
+    for (int t0 = 0, c = 0; t0 < s.len; t0 += kDC, c++) {
+        const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
+        const float* pre = d.chunks + ((s.slot + c) * d.H + h) * kDeltaChunk;
+        __syncthreads();
+        stage_tile<T, P, KP, true, true>(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n,
+                                         Kd, a.vec_k, K, KT, tid, 64 * W);
+        stage_tile<T, P, KP, true, false>(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1],
+                                          n, Kd, a.vec_q, Q, none, tid, 64 * W);
+        stage_mat<3, false>(pre, M, tid, 64 * W);
+        stage_mat<LO, false>(pre + kDeltaP, PM, tid, 64 * W);
+        for (int i = tid; i < 3 * kDC; i += 64 * W) sv[i] = pre[kDeltaG + i];
+        __syncthreads();
+        if (d.states) {       // S^T (VP, KP) before the chunk, for the backward
+            float* st = d.states + ((s.slot + c) * d.H + h) * (int64_t)(a.VP * KP);
+            if (v < a.VP)
+#pragma unroll
+                for (int kt = 0; kt < NK; kt++)
+                    *reinterpret_cast<f32x4*>(st + (int64_t)v * KP + kt * 16 + g4) = S[kt];
+        }
+        f32x4 ks[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int i = 0; i < KP / 32; i++) {
+            float x[8];
+#pragma unroll
+            for (int r = 0; r < 4; r++) x[r] = S[2 * i][r], x[4 + r] = S[2 * i + 1][r];
+            const Frag<3> b = split8<3>(x);
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                ks[m] = mma<3>(K.frag(16 * m, i, lane), b, ks[m]);
+                o[m] = mma<LO>(Q.frag(16 * m, i, lane), b, o[m]);
+            }
+        }
+        const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t0, h) + v;
+        float x[8];
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = 16 * m + g4 + r;
+                const float vv = t < n && v < V ? (float)vp[t * d.v_stride[1]] : 0.f;
+                x[4 * m + r] = sv[2 * kDC + t] * (vv - sv[t] * ks[m][r]);
+                o[m][r] *= (float)d.scale * sv[t];
+            }
+        const Frag<3> R = split8<3>(x);
+        f32x4 u[2];
+#pragma unroll
+        for (int m = 0; m < 2; m++) u[m] = mma<3>(M.frag(16 * m, 0, lane), R, f32x4{0, 0, 0, 0});
+        float y[8];
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                x[4 * m + r] = u[m][r];
+                y[4 * m + r] = u[m][r] * sv[kDC + 16 * m + g4 + r];
+            }
+        const Frag<LO> U = split8<LO>(x);
+        const Frag<3> LU = split8<3>(y);
+        T* op = out + ((s.row + t0) * d.H + h) * (int64_t)V + v;
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+            o[m] = mma<LO>(PM.frag(16 * m, 0, lane), U, o[m]);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = 16 * m + g4 + r;
+                if (t < n && v < V) op[(int64_t)t * d.H * V] = (T)o[m][r];
+            }
+        }
+        const float decay = sv[kDC - 1];
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++) S[kt] = mma<3>(KT.frag(16 * kt, 0, lane), LU, S[kt] * decay);
+    }
+    if (send && v < V)
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int k = kt * 16 + g4 + r;
+                if (k < Kd) send[sbase + (int64_t)k * V + v] = S[kt][r];
+            }
+}
+
+// Token by token. A wave owns 32 columns of V of one sequence and head: lane (kg, vg)
+// holds rows kg RPT .. + RPT - 1 and four columns, all in registers from one read of the
+// state to one write. q.S' = a q.S + (q.k) u, so one pass over the state gives both
+// read-outs. Bound by the state's bytes.
+template <typename T, int RPT>
+__global__ __launch_bounds__(64) void k_delta_step(DeltaP a, T* out, const float* s0, float* send) {
+    const SnHipDelta& d = a.d;
+    const int h = blockIdx.y, lane = threadIdx.x, kg = lane >> 3, k0 = kg * RPT;
+    const int V = (int)d.V, Kd = (int)d.K, v0 = blockIdx.x * 32 + (lane & 7) * 4;
+    const DeltaSeq s = delta_seq(d, blockIdx.z);
+    const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
+    const bool whole = (V & 3) == 0 && v0 < V;       // four columns at a 16-byte address
+    f32x4 S[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+        S[i] = f32x4{0, 0, 0, 0};
+        const int k = k0 + i;
+        if (!s0 || k >= Kd) continue;
+        const float* p = s0 + sbase + (int64_t)k * V + v0;
+        if (whole) {
+            S[i] = *reinterpret_cast<const f32x4*>(p);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (v0 + j < V) S[i][j] = p[j];
+        }
+    }
+    for (int t = 0; t < s.len; t++) {
+        const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t, h / a.rep);
+        const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t, h / a.rep);
+        const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t, h);
+        const int64_t row = (s.row + t) * d.H + h;
+        const float al = expf(d.g[row]), be = d.beta[row];
+        float q[RPT], k[RPT];
+#pragma unroll
+        for (int i = 0; i < RPT; i += 8) {
+            load8(qp + k0 + i, Kd - k0 - i, a.vec_q, q + i);
+            load8(kp + k0 + i, Kd - k0 - i, a.vec_k, k + i);
+        }
+        f32x4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
+        float qk = 0.f;
+#pragma unroll
+        for (int i = 0; i < RPT; i++) {
+            qk = fmaf(q[i], k[i], qk);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                sk[j] = fmaf(S[i][j], k[i], sk[j]);
+                sq[j] = fmaf(S[i][j], q[i], sq[j]);
+            }
+        }
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) {
+            qk += __shfl_xor(qk, o);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                sk[j] += __shfl_xor(sk[j], o);
+                sq[j] += __shfl_xor(sq[j], o);
+            }
+        }
+        f32x4 u;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float vv = v0 + j < V ? (float)vp[v0 + j] : 0.f;
+            u[j] = be * (vv - al * sk[j]);
+            const float o = (float)d.scale * (al * sq[j] + qk * u[j]);
+            if (kg == 0 && v0 + j < V) out[row * V + v0 + j] = (T)o;
+        }
+#pragma unroll
+        for (int i = 0; i < RPT; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) S[i][j] = fmaf(k[i], u[j], al * S[i][j]);
+    }
+    if (!send) return;
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+        const int k = k0 + i;
+        if (k >= Kd) continue;
+        float* p = send + sbase + (int64_t)k * V + v0;
+        if (whole) {
+            *reinterpret_cast<f32x4*>(p) = S[i];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (v0 + j < V) p[j] = S[i][j];
+        }
+    }
+}
+
+template <typename T>
+snhip_status step_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
+    const dim3 grid((unsigned)((a.d.V + 31) / 32), (unsigned)a.d.H, (unsigned)a.d.N);
+    if (a.KP == 64) k_delta_step<T, 8><<<grid, 64, 0, st>>>(a, (T*)out, a.d.s0, send);
+    else k_delta_step<T, 16><<<grid, 64, 0, st>>>(a, (T*)out, a.d.s0, send);
+    SNHIP_CHECK(hipGetLastError());
+    return SNHIP_OK;
+}
+
+template <typename T, int KP>
+snhip_status fwd_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
+    k_delta_prep<T, KP><<<dim3((unsigned)a.slots, (unsigned)a.d.H), 256, 0, st>>>(a);
+    SNHIP_CHECK(hipGetLastError());
+    const int strips = a.VP / 16;
+    const int W = strips >= 4 ? 4 : strips >= 2 ? 2 : 1;
+    const dim3 grid((unsigned)((strips + W - 1) / W), (unsigned)a.d.H, (unsigned)a.d.N);
+    if (W == 4) k_delta_scan<T, KP, 4><<<grid, 256, 0, st>>>(a, (T*)out, send);
+    else if (W == 2) k_delta_scan<T, KP, 2><<<grid, 128, 0, st>>>(a, (T*)out, send);
+    else k_delta_scan<T, KP, 1><<<grid, 64, 0, st>>>(a, (T*)out, send);
+    SNHIP_CHECK(hipGetLastError());
+    return SNHIP_OK;
+}
+
+}  // namespace
+
+// Checks d and fills in what the kernels derive from it.
+snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
+    if (!d || !d->q || !d->k || !d->v || !d->g || !d->beta) return SNHIP_E_INVAL;
+    if (d->B < 1 || d->T < 1 || d->N < 1 || d->N > 65535 || d->H < 1 || d->H > 65535 || d->Hk < 1 ||
+        d->H % d->Hk || d->K < 1 || d->K > 128 || d->V < 1 || d->V > 4096 || d->T > INT32_MAX / d->B ||
+        (d->cu ? d->B != 1 : d->N != d->B) || d->dtype < SNHIP_F32 || d->dtype > SNHIP_F16)
+        return SNHIP_E_INVAL;
+    a->d = *d;
+    a->slots = delta_slots(*d);
+    a->KP = delta_kp(d->K);
+    a->VP = delta_vp(d->V);
+    a->rep = (int)(d->H / d->Hk);
+    const int64_t step = d->dtype == SNHIP_F32 ? 4 : 8;       // elements of 16 bytes
+    auto vec = [&](const void* p, const int64_t* s) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % step == 0 && s[1] % step == 0 && s[2] % step == 0;
+    };
+    a->vec_q = vec(d->q, d->q_stride);
+    a->vec_k = vec(d->k, d->k_stride);
+    a->vec_v = vec(d->v, d->v_stride);
+    return SNHIP_OK;
+}
+
+}  // namespace snhip
+
+using namespace snhip;
+
+extern "C" {
+
+int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d) {
+    return d ? delta_slots(*d) * d->H * kDeltaChunk : 0;
+}
+int64_t snhip_op_delta_state_floats(const SnHipDelta* d) {
+    return d ? delta_slots(*d) * d->H * delta_kp(d->K) * delta_vp(d->V) : 0;
+}
+
+snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send, void* stream) {
+    DeltaP a;
+    const snhip_status rc = delta_args(d, &a);
+    if (rc != SNHIP_OK || !out || !send) return SNHIP_E_INVAL;
+    if (d->dtype == SNHIP_F32) return step_t<float>(a, out, send, as_stream(stream));
+    if (d->dtype == SNHIP_BF16) return step_t<__bf16>(a, out, send, as_stream(stream));
+    return step_t<_Float16>(a, out, send, as_stream(stream));
+}
+
+snhip_status snhip_op_delta_fwd_dev(const SnHipDelta* d, void* out, float* send, void* stream) {
+    DeltaP a;
+    const snhip_status rc = delta_args(d, &a);
+    if (rc != SNHIP_OK || !out) return SNHIP_E_INVAL;
+    const hipStream_t st = as_stream(stream);
+    if (!d->chunks) {
+        if (d->cu || d->states || d->T > 16) return SNHIP_E_INVAL;
+        if (d->dtype == SNHIP_F32) return step_t<float>(a, out, send, st);
+        if (d->dtype == SNHIP_BF16) return step_t<__bf16>(a, out, send, st);
+        return step_t<_Float16>(a, out, send, st);
+    }
+    if (a.KP == 64) {
+        if (d->dtype == SNHIP_F32) return fwd_t<float, 64>(a, out, send, st);
+        if (d->dtype == SNHIP_BF16) return fwd_t<__bf16, 64>(a, out, send, st);
+        return fwd_t<_Float16, 64>(a, out, send, st);
+    }
+    if (d->dtype == SNHIP_F32) return fwd_t<float, 128>(a, out, send, st);
+    if (d->dtype == SNHIP_BF16) return fwd_t<__bf16, 128>(a, out, send, st);
+    return fwd_t<_Float16, 128>(a, out, send, st);
+}
+
+}  // extern "C"

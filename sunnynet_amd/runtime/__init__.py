@@ -14,9 +14,14 @@ from __future__ import annotations
 import torch
 
 from .. import _native
+from .delta import GatedDelta, delta_bwd, delta_fwd, delta_step, gated_delta
+from .norm import LayerNorm, layer_norm, norm_bwd, norm_fwd
+from .sample import sample_tokens
 
-__all__ = ["FMA", "GATED", "CoreFused", "GatedScan", "core_bwd", "core_forward", "core_fwd", "gated_scan",
-           "load_runtime", "runtime_available", "scan", "scan_bwd", "step"]
+__all__ = ["FMA", "GATED", "CoreFused", "GatedDelta", "GatedScan", "LayerNorm", "core_bwd", "core_forward",
+           "core_fwd", "delta_bwd", "delta_fwd", "delta_step", "gated_delta", "gated_scan", "layer_norm",
+           "load_runtime", "norm_bwd", "norm_fwd", "runtime_available", "sample_tokens", "scan", "scan_bwd",
+           "step"]
 
 FMA = 0
 GATED = 1
