@@ -14,7 +14,7 @@
 // once. What is left is sequential over chunks but independent over the columns of V:
 // a wave owns 16 of them and keeps its (K, 16) of the state in registers, where the
 // results of one product are the operand of the next (planes.h); LDS only holds the
-// tiles that all columns share.
+// tiles that all columns share. Rows of K and tokens are both taken in pair_row's order.
 #pragma once
 
 #include "common.h"
@@ -24,15 +24,16 @@
 namespace snhip {
 
 constexpr int kDC = 32;                            // tokens per chunk
-// Per chunk and head: M, P (32 x 32 each), then G, L, beta (32 each).
-constexpr int kDeltaP = 1024, kDeltaG = 2048, kDeltaL = 2080, kDeltaB = 2112, kDeltaChunk = 2144;
+// Per chunk and head, in floats: M and P as three bf16 planes of 32 x 32 each, then G, L
+// and beta (32 each).
+constexpr int kDeltaP = 1536, kDeltaG = 3072, kDeltaChunk = 3168;
 
 struct DeltaP {
     SnHipDelta d;
     int64_t slots;          // chunk slots of all sequences
     int KP, VP;             // K and V padded: state slabs are (VP, KP), k contiguous
     int rep;                // value heads per query and key head
-    bool vec_q, vec_k, vec_v;   // 16-byte loads reach
+    bool vec_q, vec_k;          // 16-byte loads reach
 };
 
 __host__ __device__ inline int64_t delta_slots(const SnHipDelta& d) {
@@ -94,41 +95,48 @@ __device__ __forceinline__ const T* delta_at(const void* p, const int64_t* st, i
     return static_cast<const T*>(p) + b * st[0] + t * st[1] + h * st[2];
 }
 
-// Rows [0, 32) of a (tokens, K) tile into LDS, rows from n on and columns from K on 0:
-// rows by token (`rows`) and / or rows by column (`cols`).
-template <typename T, int P, int KP, bool ROWS, bool COLS>
-__device__ __forceinline__ void stage_tile(const T* src, int64_t stride, int n, int K, bool vec,
-                                           Tile<P, kDC, KP> rows, Tile<P, KP, kDC> cols, int tid, int nth) {
-    for (int i = tid; i < kDC * KP / 8; i += nth) {
-        const int t = i / (KP / 8), c = i % (KP / 8) * 8;
-        float x[8];
-        load8(src + t * stride + c, t < n ? K - c : 0, vec, x);
-        if (ROWS) {
-            rows.put4(t, c, x);
-            rows.put4(t, c + 4, x + 4);
-        }
-        if (COLS) {
+// A (32, KP) tile of a (tokens, K) array on its way from memory to LDS, held by NTH
+// threads: rows from n on and columns from K on are 0.
+template <typename T, int KP, int NTH> struct RowsFetch {
+    static constexpr int P = ElemPlanes<T>::n, N = (kDC * KP / 8 + NTH - 1) / NTH;
+    static constexpr bool whole = kDC * KP / 8 % NTH == 0;
+    Vec8<T> x[N];
+    __device__ __forceinline__ void load(const T* src, int64_t stride, int n, int K, bool vec, int tid) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) cols.put(c + j, t, x[j]);
+        for (int j = 0; j < N; j++) {
+            const int i = tid + j * NTH, t = i / (KP / 8), c = i % (KP / 8) * 8;
+            if (whole || t < kDC) x[j] = load_raw8(src + t * stride + c, t < n ? K - c : 0, vec);
         }
     }
-}
+    __device__ __forceinline__ void store(Tile<P, kDC, KP> to, int tid) const {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int i = tid + j * NTH, t = i / (KP / 8), c = i % (KP / 8) * 8;
+            if (whole || t < kDC) to.put8(t, c, split_raw8<T>(x[j]));
+        }
+    }
+};
 
-// A (32, 32) fp32 matrix into LDS, as stored or transposed.
-template <int P, bool TR>
-__device__ __forceinline__ void stage_mat(const float* src, Tile<P, kDC, kDC> m, int tid, int nth) {
-    for (int i = tid; i < kDC * kDC / 4; i += nth) {
-        const int r = i / 8, c = i % 8 * 4;
-        const f32x4 x = *reinterpret_cast<const f32x4*>(src + r * kDC + c);
-        if (TR) {
+// The first Q planes of a (32, 32) matrix of a chunk's record, likewise.
+template <int Q, int NTH> struct MatFetch {
+    static constexpr int N = (Q * 128 + NTH - 1) / NTH;
+    static constexpr bool whole = Q * 128 % NTH == 0;
+    bf16x8 x[N];
+    __device__ __forceinline__ void load(const float* rec, int tid) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) m.put(c + j, r, x[j]);
-        } else {
-            const float t[4] = {x[0], x[1], x[2], x[3]};
-            m.put4(r, c, t);
+        for (int j = 0; j < N; j++) {
+            const int i = tid + j * NTH;
+            if (whole || i < Q * 128) x[j] = *reinterpret_cast<const bf16x8*>(rec + i * 4);
         }
     }
-}
+    __device__ __forceinline__ void store(Tile<Q, kDC, kDC> to, int tid) const {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int i = tid + j * NTH;
+            if (whole || i < Q * 128) *reinterpret_cast<bf16x8*>(to.at(i >> 7, (i >> 2) & 31, (i & 3) * 8)) = x[j];
+        }
+    }
+};
 
 // g as the kernels use it: exp(-200) is 0 in fp32, and a sum of 32 such stays finite.
 __device__ __forceinline__ float delta_decay(float g) { return g < -200.f ? -200.f : g; }

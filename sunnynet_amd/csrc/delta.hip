@@ -14,20 +14,18 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
     constexpr int P = ElemPlanes<T>::n;
     __shared__ alignas(16) __bf16 sk[Tile<P, kDC, KP>::elems], sq[Tile<P, kDC, KP>::elems];
     __shared__ double sc[kDC];
-    __shared__ float sb[kDC], sA[kDC][kDC + 1], sM[kDC][kDC + 1], sT[16][17];
+    __shared__ float sb[kDC], sA[kDC][kDC + 1], sM[kDC][kDC + 1], sP[kDC][kDC + 1], sT[16][17];
     const SnHipDelta& d = a.d;
-    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15;
     DeltaSeq s;
     int chunk;
     if (!delta_chunk_of(d, blockIdx.x, &s, &chunk)) return;
     const int64_t t0 = (int64_t)chunk * kDC;
     const int n = (int)(s.len - t0 < kDC ? s.len - t0 : kDC);
     const Tile<P, kDC, KP> K{sk}, Q{sq};
-    const Tile<P, KP, kDC> none{nullptr};
-    stage_tile<T, P, KP, true, false>(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n,
-                                      (int)d.K, a.vec_k, K, none, tid, 256);
-    stage_tile<T, P, KP, true, false>(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1], n,
-                                      (int)d.K, a.vec_q, Q, none, tid, 256);
+    RowsFetch<T, KP, 256> fk, fq;
+    fk.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n, (int)d.K, a.vec_k, tid);
+    fq.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1], n, (int)d.K, a.vec_q, tid);
     if (wave == 0) {
         const int64_t at = (s.row + t0 + lane) * d.H + h;
         double c = lane < n ? (double)delta_decay(d.g[at]) : 0.0;
@@ -41,16 +39,18 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
             sb[lane] = lane < n ? d.beta[at] : 0.f;
         }
     }
+    fk.store(K, tid);
+    fq.store(Q, tid);
     __syncthreads();
     float* out = d.chunks + ((int64_t)blockIdx.x * d.H + h) * kDeltaChunk;
-    const int ti = wave >> 1, tj = wave & 1, col = tj * 16 + (lane & 15);
+    const int ti = wave >> 1, tj = wave & 1, col = tj * 16 + l16;
     f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
     if (tj <= ti) {
 #pragma unroll
-        for (int ks = 0; ks < KP / 32; ks++) {
-            const Frag<P> b = K.frag(16 * tj, ks, lane);
-            kk = mma<3>(K.frag(16 * ti, ks, lane), b, kk);
-            qk = mma<3>(Q.frag(16 * ti, ks, lane), b, qk);
+        for (int c = 0; c < KP; c += 32) {
+            const Frag<P> b = K.frag(16 * tj + l16, c, lane);
+            kk = mma<3>(K.frag(16 * ti + l16, c, lane), b, kk);
+            qk = mma<3>(Q.frag(16 * ti + l16, c, lane), b, qk);
         }
     }
 #pragma unroll
@@ -58,12 +58,12 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
         const int row = ti * 16 + (lane >> 4) * 4 + r;
         const float D = col <= row ? expf((float)(sc[row] - sc[col])) : 0.f;
         sA[row][col] = col < row ? sb[row] * D * kk[r] : 0.f;
-        out[kDeltaP + row * kDC + col] = col <= row ? (float)d.scale * D * qk[r] : 0.f;
+        sP[row][col] = col <= row ? (float)d.scale * D * qk[r] : 0.f;
     }
     if (tid < kDC) {
         out[kDeltaG + tid] = expf((float)sc[tid]);
-        out[kDeltaL + tid] = expf((float)(sc[kDC - 1] - sc[tid]));
-        out[kDeltaB + tid] = sb[tid];
+        out[kDeltaG + kDC + tid] = expf((float)(sc[kDC - 1] - sc[tid]));
+        out[kDeltaG + 2 * kDC + tid] = sb[tid];
     }
     __syncthreads();
     if (tid < 32) {
@@ -96,113 +96,159 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
         sM[16 + i][j] = v;
     }
     __syncthreads();
-    for (int i = tid; i < kDC * kDC; i += 256) out[i] = sM[i / kDC][i % kDC];
+    {
+        // eight values a thread: M by the first two waves, P by the others
+        const int i = tid & 127, row = i >> 2, c = (i & 3) * 8;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = tid < 128 ? sM[row][c + j] : sP[row][c + j];
+        const Frag<3> f = split8<3>(x);
+        float* to = out + (tid < 128 ? 0 : kDeltaP) + i * 4;
+#pragma unroll
+        for (int p = 0; p < 3; p++) *reinterpret_cast<bf16x8*>(to + p * 512) = f.p[p];
+    }
 }
 
 // The scan over chunks: W waves, 16 columns of V each. Half types read the state by
-// two planes where only out (of that type) depends on it.
+// two planes where only out (of that type) depends on it. The next chunk's tiles are
+// fetched into registers while this one is worked on, and put into the other half of LDS:
+// one barrier per chunk, no wait for memory in between.
 template <typename T, int KP, int W>
 __global__ __launch_bounds__(64 * W) void k_delta_scan(DeltaP a, T* out, float* send) {
-    constexpr int P = ElemPlanes<T>::n, NK = KP / 16;
+    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, NTH = 64 * W;
     constexpr int LO = sizeof(T) == 4 ? 3 : 2;      // planes of the products that only reach out
-    __shared__ alignas(16) __bf16 sk[Tile<P, kDC, KP>::elems], sq[Tile<P, kDC, KP>::elems],
-        skt[Tile<P, KP, kDC>::elems], sm[Tile<3, kDC, kDC>::elems], sp[Tile<LO, kDC, kDC>::elems];
-    __shared__ alignas(16) float sv[3 * kDC];
+    typedef Tile<P, kDC, KP> Rows;
+    typedef Tile<3, kDC, kDC> MatM;
+    typedef Tile<LO, kDC, kDC> MatP;
+    __shared__ alignas(16) __bf16 sk[2][Rows::elems], sq[2][Rows::elems], sm[2][MatM::elems], sp[2][MatP::elems];
+    __shared__ alignas(16) float sv[2][3 * kDC];
     const SnHipDelta& d = a.d;
-    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4;
+    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g8 = (lane >> 4) * 8;
     const DeltaSeq s = delta_seq(d, blockIdx.z);
-    const int v = (blockIdx.x * W + wave) * 16 + (lane & 15), V = (int)d.V, Kd = (int)d.K;
-    const Tile<P, kDC, KP> K{sk}, Q{sq};
-    const Tile<P, KP, kDC> KT{skt}, none{nullptr};
-    const Tile<3, kDC, kDC> M{sm};
-    const Tile<LO, kDC, kDC> PM{sp};
+    const int v = (blockIdx.x * W + wave) * 16 + l16, V = (int)d.V, Kd = (int)d.K;
     const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
+    const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0, h / a.rep);
+    const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0, h / a.rep);
+    const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0, h) + v;
+    const float* rec = d.chunks + (s.slot * d.H + h) * kDeltaChunk;
 
-    f32x4 S[NK];
+    f32x4 S[NK];           // S[2 p + e][r] is row 32 p + g8 + 4 e + r of column v
 #pragma unroll
     for (int kt = 0; kt < NK; kt++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int k = kt * 16 + g4 + r;
+            const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
             S[kt][r] = d.s0 && k < Kd && v < V ? d.s0[sbase + (int64_t)k * V + v] : 0.f;
         }
-    for (int t0 = 0, c = 0; t0 < s.len; t0 += kDC, c++) {
+    RowsFetch<T, KP, NTH> fk, fq;
+    MatFetch<3, NTH> fm;
+    MatFetch<LO, NTH> fp;
+    float fv[(3 * kDC + NTH - 1) / NTH];
+    T vv[8];
+    auto fetch = [&](int t0) {
         const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
-        const float* pre = d.chunks + ((s.slot + c) * d.H + h) * kDeltaChunk;
-        __syncthreads();
-        stage_tile<T, P, KP, true, true>(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n,
-                                         Kd, a.vec_k, K, KT, tid, 64 * W);
-        stage_tile<T, P, KP, true, false>(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1],
-                                          n, Kd, a.vec_q, Q, none, tid, 64 * W);
-        stage_mat<3, false>(pre, M, tid, 64 * W);
-        stage_mat<LO, false>(pre + kDeltaP, PM, tid, 64 * W);
-        for (int i = tid; i < 3 * kDC; i += 64 * W) sv[i] = pre[kDeltaG + i];
-        __syncthreads();
+        const float* r = rec + (int64_t)(t0 / kDC) * d.H * kDeltaChunk;
+        fk.load(kp + t0 * d.k_stride[1], d.k_stride[1], n, Kd, a.vec_k, tid);
+        fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, a.vec_q, tid);
+        fm.load(r, tid);
+        fp.load(r + kDeltaP, tid);
+#pragma unroll
+        for (int j = 0; j * NTH < 3 * kDC; j++)
+            if (tid + j * NTH < 3 * kDC) fv[j] = r[kDeltaG + tid + j * NTH];
+#pragma unroll
+        for (int i = 0; i < 8; i++) vv[i] = g8 + i < n && v < V ? vp[(t0 + g8 + i) * d.v_stride[1]] : (T)0.f;
+    };
+    auto store = [&](int b) {
+        fk.store(Rows{sk[b]}, tid);
+        fq.store(Rows{sq[b]}, tid);
+        fm.store(MatM{sm[b]}, tid);
+        fp.store(MatP{sp[b]}, tid);
+#pragma unroll
+        for (int j = 0; j * NTH < 3 * kDC; j++)
+            if (tid + j * NTH < 3 * kDC) sv[b][tid + j * NTH] = fv[j];
+    };
+    if (s.len > 0) {
+        fetch(0);
+        store(0);
+    }
+    barrier_lds();
+    for (int t0 = 0, b = 0; t0 < s.len; t0 += kDC, b ^= 1) {
+        const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
+        const Rows K{sk[b]}, Q{sq[b]};
+        float vc[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) vc[i] = (float)vv[i];
+        const bool more = t0 + kDC < s.len;
+        if (more) fetch(t0 + kDC);
         if (d.states) {       // S^T (VP, KP) before the chunk, for the backward
-            float* st = d.states + ((s.slot + c) * d.H + h) * (int64_t)(a.VP * KP);
+            float* st = d.states + ((s.slot + t0 / kDC) * d.H + h) * (int64_t)(a.VP * KP);
             if (v < a.VP)
 #pragma unroll
                 for (int kt = 0; kt < NK; kt++)
-                    *reinterpret_cast<f32x4*>(st + (int64_t)v * KP + kt * 16 + g4) = S[kt];
+                    *reinterpret_cast<f32x4*>(st + (int64_t)v * KP + (kt >> 1) * 32 + g8 + 4 * (kt & 1)) = S[kt];
         }
         f32x4 ks[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-        for (int i = 0; i < KP / 32; i++) {
+        for (int p = 0; p < KP / 32; p++) {
             float x[8];
 #pragma unroll
-            for (int r = 0; r < 4; r++) x[r] = S[2 * i][r], x[4 + r] = S[2 * i + 1][r];
-            const Frag<3> b = split8<3>(x);
+            for (int r = 0; r < 4; r++) x[r] = S[2 * p][r], x[4 + r] = S[2 * p + 1][r];
+            const Frag<3> f = split8<3>(x);
 #pragma unroll
             for (int m = 0; m < 2; m++) {
-                ks[m] = mma<3>(K.frag(16 * m, i, lane), b, ks[m]);
-                o[m] = mma<LO>(Q.frag(16 * m, i, lane), b, o[m]);
+                ks[m] = mma<3>(K.frag(pair_row(m, l16), 32 * p, lane), f, ks[m]);
+                o[m] = mma<LO>(Q.frag(pair_row(m, l16), 32 * p, lane), f, o[m]);
             }
         }
-        const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t0, h) + v;
-        float x[8];
+        float G[8], L[8], be[8], x[8], y[8];
 #pragma unroll
-        for (int m = 0; m < 2; m++)
+        for (int i = 0; i < 8; i += 4) {
+            const f32x4 t0v = *reinterpret_cast<const f32x4*>(&sv[b][g8 + i]),
+                        t1v = *reinterpret_cast<const f32x4*>(&sv[b][kDC + g8 + i]),
+                        t2v = *reinterpret_cast<const f32x4*>(&sv[b][2 * kDC + g8 + i]);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = 16 * m + g4 + r;
-                const float vv = t < n && v < V ? (float)vp[t * d.v_stride[1]] : 0.f;
-                x[4 * m + r] = sv[2 * kDC + t] * (vv - sv[t] * ks[m][r]);
-                o[m][r] *= (float)d.scale * sv[t];
-            }
+            for (int r = 0; r < 4; r++) G[i + r] = t0v[r], L[i + r] = t1v[r], be[i + r] = t2v[r];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = be[i] * (vc[i] - G[i] * ks[i >> 2][i & 3]);
+            o[i >> 2][i & 3] *= (float)d.scale * G[i];
+        }
         const Frag<3> R = split8<3>(x);
-        f32x4 u[2];
 #pragma unroll
-        for (int m = 0; m < 2; m++) u[m] = mma<3>(M.frag(16 * m, 0, lane), R, f32x4{0, 0, 0, 0});
-        float y[8];
-#pragma unroll
-        for (int m = 0; m < 2; m++)
+        for (int m = 0; m < 2; m++) {
+            const f32x4 u = mma<3>(MatM{sm[b]}.frag(pair_row(m, l16), 0, lane), R, f32x4{0, 0, 0, 0});
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                x[4 * m + r] = u[m][r];
-                y[4 * m + r] = u[m][r] * sv[kDC + 16 * m + g4 + r];
+                x[4 * m + r] = u[r];
+                y[4 * m + r] = u[r] * L[4 * m + r];
             }
+        }
         const Frag<LO> U = split8<LO>(x);
         const Frag<3> LU = split8<3>(y);
+        const float decay = sv[b][kDC - 1];
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++)
+            S[kt] = mma<3>(K.tfrag(0, (kt >> 1) * 32 + 8 * (lane & 3) + 4 * (kt & 1), lane), LU, S[kt] * decay);
         T* op = out + ((s.row + t0) * d.H + h) * (int64_t)V + v;
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            o[m] = mma<LO>(PM.frag(16 * m, 0, lane), U, o[m]);
+            o[m] = mma<LO>(MatP{sp[b]}.frag(pair_row(m, l16), 0, lane), U, o[m]);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int t = 16 * m + g4 + r;
+                const int t = g8 + 4 * m + r;
                 if (t < n && v < V) op[(int64_t)t * d.H * V] = (T)o[m][r];
             }
         }
-        const float decay = sv[kDC - 1];
-#pragma unroll
-        for (int kt = 0; kt < NK; kt++) S[kt] = mma<3>(KT.frag(16 * kt, 0, lane), LU, S[kt] * decay);
+        if (more) store(b ^ 1);
+        barrier_lds();
     }
     if (send && v < V)
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int k = kt * 16 + g4 + r;
+                const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
                 if (k < Kd) send[sbase + (int64_t)k * V + v] = S[kt][r];
             }
 }
@@ -338,7 +384,6 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
     };
     a->vec_q = vec(d->q, d->q_stride);
     a->vec_k = vec(d->k, d->k_stride);
-    a->vec_v = vec(d->v, d->v_stride);
     return SNHIP_OK;
 }
 

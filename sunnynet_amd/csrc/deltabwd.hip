@@ -22,7 +22,7 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a);
 
 namespace {
 
-// Per slot and head: dR (32, VP), then dS^T (VP, KP) after the chunk.
+// Per slot and head: dR^T (VP, 32), then dS^T (VP, KP) after the chunk.
 struct DeltaWs {
     float* dr;
     float* ds;
@@ -32,159 +32,193 @@ __host__ __device__ inline DeltaWs delta_ws(const DeltaP& a, float* ws, int64_t 
     return {ws + i * kDC * a.VP, ws + nr + i * (int64_t)(a.VP * a.KP)};
 }
 
-// Rows of 16x16 results that belong to this lane's column: 16 m + 4 (lane / 16) + r.
-__device__ __forceinline__ int res_row(int m, int lane, int r) { return 16 * m + (lane >> 4) * 4 + r; }
-
 template <typename T, int KP, int W>
 __global__ __launch_bounds__(64 * W) void k_delta_rscan(DeltaP a, SnHipDeltaGrad gr) {
-    constexpr int P = ElemPlanes<T>::n, NK = KP / 16;
-    __shared__ alignas(16) __bf16 sk[Tile<P, kDC, KP>::elems], skt[Tile<P, KP, kDC>::elems],
-        sqt[Tile<P, KP, kDC>::elems], sm[Tile<3, kDC, kDC>::elems], sp[Tile<3, kDC, kDC>::elems];
-    __shared__ alignas(16) float sv[3 * kDC];
+    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, NTH = 64 * W;
+    typedef Tile<P, kDC, KP> Rows;
+    typedef Tile<3, kDC, kDC> Mat;
+    __shared__ alignas(16) __bf16 sk[2][Rows::elems], sq[2][Rows::elems], sm[2][Mat::elems], sp[2][Mat::elems];
+    __shared__ alignas(16) float sv[2][3 * kDC];
     const SnHipDelta& d = a.d;
-    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4;
+    const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g8 = (lane >> 4) * 8;
     const DeltaSeq s = delta_seq(d, blockIdx.z);
-    const int v = (blockIdx.x * W + wave) * 16 + (lane & 15), V = (int)d.V, Kd = (int)d.K;
-    const Tile<P, kDC, KP> K{sk}, none{nullptr};
-    const Tile<P, KP, kDC> KT{skt}, QT{sqt};
-    const Tile<3, kDC, kDC> MT{sm}, PT{sp};
+    const int v = (blockIdx.x * W + wave) * 16 + l16, V = (int)d.V, Kd = (int)d.K;
     const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
+    const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0, h / a.rep);
+    const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0, h / a.rep);
+    const T* dop = static_cast<const T*>(gr.dout) + (s.row * d.H + h) * (int64_t)V + v;
+    const float* rec = d.chunks + (s.slot * d.H + h) * kDeltaChunk;
 
-    f32x4 S[NK];
+    f32x4 S[NK];           // dS, rows as k_delta_scan holds S
 #pragma unroll
     for (int kt = 0; kt < NK; kt++)
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int k = kt * 16 + g4 + r;
+            const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
             S[kt][r] = gr.dsend && k < Kd && v < V ? gr.dsend[sbase + (int64_t)k * V + v] : 0.f;
         }
-    for (int c = (s.len + kDC - 1) / kDC - 1; c >= 0; c--) {
-        const int t0 = c * kDC, n = s.len - t0 < kDC ? s.len - t0 : kDC;
-        const float* pre = d.chunks + ((s.slot + c) * d.H + h) * kDeltaChunk;
-        const DeltaWs w = delta_ws(a, gr.ws, s.slot + c, h);
-        __syncthreads();
-        stage_tile<T, P, KP, true, true>(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n,
-                                         Kd, a.vec_k, K, KT, tid, 64 * W);
-        stage_tile<T, P, KP, false, true>(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1],
-                                          n, Kd, a.vec_q, none, QT, tid, 64 * W);
-        stage_mat<3, true>(pre, MT, tid, 64 * W);
-        stage_mat<3, true>(pre + kDeltaP, PT, tid, 64 * W);
-        for (int i = tid; i < 3 * kDC; i += 64 * W) sv[i] = pre[kDeltaG + i];
-        __syncthreads();
+    RowsFetch<T, KP, NTH> fk, fq;
+    MatFetch<3, NTH> fm, fp;
+    float fv[(3 * kDC + NTH - 1) / NTH];
+    T vv[8];
+    auto fetch = [&](int t0) {
+        const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
+        const float* r = rec + (int64_t)(t0 / kDC) * d.H * kDeltaChunk;
+        fk.load(kp + t0 * d.k_stride[1], d.k_stride[1], n, Kd, a.vec_k, tid);
+        fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, a.vec_q, tid);
+        fm.load(r, tid);
+        fp.load(r + kDeltaP, tid);
+#pragma unroll
+        for (int j = 0; j * NTH < 3 * kDC; j++)
+            if (tid + j * NTH < 3 * kDC) fv[j] = r[kDeltaG + tid + j * NTH];
+#pragma unroll
+        for (int i = 0; i < 8; i++) vv[i] = g8 + i < n && v < V ? dop[(int64_t)(t0 + g8 + i) * d.H * V] : (T)0.f;
+    };
+    auto store = [&](int b) {
+        fk.store(Rows{sk[b]}, tid);
+        fq.store(Rows{sq[b]}, tid);
+        fm.store(Mat{sm[b]}, tid);
+        fp.store(Mat{sp[b]}, tid);
+#pragma unroll
+        for (int j = 0; j * NTH < 3 * kDC; j++)
+            if (tid + j * NTH < 3 * kDC) sv[b][tid + j * NTH] = fv[j];
+    };
+    const int last = s.len > 0 ? (s.len - 1) / kDC * kDC : -1;
+    if (last >= 0) {
+        fetch(last);
+        store(0);
+    }
+    barrier_lds();
+    for (int t0 = last, b = 0; t0 >= 0; t0 -= kDC, b ^= 1) {
+        const Rows K{sk[b]}, Q{sq[b]};
+        const Mat M{sm[b]}, PM{sp[b]};
+        const DeltaWs w = delta_ws(a, gr.ws, s.slot + t0 / kDC, h);
+        float G[8], L[8], be[8], x[8], y[8];
+        Vec8<T> raw;
+#pragma unroll
+        for (int i = 0; i < 8; i++) raw[i] = vv[i];
+        if (t0 > 0) fetch(t0 - kDC);
         if (v < a.VP)
 #pragma unroll
             for (int kt = 0; kt < NK; kt++)
-                *reinterpret_cast<f32x4*>(w.ds + (int64_t)v * KP + kt * 16 + g4) = S[kt];
-        const T* dop = static_cast<const T*>(gr.dout) + ((s.row + t0) * d.H + h) * (int64_t)V + v;
-        float x[8], y[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int t = res_row(i >> 2, lane, i & 3);
-            x[i] = t < n && v < V ? (float)dop[(int64_t)t * d.H * V] : 0.f;
-            y[i] = x[i] * ((float)d.scale * sv[t]);
-        }
-        const Frag<P> dO = split8<P>(x);
-        const Frag<3> GdO = split8<3>(y);
+                *reinterpret_cast<f32x4*>(w.ds + (int64_t)v * KP + (kt >> 1) * 32 + g8 + 4 * (kt & 1)) = S[kt];
         f32x4 du[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
-        for (int i = 0; i < KP / 32; i++) {
+        for (int p = 0; p < KP / 32; p++) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) x[r] = S[2 * i][r], x[4 + r] = S[2 * i + 1][r];
-            const Frag<3> b = split8<3>(x);
+            for (int r = 0; r < 4; r++) x[r] = S[2 * p][r], x[4 + r] = S[2 * p + 1][r];
+            const Frag<3> f = split8<3>(x);
 #pragma unroll
-            for (int m = 0; m < 2; m++) du[m] = mma<3>(K.frag(16 * m, i, lane), b, du[m]);
+            for (int m = 0; m < 2; m++) du[m] = mma<3>(K.frag(pair_row(m, l16), 32 * p, lane), f, du[m]);
         }
+#pragma unroll
+        for (int i = 0; i < 8; i += 4) {
+            const f32x4 t0v = *reinterpret_cast<const f32x4*>(&sv[b][g8 + i]),
+                        t1v = *reinterpret_cast<const f32x4*>(&sv[b][kDC + g8 + i]),
+                        t2v = *reinterpret_cast<const f32x4*>(&sv[b][2 * kDC + g8 + i]);
+#pragma unroll
+            for (int r = 0; r < 4; r++) G[i + r] = t0v[r], L[i + r] = t1v[r], be[i + r] = t2v[r];
+        }
+        const Frag<P> dO = split_raw8<T>(raw);
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = (float)raw[i] * ((float)d.scale * G[i]);
+        const Frag<3> GdO = split8<3>(y);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) du[m][r] *= sv[kDC + res_row(m, lane, r)];
-            du[m] = mma<3>(PT.frag(16 * m, 0, lane), dO, du[m]);
+            for (int r = 0; r < 4; r++) du[m][r] *= L[4 * m + r];
+            du[m] = mma<3>(PM.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dO, du[m]);
 #pragma unroll
             for (int r = 0; r < 4; r++) x[4 * m + r] = du[m][r];
         }
         const Frag<3> dU = split8<3>(x);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            const f32x4 dr = mma<3>(MT.frag(16 * m, 0, lane), dU, f32x4{0, 0, 0, 0});
+            const f32x4 dr = mma<3>(M.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dU, f32x4{0, 0, 0, 0});
+            if (v < a.VP) *reinterpret_cast<f32x4*>(w.dr + (int64_t)v * kDC + g8 + 4 * m) = dr;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = res_row(m, lane, r);
-                if (v < a.VP) w.dr[(int64_t)t * a.VP + v] = dr[r];
-                y[4 * m + r] = -dr[r] * sv[2 * kDC + t] * sv[t];
-            }
+            for (int r = 0; r < 4; r++) y[4 * m + r] = -dr[r] * be[4 * m + r] * G[4 * m + r];
         }
         const Frag<3> BdR = split8<3>(y);
-        const float decay = sv[kDC - 1];
+        const float decay = sv[b][kDC - 1];
 #pragma unroll
         for (int kt = 0; kt < NK; kt++) {
-            S[kt] = mma<3>(QT.frag(16 * kt, 0, lane), GdO, S[kt] * decay);
-            S[kt] = mma<3>(KT.frag(16 * kt, 0, lane), BdR, S[kt]);
+            const int block = (kt >> 1) * 32 + 8 * (lane & 3) + 4 * (kt & 1);
+            S[kt] = mma<3>(Q.tfrag(0, block, lane), GdO, S[kt] * decay);
+            S[kt] = mma<3>(K.tfrag(0, block, lane), BdR, S[kt]);
         }
+        if (t0 > 0) store(b ^ 1);
+        barrier_lds();
     }
     if (gr.ds0 && v < V)
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int k = kt * 16 + g4 + r;
+                const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
                 if (k < Kd) gr.ds0[sbase + (int64_t)k * V + v] = S[kt][r];
             }
 }
 
-// Sum over the 16 lanes that hold one result row, or over the four lane groups.
-__device__ __forceinline__ float sum16(float x) {
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o);
-    return x;
-}
 __device__ __forceinline__ float sum_groups(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
 
-// One chunk of one query and key head: a block of eight waves runs over the value
-// heads that share it, so dq and dk are summed in registers. Per head and 128 columns
-// of V a wave first owns 16 columns (X, U, dV), then 16 columns of K (the products
-// with S and dS); the 32x32 matrices are made by three waves, a tile of 16x16 each.
+// One chunk of one query and key head: a block of four waves runs over the value heads
+// that share it, so dq and dk are summed in registers. Per head and 64 columns of V a
+// wave first owns 16 columns (X, U, dV), then KP / 4 columns of K (the products with S
+// and dS); the 32x32 matrices are made by three waves, a 16x16 tile each. U and dR lie
+// in LDS by column of V, as the waves hold them, and are read transposed.
 template <typename T, int KP>
-__global__ __launch_bounds__(512) void k_delta_local(DeltaP a, SnHipDeltaGrad gr) {
-    constexpr int P = ElemPlanes<T>::n, VT = 128;
-    constexpr int KT1 = Tile<P, KP, kDC>::elems, V3 = Tile<3, kDC, VT>::elems, X1 = Tile<3, kDC, kDC>::elems;
-    constexpr int VPH = 2 * V3 + Tile<P, kDC, VT>::elems;       // U, dR, dO, then K^T and Q^T
-    constexpr int OV = VPH > 2 * KT1 ? VPH : 2 * KT1;
-    __shared__ alignas(16) __bf16 sk[Tile<P, kDC, KP>::elems], sq[Tile<P, kDC, KP>::elems], sov[OV], sx[3 * X1];
+__global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
+    constexpr int P = ElemPlanes<T>::n, VT = 64, NC = KP / 64;     // NC tiles of 16 columns of K a wave
+    typedef Tile<P, kDC, KP> Rows;
+    typedef Tile<3, VT, kDC> Cols;
+    typedef Tile<3, kDC, kDC> Mat;
+    __shared__ alignas(16) __bf16 sk[Rows::elems], sq[Rows::elems], su[Cols::elems], sr[Cols::elems],
+        so[Tile<P, kDC, VT>::elems], sx[2 * Mat::elems];
     __shared__ alignas(16) float sv[3 * kDC];
-    __shared__ float red[8][kDC], kread[8][kDC], kwrite[8][kDC], trow[3][16], tzk[3][16], tcol[3][16], dots[8];
+    __shared__ float red[4][kDC], kread[4][kDC], kwrite[4][kDC], trow[3][16], tzk[3][16], tcol[3][16], dots[4];
     __shared__ double sc[kDC];
     const SnHipDelta& d = a.d;
-    const int hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4, l16 = lane & 15;
+    const int hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4, g8 = 2 * g4,
+              l16 = lane & 15, blk16 = 4 * (lane & 3), blkp = 8 * (lane & 3);
     DeltaSeq s;
     int chunk;
     if (!delta_chunk_of(d, blockIdx.x, &s, &chunk)) return;
     const int64_t t0 = (int64_t)chunk * kDC;
     const int n = (int)(s.len - t0 < kDC ? s.len - t0 : kDC), V = (int)d.V, Kd = (int)d.K;
-    const Tile<P, kDC, KP> K{sk}, Q{sq}, none{nullptr};
-    const Tile<P, KP, kDC> KT{sov}, QT{sov + KT1}, nonet{nullptr};
-    const Tile<3, kDC, VT> U{sov}, DR{sov + V3};
-    const Tile<P, kDC, VT> DO{sov + 2 * V3};
-    const Tile<3, kDC, kDC> M{sx}, Y{sx}, YT{sx + X1}, FF{sx + 2 * X1};
-    const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, hk);
-    const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, hk);
-    stage_tile<T, P, KP, true, false>(kp, d.k_stride[1], n, Kd, a.vec_k, K, nonet, tid, 512);
-    stage_tile<T, P, KP, true, false>(qp, d.q_stride[1], n, Kd, a.vec_q, Q, nonet, tid, 512);
-    const int k0 = wave * 16;
-    const bool kwave = k0 < KP;
-    f32x4 dq[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, dk[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    const Rows K{sk}, Q{sq};
+    const Cols UT{su}, RT{sr};
+    const Tile<P, kDC, VT> DO{so};
+    const Mat M{sx}, Y{sx}, FF{sx + Mat::elems};        // Y takes M's place
+    RowsFetch<T, KP, 256> f;
+    f.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, hk), d.k_stride[1], n, Kd, a.vec_k, tid);
+    f.store(K, tid);
+    f.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, hk), d.q_stride[1], n, Kd, a.vec_q, tid);
+    f.store(Q, tid);
+    f32x4 dq[NC][2], dk[NC][2];
+#pragma unroll
+    for (int j = 0; j < NC; j++)
+#pragma unroll
+        for (int m = 0; m < 2; m++) dq[j][m] = dk[j][m] = f32x4{0, 0, 0, 0};
     const int ti = wave == 0 ? 0 : 1, tj = wave == 2 ? 1 : 0;     // waves 0..2: tiles (0,0), (1,0), (1,1)
 
     for (int h = hk * a.rep; h < (hk + 1) * a.rep; h++) {
-        const float* pre = d.chunks + ((int64_t)blockIdx.x * d.H + h) * kDeltaChunk;
+        const float* rec = d.chunks + ((int64_t)blockIdx.x * d.H + h) * kDeltaChunk;
         const float* st = d.states + ((int64_t)blockIdx.x * d.H + h) * (int64_t)(a.VP * KP);
         const DeltaWs w = delta_ws(a, gr.ws, blockIdx.x, h);
+        const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t0, h);
+        const int64_t at0 = ((s.row + t0) * d.H + h) * (int64_t)V;
         __syncthreads();
-        stage_mat<3, false>(pre, M, tid, 512);
-        for (int i = tid; i < 3 * kDC; i += 512) sv[i] = pre[kDeltaG + i];
-        if (wave == 7) {
+        {
+            MatFetch<3, 256> fm;
+            fm.load(rec, tid);
+            fm.store(M, tid);
+        }
+        if (tid < 3 * kDC) sv[tid] = rec[kDeltaG + tid];
+        if (wave == 3) {
             const int64_t at = (s.row + t0 + lane) * d.H + h;
             double c = lane < n ? (double)delta_decay(d.g[at]) : 0.0;
 #pragma unroll
@@ -195,123 +229,121 @@ __global__ __launch_bounds__(512) void k_delta_local(DeltaP a, SnHipDeltaGrad gr
             if (lane < kDC) sc[lane] = c;
         }
         __syncthreads();
-        f32x4 dp = {0, 0, 0, 0}, z = {0, 0, 0, 0};
-        f32x4 q1[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, k1[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}},
-              k2[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        float G[8], be[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) G[i] = sv[g8 + i], be[i] = sv[2 * kDC + g8 + i];
+        f32x4 dp = {0, 0, 0, 0}, z = {0, 0, 0, 0}, q1[NC][2], k1[NC][2], k2[NC][2];
+#pragma unroll
+        for (int j = 0; j < NC; j++)
+#pragma unroll
+            for (int m = 0; m < 2; m++) q1[j][m] = k1[j][m] = k2[j][m] = f32x4{0, 0, 0, 0};
         float bsum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, ss = 0.f;
         for (int vt = 0; vt < a.VP; vt += VT) {
             const int vl = wave * 16 + l16, v = vt + vl;
-            float u[8], dr[8], o[8];
+            {
+                const int t = tid >> 3, c = (tid & 7) * 8;
+                const T* op = static_cast<const T*>(gr.dout) + at0 + (int64_t)t * d.H * V + vt + c;
+                DO.put8(t, c, split_raw8<T>(load_raw8(op, t < n ? V - vt - c : 0, vec_o)));
+            }
+            float x[8], dr[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) u[i] = dr[i] = o[i] = 0.f;
+            for (int i = 0; i < 8; i++) x[i] = dr[i] = 0.f;
             if (vt + wave * 16 < a.VP) {
                 f32x4 ks[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+                float vv[8];
 #pragma unroll
-                for (int i = 0; i < KP / 32; i++) {
-                    const float* p = st + (int64_t)v * KP + 32 * i + g4;
-                    const f32x4 lo = *reinterpret_cast<const f32x4*>(p), hi = *reinterpret_cast<const f32x4*>(p + 16);
-                    const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                    const Frag<3> b = split8<3>(x);
+                for (int i = 0; i < 8; i++) vv[i] = g8 + i < n && v < V ? (float)vp[(g8 + i) * d.v_stride[1] + v] : 0.f;
+                const Vec8<float> rv = load_raw8(w.dr + (int64_t)v * kDC + g8, 8, true);
 #pragma unroll
-                    for (int m = 0; m < 2; m++) ks[m] = mma<3>(K.frag(16 * m, i, lane), b, ks[m]);
+                for (int p = 0; p < KP / 32; p++) {
+                    const Frag<3> b = split_raw8<float>(load_raw8(st + (int64_t)v * KP + 32 * p + g8, 8, true));
+#pragma unroll
+                    for (int m = 0; m < 2; m++) ks[m] = mma<3>(K.frag(pair_row(m, l16), 32 * p, lane), b, ks[m]);
                 }
-                const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t0, h) + v;
-                const int64_t at = ((s.row + t0) * d.H + h) * (int64_t)V + v;
-                float x[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const int t = res_row(i >> 2, lane, i & 3);
-                    const bool live = t < n && v < V;
-                    const float xx = (live ? (float)vp[t * d.v_stride[1]] : 0.f) - sv[t] * ks[i >> 2][i & 3];
-                    dr[i] = w.dr[(int64_t)t * a.VP + v];
-                    o[i] = live ? (float)static_cast<const T*>(gr.dout)[at + (int64_t)t * d.H * V] : 0.f;
-                    if (live) static_cast<T*>(gr.dv)[at + (int64_t)t * d.H * V] = (T)(sv[2 * kDC + t] * dr[i]);
+                    const float xx = vv[i] - G[i] * ks[i >> 2][i & 3];
+                    dr[i] = rv[i];
+                    if (g8 + i < n && v < V)
+                        static_cast<T*>(gr.dv)[at0 + (int64_t)(g8 + i) * d.H * V + v] = (T)(be[i] * dr[i]);
                     bsum[i] = fmaf(dr[i], xx, bsum[i]);
-                    x[i] = sv[2 * kDC + t] * xx;
+                    x[i] = be[i] * xx;
                 }
                 const Frag<3> R = split8<3>(x);
 #pragma unroll
                 for (int m = 0; m < 2; m++) {
-                    const f32x4 um = mma<3>(M.frag(16 * m, 0, lane), R, f32x4{0, 0, 0, 0});
+                    const f32x4 u = mma<3>(M.frag(pair_row(m, l16), 0, lane), R, f32x4{0, 0, 0, 0});
 #pragma unroll
-                    for (int r = 0; r < 4; r++) u[4 * m + r] = um[r];
+                    for (int r = 0; r < 4; r++) x[4 * m + r] = u[r];
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int t = res_row(i >> 2, lane, i & 3);
-                U.put(t, vl, u[i]);
-                DR.put(t, vl, dr[i]);
-                DO.put(t, vl, o[i]);
-            }
+            UT.put8(vl, g8, x);
+            RT.put8(vl, g8, dr);
             __syncthreads();
-            const int nv = (a.VP - vt < VT ? a.VP - vt + 31 : VT) / 32;
+            const int nv = a.VP - vt < VT ? (a.VP - vt + 31) & ~31 : VT;       // whole 32s
             if (wave < 3)
-                for (int i = 0; i < nv; i++) {
-                    const Frag<3> b = U.frag(16 * tj, i, lane);
-                    dp = mma<3>(DO.frag(16 * ti, i, lane), b, dp);
-                    z = mma<3>(DR.frag(16 * ti, i, lane), b, z);
+                for (int i = 0; i < nv; i += 32) {
+                    const Frag<3> b = UT.tfrag(i, 16 * tj + blk16, lane);
+                    dp = mma<3>(DO.frag(16 * ti + l16, i, lane), b, dp);
+                    z = mma<3>(RT.tfrag(i, 16 * ti + blk16, lane), b, z);
                 }
-            if (kwave)
-                for (int i = 0; i < nv; i++) {
-                    float x[8], y[8];
+            for (int i = 0; i < nv; i += 32) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int vv = vt + 32 * i + g4 + (j & 3) + (j >> 2) * 16;
-                        x[j] = vv < a.VP ? st[(int64_t)vv * KP + k0 + l16] : 0.f;
-                        y[j] = vv < a.VP ? w.ds[(int64_t)vv * KP + k0 + l16] : 0.f;
-                        ss = fmaf(x[j], y[j], ss);
+                for (int j = 0; j < NC; j++) {
+                    const int kc = (wave * NC + j) * 16 + l16;
+                    float sx8[8], dx8[8];
+#pragma unroll
+                    for (int l = 0; l < 8; l++) {
+                        const int vv = vt + i + g8 + l;
+                        sx8[l] = vv < a.VP ? st[(int64_t)vv * KP + kc] : 0.f;
+                        dx8[l] = vv < a.VP ? w.ds[(int64_t)vv * KP + kc] : 0.f;
+                        ss = fmaf(sx8[l], dx8[l], ss);
                     }
-                    const Frag<3> b = split8<3>(x), e = split8<3>(y);
+                    const Frag<3> b = split8<3>(sx8), e = split8<3>(dx8);
 #pragma unroll
                     for (int m = 0; m < 2; m++) {
-                        q1[m] = mma<3>(DO.frag(16 * m, i, lane), b, q1[m]);
-                        k1[m] = mma<3>(DR.frag(16 * m, i, lane), b, k1[m]);
-                        k2[m] = mma<3>(U.frag(16 * m, i, lane), e, k2[m]);
+                        q1[j][m] = mma<3>(DO.frag(pair_row(m, l16), i, lane), b, q1[j][m]);
+                        k1[j][m] = mma<3>(RT.tfrag(i, blkp + 4 * m, lane), b, k1[j][m]);
+                        k2[j][m] = mma<3>(UT.tfrag(i, blkp + 4 * m, lane), e, k2[j][m]);
                     }
                 }
+            }
             __syncthreads();
         }
-        // the V tiles are done with: K and Q by column take their place
-        stage_tile<T, P, KP, false, true>(kp, d.k_stride[1], n, Kd, a.vec_k, none, KT, tid, 512);
-        stage_tile<T, P, KP, false, true>(qp, d.q_stride[1], n, Kd, a.vec_q, none, QT, tid, 512);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const float b = sum16(bsum[i]);
-            if (l16 == 0) red[wave][res_row(i >> 2, lane, i & 3)] = b;
+            if (l16 == 0) red[wave][g8 + i] = b;
         }
-        ss = sum16(sum_groups(ss));
+        ss = sum_groups(sum16(ss));
         if (lane == 0) dots[wave] = ss;
         if (wave < 3) {
             f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < KP / 32; i++) {
-                const Frag<P> b = K.frag(16 * tj, i, lane);
-                kk = mma<3>(K.frag(16 * ti, i, lane), b, kk);
-                qk = mma<3>(Q.frag(16 * ti, i, lane), b, qk);
+            for (int c = 0; c < KP; c += 32) {
+                const Frag<P> b = K.frag(16 * tj + l16, c, lane);
+                kk = mma<3>(K.frag(16 * ti + l16, c, lane), b, kk);
+                qk = mma<3>(Q.frag(16 * ti + l16, c, lane), b, qk);
             }
             const int col = tj * 16 + l16;
             float esum = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int row = res_row(ti, lane, r);
+                const int row = 16 * ti + g4 + r;
                 const float D = col <= row ? expf((float)(sc[row] - sc[col])) : 0.f;
-                const float zd = col < row ? D * z[r] : 0.f, f = -sv[2 * kDC + row] * zd;
-                const float y = (float)d.scale * D * dp[r], e = col < row ? y * qk[r] + f * kk[r] : 0.f;
+                const float zd = col < row ? D * z[r] : 0.f, ff = -sv[2 * kDC + row] * zd;
+                const float y = (float)d.scale * D * dp[r], e = col < row ? y * qk[r] + ff * kk[r] : 0.f;
                 const float er = sum16(e), zr = sum16(zd * kk[r]);
                 if (l16 == 0) {
                     trow[wave][g4 + r] = er;
                     tzk[wave][g4 + r] = zr;
                 }
                 esum += e;
-                z[r] = f;
+                z[r] = ff;
                 Y.put(row, col, y);
-                YT.put(col, row, y);
                 if (ti != tj) {
-                    Y.put(col, row, 0.f);
-                    YT.put(row, col, 0.f);
-                    FF.put(row, col, f);
-                    FF.put(col, row, f);
+                    FF.put(row, col, ff);
+                    FF.put(col, row, ff);
                 }
             }
             esum = sum_groups(esum);
@@ -326,34 +358,44 @@ __global__ __launch_bounds__(512) void k_delta_local(DeltaP a, SnHipDeltaGrad gr
                         const float x = __shfl(z[rr], (l16 >> 2) * 16 + g4 + r);
                         if ((l16 & 3) == rr) t = x;
                     }
-                    FF.put(res_row(ti, lane, r), col, z[r] + t);
+                    FF.put(16 * ti + g4 + r, col, z[r] + t);
                 }
             }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) Y.put(g4 + r, 16 + l16, 0.f);
         }
         __syncthreads();
-        if (kwave) {
-            const int kc = k0 + l16;
-            const Frag<P> bk = KT.frag(k0, 0, lane), bq = QT.frag(k0, 0, lane);
+        float cr[8], cw[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) cr[i] = cw[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NC; j++) {
+            const int kc = (wave * NC + j) * 16;
+            const Frag<P> bk = K.tfrag(0, kc + blk16, lane), bq = Q.tfrag(0, kc + blk16, lane);
 #pragma unroll
             for (int m = 0; m < 2; m++) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int t = res_row(m, lane, r);
-                    const float G = sv[t], qv = Q.get(t, kc), kv = K.get(t, kc);
-                    q1[m][r] *= (float)d.scale * G;
-                    k1[m][r] *= -sv[2 * kDC + t] * G;
-                    k2[m][r] *= sv[kDC + t];
-                    const float cr = sum16(qv * q1[m][r] + kv * k1[m][r]), cw = sum16(kv * k2[m][r]);
-                    if (l16 == 0) {
-                        kread[wave][t] = cr;
-                        kwrite[wave][t] = cw;
-                    }
+                    const int i = 4 * m + r, t = g8 + i;
+                    const float qv = Q.get(t, kc + l16), kv = K.get(t, kc + l16);
+                    q1[j][m][r] *= (float)d.scale * G[i];
+                    k1[j][m][r] *= -be[i] * G[i];
+                    k2[j][m][r] *= sv[kDC + t];
+                    cr[i] = fmaf(qv, q1[j][m][r], fmaf(kv, k1[j][m][r], cr[i]));
+                    cw[i] = fmaf(kv, k2[j][m][r], cw[i]);
                 }
-                q1[m] = mma<3>(Y.frag(16 * m, 0, lane), bk, q1[m]);
-                k1[m] = mma<3>(YT.frag(16 * m, 0, lane), bq, k1[m] + k2[m]);
-                k1[m] = mma<3>(FF.frag(16 * m, 0, lane), bk, k1[m]);
-                dq[m] += q1[m];
-                dk[m] += k1[m];
+                dq[j][m] += mma<3>(Y.frag(pair_row(m, l16), 0, lane), bk, q1[j][m]);
+                f32x4 t = mma<3>(Y.tfrag(0, blkp + 4 * m, lane), bq, k1[j][m] + k2[j][m]);
+                dk[j][m] += mma<3>(FF.frag(pair_row(m, l16), 0, lane), bk, t);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float r = sum16(cr[i]), wr = sum16(cw[i]);
+            if (l16 == 0) {
+                kread[wave][g8 + i] = r;
+                kwrite[wave][g8 + i] = wr;
             }
         }
         __syncthreads();
@@ -364,12 +406,12 @@ __global__ __launch_bounds__(512) void k_delta_local(DeltaP a, SnHipDeltaGrad gr
             float dc = hi ? trow[1][lo] + trow[2][lo] - tcol[2][lo] : trow[0][lo] - tcol[0][lo] - tcol[1][lo];
             float db = hi ? -tzk[1][lo] - tzk[2][lo] : -tzk[0][lo];
             float wr = 0.f, all = 0.f;
-            for (int i = 0; i < KP / 16; i++) {
+            for (int i = 0; i < 4; i++) {
                 dc += kread[i][t];
                 wr += kwrite[i][t];
                 all += dots[i];
+                db += red[i][t];
             }
-            for (int i = 0; i < 8; i++) db += red[i][t];
 #pragma unroll
             for (int o = 1; o < kDC; o <<= 1) {
                 const float x = __shfl_down(dc, o, kDC), y = __shfl_up(wr, o, kDC);
@@ -384,16 +426,19 @@ __global__ __launch_bounds__(512) void k_delta_local(DeltaP a, SnHipDeltaGrad gr
             }
         }
     }
-    if (kwave && k0 + l16 < Kd)
+#pragma unroll
+    for (int j = 0; j < NC; j++) {
+        const int kc = (wave * NC + j) * 16 + l16;
+        if (kc >= Kd) continue;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int t = res_row(i >> 2, lane, i & 3);
-            const int64_t at = ((s.row + t0 + t) * d.Hk + hk) * (int64_t)Kd + k0 + l16;
-            if (t < n) {
-                static_cast<T*>(gr.dq)[at] = (T)dq[i >> 2][i & 3];
-                static_cast<T*>(gr.dk)[at] = (T)dk[i >> 2][i & 3];
+            const int64_t at = ((s.row + t0 + g8 + i) * d.Hk + hk) * (int64_t)Kd + kc;
+            if (g8 + i < n) {
+                static_cast<T*>(gr.dq)[at] = (T)dq[j][i >> 2][i & 3];
+                static_cast<T*>(gr.dk)[at] = (T)dk[j][i >> 2][i & 3];
             }
         }
+    }
 }
 
 template <typename T, int KP>
@@ -404,7 +449,8 @@ snhip_status bwd_t(const DeltaP& a, const SnHipDeltaGrad& gr, hipStream_t st) {
     else if (W == 2) k_delta_rscan<T, KP, 2><<<grid, 128, 0, st>>>(a, gr);
     else k_delta_rscan<T, KP, 1><<<grid, 64, 0, st>>>(a, gr);
     SNHIP_CHECK(hipGetLastError());
-    k_delta_local<T, KP><<<dim3((unsigned)a.slots, (unsigned)a.d.Hk), 512, 0, st>>>(a, gr);
+    const bool vec_o = a.d.V % 8 == 0 && reinterpret_cast<uintptr_t>(gr.dout) % 16 == 0;
+    k_delta_local<T, KP><<<dim3((unsigned)a.slots, (unsigned)a.d.Hk), 256, 0, st>>>(a, gr, vec_o);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }

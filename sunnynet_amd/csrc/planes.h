@@ -5,11 +5,18 @@
 // 8 LIM bits: LIM = 3 is fp32 to its last bit or two. Range is bf16's, which is
 // fp32's, so nothing is scaled. A non-finite value leaves NaN planes.
 //
-// A 16x16x32 product reads eight contraction elements per lane. A lane's group
-// g = lane / 16 holds, in this file's order, elements 4g..4g+3 and 16+4g..16+4g+3 of
-// the 32: the rows that the lane holds of two 16x16 results stacked along that axis.
-// So a result is the next product's right operand without leaving its registers, and
-// tiles in LDS store their columns in the same order (perm_col).
+// A 16x16x32 product reads eight contraction elements per lane: lane group g = lane / 16
+// holds elements 8g..8g+7 of the 32, of row (left) or column (right) lane % 16. Of the
+// 16x16 result the lane holds rows 4g..4g+3 of column lane % 16. Two results make 32
+// rows, and which row of the matrix a row of a left operand stands for is free: with row
+// i of result m standing for row pair_row(m, i) = 8 (i / 4) + 4 m + i % 4, the lane holds
+// rows 8g..8g+7 of its column, in order. So a pair of results is the next product's
+// right operand without leaving its registers.
+//
+// Tiles in LDS are row by row, eight neighbouring values (16 bytes a plane) to a write.
+// An operand whose contraction runs along a row is read as it stands (frag); one whose
+// contraction runs down the columns through the transposing LDS read (tfrag), which
+// hands four rows of a 4x16 block to the lane of each column.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -60,55 +67,105 @@ __device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4
     return acc;
 }
 
-// Where column c of a row is stored (a multiple of 4 columns moves as one).
-__host__ __device__ constexpr int perm_col(int c) {
-    return (c & ~31) + ((c & 12) << 1) + ((c & 16) >> 2) + (c & 3);
-}
+__device__ __forceinline__ int pair_row(int m, int i) { return 8 * (i >> 2) + 4 * m + (i & 3); }
 
-// A tile of P planes of R rows and C columns in LDS. Rows are padded by 8 elements
-// (16 bytes), which spreads a product's 16 rows over the banks.
+// A tile of P planes of R rows and C columns in LDS. Rows are padded by 16 bytes, which
+// spreads a product's 16 rows over the banks.
 template <int P, int R, int C> struct Tile {
     static constexpr int ld = C + 8;
     static constexpr int elems = P * R * ld;
     __bf16* s;
     __device__ __forceinline__ __bf16* at(int p, int r, int c) const { return s + (p * R + r) * ld + c; }
-    // The operand of rows r0..r0+15, contraction columns 32 ks..32 ks + 31.
-    template <int Q = P> __device__ __forceinline__ Frag<Q> frag(int r0, int ks, int lane) const {
+    // Row `row` (one per lane % 16), contraction columns c0..c0 + 31.
+    template <int Q = P> __device__ __forceinline__ Frag<Q> frag(int row, int c0, int lane) const {
         Frag<Q> f;
 #pragma unroll
-        for (int p = 0; p < Q; p++)
-            f.p[p] = *reinterpret_cast<const bf16x8*>(at(p, r0 + (lane & 15), 32 * ks + 8 * (lane >> 4)));
+        for (int p = 0; p < Q; p++) f.p[p] = *reinterpret_cast<const bf16x8*>(at(p, row, c0 + 8 * (lane >> 4)));
         return f;
     }
-    // Four neighbouring columns (c a multiple of 4) of one row.
-    __device__ __forceinline__ void put4(int r, int c, const float* x) const {
-        float t[4] = {x[0], x[1], x[2], x[3]};
+    // Contraction rows r0..r0 + 31; the lane's column is that of lane % 16 in the four
+    // blocks of four columns, of which the one at `block` is this lane's to fetch
+    // (block index lane % 4): columns 16 t + i: block = 16 t + 4 (lane % 4); columns
+    // pair_row(m, i): block = 8 (lane % 4) + 4 m. The whole wave takes part.
+    template <int Q = P> __device__ __forceinline__ Frag<Q> tfrag(int r0, int block, int lane) const {
+        Frag<Q> f;
+        const int r = r0 + 8 * (lane >> 4) + ((lane >> 2) & 3);
 #pragma unroll
-        for (int p = 0; p < P; p++) {
-            bf16x4 h;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                h[i] = (__bf16)t[i];
-                t[i] = t[i] - (float)h[i];
-            }
-            *reinterpret_cast<bf16x4*>(at(p, r, perm_col(c))) = h;
+        for (int p = 0; p < Q; p++) {
+            const bf16x4 lo = tread(at(p, r, block)), hi = tread(at(p, r + 4, block));
+            f.p[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
+        return f;
+    }
+    static __device__ __forceinline__ bf16x4 tread(__bf16* a) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds4;
+        return __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)a));
+    }
+    // Eight neighbouring columns (c a multiple of 8) of one row.
+    __device__ __forceinline__ void put8(int r, int c, const float* x) const { put8(r, c, split8<P>(x)); }
+    __device__ __forceinline__ void put8(int r, int c, const Frag<P>& f) const {
+#pragma unroll
+        for (int p = 0; p < P; p++) *reinterpret_cast<bf16x8*>(at(p, r, c)) = f.p[p];
     }
     __device__ __forceinline__ void put(int r, int c, float x) const {
 #pragma unroll
         for (int p = 0; p < P; p++) {
             const __bf16 h = (__bf16)x;
-            *at(p, r, perm_col(c)) = h;
+            *at(p, r, c) = h;
             x = x - (float)h;
         }
     }
     __device__ __forceinline__ float get(int r, int c) const {
         float x = 0.f;
 #pragma unroll
-        for (int p = P - 1; p >= 0; p--) x += (float)*at(p, r, perm_col(c));
+        for (int p = P - 1; p >= 0; p--) x += (float)*at(p, r, c);
         return x;
     }
 };
+
+template <typename T> using Vec8 = T __attribute__((ext_vector_type(8)));
+
+// Eight consecutive elements from `src`, of which the first `n` exist (the rest are 0).
+// vec: the address is 16-byte aligned.
+template <typename T> __device__ __forceinline__ Vec8<T> load_raw8(const T* src, int n, bool vec) {
+    Vec8<T> x;
+    if (vec && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
+            x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            x = *reinterpret_cast<const Vec8<T>*>(src);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = i < n ? src[i] : (T)0.f;
+    }
+    return x;
+}
+
+// The planes of eight elements, without arithmetic where one plane is the value.
+template <typename T> __device__ __forceinline__ Frag<ElemPlanes<T>::n> split_raw8(const Vec8<T>& v) {
+    if constexpr (ElemPlanes<T>::n == 1) {
+        return Frag<1>{{v}};
+    } else {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = (float)v[i];
+        return split8<ElemPlanes<T>::n>(x);
+    }
+}
+
+// Sum over the 16 lanes of a row, by row-local lane exchanges in the adder's operand.
+template <int CTRL> __device__ __forceinline__ float add_dpp(float x) {
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum16(float x) {
+    x = add_dpp<0xb1>(x);         // lanes 1, 0, 3, 2
+    x = add_dpp<0x4e>(x);         // 2, 3, 0, 1
+    x = add_dpp<0x141>(x);        // mirrored within 8
+    return add_dpp<0x140>(x);     // and within 16
+}
 
 // Eight consecutive elements from `src`, of which the first `n` exist (the rest
 // are 0). vec: the address is 16-byte aligned.
