@@ -17,6 +17,8 @@
 // tiles that all columns share. Rows of K and tokens are both taken in pair_row's order.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 #include "planes.h"
 #include "snhip_ops.h"
@@ -28,12 +30,17 @@ constexpr int kDC = 32;                            // tokens per chunk
 // and beta (32 each).
 constexpr int kDeltaP = 1536, kDeltaG = 3072, kDeltaChunk = 3168;
 
+// Waves of a block of the scans, 16 columns of V each.
+constexpr int kDeltaW = 4;
+// Token strides stay below this, so that offsets inside a chunk fit 32 bits.
+constexpr int64_t kDeltaStride = 1 << 24;
+
 struct DeltaP {
     SnHipDelta d;
     int64_t slots;          // chunk slots of all sequences
     int KP, VP;             // K and V padded: state slabs are (VP, KP), k contiguous
     int rep;                // value heads per query and key head
-    bool vec_q, vec_k;          // 16-byte loads reach
+    bool vec;               // every eight elements of a row of q or k are 16-byte aligned
 };
 
 __host__ __device__ inline int64_t delta_slots(const SnHipDelta& d) {
@@ -97,16 +104,22 @@ __device__ __forceinline__ const T* delta_at(const void* p, const int64_t* st, i
 
 // A (32, KP) tile of a (tokens, K) array on its way from memory to LDS, held by NTH
 // threads: rows from n on and columns from K on are 0.
-template <typename T, int KP, int NTH> struct RowsFetch {
+template <typename T, int KP, int NTH, bool VEC> struct RowsFetch {
     static constexpr int P = ElemPlanes<T>::n, N = (kDC * KP / 8 + NTH - 1) / NTH;
     static constexpr bool whole = kDC * KP / 8 % NTH == 0;
     Vec8<T> x[N];
-    __device__ __forceinline__ void load(const T* src, int64_t stride, int n, int K, bool vec, int tid) {
+    int off[N];            // of this thread's vectors in any chunk
+    __device__ __forceinline__ void init(int64_t stride, int K, int tid) {
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const int i = tid + j * NTH, t = i / (KP / 8), c = i % (KP / 8) * 8;
-            if (whole || t < kDC) x[j] = load_raw8(src + t * stride + c, t < n ? K - c : 0, vec);
+            off[j] = c < K ? (t * (int)stride + c) * (int)sizeof(T) : kNowhere;
         }
+    }
+    __device__ __forceinline__ void load(const T* src, int64_t stride, int n, int K, int tid) {
+        const __amdgpu_buffer_rsrc_t r = rows_window(src, stride, n, K);
+#pragma unroll
+        for (int j = 0; j < N; j++) x[j] = buf_load8<T>(r, off[j], K - (tid + j * NTH) % (KP / 8) * 8, VEC);
     }
     __device__ __forceinline__ void store(Tile<P, kDC, KP> to, int tid) const {
 #pragma unroll
@@ -117,17 +130,15 @@ template <typename T, int KP, int NTH> struct RowsFetch {
     }
 };
 
-// The first Q planes of a (32, 32) matrix of a chunk's record, likewise.
+// The first Q planes of a (32, 32) matrix of a chunk's record (at float `at`), likewise.
 template <int Q, int NTH> struct MatFetch {
     static constexpr int N = (Q * 128 + NTH - 1) / NTH;
     static constexpr bool whole = Q * 128 % NTH == 0;
     bf16x8 x[N];
-    __device__ __forceinline__ void load(const float* rec, int tid) {
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rec, int at, int tid) {
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const int i = tid + j * NTH;
-            if (whole || i < Q * 128) x[j] = *reinterpret_cast<const bf16x8*>(rec + i * 4);
-        }
+        for (int j = 0; j < N; j++)
+            x[j] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rec, (tid + j * NTH) * 16, at * 4, 0));
     }
     __device__ __forceinline__ void store(Tile<Q, kDC, kDC> to, int tid) const {
 #pragma unroll
@@ -137,6 +148,17 @@ template <int Q, int NTH> struct MatFetch {
         }
     }
 };
+
+// f(element type, padded K, vector loads) of a call, as values of types that name them.
+template <typename F> snhip_status delta_pick(const DeltaP& a, F f) {
+    auto by_vec = [&](auto t, auto kp) {
+        return a.vec ? f(t, kp, std::true_type()) : f(t, kp, std::false_type());
+    };
+    auto by_k = [&](auto t) {
+        return a.KP == 64 ? by_vec(t, std::integral_constant<int, 64>()) : by_vec(t, std::integral_constant<int, 128>());
+    };
+    return a.d.dtype == SNHIP_F32 ? by_k(float()) : a.d.dtype == SNHIP_BF16 ? by_k(__bf16()) : by_k(_Float16());
+}
 
 // g as the kernels use it: exp(-200) is 0 in fp32, and a sum of 32 such stays finite.
 __device__ __forceinline__ float delta_decay(float g) { return g < -200.f ? -200.f : g; }

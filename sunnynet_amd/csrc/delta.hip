@@ -9,7 +9,7 @@ namespace {
 // of the 32x32 matrices each. The inverse of the unit lower triangular I + A goes by
 // halves: its two diagonal 16x16 blocks by forward substitution, a column per lane,
 // then M10 = -M11 A10 M00.
-template <typename T, int KP>
+template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
     constexpr int P = ElemPlanes<T>::n;
     __shared__ alignas(16) __bf16 sk[Tile<P, kDC, KP>::elems], sq[Tile<P, kDC, KP>::elems];
@@ -23,9 +23,11 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
     const int64_t t0 = (int64_t)chunk * kDC;
     const int n = (int)(s.len - t0 < kDC ? s.len - t0 : kDC);
     const Tile<P, kDC, KP> K{sk}, Q{sq};
-    RowsFetch<T, KP, 256> fk, fq;
-    fk.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n, (int)d.K, a.vec_k, tid);
-    fq.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1], n, (int)d.K, a.vec_q, tid);
+    RowsFetch<T, KP, 256, VEC> fk, fq;
+    fk.init(d.k_stride[1], (int)d.K, tid);
+    fq.init(d.q_stride[1], (int)d.K, tid);
+    fk.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, h / a.rep), d.k_stride[1], n, (int)d.K, tid);
+    fq.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, h / a.rep), d.q_stride[1], n, (int)d.K, tid);
     if (wave == 0) {
         const int64_t at = (s.row + t0 + lane) * d.H + h;
         double c = lane < n ? (double)delta_decay(d.g[at]) : 0.0;
@@ -109,13 +111,13 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
     }
 }
 
-// The scan over chunks: W waves, 16 columns of V each. Half types read the state by
+// The scan over chunks: kDeltaW waves, 16 columns of V each. Half types read the state by
 // two planes where only out (of that type) depends on it. The next chunk's tiles are
 // fetched into registers while this one is worked on, and put into the other half of LDS:
 // one barrier per chunk, no wait for memory in between.
-template <typename T, int KP, int W>
-__global__ __launch_bounds__(64 * W) void k_delta_scan(DeltaP a, T* out, float* send) {
-    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, NTH = 64 * W;
+template <typename T, int KP, bool VEC>
+__global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, float* send) {
+    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W;
     constexpr int LO = sizeof(T) == 4 ? 3 : 2;      // planes of the products that only reach out
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, kDC, kDC> MatM;
@@ -129,7 +131,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_scan(DeltaP a, T* out, float* 
     const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
     const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0, h / a.rep);
     const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0, h / a.rep);
-    const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0, h) + v;
+    const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0, h);
     const float* rec = d.chunks + (s.slot * d.H + h) * kDeltaChunk;
 
     f32x4 S[NK];           // S[2 p + e][r] is row 32 p + g8 + 4 e + r of column v
@@ -140,23 +142,27 @@ __global__ __launch_bounds__(64 * W) void k_delta_scan(DeltaP a, T* out, float* 
             const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
             S[kt][r] = d.s0 && k < Kd && v < V ? d.s0[sbase + (int64_t)k * V + v] : 0.f;
         }
-    RowsFetch<T, KP, NTH> fk, fq;
+    RowsFetch<T, KP, NTH, VEC> fk, fq;
     MatFetch<3, NTH> fm;
     MatFetch<LO, NTH> fp;
     float fv[(3 * kDC + NTH - 1) / NTH];
-    T vv[8];
+    unsigned vv[8];
+    fk.init(d.k_stride[1], Kd, tid);
+    fq.init(d.q_stride[1], Kd, tid);
+    const int E = (int)sizeof(T), v_step = (int)d.v_stride[1] * E, v_off = v < V ? g8 * v_step + v * E : kNowhere;
+    const int o_step = (int)d.H * V * E, o_off = v < V ? g8 * o_step + v * E : kNowhere;
     auto fetch = [&](int t0) {
         const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
-        const float* r = rec + (int64_t)(t0 / kDC) * d.H * kDeltaChunk;
-        fk.load(kp + t0 * d.k_stride[1], d.k_stride[1], n, Kd, a.vec_k, tid);
-        fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, a.vec_q, tid);
-        fm.load(r, tid);
-        fp.load(r + kDeltaP, tid);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(rec + (int64_t)(t0 / kDC) * d.H * kDeltaChunk, kDeltaChunk * 4);
+        fk.load(kp + t0 * d.k_stride[1], d.k_stride[1], n, Kd, tid);
+        fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, tid);
+        fm.load(r, 0, tid);
+        fp.load(r, kDeltaP, tid);
 #pragma unroll
-        for (int j = 0; j * NTH < 3 * kDC; j++)
-            if (tid + j * NTH < 3 * kDC) fv[j] = r[kDeltaG + tid + j * NTH];
+        for (int j = 0; j * NTH < 3 * kDC; j++) fv[j] = buf_load<float>(r, (kDeltaG + tid + j * NTH) * 4);
+        const __amdgpu_buffer_rsrc_t rv = rows_window(vp + t0 * d.v_stride[1], d.v_stride[1], n, V);
 #pragma unroll
-        for (int i = 0; i < 8; i++) vv[i] = g8 + i < n && v < V ? vp[(t0 + g8 + i) * d.v_stride[1]] : (T)0.f;
+        for (int i = 0; i < 8; i++) vv[i] = buf_load_bits<T>(rv, v_off + i * v_step);
     };
     auto store = [&](int b) {
         fk.store(Rows{sk[b]}, tid);
@@ -177,15 +183,15 @@ __global__ __launch_bounds__(64 * W) void k_delta_scan(DeltaP a, T* out, float* 
         const Rows K{sk[b]}, Q{sq[b]};
         float vc[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) vc[i] = (float)vv[i];
+        for (int i = 0; i < 8; i++) vc[i] = float_of_bits<T>(vv[i]);
         const bool more = t0 + kDC < s.len;
         if (more) fetch(t0 + kDC);
         if (d.states) {       // S^T (VP, KP) before the chunk, for the backward
-            float* st = d.states + ((s.slot + t0 / kDC) * d.H + h) * (int64_t)(a.VP * KP);
-            if (v < a.VP)
+            const __amdgpu_buffer_rsrc_t st = make_rsrc(
+                d.states + ((s.slot + t0 / kDC) * d.H + h) * (int64_t)(a.VP * KP), (uint32_t)(a.VP * KP * 4));
 #pragma unroll
-                for (int kt = 0; kt < NK; kt++)
-                    *reinterpret_cast<f32x4*>(st + (int64_t)v * KP + (kt >> 1) * 32 + g8 + 4 * (kt & 1)) = S[kt];
+            for (int kt = 0; kt < NK; kt++)
+                buf_store4(st, (v * KP + g8) * 4 + ((kt >> 1) * 32 + 4 * (kt & 1)) * 4, S[kt]);
         }
         f32x4 ks[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
@@ -230,15 +236,13 @@ __global__ __launch_bounds__(64 * W) void k_delta_scan(DeltaP a, T* out, float* 
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
             S[kt] = mma<3>(K.tfrag(0, (kt >> 1) * 32 + 8 * (lane & 3) + 4 * (kt & 1), lane), LU, S[kt] * decay);
-        T* op = out + ((s.row + t0) * d.H + h) * (int64_t)V + v;
+        const __amdgpu_buffer_rsrc_t ro =
+            rows_window(out + ((s.row + t0) * d.H + h) * (int64_t)V, d.H * (int64_t)V, n, V);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             o[m] = mma<LO>(MatP{sp[b]}.frag(pair_row(m, l16), 0, lane), U, o[m]);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = g8 + 4 * m + r;
-                if (t < n && v < V) op[(int64_t)t * d.H * V] = (T)o[m][r];
-            }
+            for (int r = 0; r < 4; r++) buf_store<T>(ro, o_off + (4 * m + r) * o_step, (T)o[m][r]);
         }
         if (more) store(b ^ 1);
         barrier_lds();
@@ -289,8 +293,8 @@ __global__ __launch_bounds__(64) void k_delta_step(DeltaP a, T* out, const float
         float q[RPT], k[RPT];
 #pragma unroll
         for (int i = 0; i < RPT; i += 8) {
-            load8(qp + k0 + i, Kd - k0 - i, a.vec_q, q + i);
-            load8(kp + k0 + i, Kd - k0 - i, a.vec_k, k + i);
+            load8(qp + k0 + i, Kd - k0 - i, a.vec, q + i);
+            load8(kp + k0 + i, Kd - k0 - i, a.vec, k + i);
         }
         f32x4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
         float qk = 0.f;
@@ -350,16 +354,12 @@ snhip_status step_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
     return SNHIP_OK;
 }
 
-template <typename T, int KP>
+template <typename T, int KP, bool VEC>
 snhip_status fwd_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
-    k_delta_prep<T, KP><<<dim3((unsigned)a.slots, (unsigned)a.d.H), 256, 0, st>>>(a);
+    k_delta_prep<T, KP, VEC><<<dim3((unsigned)a.slots, (unsigned)a.d.H), 256, 0, st>>>(a);
     SNHIP_CHECK(hipGetLastError());
-    const int strips = a.VP / 16;
-    const int W = strips >= 4 ? 4 : strips >= 2 ? 2 : 1;
-    const dim3 grid((unsigned)((strips + W - 1) / W), (unsigned)a.d.H, (unsigned)a.d.N);
-    if (W == 4) k_delta_scan<T, KP, 4><<<grid, 256, 0, st>>>(a, (T*)out, send);
-    else if (W == 2) k_delta_scan<T, KP, 2><<<grid, 128, 0, st>>>(a, (T*)out, send);
-    else k_delta_scan<T, KP, 1><<<grid, 64, 0, st>>>(a, (T*)out, send);
+    const dim3 grid((unsigned)((a.VP / 16 + kDeltaW - 1) / kDeltaW), (unsigned)a.d.H, (unsigned)a.d.N);
+    k_delta_scan<T, KP, VEC><<<grid, 64 * kDeltaW, 0, st>>>(a, (T*)out, send);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
@@ -371,8 +371,10 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
     if (!d || !d->q || !d->k || !d->v || !d->g || !d->beta) return SNHIP_E_INVAL;
     if (d->B < 1 || d->T < 1 || d->N < 1 || d->N > 65535 || d->H < 1 || d->H > 65535 || d->Hk < 1 ||
         d->H % d->Hk || d->K < 1 || d->K > 128 || d->V < 1 || d->V > 4096 || d->T > INT32_MAX / d->B ||
-        (d->cu ? d->B != 1 : d->N != d->B) || d->dtype < SNHIP_F32 || d->dtype > SNHIP_F16)
+        (d->cu ? d->B != 1 : d->N != d->B) || d->H * d->V >= kDeltaStride || d->H * d->K >= kDeltaStride || d->dtype < SNHIP_F32 || d->dtype > SNHIP_F16)
         return SNHIP_E_INVAL;
+    for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride})
+        if (st[1] < 0 || st[1] >= kDeltaStride) return SNHIP_E_INVAL;
     a->d = *d;
     a->slots = delta_slots(*d);
     a->KP = delta_kp(d->K);
@@ -382,8 +384,7 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
     auto vec = [&](const void* p, const int64_t* s) {
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % step == 0 && s[1] % step == 0 && s[2] % step == 0;
     };
-    a->vec_q = vec(d->q, d->q_stride);
-    a->vec_k = vec(d->k, d->k_stride);
+    a->vec = d->K % 8 == 0 && vec(d->q, d->q_stride) && vec(d->k, d->k_stride);
     return SNHIP_OK;
 }
 
@@ -420,14 +421,9 @@ snhip_status snhip_op_delta_fwd_dev(const SnHipDelta* d, void* out, float* send,
         if (d->dtype == SNHIP_BF16) return step_t<__bf16>(a, out, send, st);
         return step_t<_Float16>(a, out, send, st);
     }
-    if (a.KP == 64) {
-        if (d->dtype == SNHIP_F32) return fwd_t<float, 64>(a, out, send, st);
-        if (d->dtype == SNHIP_BF16) return fwd_t<__bf16, 64>(a, out, send, st);
-        return fwd_t<_Float16, 64>(a, out, send, st);
-    }
-    if (d->dtype == SNHIP_F32) return fwd_t<float, 128>(a, out, send, st);
-    if (d->dtype == SNHIP_BF16) return fwd_t<__bf16, 128>(a, out, send, st);
-    return fwd_t<_Float16, 128>(a, out, send, st);
+    return delta_pick(a, [&](auto t, auto kp, auto vec) {
+        return fwd_t<decltype(t), decltype(kp)::value, decltype(vec)::value>(a, out, send, st);
+    });
 }
 
 }  // extern "C"

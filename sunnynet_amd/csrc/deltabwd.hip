@@ -32,9 +32,9 @@ __host__ __device__ inline DeltaWs delta_ws(const DeltaP& a, float* ws, int64_t 
     return {ws + i * kDC * a.VP, ws + nr + i * (int64_t)(a.VP * a.KP)};
 }
 
-template <typename T, int KP, int W>
-__global__ __launch_bounds__(64 * W) void k_delta_rscan(DeltaP a, SnHipDeltaGrad gr) {
-    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, NTH = 64 * W;
+template <typename T, int KP, bool VEC>
+__global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDeltaGrad gr) {
+    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W;
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, kDC, kDC> Mat;
     __shared__ alignas(16) __bf16 sk[2][Rows::elems], sq[2][Rows::elems], sm[2][Mat::elems], sp[2][Mat::elems];
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_rscan(DeltaP a, SnHipDeltaGrad
     const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
     const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0, h / a.rep);
     const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0, h / a.rep);
-    const T* dop = static_cast<const T*>(gr.dout) + (s.row * d.H + h) * (int64_t)V + v;
+    const T* dop = static_cast<const T*>(gr.dout) + (s.row * d.H + h) * (int64_t)V;
     const float* rec = d.chunks + (s.slot * d.H + h) * kDeltaChunk;
 
     f32x4 S[NK];           // dS, rows as k_delta_scan holds S
@@ -57,22 +57,25 @@ __global__ __launch_bounds__(64 * W) void k_delta_rscan(DeltaP a, SnHipDeltaGrad
             const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
             S[kt][r] = gr.dsend && k < Kd && v < V ? gr.dsend[sbase + (int64_t)k * V + v] : 0.f;
         }
-    RowsFetch<T, KP, NTH> fk, fq;
+    RowsFetch<T, KP, NTH, VEC> fk, fq;
     MatFetch<3, NTH> fm, fp;
     float fv[(3 * kDC + NTH - 1) / NTH];
-    T vv[8];
+    unsigned vv[8];
+    fk.init(d.k_stride[1], Kd, tid);
+    fq.init(d.q_stride[1], Kd, tid);
+    const int E = (int)sizeof(T), o_step = (int)d.H * V * E, o_off = v < V ? g8 * o_step + v * E : kNowhere;
     auto fetch = [&](int t0) {
         const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
-        const float* r = rec + (int64_t)(t0 / kDC) * d.H * kDeltaChunk;
-        fk.load(kp + t0 * d.k_stride[1], d.k_stride[1], n, Kd, a.vec_k, tid);
-        fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, a.vec_q, tid);
-        fm.load(r, tid);
-        fp.load(r + kDeltaP, tid);
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(rec + (int64_t)(t0 / kDC) * d.H * kDeltaChunk, kDeltaChunk * 4);
+        fk.load(kp + t0 * d.k_stride[1], d.k_stride[1], n, Kd, tid);
+        fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, tid);
+        fm.load(r, 0, tid);
+        fp.load(r, kDeltaP, tid);
 #pragma unroll
-        for (int j = 0; j * NTH < 3 * kDC; j++)
-            if (tid + j * NTH < 3 * kDC) fv[j] = r[kDeltaG + tid + j * NTH];
+        for (int j = 0; j * NTH < 3 * kDC; j++) fv[j] = buf_load<float>(r, (kDeltaG + tid + j * NTH) * 4);
+        const __amdgpu_buffer_rsrc_t ro = rows_window(dop + t0 * d.H * V, d.H * V, n, V);
 #pragma unroll
-        for (int i = 0; i < 8; i++) vv[i] = g8 + i < n && v < V ? dop[(int64_t)(t0 + g8 + i) * d.H * V] : (T)0.f;
+        for (int i = 0; i < 8; i++) vv[i] = buf_load_bits<T>(ro, o_off + i * o_step);
     };
     auto store = [&](int b) {
         fk.store(Rows{sk[b]}, tid);
@@ -94,14 +97,15 @@ __global__ __launch_bounds__(64 * W) void k_delta_rscan(DeltaP a, SnHipDeltaGrad
         const Mat M{sm[b]}, PM{sp[b]};
         const DeltaWs w = delta_ws(a, gr.ws, s.slot + t0 / kDC, h);
         float G[8], L[8], be[8], x[8], y[8];
-        Vec8<T> raw;
+        float od[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) raw[i] = vv[i];
+        for (int i = 0; i < 8; i++) od[i] = float_of_bits<T>(vv[i]);
         if (t0 > 0) fetch(t0 - kDC);
-        if (v < a.VP)
+        const __amdgpu_buffer_rsrc_t rds = make_rsrc(w.ds, (uint32_t)(a.VP * KP * 4)),
+                                     rdr = make_rsrc(w.dr, (uint32_t)(a.VP * kDC * 4));
 #pragma unroll
-            for (int kt = 0; kt < NK; kt++)
-                *reinterpret_cast<f32x4*>(w.ds + (int64_t)v * KP + (kt >> 1) * 32 + g8 + 4 * (kt & 1)) = S[kt];
+        for (int kt = 0; kt < NK; kt++)
+            buf_store4(rds, (v * KP + g8) * 4 + ((kt >> 1) * 32 + 4 * (kt & 1)) * 4, S[kt]);
         f32x4 du[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
         for (int p = 0; p < KP / 32; p++) {
@@ -119,9 +123,9 @@ __global__ __launch_bounds__(64 * W) void k_delta_rscan(DeltaP a, SnHipDeltaGrad
 #pragma unroll
             for (int r = 0; r < 4; r++) G[i + r] = t0v[r], L[i + r] = t1v[r], be[i + r] = t2v[r];
         }
-        const Frag<P> dO = split_raw8<T>(raw);
+        const Frag<P> dO = split8<P>(od);
 #pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = (float)raw[i] * ((float)d.scale * G[i]);
+        for (int i = 0; i < 8; i++) y[i] = od[i] * ((float)d.scale * G[i]);
         const Frag<3> GdO = split8<3>(y);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
@@ -135,7 +139,7 @@ __global__ __launch_bounds__(64 * W) void k_delta_rscan(DeltaP a, SnHipDeltaGrad
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             const f32x4 dr = mma<3>(M.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dU, f32x4{0, 0, 0, 0});
-            if (v < a.VP) *reinterpret_cast<f32x4*>(w.dr + (int64_t)v * kDC + g8 + 4 * m) = dr;
+            buf_store4(rdr, (v * kDC + g8 + 4 * m) * 4, dr);
 #pragma unroll
             for (int r = 0; r < 4; r++) y[4 * m + r] = -dr[r] * be[4 * m + r] * G[4 * m + r];
         }
@@ -170,7 +174,7 @@ __device__ __forceinline__ float sum_groups(float x) {
 // wave first owns 16 columns (X, U, dV), then KP / 4 columns of K (the products with S
 // and dS); the 32x32 matrices are made by three waves, a 16x16 tile each. U and dR lie
 // in LDS by column of V, as the waves hold them, and are read transposed.
-template <typename T, int KP>
+template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
     constexpr int P = ElemPlanes<T>::n, VT = 64, NC = KP / 64;     // NC tiles of 16 columns of K a wave
     typedef Tile<P, kDC, KP> Rows;
@@ -193,10 +197,12 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
     const Cols UT{su}, RT{sr};
     const Tile<P, kDC, VT> DO{so};
     const Mat M{sx}, Y{sx}, FF{sx + Mat::elems};        // Y takes M's place
-    RowsFetch<T, KP, 256> f;
-    f.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, hk), d.k_stride[1], n, Kd, a.vec_k, tid);
+    RowsFetch<T, KP, 256, VEC> f;
+    f.init(d.k_stride[1], Kd, tid);
+    f.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, hk), d.k_stride[1], n, Kd, tid);
     f.store(K, tid);
-    f.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, hk), d.q_stride[1], n, Kd, a.vec_q, tid);
+    f.init(d.q_stride[1], Kd, tid);
+    f.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, hk), d.q_stride[1], n, Kd, tid);
     f.store(Q, tid);
     f32x4 dq[NC][2], dk[NC][2];
 #pragma unroll
@@ -214,7 +220,7 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
         __syncthreads();
         {
             MatFetch<3, 256> fm;
-            fm.load(rec, tid);
+            fm.load(make_rsrc(rec, kDeltaChunk * 4), 0, tid);
             fm.store(M, tid);
         }
         if (tid < 3 * kDC) sv[tid] = rec[kDeltaG + tid];
@@ -441,16 +447,13 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
     }
 }
 
-template <typename T, int KP>
+template <typename T, int KP, bool VEC>
 snhip_status bwd_t(const DeltaP& a, const SnHipDeltaGrad& gr, hipStream_t st) {
-    const int strips = a.VP / 16, W = strips >= 4 ? 4 : strips >= 2 ? 2 : 1;
-    const dim3 grid((unsigned)((strips + W - 1) / W), (unsigned)a.d.H, (unsigned)a.d.N);
-    if (W == 4) k_delta_rscan<T, KP, 4><<<grid, 256, 0, st>>>(a, gr);
-    else if (W == 2) k_delta_rscan<T, KP, 2><<<grid, 128, 0, st>>>(a, gr);
-    else k_delta_rscan<T, KP, 1><<<grid, 64, 0, st>>>(a, gr);
+    const dim3 grid((unsigned)((a.VP / 16 + kDeltaW - 1) / kDeltaW), (unsigned)a.d.H, (unsigned)a.d.N);
+    k_delta_rscan<T, KP, VEC><<<grid, 64 * kDeltaW, 0, st>>>(a, gr);
     SNHIP_CHECK(hipGetLastError());
     const bool vec_o = a.d.V % 8 == 0 && reinterpret_cast<uintptr_t>(gr.dout) % 16 == 0;
-    k_delta_local<T, KP><<<dim3((unsigned)a.slots, (unsigned)a.d.Hk), 256, 0, st>>>(a, gr, vec_o);
+    k_delta_local<T, KP, VEC><<<dim3((unsigned)a.slots, (unsigned)a.d.Hk), 256, 0, st>>>(a, gr, vec_o);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
@@ -473,14 +476,9 @@ snhip_status snhip_op_delta_bwd_dev(const SnHipDelta* d, const SnHipDeltaGrad* g
         !gr->dg || !gr->dbeta || !gr->ws)
         return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);
-    if (a.KP == 64) {
-        if (d->dtype == SNHIP_F32) return bwd_t<float, 64>(a, *gr, st);
-        if (d->dtype == SNHIP_BF16) return bwd_t<__bf16, 64>(a, *gr, st);
-        return bwd_t<_Float16, 64>(a, *gr, st);
-    }
-    if (d->dtype == SNHIP_F32) return bwd_t<float, 128>(a, *gr, st);
-    if (d->dtype == SNHIP_BF16) return bwd_t<__bf16, 128>(a, *gr, st);
-    return bwd_t<_Float16, 128>(a, *gr, st);
+    return delta_pick(a, [&](auto t, auto kp, auto vec) {
+        return bwd_t<decltype(t), decltype(kp)::value, decltype(vec)::value>(a, *gr, st);
+    });
 }
 
 }  // extern "C"

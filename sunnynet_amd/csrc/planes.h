@@ -23,6 +23,8 @@
 
 #include <cstdint>
 
+#include "bufio.h"
+
 namespace snhip {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -38,16 +40,18 @@ template <> struct ElemPlanes<__bf16> { static constexpr int n = 1; };
 template <int P> struct Frag { bf16x8 p[P]; };
 
 template <int P> __device__ __forceinline__ Frag<P> split8(const float* x) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
     Frag<P> f;
-    float r[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) r[i] = x[i];
+    for (int i = 0; i < 8; i += 2) {       // by pairs: one instruction rounds and packs two
+        f32x2 r = {x[i], x[i + 1]};
 #pragma unroll
-    for (int p = 0; p < P; p++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            f.p[p][i] = (__bf16)r[i];
-            r[i] = r[i] - (float)f.p[p][i];
+        for (int p = 0; p < P; p++) {
+            const bf16x2 h = __builtin_convertvector(r, bf16x2);
+            f.p[p][i] = h[0];
+            f.p[p][i + 1] = h[1];
+            if (p + 1 < P) r = r - __builtin_convertvector(h, f32x2);
         }
     }
     return f;
@@ -140,6 +144,56 @@ template <typename T> __device__ __forceinline__ Vec8<T> load_raw8(const T* src,
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = i < n ? src[i] : (T)0.f;
+    }
+    return x;
+}
+
+// A window of n rows of `len` elements, `stride` elements apart, as a buffer: an offset
+// past it reads 0 and writes nothing, so no row or column needs a branch. kNowhere is
+// such an offset. Strides are below 2^24 elements, so offsets fit 32 bits.
+constexpr int kNowhere = (int)0x80000000u;
+template <typename T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_window(const T* p, int64_t stride, int n, int len) {
+    return make_rsrc(p, (uint32_t)((uint32_t)(n - 1) * (uint32_t)stride + (uint32_t)len) * (uint32_t)sizeof(T));
+}
+template <typename T> __device__ __forceinline__ T buf_load(__amdgpu_buffer_rsrc_t r, int off) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0));
+    else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0));
+}
+// The same as a register of its own, to be held while later work runs: 16-bit values
+// would be packed in pairs on arrival, which waits for them.
+template <typename T> __device__ __forceinline__ unsigned buf_load_bits(__amdgpu_buffer_rsrc_t r, int off) {
+    if constexpr (sizeof(T) == 4) return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    else return (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+}
+template <typename T> __device__ __forceinline__ float float_of_bits(unsigned b) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(b);
+    else return (float)__builtin_bit_cast(T, (unsigned short)b);
+}
+template <typename T> __device__ __forceinline__ void buf_store(__amdgpu_buffer_rsrc_t r, int off, T x) {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, x), r, off, 0, 0);
+}
+__device__ __forceinline__ f32x4 buf_load4(__amdgpu_buffer_rsrc_t r, int off) {
+    return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+}
+__device__ __forceinline__ void buf_store4(__amdgpu_buffer_rsrc_t r, int off, f32x4 x) {
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), r, off, 0, 0);
+}
+// Eight elements from `off`, of which the first n are wanted (n < 8 only without vec);
+// vec: 16-byte aligned.
+template <typename T> __device__ __forceinline__ Vec8<T> buf_load8(__amdgpu_buffer_rsrc_t r, int off, int n, bool vec) {
+    Vec8<T> x;
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 a = buf_load4(r, off), b = buf_load4(r, off + 16);
+            x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            x = __builtin_bit_cast(Vec8<T>, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = buf_load<T>(r, i < n ? off + i * (int)sizeof(T) : kNowhere);
     }
     return x;
 }
