@@ -1,252 +1,526 @@
 // The next token of every row of logits from one given random number per row.
 //
-// With z = logit / T and m = max z, token i weighs exp(z_i - m). The filters keep, in
-// the descending order of z, a prefix each: top-k by count, top-p by share, min-p by
-// weight. So a row needs no sort: it needs the value at which a prefix ends. That value
-// is found on a monotone 32-bit image of the logit (sort_key), 2048 bins at a time:
-// counts or sums per bin in LDS, the bin in which the prefix ends, then the same over
-// that bin's keys until it is one key. The token is the first index up to which the kept
-// weights sum to more than u of their total; a wave sums a span of indices, and the span
-// that holds the point is divided again.
+// With m the largest logit, token i weighs exp((x_i - m) / T). The filters keep, in the
+// descending order of the logits, a prefix each: top-k by count, top-p by share, min-p by
+// weight. So a row needs no sort: it needs the place at which a prefix ends. A block holds
+// its row in registers (rows of up to 65536; longer ones are read again) and
+//   - counts, or sums, the row into 2048 bins of equal width of (m - x) / T in LDS, down to
+//     where weights are 0, and finds the bin in which the prefix ends;
+//   - takes that bin's few tokens (for top-k all tokens from it up, if few) into a list and
+//     orders them by comparing all pairs; a bin of many (equal logits, mostly) is divided
+//     again by the bits of the logits until it is one value, whose tokens go by index;
+//   - sums the kept weights by groups of 256 neighbouring indices and walks those sums to
+//     the first index up to which they exceed u of their total.
 //
 // Weights are computed in 64 bits and summed as whole numbers (scaled by a power of two
 // that lets a row's sum stay below 2^62): sums do not depend on their order, so neither
 // the LDS atomics nor the division of the row change a result, and the rounding of a
-// weight (2^-42 of the largest for 2^20 tokens, 2^-47 for 32000) is far below what a
-// sum of 32-bit floats would leave.
+// weight (2^-42 of the largest for 2^20 tokens, 2^-47 for 32000) is far below what a sum
+// of 32-bit floats would leave.
 #include "common.h"
+#include "planes.h"
 #include "snhip_ops.h"
 
 namespace snhip {
 namespace {
 
-constexpr int kBins = 2048;
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kBins = 2048, kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kSlab = 4 * kThreads;          // tokens of one pass: four neighbours a thread
+constexpr int kHeld = 16;                    // slabs that registers hold
+constexpr int kSlabs = (1 << 20) / kSlab;
+constexpr int kList = 256;
+constexpr float kRange = 44.f;               // exp(-44) is 0 in the scaled weights
 typedef unsigned long long u64;
-
-__device__ __forceinline__ float logit_f(float x) { return x; }
-__device__ __forceinline__ float logit_f(__bf16 x) { return (float)x; }
-__device__ __forceinline__ float logit_f(_Float16 x) { return (float)x; }
 
 // Larger logits have larger keys; -0 and 0 are one.
 __device__ __forceinline__ unsigned sort_key(float x) {
     const unsigned b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-
-struct Row {
-    double temperature, zmax, scale;
-};
-
-// The weight of a logit as a whole number; a NaN or a logit of -inf weighs nothing.
-__device__ __forceinline__ u64 weight(const Row& r, float x) {
-    const double w = exp((double)x / r.temperature - r.zmax);
-    return w > 0. ? (u64)rint(w * r.scale) : 0;
+__device__ __forceinline__ float key_logit(unsigned k) {
+    return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
 struct Shared {
-    u64 sum[kBins];
+    u64 sum[kBins];                // of bins; the groups' sums at the end
     unsigned count[kBins];
+    double exp2[128];              // 2^(j / 128)
     u64 wsum[kWaves];
     unsigned wcount[kWaves];
-    u64 pick_sum;              // what the search found
-    unsigned pick_bin, pick_count;
+    float lx[kList];               // the list: logits, indices, weights
+    int li[kList];
+    u64 lw[kList];
     float wmax[kWaves];
-    int warg[kWaves], wnan[kWaves];
+    int windex[kWaves];
+    unsigned listed, low_key, high_key;
+    int bin, pick;
+    u64 above_sum, total;
+    unsigned above_count;
+    u64 group[kSlabs][kWaves];     // kept weight of 256 neighbouring tokens
 };
 
-__device__ __forceinline__ u64 wave_sum(u64 x) {
+// exp((x - m) / T) 2^bits, in 64 bits: 2^(n / 128) from the table, the rest (below
+// 2^-8 log 2) by its Taylor polynomial of degree 4, 1e-15 of the value.
+struct Weights {
+    double m, step, scale, low;    // step: 128 / (T log 2)
+    int bits;
+    __device__ __forceinline__ double real(float x, const Shared& s) const {
+        const double t = ((double)x - m) * step;
+        if (!(t > -128. * 70.)) return 0.;
+        const double n = rint(t), r = (t - n) * (0.69314718055994530942 / 128.);
+        const int i = (int)n;
+        const double p = fma(r, fma(r, fma(r, fma(r, 1. / 24., 1. / 6.), 0.5), 1.), 1.);
+        return ldexp(s.exp2[i & 127] * p, (i >> 7) + bits);
+    }
+    // Rounded to a whole number (below 2^52), by adding 2^52.
+    __device__ __forceinline__ u64 whole(double w) const {
+        return (u64)__double_as_longlong(w + 0x1p52) - (u64)__double_as_longlong(0x1p52);
+    }
+    __device__ __forceinline__ u64 operator()(float x, const Shared& s) const { return whole(real(x, s)); }
+};
+
+template <typename V> __device__ __forceinline__ V wave_sum(V x) {
     for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
     return x;
 }
 
-// In the descending order of keys from `top` down, where a prefix ends: the key of the
-// last token before which `limit` is not yet passed (by count: fewer than `limit` tokens
-// before it; by sum: the weights before it sum to at most `limit`). Also the number and
-// sum of the tokens above that key. Tokens below `low` do not take part.
-struct Cut {
-    unsigned key, above;
-    u64 sum;
+// A row: NJ slabs in registers, or (NJ = 0) read where they are used. Tokens past the
+// row's end read as -inf.
+template <typename T, int NJ> struct RowData {
+    f32x4 x[NJ ? NJ : 1];
+    const T* p;
+    int V, slabs;
+    bool vec;
+    __device__ __forceinline__ f32x4 load(int j) const {
+        const int i = j * kSlab + 4 * threadIdx.x;
+        f32x4 v;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        if (vec && i + 4 <= V) {
+            const T4 t = *reinterpret_cast<const T4*>(p + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = (float)t[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = i + e < V ? (float)p[i + e] : -INFINITY;
+        }
+        return v;
+    }
+    // f(index, logit) for every token of this thread.
+    template <typename F> __device__ __forceinline__ void each(F f) const {
+        if constexpr (NJ > 0) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) f(j * kSlab + 4 * (int)threadIdx.x + e, x[j][e]);
+                __builtin_amdgcn_sched_barrier(0);      // slabs at once would need registers for all
+            }
+        } else {
+            for (int j = 0; j < slabs; j++) {
+                const f32x4 v = load(j);
+#pragma unroll
+                for (int e = 0; e < 4; e++) f(j * kSlab + 4 * (int)threadIdx.x + e, v[e]);
+            }
+        }
+    }
+    template <typename F> __device__ __forceinline__ void each_slab(F f) const {
+        if constexpr (NJ > 0) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                f(j, x[j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            for (int j = 0; j < slabs; j++) f(j, load(j));
+        }
+    }
 };
-template <typename T>
-__device__ Cut find_cut(const T* x, int V, const Row& row, unsigned top, unsigned low, bool by_sum, u64 limit,
-                        Shared& s) {
-    const int tid = threadIdx.x;
-    Cut c{0, 0, 0};
-    unsigned hi = top, lo = low;               // the keys in question
+
+__device__ __forceinline__ void clear_bins(Shared& s) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+        s.sum[i] = 0;
+        s.count[i] = 0;
+    }
+    if (threadIdx.x == 0) {
+        s.bin = -1;
+        s.listed = 0;
+        s.low_key = ~0u;
+        s.high_key = 0;
+    }
+}
+
+// The last used bin before which fewer than `limit` tokens lie (or, by sum, a weight of
+// at most `limit`), counting from (count, sum) above the first bin. -1: no bin is used.
+// Leaves the bin and what lies above it in s.
+__device__ void end_bin(bool by_sum, u64 limit, unsigned count, u64 sum, Shared& s) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __syncthreads();
+    const unsigned c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+    const u64 s0 = s.sum[2 * tid], s1 = s.sum[2 * tid + 1];
+    unsigned c = c0 + c1;
+    u64 t = s0 + s1;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned y = __shfl_up(c, o);
+        const u64 z = __shfl_up(t, o);
+        if (lane >= o) c += y, t += z;
+    }
+    if (lane == 63) s.wcount[wave] = c, s.wsum[wave] = t;
+    __syncthreads();
+    for (int w = 0; w < wave; w++) c += s.wcount[w], t += s.wsum[w];
+    c += count - (c0 + c1);            // above the first of this thread's two bins
+    t += sum - (s0 + s1);
+    const bool a0 = c0 && (by_sum ? t <= limit : c < limit);
+    const bool a1 = c1 && (by_sum ? t + s0 <= limit : c + c0 < limit);
+    const int mine = a1 ? 2 * tid + 1 : a0 ? 2 * tid : -1;
+    if (mine >= 0) atomicMax(&s.bin, mine);
+    __syncthreads();
+    if (mine >= 0 && mine == s.bin) {
+        s.above_count = a1 ? c + c0 : c;
+        s.above_sum = a1 ? t + s0 : t;
+    }
+    __syncthreads();
+}
+
+// Where a prefix ends: tokens above `x`, and of those equal to it the indices below
+// `end`, are in it.
+struct Cut {
+    float x;
+    int end;
+    __device__ __forceinline__ bool keeps(int i, float y) const { return y > x || (y == x && i < end); }
+};
+
+// The first index at which the running total of val(i, x) over indices exceeds
+// point(total); -1 if there is none.
+template <typename D, typename F, typename G> __device__ int find_index(const D& row, Shared& s, F val, G point_of) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __syncthreads();
+    if (tid == 0) s.pick = s.bin = -1;
+    row.each_slab([&](int j, f32x4 x) {
+        u64 t = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) t += val(j * kSlab + 4 * tid + e, x[e]);
+        t = wave_sum(t);
+        if (lane == 0) s.group[j][wave] = t;
+    });
+    __syncthreads();
+    // wave 0 walks the groups, 64 at a time
+    const u64* g = &s.group[0][0];
+    const int n = row.slabs * kWaves;
+    if (wave == 0) {
+        u64 before = 0, total = 0;
+        for (int i = lane; i < n; i += 64) total += g[i];
+        total = wave_sum(total);
+        if (lane == 0) s.total = total;
+        const u64 point = point_of(total);
+        for (int i = 0; i < n; i += 64) {
+            u64 t = i + lane < n ? g[i + lane] : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const u64 y = __shfl_up(t, o);
+                if (lane >= o) t += y;
+            }
+            const u64 m = __ballot(before + t > point);
+            if (m) {
+                const int l = __ffsll(m) - 1;
+                const u64 upto = before + __shfl(t, l);
+                if (lane == 0) {
+                    s.bin = i + l;
+                    s.above_sum = upto - g[i + l];
+                }
+                break;
+            }
+            before += __shfl(t, 63);
+        }
+    }
+    __syncthreads();
+    const int at = s.bin;
+    const u64 point = point_of(s.total);
+    if (at >= 0 && wave == at % kWaves) {
+        const f32x4 x = row.load(at / kWaves);
+        const int i = at / kWaves * kSlab + 4 * tid;
+        u64 w[4], t = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) t += w[e] = val(i + e, x[e]);
+        u64 run = t;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const u64 y = __shfl_up(run, o);
+            if (lane >= o) run += y;
+        }
+        run += s.above_sum;
+        const u64 m = __ballot(run > point);
+        if (m && lane == __ffsll(m) - 1) {
+            run -= t;
+            int e = 0;
+            while (e < 3 && run + w[e] <= point) run += w[e++];
+            s.pick = i + e;
+        }
+    }
+    __syncthreads();
+    return s.pick;
+}
+
+// The cut of a prefix that ends among the tokens with keys [low, high], of which there
+// are many: by the bits of the keys, then by index.
+template <typename D>
+__device__ Cut cut_by_keys(const D& row, const Weights& w, unsigned low, unsigned high, bool by_sum, u64 limit,
+                           unsigned count, u64 sum, Shared& s) {
     for (;;) {
-        const unsigned span = hi - lo;         // bins of 2^shift keys, the first at hi
+        const unsigned span = high - low;         // bins of 2^shift keys, the first at `high`
         int shift = 0;
         while ((span >> shift) >= kBins) shift++;
-        for (int i = tid; i < kBins; i += kThreads) {
-            s.sum[i] = 0;
-            s.count[i] = 0;
-        }
         __syncthreads();
-        for (int i = tid; i < V; i += kThreads) {
-            const float f = logit_f(x[i]);
-            const unsigned k = sort_key(f);
-            if (f == f && k >= lo && k <= hi) {
-                const unsigned b = (hi - k) >> shift;
+        clear_bins(s);
+        __syncthreads();
+        row.each([&](int i, float x) {
+            const unsigned k = sort_key(x);
+            if (k >= low && k <= high) {
+                const unsigned b = (high - k) >> shift;
                 atomicAdd(&s.count[b], 1u);
-                atomicAdd(&s.sum[b], weight(row, f));
+                if (by_sum) atomicAdd(&s.sum[b], w(x, s));
             }
-        }
-        __syncthreads();
-        if (tid == 0) {                        // the bin in which the prefix ends
-            u64 sum = c.sum;
-            unsigned n = c.above, b = 0, last = 0;
-            u64 lsum = sum;
-            unsigned ln = n;
-            bool any = false;
-            for (b = 0; b < kBins; b++) {
-                if (!s.count[b]) continue;
-                if (any && (by_sum ? sum > limit : n >= limit)) break;
-                any = true;
-                last = b;
-                lsum = sum;
-                ln = n;
-                sum += s.sum[b];
-                n += s.count[b];
-            }
-            s.pick_bin = last;
-            s.pick_sum = lsum;
-            s.pick_count = ln;
-        }
-        __syncthreads();
-        c.sum = s.pick_sum;
-        c.above = s.pick_count;
-        hi = hi - (s.pick_bin << shift);
+        });
+        end_bin(by_sum, limit, count, sum, s);
+        count = s.above_count;
+        sum = s.above_sum;
+        high -= (unsigned)s.bin << shift;
         const unsigned width = (1u << shift) - 1;
-        lo = hi - lo > width ? hi - width : lo;
-        __syncthreads();
-        if (!shift) {
-            c.key = hi;
-            return c;
-        }
+        low = high - low > width ? high - width : low;
+        if (!shift) break;
     }
+    const float x = key_logit(high);
+    if (!by_sum) return {x, INT32_MAX};           // all that equal the k-th stay
+    const u64 one = w(x, s), n = one ? (limit - sum) / one + 1 : (u64)row.V;
+    if (n >= (u64)row.V) return {x, INT32_MAX};
+    const int end = find_index(row, s, [&](int, float y) -> u64 { return y == x; }, [&](u64) { return n; });
+    return {x, end < 0 ? INT32_MAX : end};
 }
 
-// The first index at which a running total over indices [0, V) of val(i) exceeds
-// `point`, and the total before its span; V if there is none. The row is divided into
-// kWaves spans, the span with the point again, down to 64 indices.
-template <typename F> __device__ int find_index(int V, u64 point, Shared& s, F val) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int lo = 0, hi = V;
-    u64 before = 0;
-    while (hi - lo > 64) {
-        const int span = ((hi - lo + kWaves - 1) / kWaves + 63) & ~63;
-        const int a = lo + wave * span, e = a + span < hi ? a + span : hi;
-        u64 t = 0;
-        for (int i = a + lane; i < e; i += 64) t += val(i);
-        t = wave_sum(t);
-        __syncthreads();
-        if (lane == 0) s.wsum[wave] = t;
-        __syncthreads();
-        int w = 0;
-        u64 sum = before;
-        while (w < kWaves && sum + s.wsum[w] <= point) sum += s.wsum[w++];
-        if (w == kWaves) return V;
-        before = sum;
-        lo = lo + w * span;
-        hi = lo + span < hi ? lo + span : hi;
-    }
-    // every wave does the same last step
-    u64 t = lo + lane < hi ? val(lo + lane) : 0;
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(t, o);
-        if (lane >= o) t += y;
-    }
-    const u64 m = __ballot(lo + lane < hi && before + t > point);
-    return m ? lo + __ffsll(m) - 1 : V;
+// Sum over the listed tokens j of f(j), for the listed token of this thread's group of
+// kThreads / kList threads (0 for groups past the list); every thread of the group has it.
+constexpr int kPer = kThreads / kList;
+template <typename V, typename F> __device__ __forceinline__ V over_list(int n, F f) {
+    V t = 0;
+    for (int j = threadIdx.x % kPer; j < n; j += kPer) t += f(j);
+#pragma unroll
+    for (int o = 1; o < kPer; o <<= 1) t += __shfl_xor(t, o);
+    return t;
 }
 
-template <typename T> __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens) {
+template <typename T, int NJ> __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens, bool vec) {
     __shared__ Shared s;
     const int64_t b = blockIdx.x;
-    const int V = (int)a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const T* x = static_cast<const T*>(a.logits) + b * a.stride;
-    Row row;
-    row.temperature = a.temperature ? a.temperature[b] : a.temperature0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    RowData<T, NJ> row;
+    row.p = static_cast<const T*>(a.logits) + b * a.stride;
+    row.V = (int)a.V;
+    row.slabs = (row.V + kSlab - 1) / kSlab;
+    row.vec = vec;
+    if constexpr (NJ > 0) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) row.x[j] = row.load(j);
+    }
+    const double temperature = a.temperature ? a.temperature[b] : a.temperature0;
     const double top_p = a.top_p ? a.top_p[b] : a.top_p0, min_p = a.min_p ? a.min_p[b] : a.min_p0;
     const int64_t top_k = a.top_k ? a.top_k[b] : a.top_k0;
+    const double u = a.u[b];
+    if (tid < 128) s.exp2[tid] = exp2((double)tid / 128.);
+    clear_bins(s);
 
-    // the first maximal logit; NaN counts as maximal
+    // the largest logit; a NaN makes it NaN
     float m = -INFINITY;
-    int at = V, nan = V;
-    for (int i = tid; i < V; i += kThreads) {
-        const float f = logit_f(x[i]);
-        if (f != f) nan = nan < i ? nan : i;
-        else if (at == V || f > m) m = f, at = i;
-    }
-    for (int o = 32; o; o >>= 1) {
-        const float om = __shfl_xor(m, o);
-        const int oa = __shfl_xor(at, o), on = __shfl_xor(nan, o);
-        if (oa < V && (at == V || om > m || (om == m && oa < at))) m = om, at = oa;
-        nan = nan < on ? nan : on;
-    }
-    if (lane == 0) s.wmax[wave] = m, s.warg[wave] = at, s.wnan[wave] = nan;
+    bool nan = false;
+    row.each([&](int, float x) {
+        m = fmaxf(m, x);
+        nan |= x != x;
+    });
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (__any(nan)) m = NAN;
+    if (lane == 0) s.wmax[wave] = m;
     __syncthreads();
-    m = s.wmax[0], at = s.warg[0], nan = s.wnan[0];
-    for (int w = 1; w < kWaves; w++) {
-        const int oa = s.warg[w];
-        if (oa < V && (at == V || s.wmax[w] > m || (s.wmax[w] == m && oa < at))) m = s.wmax[w], at = oa;
-        nan = nan < s.wnan[w] ? nan : s.wnan[w];
-    }
-    const int greedy = nan < V ? nan : at;
-    row.zmax = (double)m / row.temperature;
-    int bits = 0;
-    while ((1 << bits) < V) bits++;
-    row.scale = ldexp(1.0, 62 - bits);
-    if (!(row.temperature > 0.) || nan < V || !(fabs(row.zmax) < INFINITY)) {
-        if (tid == 0) tokens[b] = greedy;
-        return;
-    }
-    const unsigned top = sort_key(m), all = sort_key(-INFINITY);
-    unsigned low = all;                        // the smallest key that is kept
-    int ties = V;                              // and the first index from which it is not
-    if (top_k > 0 && top_k < V) low = find_cut(x, V, row, top, all, false, (u64)top_k, s).key;
-    if (top_p > 0. && top_p < 1.) {
-        __syncthreads();
-        u64 t = 0;
-        for (int i = tid; i < V; i += kThreads) {
-            const float f = logit_f(x[i]);
-            if (sort_key(f) >= low) t += weight(row, f);
+    m = s.wmax[0];
+    for (int w = 1; w < kWaves; w++) m = s.wmax[w] > m || s.wmax[w] != s.wmax[w] ? s.wmax[w] : m;
+    // written so that one NaN wins: a NaN m compares false, and a later number does not replace it
+    const double zmax = (double)m / temperature;
+    auto first_max = [&] {
+        int at = row.V;
+        row.each([&](int i, float x) {
+            if ((m != m ? x != x : x == m) && i < at) at = i;
+        });
+        for (int o = 32; o; o >>= 1) {
+            const int y = __shfl_xor(at, o);
+            at = at < y ? at : y;
         }
+        __syncthreads();
+        if (lane == 0) s.windex[wave] = at;
+        __syncthreads();
+        for (int w = 0; w < kWaves; w++) at = at < s.windex[w] ? at : s.windex[w];
+        if (tid == 0) tokens[b] = at;
+    };
+    if (!(temperature > 0.) || !(fabs(zmax) < INFINITY)) return first_max();
+    auto point_of = [&](u64 total) -> u64 {
+        const u64 point = u > 0. ? (u64)(fmin(u, 1.) * (double)total) : 0;
+        return total && point >= total ? total - 1 : point;
+    };
+    Weights w;
+    int bits = 0;
+    while ((1 << bits) < row.V) bits++;
+    w.bits = 62 - bits < 51 ? 62 - bits : 51;
+    w.m = (double)m;
+    w.step = fmin(128. / (0.69314718055994530942 * temperature), 1e300);
+    w.scale = ldexp(1., w.bits);
+    w.low = min_p * w.scale;
+    const float per = (float)fmin((double)kBins / ((double)kRange * temperature), 1e30);
+    auto bin_of = [&](float x) { return (int)fminf((m - x) * per, 2.f * kBins); };     // kBins and up: weight 0
+
+    Cut cut{-INFINITY, INT32_MAX};
+    const bool some_k = top_k > 0 && top_k < row.V, some_p = top_p > 0. && top_p < 1.;
+    if (some_k) {
+        row.each([&](int, float x) {
+            const int i = bin_of(x);
+            if (i < kBins) atomicAdd(&s.count[i], 1u);
+        });
+        end_bin(false, (u64)top_k, 0, 0, s);
+        const int last = s.bin;
+        const unsigned above = s.above_count, in = s.count[last];
+        const bool all = above + in <= (unsigned)kList;          // every candidate fits the list
+        row.each([&](int i, float x) {
+            const int q = bin_of(x);
+            if (q == last || (all && q < last)) {
+                const unsigned at = atomicAdd(&s.listed, 1u);
+                if (at < (unsigned)kList) s.lx[at] = x, s.li[at] = i;
+                if (!all) {
+                    atomicMin(&s.low_key, sort_key(x));
+                    atomicMax(&s.high_key, sort_key(x));
+                }
+            }
+        });
+        __syncthreads();
+        if (all) {
+            // the rest on the list alone: a group of threads per token
+            const int n = (int)s.listed, me = tid / kPer;
+            const float x = me < n ? s.lx[me] : 0.f;
+            const int at = me < n ? s.li[me] : 0;
+            const unsigned rank = over_list<unsigned>(n, [&](int j) -> unsigned { return s.lx[j] > x; });
+            u64 mine = me < n && rank < (u64)top_k ? w(x, s) : 0;
+            if (tid % kPer == 0 && me < n) s.lw[me] = mine;
+            __syncthreads();
+            const u64 total = over_list<u64>(n, [&](int j) { return s.lw[j]; });
+            if (some_p) {
+                const u64 before = over_list<u64>(n, [&](int j) -> u64 {
+                    return s.lx[j] > x || (s.lx[j] == x && s.li[j] < at) ? s.lw[j] : 0;
+                });
+                if (before > (u64)(top_p * (double)total)) mine = 0;
+            }
+            if (mine && w.real(x, s) < w.low) mine = 0;
+            __syncthreads();
+            if (tid % kPer == 0 && me < n) s.lw[me] = mine;
+            if (tid == 0) s.pick = -1;
+            __syncthreads();
+            const u64 kept = over_list<u64>(n, [&](int j) { return s.lw[j]; });
+            const u64 before = over_list<u64>(n, [&](int j) -> u64 { return s.li[j] < at ? s.lw[j] : 0; });
+            const u64 point = point_of(kept);
+            if (tid % kPer == 0 && mine && before <= point && point < before + mine) s.pick = at;
+            __syncthreads();
+            if (s.pick < 0) return first_max();        // min-p leaves nothing
+            if (tid == 0) tokens[b] = s.pick;
+            return;
+        } else if (in <= (unsigned)kList) {
+            const int n = (int)s.listed, me = tid / kPer;
+            const float x = me < n ? s.lx[me] : 0.f;
+            const unsigned rank = above + over_list<unsigned>(n, [&](int j) -> unsigned { return s.lx[j] > x; });
+            // the smallest kept one: fewer than k above it, and k with its equals
+            const unsigned upto = rank + over_list<unsigned>(n, [&](int j) -> unsigned { return s.lx[j] == x; });
+            if (tid % kPer == 0 && me < n && rank < (u64)top_k && (upto >= (u64)top_k || upto == above + in)) s.wmax[0] = x;
+            __syncthreads();
+            cut.x = s.wmax[0];
+        } else {
+            cut = cut_by_keys(row, w, s.low_key, s.high_key, false, (u64)top_k, above, 0, s);
+        }
+        __syncthreads();
+        clear_bins(s);
+        __syncthreads();
+    }
+    if (some_p) {
+        u64 t = 0;
+        row.each([&](int, float x) {
+            const int i = bin_of(x);
+            if (i < kBins && x >= cut.x) {
+                const u64 y = w(x, s);
+                t += y;
+                atomicAdd(&s.count[i], 1u);
+                atomicAdd(&s.sum[i], y);
+            }
+        });
         t = wave_sum(t);
         if (lane == 0) s.wsum[wave] = t;
         __syncthreads();
         t = 0;
-        for (int w = 0; w < kWaves; w++) t += s.wsum[w];
+        for (int i = 0; i < kWaves; i++) t += s.wsum[i];
         const u64 limit = (u64)(top_p * (double)t);
-        const Cut c = find_cut(x, V, row, top, low, true, limit, s);
-        low = c.key;
-        // of the equal ones at the end, those before which the sum is at most the limit
-        const unsigned kb = low & 0x80000000u ? low & 0x7fffffffu : ~low;
-        const u64 w = weight(row, __uint_as_float(kb));
-        const u64 n = w ? (limit - c.sum) / w + 1 : V;
-        if (n < (u64)V) ties = find_index(V, n, s, [&](int i) -> u64 { return sort_key(logit_f(x[i])) == low; });
+        end_bin(true, limit, 0, 0, s);
+        const int last = s.bin;
+        const u64 above = s.above_sum;
+        const unsigned in = s.count[last];
+        const float floor_x = cut.x;
+        row.each([&](int i, float x) {
+            if (bin_of(x) == last && x >= floor_x) {
+                const unsigned at = atomicAdd(&s.listed, 1u);
+                if (at < (unsigned)kList) s.lx[at] = x, s.li[at] = i, s.lw[at] = w(x, s);
+                if (in > (unsigned)kList) {
+                    atomicMin(&s.low_key, sort_key(x));
+                    atomicMax(&s.high_key, sort_key(x));
+                }
+            }
+        });
+        __syncthreads();
+        if (in <= (unsigned)kList) {
+            // in order, the last token before which the sum is within the limit
+            const int n = (int)s.listed, me = tid / kPer;
+            const float x = me < n ? s.lx[me] : 0.f;
+            const int at = me < n ? s.li[me] : 0;
+            const u64 before = above + over_list<u64>(n, [&](int j) -> u64 {
+                return s.lx[j] > x || (s.lx[j] == x && s.li[j] < at) ? s.lw[j] : 0;
+            });
+            const bool in_it = me < n && before <= limit;
+            const unsigned rank = over_list<unsigned>(n, [&](int j) -> unsigned {
+                return s.lx[j] > x || (s.lx[j] == x && s.li[j] < at);
+            });
+            __syncthreads();
+            if (tid == 0) s.pick = -1;
+            __syncthreads();
+            if (in_it && tid % kPer == 0) atomicMax(&s.pick, (int)rank);
+            __syncthreads();
+            if (in_it && tid % kPer == 0 && (int)rank == s.pick) {
+                s.wmax[0] = x;
+                s.windex[0] = at + 1;
+            }
+            __syncthreads();
+            cut = {s.wmax[0], s.windex[0]};
+        } else {
+            cut = cut_by_keys(row, w, s.low_key, s.high_key, true, limit, s.above_count, above, s);
+        }
     }
-    auto kept = [&](int i) -> u64 {
-        const float f = logit_f(x[i]);
-        const unsigned k = sort_key(f);
-        if (k < low || (k == low && i >= ties)) return 0;
-        const double w = exp((double)f / row.temperature - row.zmax);
-        return w < min_p ? 0 : (u64)rint(w * row.scale);
+    auto kept = [&](int i, float x) -> u64 {
+        if (!cut.keeps(i, x)) return 0;
+        const double y = w.real(x, s);
+        return y < w.low ? 0 : w.whole(y);
     };
-    __syncthreads();
-    u64 t = 0;
-    for (int i = tid; i < V; i += kThreads) t += kept(i);
-    t = wave_sum(t);
-    if (lane == 0) s.wsum[wave] = t;
-    __syncthreads();
-    t = 0;
-    for (int w = 0; w < kWaves; w++) t += s.wsum[w];
-    const double u = a.u[b];
-    u64 point = u > 0. ? (u64)(u * (double)t) : 0;
-    if (t && point >= t) point = t - 1;
-    const int pick = t ? find_index(V, point, s, kept) : greedy;
+    const int pick = find_index(row, s, kept, point_of);
+    if (pick < 0) return first_max();
     if (tid == 0) tokens[b] = pick;
+}
+
+template <typename T> void sample_t(const SnHipSample& a, int* tokens, hipStream_t st) {
+    const bool vec = reinterpret_cast<uintptr_t>(a.logits) % (4 * sizeof(T)) == 0 && a.stride % 4 == 0;
+    const int slabs = (int)((a.V + kSlab - 1) / kSlab);
+    const unsigned B = (unsigned)a.B;
+    if (slabs <= 1) k_sample<T, 1><<<B, kThreads, 0, st>>>(a, tokens, vec);
+    else if (slabs <= 2) k_sample<T, 2><<<B, kThreads, 0, st>>>(a, tokens, vec);
+    else if (slabs <= 4) k_sample<T, 4><<<B, kThreads, 0, st>>>(a, tokens, vec);
+    else if (slabs <= 8) k_sample<T, 8><<<B, kThreads, 0, st>>>(a, tokens, vec);
+    else if (slabs <= kHeld) k_sample<T, kHeld><<<B, kThreads, 0, st>>>(a, tokens, vec);
+    else k_sample<T, 0><<<B, kThreads, 0, st>>>(a, tokens, vec);
 }
 
 }  // namespace
@@ -259,9 +533,9 @@ extern "C" snhip_status snhip_op_sample_dev(const SnHipSample* s, int32_t* token
         s->stride < 0 || s->dtype < SNHIP_F32 || s->dtype > SNHIP_F16)
         return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);
-    if (s->dtype == SNHIP_F32) k_sample<float><<<(unsigned)s->B, kThreads, 0, st>>>(*s, tokens);
-    else if (s->dtype == SNHIP_BF16) k_sample<__bf16><<<(unsigned)s->B, kThreads, 0, st>>>(*s, tokens);
-    else k_sample<_Float16><<<(unsigned)s->B, kThreads, 0, st>>>(*s, tokens);
+    if (s->dtype == SNHIP_F32) sample_t<float>(*s, tokens, st);
+    else if (s->dtype == SNHIP_BF16) sample_t<__bf16>(*s, tokens, st);
+    else sample_t<_Float16>(*s, tokens, st);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
