@@ -26,7 +26,6 @@ namespace {
 
 constexpr int kBins = 2048, kThreads = 1024, kWaves = kThreads / 64;
 constexpr int kSlab = 4 * kThreads;          // tokens of one pass: four neighbours a thread
-constexpr int kHeld = 16;                    // slabs that registers hold
 constexpr int kSlabs = (1 << 20) / kSlab;
 constexpr int kList = 256;
 constexpr float kRange = 44.f;               // exp(-44) is 0 in the scaled weights
@@ -60,78 +59,108 @@ struct Shared {
 };
 
 // exp((x - m) / T) 2^bits, in 64 bits: 2^(n / 128) from the table, the rest (below
-// 2^-8 log 2) by its Taylor polynomial of degree 4, 1e-15 of the value.
+// 2^-8 log 2) by its Taylor polynomial of degree 4, 1e-15 of the value. n comes from
+// adding 1.5 2^52, whose last bits it is; the power of two is added to the exponent's bits
+// (the value stays above 2^-72).
 struct Weights {
-    double m, step, scale, low;    // step: 128 / (T log 2)
+    double m, step, low;           // step: 128 / (T log 2)
     int bits;
     __device__ __forceinline__ double real(float x, const Shared& s) const {
-        const double t = ((double)x - m) * step;
-        if (!(t > -128. * 70.)) return 0.;
-        const double n = rint(t), r = (t - n) * (0.69314718055994530942 / 128.);
-        const int i = (int)n;
+        const double t = ((double)x - m) * step, c = 0x1.8p52;
+        const double q = t + c, r = (t - (q - c)) * (0.69314718055994530942 / 128.);
+        const int i = (int)(unsigned)__double_as_longlong(q);
         const double p = fma(r, fma(r, fma(r, fma(r, 1. / 24., 1. / 6.), 0.5), 1.), 1.);
-        return ldexp(s.exp2[i & 127] * p, (i >> 7) + bits);
+        const double w = __longlong_as_double(__double_as_longlong(s.exp2[i & 127] * p) + ((long long)((i >> 7) + bits) << 52));
+        return t > -128. * 70. ? w : 0.;
     }
     // Rounded to a whole number (below 2^52), by adding 2^52.
     __device__ __forceinline__ u64 whole(double w) const {
-        return (u64)__double_as_longlong(w + 0x1p52) - (u64)__double_as_longlong(0x1p52);
+        return (u64)__double_as_longlong(w + 0x1p52) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ u64 operator()(float x, const Shared& s) const { return whole(real(x, s)); }
 };
 
-template <typename V> __device__ __forceinline__ V wave_sum(V x) {
-    for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-    return x;
+// Sum over the wave: rows of 16 lanes by row-local exchanges, then four scalars.
+template <int CTRL> __device__ __forceinline__ u64 add_dpp64(u64 x) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)x, CTRL, 0xf, 0xf, true),
+                   hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(x >> 32), CTRL, 0xf, 0xf, true);
+    return x + ((u64)hi << 32 | lo);
+}
+__device__ __forceinline__ u64 wave_sum(u64 x) {
+    x = add_dpp64<0xb1>(x);
+    x = add_dpp64<0x4e>(x);
+    x = add_dpp64<0x141>(x);
+    x = add_dpp64<0x140>(x);
+    u64 t = 0;
+#pragma unroll
+    for (int l = 0; l < 64; l += 16)
+        t += (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), l) << 32 |
+             (unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, l);
+    return t;
 }
 
-// A row: NJ slabs in registers, or (NJ = 0) read where they are used. Tokens past the
-// row's end read as -inf.
-template <typename T, int NJ> struct RowData {
-    f32x4 x[NJ ? NJ : 1];
+// A row, read where it is used: a slab of kSlab tokens at a time, the next one on its way
+// (a row of 65536 fp32 is 256 KB, in L2 after the first pass; held in registers it made
+// every pass spill). A thread has four neighbouring tokens of a slab, from first(j) on. In
+// the last, partial slab that is at most V - 4, so that every read is of four tokens inside
+// the row; those that a neighbour has already, and whole reads past the end, count as -inf.
+// Rows of fewer than four tokens (ONE) are read one by one.
+template <typename T, bool ONE> struct RowData {
+    typedef T T4 __attribute__((ext_vector_type(4)));
     const T* p;
-    int V, slabs;
-    bool vec;
-    __device__ __forceinline__ f32x4 load(int j) const {
-        const int i = j * kSlab + 4 * threadIdx.x;
-        f32x4 v;
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        if (vec && i + 4 <= V) {
-            const T4 t = *reinterpret_cast<const T4*>(p + i);
+    int V, full, slabs;            // whole slabs, and all
+    __device__ __forceinline__ void init(const T* at, int n) {
+        p = at;
+        V = n;
+        full = V / kSlab;
+        slabs = (V + kSlab - 1) / kSlab;
+    }
+    __device__ __forceinline__ int first(int j) const {
+        const int i = j * kSlab + 4 * (int)threadIdx.x;
+        return ONE || i < V - 4 ? i : V - 4;
+    }
+    __device__ __forceinline__ T4 fetch(int i) const {
+        typedef T4 T4any __attribute__((aligned(sizeof(T))));
+        if constexpr (ONE) {
+            T4 t;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = (float)t[e];
+            for (int e = 0; e < 4; e++) t[e] = p[i + e < V ? i + e : V - 1];
+            return t;
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = i + e < V ? (float)p[i + e] : -INFINITY;
+            return *reinterpret_cast<const T4any*>(p + i);
         }
+    }
+    __device__ __forceinline__ f32x4 load(int j) const {
+        const int want = j * kSlab + 4 * (int)threadIdx.x, i = first(j);
+        const T4 t = fetch(i);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = i + e >= want && i + e < V ? (float)t[e] : -INFINITY;
         return v;
+    }
+    // f(slab, first index, four logits) for this thread's part of every slab.
+    template <typename F> __device__ __forceinline__ void each_slab(F f) const {
+        if (full) {
+            int i = 4 * (int)threadIdx.x;
+            T4 t = fetch(i);
+#pragma unroll 1
+            for (int j = 0; j < full; j++, i += kSlab) {
+                const T4 next = fetch(j + 1 < full ? i + kSlab : i);
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = (float)t[e];
+                f(j, i, v);
+                t = next;
+            }
+        }
+        if (full < slabs) f(full, first(full), load(full));
     }
     // f(index, logit) for every token of this thread.
     template <typename F> __device__ __forceinline__ void each(F f) const {
-        if constexpr (NJ > 0) {
+        each_slab([&](int, int i, f32x4 v) {
 #pragma unroll
-            for (int j = 0; j < NJ; j++) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) f(j * kSlab + 4 * (int)threadIdx.x + e, x[j][e]);
-                __builtin_amdgcn_sched_barrier(0);      // slabs at once would need registers for all
-            }
-        } else {
-            for (int j = 0; j < slabs; j++) {
-                const f32x4 v = load(j);
-#pragma unroll
-                for (int e = 0; e < 4; e++) f(j * kSlab + 4 * (int)threadIdx.x + e, v[e]);
-            }
-        }
-    }
-    template <typename F> __device__ __forceinline__ void each_slab(F f) const {
-        if constexpr (NJ > 0) {
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-                f(j, x[j]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        } else {
-            for (int j = 0; j < slabs; j++) f(j, load(j));
-        }
+            for (int e = 0; e < 4; e++) f(i + e, v[e]);
+        });
     }
 };
 
@@ -151,7 +180,7 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
 // The last used bin before which fewer than `limit` tokens lie (or, by sum, a weight of
 // at most `limit`), counting from (count, sum) above the first bin. -1: no bin is used.
 // Leaves the bin and what lies above it in s.
-__device__ void end_bin(bool by_sum, u64 limit, unsigned count, u64 sum, Shared& s) {
+__device__ __forceinline__ void end_bin(bool by_sum, u64 limit, unsigned count, u64 sum, Shared& s) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __syncthreads();
     const unsigned c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
@@ -166,7 +195,11 @@ __device__ void end_bin(bool by_sum, u64 limit, unsigned count, u64 sum, Shared&
     }
     if (lane == 63) s.wcount[wave] = c, s.wsum[wave] = t;
     __syncthreads();
-    for (int w = 0; w < wave; w++) c += s.wcount[w], t += s.wsum[w];
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) {
+        c += w < wave ? s.wcount[w] : 0;
+        t += w < wave ? s.wsum[w] : 0;
+    }
     c += count - (c0 + c1);            // above the first of this thread's two bins
     t += sum - (s0 + s1);
     const bool a0 = c0 && (by_sum ? t <= limit : c < limit);
@@ -191,14 +224,14 @@ struct Cut {
 
 // The first index at which the running total of val(i, x) over indices exceeds
 // point(total); -1 if there is none.
-template <typename D, typename F, typename G> __device__ int find_index(const D& row, Shared& s, F val, G point_of) {
+template <typename D, typename F, typename G> __device__ __forceinline__ int find_index(D& row, Shared& s, F val, G point_of) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __syncthreads();
     if (tid == 0) s.pick = s.bin = -1;
-    row.each_slab([&](int j, f32x4 x) {
+    row.each_slab([&](int j, int i, f32x4 x) {
         u64 t = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) t += val(j * kSlab + 4 * tid + e, x[e]);
+        for (int e = 0; e < 4; e++) t += val(i + e, x[e]);
         t = wave_sum(t);
         if (lane == 0) s.group[j][wave] = t;
     });
@@ -237,7 +270,7 @@ template <typename D, typename F, typename G> __device__ int find_index(const D&
     const u64 point = point_of(s.total);
     if (at >= 0 && wave == at % kWaves) {
         const f32x4 x = row.load(at / kWaves);
-        const int i = at / kWaves * kSlab + 4 * tid;
+        const int i = row.first(at / kWaves);
         u64 w[4], t = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) t += w[e] = val(i + e, x[e]);
@@ -263,7 +296,7 @@ template <typename D, typename F, typename G> __device__ int find_index(const D&
 // The cut of a prefix that ends among the tokens with keys [low, high], of which there
 // are many: by the bits of the keys, then by index.
 template <typename D>
-__device__ Cut cut_by_keys(const D& row, const Weights& w, unsigned low, unsigned high, bool by_sum, u64 limit,
+__device__ __forceinline__ Cut cut_by_keys(D& row, const Weights& w, unsigned low, unsigned high, bool by_sum, u64 limit,
                            unsigned count, u64 sum, Shared& s) {
     for (;;) {
         const unsigned span = high - low;         // bins of 2^shift keys, the first at `high`
@@ -290,36 +323,44 @@ __device__ Cut cut_by_keys(const D& row, const Weights& w, unsigned low, unsigne
     }
     const float x = key_logit(high);
     if (!by_sum) return {x, INT32_MAX};           // all that equal the k-th stay
-    const u64 one = w(x, s), n = one ? (limit - sum) / one + 1 : (u64)row.V;
+    const u64 one = w(x, s), room = limit - sum;
+    u64 n = row.V;                                // room / one + 1 of them stay
+    if (one && (double)room < (double)one * (double)row.V) {
+        n = (u64)((double)room / (double)one);
+        while (n * one > room) n--;
+        while (n * one <= room) n++;
+    }
     if (n >= (u64)row.V) return {x, INT32_MAX};
     const int end = find_index(row, s, [&](int, float y) -> u64 { return y == x; }, [&](u64) { return n; });
     return {x, end < 0 ? INT32_MAX : end};
 }
 
-// Sum over the listed tokens j of f(j), for the listed token of this thread's group of
-// kThreads / kList threads (0 for groups past the list); every thread of the group has it.
-constexpr int kPer = kThreads / kList;
-template <typename V, typename F> __device__ __forceinline__ V over_list(int n, F f) {
-    V t = 0;
-    for (int j = threadIdx.x % kPer; j < n; j += kPer) t += f(j);
-#pragma unroll
-    for (int o = 1; o < kPer; o <<= 1) t += __shfl_xor(t, o);
-    return t;
-}
+// The block's threads in groups of equal size, one group per listed token.
+struct ListView {
+    int n, per, me;                // listed tokens, threads a group, this group's token
+    __device__ __forceinline__ explicit ListView(int n_) : n(n_) {
+        per = n <= 64 ? 16 : n <= 128 ? 8 : 4;
+        me = (int)threadIdx.x / per;
+    }
+    __device__ __forceinline__ bool first() const { return me < n && (int)threadIdx.x % per == 0; }
+    // Sum over the listed tokens j of f(j), in every thread of the group.
+    template <typename V, typename F> __device__ __forceinline__ V sum(F f) const {
+        V t = 0;
+#pragma unroll 4
+        for (int j = (int)threadIdx.x % per; j < n; j += per) t += f(j);
+        for (int o = 1; o < per; o <<= 1) t += __shfl_xor(t, o);
+        return t;
+    }
+};
+static_assert(kThreads >= 4 * kList, "a group of threads for every listed token");
 
-template <typename T, int NJ> __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens, bool vec) {
+template <typename T, bool ONE>
+__global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens) {
     __shared__ Shared s;
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    RowData<T, NJ> row;
-    row.p = static_cast<const T*>(a.logits) + b * a.stride;
-    row.V = (int)a.V;
-    row.slabs = (row.V + kSlab - 1) / kSlab;
-    row.vec = vec;
-    if constexpr (NJ > 0) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) row.x[j] = row.load(j);
-    }
+    RowData<T, ONE> row;
+    row.init(static_cast<const T*>(a.logits) + b * a.stride, (int)a.V);
     const double temperature = a.temperature ? a.temperature[b] : a.temperature0;
     const double top_p = a.top_p ? a.top_p[b] : a.top_p0, min_p = a.min_p ? a.min_p[b] : a.min_p0;
     const int64_t top_k = a.top_k ? a.top_k[b] : a.top_k0;
@@ -368,8 +409,7 @@ template <typename T, int NJ> __global__ __launch_bounds__(kThreads) void k_samp
     w.bits = 62 - bits < 51 ? 62 - bits : 51;
     w.m = (double)m;
     w.step = fmin(128. / (0.69314718055994530942 * temperature), 1e300);
-    w.scale = ldexp(1., w.bits);
-    w.low = min_p * w.scale;
+    w.low = min_p * ldexp(1., w.bits);
     const float per = (float)fmin((double)kBins / ((double)kRange * temperature), 1e30);
     auto bin_of = [&](float x) { return (int)fminf((m - x) * per, 2.f * kBins); };     // kBins and up: weight 0
 
@@ -398,40 +438,42 @@ template <typename T, int NJ> __global__ __launch_bounds__(kThreads) void k_samp
         __syncthreads();
         if (all) {
             // the rest on the list alone: a group of threads per token
-            const int n = (int)s.listed, me = tid / kPer;
+            const ListView list((int)s.listed);
+            const int n = list.n, me = list.me;
             const float x = me < n ? s.lx[me] : 0.f;
             const int at = me < n ? s.li[me] : 0;
-            const unsigned rank = over_list<unsigned>(n, [&](int j) -> unsigned { return s.lx[j] > x; });
+            const unsigned rank = list.sum<unsigned>([&](int j) -> unsigned { return s.lx[j] > x; });
             u64 mine = me < n && rank < (u64)top_k ? w(x, s) : 0;
-            if (tid % kPer == 0 && me < n) s.lw[me] = mine;
+            if (list.first()) s.lw[me] = mine;
             __syncthreads();
-            const u64 total = over_list<u64>(n, [&](int j) { return s.lw[j]; });
+            const u64 total = list.sum<u64>([&](int j) { return s.lw[j]; });
             if (some_p) {
-                const u64 before = over_list<u64>(n, [&](int j) -> u64 {
+                const u64 before = list.sum<u64>([&](int j) -> u64 {
                     return s.lx[j] > x || (s.lx[j] == x && s.li[j] < at) ? s.lw[j] : 0;
                 });
                 if (before > (u64)(top_p * (double)total)) mine = 0;
             }
             if (mine && w.real(x, s) < w.low) mine = 0;
             __syncthreads();
-            if (tid % kPer == 0 && me < n) s.lw[me] = mine;
+            if (list.first()) s.lw[me] = mine;
             if (tid == 0) s.pick = -1;
             __syncthreads();
-            const u64 kept = over_list<u64>(n, [&](int j) { return s.lw[j]; });
-            const u64 before = over_list<u64>(n, [&](int j) -> u64 { return s.li[j] < at ? s.lw[j] : 0; });
+            const u64 kept = list.sum<u64>([&](int j) { return s.lw[j]; });
+            const u64 before = list.sum<u64>([&](int j) -> u64 { return s.li[j] < at ? s.lw[j] : 0; });
             const u64 point = point_of(kept);
-            if (tid % kPer == 0 && mine && before <= point && point < before + mine) s.pick = at;
+            if (list.first() && mine && before <= point && point < before + mine) s.pick = at;
             __syncthreads();
             if (s.pick < 0) return first_max();        // min-p leaves nothing
             if (tid == 0) tokens[b] = s.pick;
             return;
         } else if (in <= (unsigned)kList) {
-            const int n = (int)s.listed, me = tid / kPer;
+            const ListView list((int)s.listed);
+            const int n = list.n, me = list.me;
             const float x = me < n ? s.lx[me] : 0.f;
-            const unsigned rank = above + over_list<unsigned>(n, [&](int j) -> unsigned { return s.lx[j] > x; });
+            const unsigned rank = above + list.sum<unsigned>([&](int j) -> unsigned { return s.lx[j] > x; });
             // the smallest kept one: fewer than k above it, and k with its equals
-            const unsigned upto = rank + over_list<unsigned>(n, [&](int j) -> unsigned { return s.lx[j] == x; });
-            if (tid % kPer == 0 && me < n && rank < (u64)top_k && (upto >= (u64)top_k || upto == above + in)) s.wmax[0] = x;
+            const unsigned upto = rank + list.sum<unsigned>([&](int j) -> unsigned { return s.lx[j] == x; });
+            if (list.first() && rank < (u64)top_k && (upto >= (u64)top_k || upto == above + in)) s.wmax[0] = x;
             __syncthreads();
             cut.x = s.wmax[0];
         } else {
@@ -476,22 +518,23 @@ template <typename T, int NJ> __global__ __launch_bounds__(kThreads) void k_samp
         __syncthreads();
         if (in <= (unsigned)kList) {
             // in order, the last token before which the sum is within the limit
-            const int n = (int)s.listed, me = tid / kPer;
+            const ListView list((int)s.listed);
+            const int n = list.n, me = list.me;
             const float x = me < n ? s.lx[me] : 0.f;
             const int at = me < n ? s.li[me] : 0;
-            const u64 before = above + over_list<u64>(n, [&](int j) -> u64 {
+            const u64 before = above + list.sum<u64>([&](int j) -> u64 {
                 return s.lx[j] > x || (s.lx[j] == x && s.li[j] < at) ? s.lw[j] : 0;
             });
             const bool in_it = me < n && before <= limit;
-            const unsigned rank = over_list<unsigned>(n, [&](int j) -> unsigned {
+            const unsigned rank = list.sum<unsigned>([&](int j) -> unsigned {
                 return s.lx[j] > x || (s.lx[j] == x && s.li[j] < at);
             });
             __syncthreads();
             if (tid == 0) s.pick = -1;
             __syncthreads();
-            if (in_it && tid % kPer == 0) atomicMax(&s.pick, (int)rank);
+            if (in_it && list.first()) atomicMax(&s.pick, (int)rank);
             __syncthreads();
-            if (in_it && tid % kPer == 0 && (int)rank == s.pick) {
+            if (in_it && list.first() && (int)rank == s.pick) {
                 s.wmax[0] = x;
                 s.windex[0] = at + 1;
             }
@@ -512,15 +555,8 @@ template <typename T, int NJ> __global__ __launch_bounds__(kThreads) void k_samp
 }
 
 template <typename T> void sample_t(const SnHipSample& a, int* tokens, hipStream_t st) {
-    const bool vec = reinterpret_cast<uintptr_t>(a.logits) % (4 * sizeof(T)) == 0 && a.stride % 4 == 0;
-    const int slabs = (int)((a.V + kSlab - 1) / kSlab);
-    const unsigned B = (unsigned)a.B;
-    if (slabs <= 1) k_sample<T, 1><<<B, kThreads, 0, st>>>(a, tokens, vec);
-    else if (slabs <= 2) k_sample<T, 2><<<B, kThreads, 0, st>>>(a, tokens, vec);
-    else if (slabs <= 4) k_sample<T, 4><<<B, kThreads, 0, st>>>(a, tokens, vec);
-    else if (slabs <= 8) k_sample<T, 8><<<B, kThreads, 0, st>>>(a, tokens, vec);
-    else if (slabs <= kHeld) k_sample<T, kHeld><<<B, kThreads, 0, st>>>(a, tokens, vec);
-    else k_sample<T, 0><<<B, kThreads, 0, st>>>(a, tokens, vec);
+    if (a.V < 4) k_sample<T, true><<<(unsigned)a.B, kThreads, 0, st>>>(a, tokens);
+    else k_sample<T, false><<<(unsigned)a.B, kThreads, 0, st>>>(a, tokens);
 }
 
 }  // namespace
