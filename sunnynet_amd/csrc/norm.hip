@@ -17,7 +17,7 @@ namespace snhip {
 namespace {
 
 constexpr int kNormMaxD = 16384;
-constexpr int kNormBlocks = 1024;      // partial rows of the backward, at most
+constexpr int kNormBlocks = 256;       // partial rows of the backward, at most: a block a CU
 
 template <typename T> __device__ __forceinline__ void store8(T* dst, int n, bool vec, const float* x) {
     if (vec && n >= 8) {
@@ -108,24 +108,30 @@ __global__ __launch_bounds__(64 * norm_waves(WPR)) void k_norm_fwd(const T* x, c
     }
 }
 
+constexpr int kBwdWaves = 16;          // waves of a block of the backward
+
 template <typename T, int NV, int WPR>
-__global__ __launch_bounds__(64 * norm_waves(WPR)) void k_norm_bwd(const T* dy, const T* x, const float* w,
-                                                                   const float* mean, const float* rstd, T* dx,
-                                                                   float* part, int64_t R, int D, bool vec) {
-    constexpr int RPB = norm_waves(WPR) / WPR;
-    __shared__ float slot[4][norm_waves(WPR)];
-    __shared__ float acc[RPB > 1 ? RPB : 1][RPB > 1 ? NV * WPR * 512 : 1];
+__global__ __launch_bounds__(64 * kBwdWaves) void k_norm_bwd(const T* dy, const T* x, const float* w, const float* mean,
+                                                             const float* rstd, T* dx, float* part, int64_t R, int D,
+                                                             bool vec) {
+    constexpr int RPB = kBwdWaves / WPR;
+    __shared__ float slot[4][kBwdWaves];
+    __shared__ float acc[RPB][RPB > 1 ? NV * WPR * 512 : 1];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr bool hold = WPR <= 4;       // the weights too; wider rows have no registers left
     float ws[NV][8], aw[NV][8], ab[NV][8];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
+    auto weights = [&](int i) {
         const int c = ((i * WPR + wave % WPR) * 64 + lane) * 8;
         if (w) load8(w + c, D - c, vec, ws[i]);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            aw[i][j] = ab[i][j] = 0.f;
+        for (int j = 0; j < 8; j++)
             if (!w) ws[i][j] = 1.f;
-        }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        if (hold) weights(i);
+#pragma unroll
+        for (int j = 0; j < 8; j++) aw[i][j] = ab[i][j] = 0.f;
     }
     int odd = 0;
     for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < R; r0 += (int64_t)gridDim.x * RPB, odd ^= 2) {
@@ -142,6 +148,7 @@ __global__ __launch_bounds__(64 * norm_waves(WPR)) void k_norm_bwd(const T* dy, 
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = ((i * WPR + wave % WPR) * 64 + lane) * 8;
+            if (!hold) weights(i);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 h[i][j] = live && c + j < D ? (h[i][j] - mu) * rs : 0.f;
@@ -177,7 +184,7 @@ __global__ __launch_bounds__(64 * norm_waves(WPR)) void k_norm_bwd(const T* dy, 
                 for (int j = 0; j < 8; j++)
                     acc[wave / WPR][((i * WPR + wave % WPR) * 64 + lane) * 8 + j] = k ? ab[i][j] : aw[i][j];
             __syncthreads();
-            for (int c = threadIdx.x; c < D; c += 64 * norm_waves(WPR)) {
+            for (int c = threadIdx.x; c < D; c += 64 * kBwdWaves) {
                 float t = 0.f;
                 for (int i = 0; i < RPB; i++) t += acc[i][c];
                 out[c] = t;
@@ -200,6 +207,7 @@ __global__ __launch_bounds__(1024) void k_norm_sum(const float* part, float* dw,
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
     float t = 0.f;
     if (c < D)
+#pragma unroll 16
         for (int i = wave; i < n; i += 16) t += part[((int64_t)2 * i + blockIdx.y) * D + c];
     s[wave][lane] = t;
     __syncthreads();
@@ -225,7 +233,7 @@ int norm_wpr(int64_t D) { return D <= 1024 ? 1 : D <= 2048 ? 2 : D <= 4096 ? 4 :
 
 // Blocks of the backward, one partial row each.
 int64_t norm_blocks(int64_t R, int64_t D) {
-    const int64_t rpb = norm_waves(norm_wpr(D)) / norm_wpr(D), n = (R + rpb - 1) / rpb;
+    const int64_t rpb = kBwdWaves / norm_wpr(D), n = (R + rpb - 1) / rpb;
     return n < kNormBlocks ? n : kNormBlocks;
 }
 
@@ -252,7 +260,7 @@ snhip_status norm_bwd_t(const void* dy, const void* x, const float* w, const flo
     const bool sums = dw || db;
     return norm_shape(D, [&](auto nv, auto wpr) -> snhip_status {
         constexpr int NV = decltype(nv)::value, WPR = decltype(wpr)::value;
-        k_norm_bwd<T, NV, WPR><<<n, 64 * norm_waves(WPR), 0, st>>>(
+        k_norm_bwd<T, NV, WPR><<<n, 64 * kBwdWaves, 0, st>>>(
             (const T*)dy, (const T*)x, w, mean, rstd, (T*)dx, sums ? ws : nullptr, R, (int)D, vec);
         SNHIP_CHECK(hipGetLastError());
         if (sums) {
