@@ -3,8 +3,8 @@
 // Mathematics, per sequence and value head, in chunks of C = 32 tokens. With c the
 // running sum of g inside the chunk, G_i = exp(c_i), D_ij = exp(c_i - c_j) for j <= i
 // (0 above), S the state before the chunk and everything row by token:
-//   A_ij = beta_i D_ij k_i.k_j (j < i)      M = (I + A)^-1
-//   R = beta (V - G (K S))                   U = M R         (the writes)
+//   N_ij = D_ij k_i.k_j (j < i)              M = (I + N diag(beta))^-1
+//   X = V - G (K S)    E = M X (the errors)  U = beta E (the writes)
 //   P_ij = scale D_ij q_i.k_j (j <= i)       O = scale G (Q S) + P U
 //   S' = G_C S + K^T (L U)                   L_j = exp(c_C - c_j)
 // All exponents are differences of running sums, held in 64 bits: their difference
@@ -38,7 +38,7 @@ constexpr int64_t kDeltaStride = 1 << 24;
 struct DeltaP {
     SnHipDelta d;
     int64_t slots;          // chunk slots of all sequences
-    int KP, VP;             // K and V padded: state slabs are (VP, KP), k contiguous
+    int KP, VP;             // K and V padded: saved states are (KP, VP), errors (VP, 32)
     int rep;                // value heads per query and key head
     bool vec;               // every eight elements of a row of q or k are 16-byte aligned
 };
@@ -48,6 +48,15 @@ __host__ __device__ inline int64_t delta_slots(const SnHipDelta& d) {
 }
 __host__ __device__ inline int delta_kp(int64_t K) { return K <= 64 ? 64 : 128; }
 __host__ __device__ inline int delta_vp(int64_t V) { return (int)((V + 15) / 16 * 16); }
+
+// What the forward keeps for the backward, per slot and head: S (KP, VP) before the chunk,
+// and behind all of those E^T (VP, 32).
+__host__ __device__ inline float* delta_state(const DeltaP& a, int64_t slot, int h) {
+    return a.d.states + (slot * a.d.H + h) * (int64_t)(a.VP * a.KP);
+}
+__host__ __device__ inline float* delta_errors(const DeltaP& a, int64_t slot, int h) {
+    return a.d.states + a.slots * a.d.H * (int64_t)(a.VP * a.KP) + (slot * a.d.H + h) * (int64_t)(a.VP * kDC);
+}
 
 // A sequence: its first token as a row of the contiguous arrays, its batch entry and
 // first token there, its length, and the slot of its first chunk. With cu the slots of

@@ -6,7 +6,7 @@ namespace snhip {
 namespace {
 
 // M, P, G, L, beta of one chunk and value head: a block of four waves, one 16x16 tile
-// of the 32x32 matrices each. The inverse of the unit lower triangular I + A goes by
+// of the 32x32 matrices each. The inverse of the unit lower triangular I + A, A = N diag(beta), goes by
 // halves: its two diagonal 16x16 blocks by forward substitution, a column per lane,
 // then M10 = -M11 A10 M00.
 template <typename T, int KP, bool VEC>
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
     for (int r = 0; r < 4; r++) {
         const int row = ti * 16 + (lane >> 4) * 4 + r;
         const float D = col <= row ? expf((float)(sc[row] - sc[col])) : 0.f;
-        sA[row][col] = col < row ? sb[row] * D * kk[r] : 0.f;
+        sA[row][col] = col < row ? sb[col] * D * kk[r] : 0.f;
         sP[row][col] = col <= row ? (float)d.scale * D * qk[r] : 0.f;
     }
     if (tid < kDC) {
@@ -186,12 +186,15 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
         for (int i = 0; i < 8; i++) vc[i] = float_of_bits<T>(vv[i]);
         const bool more = t0 + kDC < s.len;
         if (more) fetch(t0 + kDC);
-        if (d.states) {       // S^T (VP, KP) before the chunk, for the backward
-            const __amdgpu_buffer_rsrc_t st = make_rsrc(
-                d.states + ((s.slot + t0 / kDC) * d.H + h) * (int64_t)(a.VP * KP), (uint32_t)(a.VP * KP * 4));
+        if (d.states) {       // S (KP, VP) before the chunk, for the backward
+            const __amdgpu_buffer_rsrc_t st = make_rsrc(delta_state(a, s.slot + t0 / kDC, h), (uint32_t)(a.VP * KP * 4));
+            const int at = v < a.VP ? (g8 * a.VP + v) * 4 : kNowhere;
 #pragma unroll
             for (int kt = 0; kt < NK; kt++)
-                buf_store4(st, (v * KP + g8) * 4 + ((kt >> 1) * 32 + 4 * (kt & 1)) * 4, S[kt]);
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[kt][r]), st, at,
+                                                          ((kt >> 1) * 32 + 4 * (kt & 1) + r) * a.VP * 4, 0);
         }
         f32x4 ks[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
@@ -217,18 +220,24 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
         }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            x[i] = be[i] * (vc[i] - G[i] * ks[i >> 2][i & 3]);
+            x[i] = vc[i] - G[i] * ks[i >> 2][i & 3];
             o[i >> 2][i & 3] *= (float)d.scale * G[i];
         }
-        const Frag<3> R = split8<3>(x);
+        const Frag<3> X = split8<3>(x);
+        f32x4 e[2];
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            const f32x4 u = mma<3>(MatM{sm[b]}.frag(pair_row(m, l16), 0, lane), R, f32x4{0, 0, 0, 0});
+            e[m] = mma<3>(MatM{sm[b]}.frag(pair_row(m, l16), 0, lane), X, f32x4{0, 0, 0, 0});
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                x[4 * m + r] = u[r];
-                y[4 * m + r] = u[r] * L[4 * m + r];
+                x[4 * m + r] = e[m][r] * be[4 * m + r];
+                y[4 * m + r] = x[4 * m + r] * L[4 * m + r];
             }
+        }
+        if (d.states) {
+            const __amdgpu_buffer_rsrc_t re = make_rsrc(delta_errors(a, s.slot + t0 / kDC, h), (uint32_t)(a.VP * kDC * 4));
+#pragma unroll
+            for (int m = 0; m < 2; m++) buf_store4(re, (v * kDC + g8 + 4 * m) * 4, e[m]);
         }
         const Frag<LO> U = split8<LO>(x);
         const Frag<3> LU = split8<3>(y);
@@ -398,7 +407,7 @@ int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d) {
     return d ? delta_slots(*d) * d->H * kDeltaChunk : 0;
 }
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d) {
-    return d ? delta_slots(*d) * d->H * delta_kp(d->K) * delta_vp(d->V) : 0;
+    return d ? delta_slots(*d) * d->H * delta_vp(d->V) * (kDC + (int64_t)delta_kp(d->K)) : 0;
 }
 
 snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send, void* stream) {

@@ -1,19 +1,19 @@
 // Gated delta rule, backward. With dS the gradient of the state after a chunk
 // (names of delta.h):
-//   dU = P^T dO + L (K dS)       dR = M^T dU        dV = beta dR
-//   dS before = G_C dS + scale Q^T (G dO) - K^T (beta G dR)
+//   dU = P^T dO + L (K dS)       W = M^T (beta dU) = dV
+//   dS before = G_C dS + scale Q^T (G dO) - K^T (G W)
 // is sequential over chunks, from the last to the first, and independent over the
-// columns of V (k_delta_rscan); it leaves dR and each chunk's dS. The rest is a sum
-// over V per chunk (k_delta_local), with X = V - G (K S), U = M (beta X):
-//   dP = dO U^T (j <= i)         Z = dR U^T (j < i; dA = -Z)
-//   dQ = scale G (dO S^T) + Y K,            Y_ij = scale D_ij dP_ij
-//   dK = L (U dS^T) - beta G (dR S^T) + Y^T Q + (F + F^T) K,  F_ij = -beta_i D_ij Z_ij
-//   dbeta_i = dR_i.X_i - sum_j Z_ij D_ij k_i.k_j
-// and, with E = Y (q.k) + F (k.k) elementwise below the diagonal (on it a decay of 1
+// columns of V (k_delta_rscan); it leaves W, each chunk's dS, and its columns' part of
+// E_i.dU_i. The rest is a sum over V per chunk (k_delta_local):
+//   Y_ij = scale D_ij beta_j dO_i.E_j (j <= i)   Z_ij = W_i.E_j, F_ij = -D_ij beta_j Z_ij (j < i)
+//   dQ = scale G (dO S^T) + Y K
+//   dK = L beta (E dS^T) - G (W S^T) + Y^T Q + (F + F^T) K
+//   dbeta_j = E_j.dU_j - sum over i > j of Z_ij D_ij k_i.k_j
+// and, with H = Y (q.k) + F (k.k) elementwise below the diagonal (on it a decay of 1
 // has no gradient: its two shares are left out, not cancelled),
-//   dg_t = sum over i >= t of [ sum_j E_ij - sum_j E_ji
-//                               + scale G q_i.(dO S^T)_i - beta G k_i.(dR S^T)_i ]
-//          + sum over i < t of L k_i.(U dS^T)_i + G_C <S, dS>.
+//   dg_t = sum over i >= t of [ sum_j H_ij - sum_j H_ji
+//                               + scale G q_i.(dO S^T)_i - G k_i.(W S^T)_i ]
+//          + sum over i < t of L beta k_i.(E dS^T)_i + G_C <S, dS>.
 #include "delta.h"
 
 namespace snhip {
@@ -22,14 +22,16 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a);
 
 namespace {
 
-// Per slot and head: dR^T (VP, 32), then dS^T (VP, KP) after the chunk.
+// Per slot and head: W^T (VP, 32), dS (KP, VP) after the chunk, and (VP / 16, 32) sums of
+// E dU over 16 columns.
 struct DeltaWs {
-    float* dr;
+    float* w;
     float* ds;
+    float* eu;
 };
 __host__ __device__ inline DeltaWs delta_ws(const DeltaP& a, float* ws, int64_t slot, int h) {
-    const int64_t i = slot * a.d.H + h, nr = a.slots * a.d.H * kDC * a.VP;
-    return {ws + i * kDC * a.VP, ws + nr + i * (int64_t)(a.VP * a.KP)};
+    const int64_t i = slot * a.d.H + h, n = a.slots * a.d.H, w = kDC * a.VP, ds = (int64_t)a.VP * a.KP;
+    return {ws + i * w, ws + n * w + i * ds, ws + n * (w + ds) + i * (a.VP / 16 * kDC)};
 }
 
 template <typename T, int KP, bool VEC>
@@ -61,6 +63,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
     MatFetch<3, NTH> fm, fp;
     float fv[(3 * kDC + NTH - 1) / NTH];
     unsigned vv[8];
+    f32x4 ev[2];
     fk.init(d.k_stride[1], Kd, tid);
     fq.init(d.q_stride[1], Kd, tid);
     const int E = (int)sizeof(T), o_step = (int)d.H * V * E, o_off = v < V ? g8 * o_step + v * E : kNowhere;
@@ -76,6 +79,9 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
         const __amdgpu_buffer_rsrc_t ro = rows_window(dop + t0 * d.H * V, d.H * V, n, V);
 #pragma unroll
         for (int i = 0; i < 8; i++) vv[i] = buf_load_bits<T>(ro, o_off + i * o_step);
+        const __amdgpu_buffer_rsrc_t re = make_rsrc(delta_errors(a, s.slot + t0 / kDC, h), (uint32_t)(a.VP * kDC * 4));
+#pragma unroll
+        for (int m = 0; m < 2; m++) ev[m] = buf_load4(re, (v * kDC + g8 + 4 * m) * 4);
     };
     auto store = [&](int b) {
         fk.store(Rows{sk[b]}, tid);
@@ -96,16 +102,22 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
         const Rows K{sk[b]}, Q{sq[b]};
         const Mat M{sm[b]}, PM{sp[b]};
         const DeltaWs w = delta_ws(a, gr.ws, s.slot + t0 / kDC, h);
-        float G[8], L[8], be[8], x[8], y[8];
-        float od[8];
+        const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
+        float G[8], L[8], be[8], x[8], y[8], od[8];
+        const f32x4 e[2] = {ev[0], ev[1]};
 #pragma unroll
         for (int i = 0; i < 8; i++) od[i] = float_of_bits<T>(vv[i]);
         if (t0 > 0) fetch(t0 - kDC);
         const __amdgpu_buffer_rsrc_t rds = make_rsrc(w.ds, (uint32_t)(a.VP * KP * 4)),
-                                     rdr = make_rsrc(w.dr, (uint32_t)(a.VP * kDC * 4));
+                                     rw = make_rsrc(w.w, (uint32_t)(a.VP * kDC * 4)),
+                                     reu = make_rsrc(w.eu, (uint32_t)(a.VP / 16 * kDC * 4));
+        const int at = v < a.VP ? (g8 * a.VP + v) * 4 : kNowhere;
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
-            buf_store4(rds, (v * KP + g8) * 4 + ((kt >> 1) * 32 + 4 * (kt & 1)) * 4, S[kt]);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[kt][r]), rds, at,
+                                                      ((kt >> 1) * 32 + 4 * (kt & 1) + r) * a.VP * 4, 0);
         f32x4 du[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
         for (int p = 0; p < KP / 32; p++) {
@@ -133,23 +145,32 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
             for (int r = 0; r < 4; r++) du[m][r] *= L[4 * m + r];
             du[m] = mma<3>(PM.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dO, du[m]);
 #pragma unroll
-            for (int r = 0; r < 4; r++) x[4 * m + r] = du[m][r];
+            for (int r = 0; r < 4; r++) {
+                x[4 * m + r] = du[m][r] * be[4 * m + r];
+                const float eu = sum16(e[m][r] * du[m][r]);
+                buf_store<float>(reu, l16 == 0 ? ((v >> 4) * kDC + g8 + 4 * m + r) * 4 : kNowhere, eu);
+            }
         }
-        const Frag<3> dU = split8<3>(x);
+        const Frag<3> dE = split8<3>(x);
+        const __amdgpu_buffer_rsrc_t rdv =
+            rows_window(static_cast<T*>(gr.dv) + ((s.row + t0) * d.H + h) * (int64_t)V, d.H * (int64_t)V, n, V);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            const f32x4 dr = mma<3>(M.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dU, f32x4{0, 0, 0, 0});
-            buf_store4(rdr, (v * kDC + g8 + 4 * m) * 4, dr);
+            const f32x4 wv = mma<3>(M.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dE, f32x4{0, 0, 0, 0});
+            buf_store4(rw, (v * kDC + g8 + 4 * m) * 4, wv);
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[4 * m + r] = -dr[r] * be[4 * m + r] * G[4 * m + r];
+            for (int r = 0; r < 4; r++) {
+                buf_store<T>(rdv, o_off + (4 * m + r) * o_step, (T)wv[r]);
+                y[4 * m + r] = -wv[r] * G[4 * m + r];
+            }
         }
-        const Frag<3> BdR = split8<3>(y);
+        const Frag<3> GW = split8<3>(y);
         const float decay = sv[b][kDC - 1];
 #pragma unroll
         for (int kt = 0; kt < NK; kt++) {
             const int block = (kt >> 1) * 32 + 8 * (lane & 3) + 4 * (kt & 1);
             S[kt] = mma<3>(Q.tfrag(0, block, lane), GdO, S[kt] * decay);
-            S[kt] = mma<3>(K.tfrag(0, block, lane), BdR, S[kt]);
+            S[kt] = mma<3>(K.tfrag(0, block, lane), GW, S[kt]);
         }
         if (t0 > 0) store(b ^ 1);
         barrier_lds();
@@ -169,21 +190,22 @@ __device__ __forceinline__ float sum_groups(float x) {
     return x + __shfl_xor(x, 32);
 }
 
-// One chunk of one query and key head: a block of four waves runs over the value heads
-// that share it, so dq and dk are summed in registers. Per head and 64 columns of V a
-// wave first owns 16 columns (X, U, dV), then KP / 4 columns of K (the products with S
-// and dS); the 32x32 matrices are made by three waves, a 16x16 tile each. U and dR lie
-// in LDS by column of V, as the waves hold them, and are read transposed.
+// One chunk of one query and key head: a block of KP / 16 waves runs over the value heads
+// that share it, so dq and dk are summed in registers. Per head and 64 columns of V, E, W
+// and dO go through LDS (E and W by column, as the scans leave them, read transposed), and
+// a wave owns 16 columns of K in the products with S and dS; the 32x32 matrices are
+// made by three waves, a 16x16 tile each. What the next step reads is fetched into
+// registers a step ahead. Bound by the bytes of S and dS.
 template <typename T, int KP, bool VEC>
-__global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
-    constexpr int P = ElemPlanes<T>::n, VT = 64, NC = KP / 64;     // NC tiles of 16 columns of K a wave
+__global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
+    constexpr int P = ElemPlanes<T>::n, VT = 64, NW = KP / 16, NTH = 64 * NW;
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, VT, kDC> Cols;
     typedef Tile<3, kDC, kDC> Mat;
-    __shared__ alignas(16) __bf16 sk[Rows::elems], sq[Rows::elems], su[Cols::elems], sr[Cols::elems],
-        so[Tile<P, kDC, VT>::elems], sx[2 * Mat::elems];
-    __shared__ alignas(16) float sv[3 * kDC];
-    __shared__ float red[4][kDC], kread[4][kDC], kwrite[4][kDC], trow[3][16], tzk[3][16], tcol[3][16], dots[4];
+    static_assert(Cols::elems >= Mat::elems, "Y and F take the places of E and W");
+    __shared__ alignas(16) __bf16 sk[Rows::elems], sq[Rows::elems], se[Cols::elems], sw[Cols::elems],
+        so[Tile<P, kDC, VT>::elems];
+    __shared__ float sv[3 * kDC], seu[kDC], kread[NW][kDC], kwrite[NW][kDC], trow[3][16], tcol[3][16], tzk[3][16], dots[NW];
     __shared__ double sc[kDC];
     const SnHipDelta& d = a.d;
     const int hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4, g8 = 2 * g4,
@@ -194,37 +216,53 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
     const int64_t t0 = (int64_t)chunk * kDC;
     const int n = (int)(s.len - t0 < kDC ? s.len - t0 : kDC), V = (int)d.V, Kd = (int)d.K;
     const Rows K{sk}, Q{sq};
-    const Cols UT{su}, RT{sr};
+    const Cols ET{se}, WT{sw};
     const Tile<P, kDC, VT> DO{so};
-    const Mat M{sx}, Y{sx}, FF{sx + Mat::elems};        // Y takes M's place
-    RowsFetch<T, KP, 256, VEC> f;
-    f.init(d.k_stride[1], Kd, tid);
-    f.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, hk), d.k_stride[1], n, Kd, tid);
-    f.store(K, tid);
-    f.init(d.q_stride[1], Kd, tid);
-    f.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, hk), d.q_stride[1], n, Kd, tid);
-    f.store(Q, tid);
-    f32x4 dq[NC][2], dk[NC][2];
+    const Mat Y{se}, FF{sw};
+    RowsFetch<T, KP, NTH, VEC> fk, fq;
+    fk.init(d.k_stride[1], Kd, tid);
+    fq.init(d.q_stride[1], Kd, tid);
+    fk.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, hk), d.k_stride[1], n, Kd, tid);
+    fq.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, hk), d.q_stride[1], n, Kd, tid);
+
+    // Fetches ahead. Tiles: 64 columns of V of E^T, then of W^T (four vectors of eight tokens
+    // a column), and dO (eight vectors a token).
+    constexpr int NEW = 512 / NTH;
+    Vec8<float> pe[NEW];
+    Vec8<T> po;
+    const int o_step = (int)d.H * V;
+    auto fetch_tiles = [&](int h, int vt) {
+        const uint32_t bytes = (uint32_t)(a.VP * kDC * 4);
+        const __amdgpu_buffer_rsrc_t re = make_rsrc(delta_errors(a, blockIdx.x, h), bytes),
+                                     rw = make_rsrc(delta_ws(a, gr.ws, blockIdx.x, h).w, bytes);
 #pragma unroll
-    for (int j = 0; j < NC; j++)
-#pragma unroll
-        for (int m = 0; m < 2; m++) dq[j][m] = dk[j][m] = f32x4{0, 0, 0, 0};
+        for (int j = 0; j < NEW; j++) {
+            const int u = tid + j * NTH;
+            pe[j] = buf_load8<float>(u < 256 ? re : rw, (vt * kDC + (u & 255) * 8) * 4, 8, true);
+        }
+        const int c = vt + (tid & 7) * 8;
+        const T* op = static_cast<const T*>(gr.dout) + ((s.row + t0) * d.H + h) * (int64_t)V;
+        po = buf_load8<T>(rows_window(op, o_step, n, V),
+                          c < V && tid < 256 ? ((tid >> 3) * o_step + c) * (int)sizeof(T) : kNowhere, V - c, vec_o);
+    };
+    // States: 32 columns of V from `v0` on of S and dS, the rows of K of this wave.
+    const int kc = wave * 16;
+    Vec8<float> ps, pd;
+    auto fetch_states = [&](int h, int v0) {
+        const int at = v0 + g8 < a.VP ? ((kc + l16) * a.VP + v0 + g8) * 4 : kNowhere;
+        ps = buf_load8<float>(make_rsrc(delta_state(a, blockIdx.x, h), (uint32_t)(a.VP * KP * 4)), at, 8, true);
+        pd = buf_load8<float>(make_rsrc(delta_ws(a, gr.ws, blockIdx.x, h).ds, (uint32_t)(a.VP * KP * 4)), at, 8, true);
+    };
+    fetch_tiles(hk * a.rep, 0);
+    fetch_states(hk * a.rep, 0);
+    fk.store(K, tid);
+    fq.store(Q, tid);
+    f32x4 dq[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, dk[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     const int ti = wave == 0 ? 0 : 1, tj = wave == 2 ? 1 : 0;     // waves 0..2: tiles (0,0), (1,0), (1,1)
 
-    for (int h = hk * a.rep; h < (hk + 1) * a.rep; h++) {
-        const float* rec = d.chunks + ((int64_t)blockIdx.x * d.H + h) * kDeltaChunk;
-        const float* st = d.states + ((int64_t)blockIdx.x * d.H + h) * (int64_t)(a.VP * KP);
-        const DeltaWs w = delta_ws(a, gr.ws, blockIdx.x, h);
-        const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t0, h);
-        const int64_t at0 = ((s.row + t0) * d.H + h) * (int64_t)V;
-        __syncthreads();
-        {
-            MatFetch<3, 256> fm;
-            fm.load(make_rsrc(rec, kDeltaChunk * 4), 0, tid);
-            fm.store(M, tid);
-        }
-        if (tid < 3 * kDC) sv[tid] = rec[kDeltaG + tid];
-        if (wave == 3) {
+    for (int h = hk * a.rep, end = h + a.rep; h < end; h++) {
+        if (tid < 3 * kDC) sv[tid] = d.chunks[((int64_t)blockIdx.x * d.H + h) * kDeltaChunk + kDeltaG + tid];
+        if (wave == 3) {        // decays, and the parts of E dU
             const int64_t at = (s.row + t0 + lane) * d.H + h;
             double c = lane < n ? (double)delta_decay(d.g[at]) : 0.0;
 #pragma unroll
@@ -232,94 +270,49 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
                 const double y = __shfl_up(c, o, kDC);
                 if ((lane & 31) >= o) c += y;
             }
-            if (lane < kDC) sc[lane] = c;
+            if (lane < kDC) {
+                sc[lane] = c;
+                const float* eu = delta_ws(a, gr.ws, blockIdx.x, h).eu;
+                float t = 0.f;
+                for (int i = 0; i < a.VP / 16; i++) t += eu[i * kDC + lane];
+                seu[lane] = t;
+            }
         }
-        __syncthreads();
-        float G[8], be[8];
+        f32x4 dp = {0, 0, 0, 0}, z = {0, 0, 0, 0}, q1[2], k1[2], k2[2];
 #pragma unroll
-        for (int i = 0; i < 8; i++) G[i] = sv[g8 + i], be[i] = sv[2 * kDC + g8 + i];
-        f32x4 dp = {0, 0, 0, 0}, z = {0, 0, 0, 0}, q1[NC][2], k1[NC][2], k2[NC][2];
-#pragma unroll
-        for (int j = 0; j < NC; j++)
-#pragma unroll
-            for (int m = 0; m < 2; m++) q1[j][m] = k1[j][m] = k2[j][m] = f32x4{0, 0, 0, 0};
-        float bsum[8] = {0, 0, 0, 0, 0, 0, 0, 0}, ss = 0.f;
+        for (int m = 0; m < 2; m++) q1[m] = k1[m] = k2[m] = f32x4{0, 0, 0, 0};
+        float ss = 0.f;
         for (int vt = 0; vt < a.VP; vt += VT) {
-            const int vl = wave * 16 + l16, v = vt + vl;
-            {
-                const int t = tid >> 3, c = (tid & 7) * 8;
-                const T* op = static_cast<const T*>(gr.dout) + at0 + (int64_t)t * d.H * V + vt + c;
-                DO.put8(t, c, split_raw8<T>(load_raw8(op, t < n ? V - vt - c : 0, vec_o)));
+#pragma unroll
+            for (int j = 0; j < NEW; j++) {
+                const int u = tid + j * NTH, r = (u & 255) >> 2, c = (u & 3) * 8;
+                (u < 256 ? ET : WT).put8(r, c, split_raw8<float>(pe[j]));
             }
-            float x[8], dr[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = dr[i] = 0.f;
-            if (vt + wave * 16 < a.VP) {
-                f32x4 ks[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-                float vv[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) vv[i] = g8 + i < n && v < V ? (float)vp[(g8 + i) * d.v_stride[1] + v] : 0.f;
-                const Vec8<float> rv = load_raw8(w.dr + (int64_t)v * kDC + g8, 8, true);
-#pragma unroll
-                for (int p = 0; p < KP / 32; p++) {
-                    const Frag<3> b = split_raw8<float>(load_raw8(st + (int64_t)v * KP + 32 * p + g8, 8, true));
-#pragma unroll
-                    for (int m = 0; m < 2; m++) ks[m] = mma<3>(K.frag(pair_row(m, l16), 32 * p, lane), b, ks[m]);
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float xx = vv[i] - G[i] * ks[i >> 2][i & 3];
-                    dr[i] = rv[i];
-                    if (g8 + i < n && v < V)
-                        static_cast<T*>(gr.dv)[at0 + (int64_t)(g8 + i) * d.H * V + v] = (T)(be[i] * dr[i]);
-                    bsum[i] = fmaf(dr[i], xx, bsum[i]);
-                    x[i] = be[i] * xx;
-                }
-                const Frag<3> R = split8<3>(x);
-#pragma unroll
-                for (int m = 0; m < 2; m++) {
-                    const f32x4 u = mma<3>(M.frag(pair_row(m, l16), 0, lane), R, f32x4{0, 0, 0, 0});
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x[4 * m + r] = u[r];
-                }
-            }
-            UT.put8(vl, g8, x);
-            RT.put8(vl, g8, dr);
-            __syncthreads();
+            if (tid < 256) DO.put8(tid >> 3, (tid & 7) * 8, split_raw8<T>(po));
+            barrier_lds();
+            if (vt + VT < a.VP) fetch_tiles(h, vt + VT);
+            else if (h + 1 < end) fetch_tiles(h + 1, 0);
             const int nv = a.VP - vt < VT ? (a.VP - vt + 31) & ~31 : VT;       // whole 32s
             if (wave < 3)
                 for (int i = 0; i < nv; i += 32) {
-                    const Frag<3> b = UT.tfrag(i, 16 * tj + blk16, lane);
+                    const Frag<3> b = ET.tfrag(i, 16 * tj + blk16, lane);
                     dp = mma<3>(DO.frag(16 * ti + l16, i, lane), b, dp);
-                    z = mma<3>(RT.tfrag(i, 16 * ti + blk16, lane), b, z);
+                    z = mma<3>(WT.tfrag(i, 16 * ti + blk16, lane), b, z);
                 }
             for (int i = 0; i < nv; i += 32) {
 #pragma unroll
-                for (int j = 0; j < NC; j++) {
-                    const int kc = (wave * NC + j) * 16 + l16;
-                    float sx8[8], dx8[8];
+                for (int l = 0; l < 8; l++) ss = fmaf(ps[l], pd[l], ss);
+                const Frag<3> b = split_raw8<float>(ps), e = split_raw8<float>(pd);
+                if (vt + i + 32 < a.VP) fetch_states(h, vt + i + 32);
+                else if (h + 1 < end) fetch_states(h + 1, 0);
 #pragma unroll
-                    for (int l = 0; l < 8; l++) {
-                        const int vv = vt + i + g8 + l;
-                        sx8[l] = vv < a.VP ? st[(int64_t)vv * KP + kc] : 0.f;
-                        dx8[l] = vv < a.VP ? w.ds[(int64_t)vv * KP + kc] : 0.f;
-                        ss = fmaf(sx8[l], dx8[l], ss);
-                    }
-                    const Frag<3> b = split8<3>(sx8), e = split8<3>(dx8);
-#pragma unroll
-                    for (int m = 0; m < 2; m++) {
-                        q1[j][m] = mma<3>(DO.frag(pair_row(m, l16), i, lane), b, q1[j][m]);
-                        k1[j][m] = mma<3>(RT.tfrag(i, blkp + 4 * m, lane), b, k1[j][m]);
-                        k2[j][m] = mma<3>(UT.tfrag(i, blkp + 4 * m, lane), e, k2[j][m]);
-                    }
+                for (int m = 0; m < 2; m++) {
+                    q1[m] = mma<3>(DO.frag(pair_row(m, l16), i, lane), b, q1[m]);
+                    k1[m] = mma<3>(WT.tfrag(i, blkp + 4 * m, lane), b, k1[m]);
+                    k2[m] = mma<3>(ET.tfrag(i, blkp + 4 * m, lane), e, k2[m]);
                 }
             }
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float b = sum16(bsum[i]);
-            if (l16 == 0) red[wave][g8 + i] = b;
+            barrier_lds();
         }
         ss = sum_groups(sum16(ss));
         if (lane == 0) dots[wave] = ss;
@@ -332,19 +325,18 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
                 qk = mma<3>(Q.frag(16 * ti + l16, c, lane), b, qk);
             }
             const int col = tj * 16 + l16;
-            float esum = 0.f;
+            const float bj = sv[2 * kDC + col];
+            float hsum = 0.f, zsum = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int row = 16 * ti + g4 + r;
                 const float D = col <= row ? expf((float)(sc[row] - sc[col])) : 0.f;
-                const float zd = col < row ? D * z[r] : 0.f, ff = -sv[2 * kDC + row] * zd;
-                const float y = (float)d.scale * D * dp[r], e = col < row ? y * qk[r] + ff * kk[r] : 0.f;
-                const float er = sum16(e), zr = sum16(zd * kk[r]);
-                if (l16 == 0) {
-                    trow[wave][g4 + r] = er;
-                    tzk[wave][g4 + r] = zr;
-                }
-                esum += e;
+                const float zd = col < row ? D * z[r] : 0.f, ff = -bj * zd;
+                const float y = (float)d.scale * D * bj * dp[r], e = col < row ? y * qk[r] + ff * kk[r] : 0.f;
+                const float er = sum16(e);
+                if (l16 == 0) trow[wave][g4 + r] = er;
+                hsum += e;
+                zsum = fmaf(zd, kk[r], zsum);
                 z[r] = ff;
                 Y.put(row, col, y);
                 if (ti != tj) {
@@ -352,8 +344,12 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
                     FF.put(col, row, ff);
                 }
             }
-            esum = sum_groups(esum);
-            if (lane < 16) tcol[wave][lane] = esum;
+            hsum = sum_groups(hsum);
+            zsum = sum_groups(zsum);
+            if (lane < 16) {
+                tcol[wave][lane] = hsum;
+                tzk[wave][lane] = zsum;
+            }
             if (ti == tj) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
@@ -367,56 +363,43 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
                     FF.put(16 * ti + g4 + r, col, z[r] + t);
                 }
             }
-        } else {
+        } else if (wave == 3) {
 #pragma unroll
             for (int r = 0; r < 4; r++) Y.put(g4 + r, 16 + l16, 0.f);
         }
-        __syncthreads();
-        float cr[8], cw[8];
+        barrier_lds();
+        const Frag<P> bk = K.tfrag(0, kc + blk16, lane), bq = Q.tfrag(0, kc + blk16, lane);
 #pragma unroll
-        for (int i = 0; i < 8; i++) cr[i] = cw[i] = 0.f;
+        for (int m = 0; m < 2; m++) {
 #pragma unroll
-        for (int j = 0; j < NC; j++) {
-            const int kc = (wave * NC + j) * 16;
-            const Frag<P> bk = K.tfrag(0, kc + blk16, lane), bq = Q.tfrag(0, kc + blk16, lane);
-#pragma unroll
-            for (int m = 0; m < 2; m++) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int i = 4 * m + r, t = g8 + i;
-                    const float qv = Q.get(t, kc + l16), kv = K.get(t, kc + l16);
-                    q1[j][m][r] *= (float)d.scale * G[i];
-                    k1[j][m][r] *= -be[i] * G[i];
-                    k2[j][m][r] *= sv[kDC + t];
-                    cr[i] = fmaf(qv, q1[j][m][r], fmaf(kv, k1[j][m][r], cr[i]));
-                    cw[i] = fmaf(kv, k2[j][m][r], cw[i]);
+            for (int r = 0; r < 4; r++) {
+                const int t = g8 + 4 * m + r;
+                const float qv = Q.get(t, kc + l16), kv = K.get(t, kc + l16), G = sv[t];
+                q1[m][r] *= (float)d.scale * G;
+                k1[m][r] *= -G;
+                k2[m][r] *= sv[kDC + t] * sv[2 * kDC + t];
+                const float cr = sum16(fmaf(qv, q1[m][r], kv * k1[m][r])), cw = sum16(kv * k2[m][r]);
+                if (l16 == 0) {
+                    kread[wave][t] = cr;
+                    kwrite[wave][t] = cw;
                 }
-                dq[j][m] += mma<3>(Y.frag(pair_row(m, l16), 0, lane), bk, q1[j][m]);
-                f32x4 t = mma<3>(Y.tfrag(0, blkp + 4 * m, lane), bq, k1[j][m] + k2[j][m]);
-                dk[j][m] += mma<3>(FF.frag(pair_row(m, l16), 0, lane), bk, t);
             }
+            dq[m] += mma<3>(Y.frag(pair_row(m, l16), 0, lane), bk, q1[m]);
+            const f32x4 t = mma<3>(Y.tfrag(0, blkp + 4 * m, lane), bq, k1[m] + k2[m]);
+            dk[m] += mma<3>(FF.frag(pair_row(m, l16), 0, lane), bk, t);
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float r = sum16(cr[i]), wr = sum16(cw[i]);
-            if (l16 == 0) {
-                kread[wave][g8 + i] = r;
-                kwrite[wave][g8 + i] = wr;
-            }
-        }
-        __syncthreads();
+        barrier_lds();
         if (tid < kDC) {
-            // dg_t: reads and E by later tokens, less E's columns there, and the writes of
+            // dg_t: reads and H by later tokens, less H's columns there, and the writes of
             // earlier ones (a write's share in dc_C less its own dc is left of its token)
             const int t = tid, hi = t >> 4, lo = t & 15;
             float dc = hi ? trow[1][lo] + trow[2][lo] - tcol[2][lo] : trow[0][lo] - tcol[0][lo] - tcol[1][lo];
-            float db = hi ? -tzk[1][lo] - tzk[2][lo] : -tzk[0][lo];
+            const float db = seu[t] - (hi ? tzk[2][lo] : tzk[0][lo] + tzk[1][lo]);
             float wr = 0.f, all = 0.f;
-            for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < NW; i++) {
                 dc += kread[i][t];
                 wr += kwrite[i][t];
                 all += dots[i];
-                db += red[i][t];
             }
 #pragma unroll
             for (int o = 1; o < kDC; o <<= 1) {
@@ -431,18 +414,15 @@ __global__ __launch_bounds__(256, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad
                 gr.dbeta[(s.row + t0 + t) * d.H + h] = db;
             }
         }
+        barrier_lds();        // sv, sc and the sums are the next head's
     }
+    if (kc + l16 >= Kd) return;
 #pragma unroll
-    for (int j = 0; j < NC; j++) {
-        const int kc = (wave * NC + j) * 16 + l16;
-        if (kc >= Kd) continue;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int64_t at = ((s.row + t0 + g8 + i) * d.Hk + hk) * (int64_t)Kd + kc;
-            if (g8 + i < n) {
-                static_cast<T*>(gr.dq)[at] = (T)dq[j][i >> 2][i & 3];
-                static_cast<T*>(gr.dk)[at] = (T)dk[j][i >> 2][i & 3];
-            }
+    for (int i = 0; i < 8; i++) {
+        const int64_t at = ((s.row + t0 + g8 + i) * d.Hk + hk) * (int64_t)Kd + kc + l16;
+        if (g8 + i < n) {
+            static_cast<T*>(gr.dq)[at] = (T)dq[i >> 2][i & 3];
+            static_cast<T*>(gr.dk)[at] = (T)dk[i >> 2][i & 3];
         }
     }
 }
@@ -453,7 +433,7 @@ snhip_status bwd_t(const DeltaP& a, const SnHipDeltaGrad& gr, hipStream_t st) {
     k_delta_rscan<T, KP, VEC><<<grid, 64 * kDeltaW, 0, st>>>(a, gr);
     SNHIP_CHECK(hipGetLastError());
     const bool vec_o = a.d.V % 8 == 0 && reinterpret_cast<uintptr_t>(gr.dout) % 16 == 0;
-    k_delta_local<T, KP, VEC><<<dim3((unsigned)a.slots, (unsigned)a.d.Hk), 256, 0, st>>>(a, gr, vec_o);
+    k_delta_local<T, KP, VEC><<<dim3((unsigned)a.slots, (unsigned)a.d.Hk), 4 * KP, 0, st>>>(a, gr, vec_o);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
@@ -466,7 +446,7 @@ using namespace snhip;
 extern "C" {
 
 int64_t snhip_op_delta_bwd_floats(const SnHipDelta* d) {
-    return d ? delta_slots(*d) * d->H * delta_vp(d->V) * (kDC + (int64_t)delta_kp(d->K)) : 0;
+    return d ? delta_slots(*d) * d->H * delta_vp(d->V) * (kDC + (int64_t)delta_kp(d->K) + kDC / 16) : 0;
 }
 
 snhip_status snhip_op_delta_bwd_dev(const SnHipDelta* d, const SnHipDeltaGrad* gr, void* stream) {

@@ -127,6 +127,6 @@ def test_workspace_sizes():
     assert size[0] == size[1] and size[2] == 2 * size[1]
     # packed sequences: a chunk more for each of them at most
     assert L.snhip_op_delta_chunk_floats(_delta(cu=P, dims=(1, 100, 7, Hk, H, K, V))) == (100 // 32 + 7) * size[0] // B
-    assert L.snhip_op_delta_state_floats(_delta(dims=(1, 32, 1, 1, 1, 65, 17))) == 128 * 32
+    assert L.snhip_op_delta_state_floats(_delta(dims=(1, 32, 1, 1, 1, 65, 17))) == (128 + 32) * 32
     assert L.snhip_op_norm_bwd_floats(0, 8) == 0 and L.snhip_op_norm_bwd_floats(1, 8) == 2 * 8
     assert L.snhip_op_norm_bwd_floats(10 ** 6, 8) == L.snhip_op_norm_bwd_floats(10 ** 7, 8) > 0
