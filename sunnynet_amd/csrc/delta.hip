@@ -203,11 +203,10 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
 #pragma unroll
             for (int r = 0; r < 4; r++) x[r] = S[2 * p][r], x[4 + r] = S[2 * p + 1][r];
             const Frag<3> f = split8<3>(x);
-#pragma unroll
-            for (int m = 0; m < 2; m++) {
-                ks[m] = mma<3>(K.frag(pair_row(m, l16), 32 * p, lane), f, ks[m]);
-                o[m] = mma<LO>(Q.frag(pair_row(m, l16), 32 * p, lane), f, o[m]);
-            }
+            const Frag<P> kf[2] = {K.frag(pair_row(0, l16), 32 * p, lane), K.frag(pair_row(1, l16), 32 * p, lane)},
+                          qf[2] = {Q.frag(pair_row(0, l16), 32 * p, lane), Q.frag(pair_row(1, l16), 32 * p, lane)};
+            mma_n<3>(kf, f, ks);
+            mma_n<LO>(qf, f, o);
         }
         float G[8], L[8], be[8], x[8], y[8];
 #pragma unroll
@@ -224,10 +223,12 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             o[i >> 2][i & 3] *= (float)d.scale * G[i];
         }
         const Frag<3> X = split8<3>(x);
-        f32x4 e[2];
+        const MatM M{sm[b]};
+        const Frag<3> mf[2] = {M.frag(pair_row(0, l16), 0, lane), M.frag(pair_row(1, l16), 0, lane)};
+        f32x4 e[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        mma_n<3>(mf, X, e);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            e[m] = mma<3>(MatM{sm[b]}.frag(pair_row(m, l16), 0, lane), X, f32x4{0, 0, 0, 0});
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 x[4 * m + r] = e[m][r] * be[4 * m + r];
@@ -243,8 +244,18 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
         const Frag<3> LU = split8<3>(y);
         const float decay = sv[b][kDC - 1];
 #pragma unroll
-        for (int kt = 0; kt < NK; kt++)
-            S[kt] = mma<3>(K.tfrag(0, (kt >> 1) * 32 + 8 * (lane & 3) + 4 * (kt & 1), lane), LU, S[kt] * decay);
+        for (int k4 = 0; k4 < NK; k4 += 4) {
+            Frag<P> kf[4];
+            f32x4 t[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                kf[i] = K.tfrag(0, ((k4 + i) >> 1) * 32 + 8 * (lane & 3) + 4 * (i & 1), lane);
+                t[i] = S[k4 + i] * decay;
+            }
+            mma_n<3>(kf, LU, t);
+#pragma unroll
+            for (int i = 0; i < 4; i++) S[k4 + i] = t[i];
+        }
         const __amdgpu_buffer_rsrc_t ro =
             rows_window(out + ((s.row + t0) * d.H + h) * (int64_t)V, d.H * (int64_t)V, n, V);
 #pragma unroll

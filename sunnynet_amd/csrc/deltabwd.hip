@@ -124,8 +124,8 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
 #pragma unroll
             for (int r = 0; r < 4; r++) x[r] = S[2 * p][r], x[4 + r] = S[2 * p + 1][r];
             const Frag<3> f = split8<3>(x);
-#pragma unroll
-            for (int m = 0; m < 2; m++) du[m] = mma<3>(K.frag(pair_row(m, l16), 32 * p, lane), f, du[m]);
+            const Frag<P> kf[2] = {K.frag(pair_row(0, l16), 32 * p, lane), K.frag(pair_row(1, l16), 32 * p, lane)};
+            mma_n<3>(kf, f, du);
         }
 #pragma unroll
         for (int i = 0; i < 8; i += 4) {
@@ -140,10 +140,11 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
         for (int i = 0; i < 8; i++) y[i] = od[i] * ((float)d.scale * G[i]);
         const Frag<3> GdO = split8<3>(y);
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
+        for (int i = 0; i < 8; i++) du[i >> 2][i & 3] *= L[i];
+        const Frag<3> pf[2] = {PM.tfrag(0, 8 * (lane & 3), lane), PM.tfrag(0, 8 * (lane & 3) + 4, lane)};
+        mma_n<3>(pf, dO, du);
 #pragma unroll
-            for (int r = 0; r < 4; r++) du[m][r] *= L[4 * m + r];
-            du[m] = mma<3>(PM.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dO, du[m]);
+        for (int m = 0; m < 2; m++) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 x[4 * m + r] = du[m][r] * be[4 * m + r];
@@ -154,9 +155,12 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
         const Frag<3> dE = split8<3>(x);
         const __amdgpu_buffer_rsrc_t rdv =
             rows_window(static_cast<T*>(gr.dv) + ((s.row + t0) * d.H + h) * (int64_t)V, d.H * (int64_t)V, n, V);
+        const Frag<3> mf[2] = {M.tfrag(0, 8 * (lane & 3), lane), M.tfrag(0, 8 * (lane & 3) + 4, lane)};
+        f32x4 wm[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        mma_n<3>(mf, dE, wm);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            const f32x4 wv = mma<3>(M.tfrag(0, 8 * (lane & 3) + 4 * m, lane), dE, f32x4{0, 0, 0, 0});
+            const f32x4 wv = wm[m];
             buf_store4(rw, (v * kDC + g8 + 4 * m) * 4, wv);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
@@ -167,10 +171,20 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
         const Frag<3> GW = split8<3>(y);
         const float decay = sv[b][kDC - 1];
 #pragma unroll
-        for (int kt = 0; kt < NK; kt++) {
-            const int block = (kt >> 1) * 32 + 8 * (lane & 3) + 4 * (kt & 1);
-            S[kt] = mma<3>(Q.tfrag(0, block, lane), GdO, S[kt] * decay);
-            S[kt] = mma<3>(K.tfrag(0, block, lane), GW, S[kt]);
+        for (int k4 = 0; k4 < NK; k4 += 4) {
+            Frag<P> kf[4], qf[4];
+            f32x4 t[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int block = ((k4 + i) >> 1) * 32 + 8 * (lane & 3) + 4 * (i & 1);
+                qf[i] = Q.tfrag(0, block, lane);
+                kf[i] = K.tfrag(0, block, lane);
+                t[i] = S[k4 + i] * decay;
+            }
+            mma_n<3>(qf, GdO, t);
+            mma_n<3>(kf, GW, t);
+#pragma unroll
+            for (int i = 0; i < 4; i++) S[k4 + i] = t[i];
         }
         if (t0 > 0) store(b ^ 1);
         barrier_lds();
@@ -193,19 +207,19 @@ __device__ __forceinline__ float sum_groups(float x) {
 // One chunk of one query and key head: a block of KP / 16 waves runs over the value heads
 // that share it, so dq and dk are summed in registers. Per head and 64 columns of V, E, W
 // and dO go through LDS (E and W by column, as the scans leave them, read transposed), and
-// a wave owns 16 columns of K in the products with S and dS; the 32x32 matrices are
-// made by three waves, a 16x16 tile each. What the next step reads is fetched into
+// a wave owns 16 columns of K in the products with S and dS; the 32x32 matrices Y and F
+// are six tasks of a 16x16 tile each. What the next step reads is fetched into
 // registers a step ahead. Bound by the bytes of S and dS.
 template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
-    constexpr int P = ElemPlanes<T>::n, VT = 64, NW = KP / 16, NTH = 64 * NW;
+    constexpr int P = ElemPlanes<T>::n, VT = 64, NW = KP / 16, NTH = 64 * NW, NT = 6 / NW + 1;
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, VT, kDC> Cols;
     typedef Tile<3, kDC, kDC> Mat;
     static_assert(Cols::elems >= Mat::elems, "Y and F take the places of E and W");
     __shared__ alignas(16) __bf16 sk[Rows::elems], sq[Rows::elems], se[Cols::elems], sw[Cols::elems],
         so[Tile<P, kDC, VT>::elems];
-    __shared__ float sv[3 * kDC], seu[kDC], kread[NW][kDC], kwrite[NW][kDC], trow[3][16], tcol[3][16], tzk[3][16], dots[NW];
+    __shared__ float sv[3 * kDC], seu[kDC], kread[NW][kDC], kwrite[NW][kDC], trow[6][16], tcol[6][16], tzk[3][16], dots[NW];
     __shared__ double sc[kDC];
     const SnHipDelta& d = a.d;
     const int hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4, g8 = 2 * g4,
@@ -258,7 +272,6 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
     fk.store(K, tid);
     fq.store(Q, tid);
     f32x4 dq[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, dk[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    const int ti = wave == 0 ? 0 : 1, tj = wave == 2 ? 1 : 0;     // waves 0..2: tiles (0,0), (1,0), (1,1)
 
     for (int h = hk * a.rep, end = h + a.rep; h < end; h++) {
         if (tid < 3 * kDC) sv[tid] = d.chunks[((int64_t)blockIdx.x * d.H + h) * kDeltaChunk + kDeltaG + tid];
@@ -278,7 +291,9 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
                 seu[lane] = t;
             }
         }
-        f32x4 dp = {0, 0, 0, 0}, z = {0, 0, 0, 0}, q1[2], k1[2], k2[2];
+        f32x4 small[NT], q1[2], k1[2], k2[2];
+#pragma unroll
+        for (int j = 0; j < NT; j++) small[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int m = 0; m < 2; m++) q1[m] = k1[m] = k2[m] = f32x4{0, 0, 0, 0};
         float ss = 0.f;
@@ -293,12 +308,16 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
             if (vt + VT < a.VP) fetch_tiles(h, vt + VT);
             else if (h + 1 < end) fetch_tiles(h + 1, 0);
             const int nv = a.VP - vt < VT ? (a.VP - vt + 31) & ~31 : VT;       // whole 32s
-            if (wave < 3)
-                for (int i = 0; i < nv; i += 32) {
-                    const Frag<3> b = ET.tfrag(i, 16 * tj + blk16, lane);
-                    dp = mma<3>(DO.frag(16 * ti + l16, i, lane), b, dp);
-                    z = mma<3>(WT.tfrag(i, 16 * ti + blk16, lane), b, z);
-                }
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const int task = wave + j * NW, ti = task % 3 ? 1 : 0, tj = task % 3 == 2 ? 1 : 0;
+                if (task < 6)
+                    for (int i = 0; i < nv; i += 32) {
+                        const Frag<3> b = ET.tfrag(i, 16 * tj + blk16, lane);
+                        small[j] = task < 3 ? mma<3>(DO.frag(16 * ti + l16, i, lane), b, small[j])
+                                            : mma<3>(WT.tfrag(i, 16 * ti + blk16, lane), b, small[j]);
+                    }
+            }
             for (int i = 0; i < nv; i += 32) {
 #pragma unroll
                 for (int l = 0; l < 8; l++) ss = fmaf(ps[l], pd[l], ss);
@@ -316,54 +335,63 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
         }
         ss = sum_groups(sum16(ss));
         if (lane == 0) dots[wave] = ss;
-        if (wave < 3) {
-            f32x4 kk = {0, 0, 0, 0}, qk = {0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < KP; c += 32) {
-                const Frag<P> b = K.frag(16 * tj + l16, c, lane);
-                kk = mma<3>(K.frag(16 * ti + l16, c, lane), b, kk);
-                qk = mma<3>(Q.frag(16 * ti + l16, c, lane), b, qk);
-            }
+        for (int j = 0; j < NT; j++) {
+            // tiles (0,0), (1,0), (1,1) of Y with its part of H, then of F with its part
+            const int task = wave + j * NW, ti = task % 3 ? 1 : 0, tj = task % 3 == 2 ? 1 : 0;
+            if (task >= 6) break;
+            const Rows A{task < 3 ? sq : sk};
+            f32x4 qk = {0, 0, 0, 0};       // q.k, or k.k
+#pragma unroll
+            for (int c = 0; c < KP; c += 32)
+                qk = mma<3>(A.frag(16 * ti + l16, c, lane), K.frag(16 * tj + l16, c, lane), qk);
             const int col = tj * 16 + l16;
             const float bj = sv[2 * kDC + col];
-            float hsum = 0.f, zsum = 0.f;
+            float hsum = 0.f, zsum = 0.f, f[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int row = 16 * ti + g4 + r;
                 const float D = col <= row ? expf((float)(sc[row] - sc[col])) : 0.f;
-                const float zd = col < row ? D * z[r] : 0.f, ff = -bj * zd;
-                const float y = (float)d.scale * D * bj * dp[r], e = col < row ? y * qk[r] + ff * kk[r] : 0.f;
-                const float er = sum16(e);
-                if (l16 == 0) trow[wave][g4 + r] = er;
-                hsum += e;
-                zsum = fmaf(zd, kk[r], zsum);
-                z[r] = ff;
-                Y.put(row, col, y);
-                if (ti != tj) {
-                    FF.put(row, col, ff);
-                    FF.put(col, row, ff);
+                float e;
+                if (task < 3) {
+                    const float y = (float)d.scale * D * bj * small[j][r];
+                    e = col < row ? y * qk[r] : 0.f;
+                    Y.put(row, col, y);
+                } else {
+                    const float zd = col < row ? D * small[j][r] : 0.f;
+                    f[r] = -bj * zd;
+                    e = f[r] * qk[r];
+                    zsum = fmaf(zd, qk[r], zsum);
+                    if (ti != tj) {
+                        FF.put(row, col, f[r]);
+                        FF.put(col, row, f[r]);
+                    }
                 }
+                const float er = sum16(e);
+                if (l16 == 0) trow[task][g4 + r] = er;
+                hsum += e;
             }
             hsum = sum_groups(hsum);
-            zsum = sum_groups(zsum);
-            if (lane < 16) {
-                tcol[wave][lane] = hsum;
-                tzk[wave][lane] = zsum;
-            }
-            if (ti == tj) {
+            if (lane < 16) tcol[task][lane] = hsum;
+            if (task >= 3) {
+                zsum = sum_groups(zsum);
+                if (lane < 16) tzk[task - 3][lane] = zsum;
+                if (ti == tj) {
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    // F_ji of this lane's (i, j): row j of column i, in lane 16 (j / 4) + i
-                    float t = 0.f;
+                    for (int r = 0; r < 4; r++) {
+                        // F_ji of this lane's (i, j): row j of column i, in lane 16 (j / 4) + i
+                        float t = 0.f;
 #pragma unroll
-                    for (int rr = 0; rr < 4; rr++) {
-                        const float x = __shfl(z[rr], (l16 >> 2) * 16 + g4 + r);
-                        if ((l16 & 3) == rr) t = x;
+                        for (int rr = 0; rr < 4; rr++) {
+                            const float x = __shfl(f[rr], (l16 >> 2) * 16 + g4 + r);
+                            if ((l16 & 3) == rr) t = x;
+                        }
+                        FF.put(16 * ti + g4 + r, col, f[r] + t);
                     }
-                    FF.put(16 * ti + g4 + r, col, z[r] + t);
                 }
             }
-        } else if (wave == 3) {
+        }
+        if (wave == 3) {
 #pragma unroll
             for (int r = 0; r < 4; r++) Y.put(g4 + r, 16 + l16, 0.f);
         }
@@ -393,7 +421,10 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
             // dg_t: reads and H by later tokens, less H's columns there, and the writes of
             // earlier ones (a write's share in dc_C less its own dc is left of its token)
             const int t = tid, hi = t >> 4, lo = t & 15;
-            float dc = hi ? trow[1][lo] + trow[2][lo] - tcol[2][lo] : trow[0][lo] - tcol[0][lo] - tcol[1][lo];
+            float dc = 0.f;
+            for (int i = 0; i < 6; i += 3)       // Y's part, F's part
+                dc += hi ? trow[i + 1][lo] + trow[i + 2][lo] - tcol[i + 2][lo]
+                         : trow[i][lo] - tcol[i][lo] - tcol[i + 1][lo];
             const float db = seu[t] - (hi ? tzk[2][lo] : tzk[0][lo] + tzk[1][lo]);
             float wr = 0.f, all = 0.f;
             for (int i = 0; i < NW; i++) {

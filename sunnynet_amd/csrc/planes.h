@@ -71,6 +71,22 @@ __device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4
     return acc;
 }
 
+// The same for N left operands at once: neighbouring products are independent, so none
+// waits for the one before it.
+template <int LIM, int N, int NA, int NB>
+__device__ __forceinline__ void mma_n(const Frag<NA> (&a)[N], const Frag<NB>& b, f32x4 (&acc)[N]) {
+#pragma unroll
+    for (int s = LIM - 1; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < NA; i++) {
+            const int j = s - i;
+            if (j >= 0 && j < NB)
+#pragma unroll
+                for (int n = 0; n < N; n++)
+                    acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n].p[i], b.p[j], acc[n], 0, 0, 0);
+        }
+}
+
 __device__ __forceinline__ int pair_row(int m, int i) { return 8 * (i >> 2) + 4 * m + (i & 3); }
 
 // A tile of P planes of R rows and C columns in LDS. Rows are padded by 16 bytes, which
