@@ -188,23 +188,14 @@ def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-class on_device:
-    """Makes a tensor's device the current one for a launch, as the library's
-    operators expect; nothing if it is already."""
-
-    def __init__(self, device):
-        self.at = device.index
-        self.was = -1
-
-    def __enter__(self):
-        now = torch.cuda.current_device()
-        if now != self.at:
-            self.was = now
-            torch.cuda.set_device(self.at)
-
-    def __exit__(self, *exc):
-        if self.was >= 0:
-            torch.cuda.set_device(self.was)
+def on_device(device, call, *args) -> int:
+    """call(*args, stream) on torch's current stream of `device`, with that device the
+    current one, as the library's operators expect."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device.index:
+        return call(*args, stream)
+    with torch.cuda.device(device):
+        return call(*args, stream)
 
 
 def ptr(t) -> int:

@@ -24,7 +24,7 @@ from .. import _native
 __all__ = ["GatedDelta", "delta_bwd", "delta_fwd", "delta_step", "gated_delta"]
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-MAX_K, MAX_V, MAX_HEADS = 128, 4096, 65535
+MAX_K, MAX_V, MAX_HEADS, MAX_STRIDE = 128, 4096, 65535, 1 << 24
 STEP_TOKENS = 16               # at most this many tokens run token by token
 _ARGS = struct.Struct("7P9q8qd2P")     # SnHipDelta
 _GRAD = struct.Struct("9P")            # SnHipDeltaGrad
@@ -47,6 +47,8 @@ def _shapes(q, k, v, g, beta, s0, cu):
     if not 1 <= K <= MAX_K or not 1 <= V <= MAX_V or H > MAX_HEADS:
         raise ValueError(f"head sizes up to K = {MAX_K}, V = {MAX_V} and up to {MAX_HEADS} heads: "
                          f"got K = {K}, V = {V}, {H} heads")
+    if H * max(K, V) >= MAX_STRIDE:
+        raise ValueError(f"H * K and H * V must be below {MAX_STRIDE}")
     if B * T >= 1 << 31:
         raise ValueError("B * T must be below 2^31")
     if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
@@ -76,8 +78,10 @@ def _check_state(s, shape, name):
 
 
 def _rows(t):
-    """t with its last axis contiguous (others may have any stride)."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t with its last axis contiguous; the others may have any stride below MAX_STRIDE."""
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 4 or t.stride(1) < MAX_STRIDE):
+        return t
+    return t.contiguous()
 
 
 def _pack(q, k, v, g, beta, s0, cu, dims, scale, chunks=None, states=None):
@@ -110,9 +114,9 @@ def delta_fwd(q, k, v, g, beta, s0=None, *, scale=None, cu_seqlens=None, keep=Fa
         chunks = torch.empty(L.snhip_op_delta_chunk_floats(sizes), device=q.device)
         if keep:
             states = torch.empty(L.snhip_op_delta_state_floats(sizes), device=q.device)
-    with _native.on_device(q.device):
-        rc = L.snhip_op_delta_fwd_dev(_pack(q, k, v, g, beta, s0, cu_seqlens, dims, scale, chunks, states),
-                                      out.data_ptr(), send.data_ptr(), _native.stream_handle(q.device))
+    rc = _native.on_device(q.device, L.snhip_op_delta_fwd_dev,
+                           _pack(q, k, v, g, beta, s0, cu_seqlens, dims, scale, chunks, states), out.data_ptr(),
+                           send.data_ptr())
     _native.check(rc, "snhip_op_delta_fwd_dev")
     return out, send, (chunks, states) if keep else None
 
@@ -147,8 +151,7 @@ def delta_bwd(q, k, v, g, beta, s0, saved, dout, dsend=None, *, scale=None, cu_s
     ws = torch.empty(L.snhip_op_delta_bwd_floats(args), device=q.device)
     grads = _GRAD.pack(dout.data_ptr(), _ptr(dsend), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
                        db.data_ptr(), _ptr(ds0), ws.data_ptr())
-    with _native.on_device(q.device):
-        rc = L.snhip_op_delta_bwd_dev(args, grads, _native.stream_handle(q.device))
+    rc = _native.on_device(q.device, L.snhip_op_delta_bwd_dev, args, grads)
     _native.check(rc, "snhip_op_delta_bwd_dev")
     return dq, dk, dv, dg, db, ds0
 
@@ -184,7 +187,11 @@ class GatedDelta(torch.autograd.Function):
 def gated_delta(q, k, v, g, beta, s0=None, *, scale=None, cu_seqlens=None):
     """(out, send) of the gated delta rule under autograd (shapes: delta_fwd). Without
     a gradient to keep anything for, calls of up to 16 tokens run token by token."""
-    return GatedDelta.apply(q, k, v, g, beta, s0, scale, cu_seqlens)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, s0)):
+        return GatedDelta.apply(q, k, v, g, beta, s0, scale, cu_seqlens)
+    if s0 is not None:
+        s0 = s0.contiguous()
+    return delta_fwd(q, k, v, g, beta, s0, scale=scale, cu_seqlens=cu_seqlens)[:2]
 
 
 def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
@@ -206,8 +213,7 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
     if B == 0:
         return out
     scale = K ** -0.5 if scale is None else float(scale)
-    with _native.on_device(q.device):
-        rc = _native.lib().snhip_op_delta_step_dev(_pack(q, k, v, g, beta, s, None, dims, scale), out.data_ptr(),
-                                                   send.data_ptr(), _native.stream_handle(q.device))
+    rc = _native.on_device(q.device, _native.lib().snhip_op_delta_step_dev,
+                           _pack(q, k, v, g, beta, s, None, dims, scale), out.data_ptr(), send.data_ptr())
     _native.check(rc, "snhip_op_delta_step_dev")
     return out

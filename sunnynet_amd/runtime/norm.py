@@ -38,10 +38,8 @@ def norm_fwd(x, weight=None, bias=None, eps=1e-5, *, keep=False):
     y = torch.empty_like(x)
     mean, rstd = (torch.empty(R, device=x.device) for _ in range(2)) if keep else (None, None)
     if R:
-        with _native.on_device(x.device):
-            rc = _native.lib().snhip_op_norm_fwd_dev(x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(),
-                                                     _ptr(mean), _ptr(rstd), R, D, eps, DTYPES[x.dtype],
-                                                     _native.stream_handle(x.device))
+        rc = _native.on_device(x.device, _native.lib().snhip_op_norm_fwd_dev, x.data_ptr(), _ptr(weight), _ptr(bias),
+                               y.data_ptr(), _ptr(mean), _ptr(rstd), R, D, eps, DTYPES[x.dtype])
         _native.check(rc, "snhip_op_norm_fwd_dev")
     return y, mean, rstd
 
@@ -61,10 +59,9 @@ def norm_bwd(dy, x, weight, mean, rstd, *, need=(True, True, True)):
     dw, db = (new(D, device=x.device) if n else None for n in need[1:])
     if R and any(need):
         ws = torch.empty(L.snhip_op_norm_bwd_floats(R, D), device=x.device) if need[1] or need[2] else None
-        with _native.on_device(x.device):
-            rc = L.snhip_op_norm_bwd_dev(dy.data_ptr(), x.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(),
-                                         _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), R, D, DTYPES[x.dtype],
-                                         _native.stream_handle(x.device))
+        rc = _native.on_device(x.device, L.snhip_op_norm_bwd_dev, dy.data_ptr(), x.data_ptr(), _ptr(weight),
+                               mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), R, D,
+                               DTYPES[x.dtype])
         _native.check(rc, "snhip_op_norm_bwd_dev")
     return dx, dw, db
 
@@ -91,4 +88,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis, under
     autograd: x (..., D) float32, bfloat16 or float16, weight and bias (D) float32 or
     None. Statistics and sums are float32."""
-    return LayerNorm.apply(x, weight, bias, float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return LayerNorm.apply(x, weight, bias, float(eps))
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    return norm_fwd(x.contiguous(), weight, bias, float(eps))[0]

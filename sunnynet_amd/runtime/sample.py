@@ -65,7 +65,6 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     m, m0 = _setting(min_p, "min_p", B, dev, f64)
     args = _ARGS.pack(logits.data_ptr(), u.data_ptr(), *(0 if x is None else x.data_ptr() for x in (t, k, p, m)),
                       float(t0), float(p0), float(m0), int(k0), B, V, logits.stride(0), DTYPES[logits.dtype])
-    with _native.on_device(dev):
-        rc = _native.lib().snhip_op_sample_dev(args, tokens.data_ptr(), _native.stream_handle(dev))
+    rc = _native.on_device(dev, _native.lib().snhip_op_sample_dev, args, tokens.data_ptr())
     _native.check(rc, "snhip_op_sample_dev")
     return tokens

@@ -18,7 +18,8 @@ while it is prefilling, as ``sn_prefill`` steps through a prompt,
 ``sunnynet.c:347-349``, else its last generated token), all active requests
 step together as sequences ``[0, n)`` of the batched step, and the logits of
 requests past their prompt give their next token (greedy, or the reference's
-``sample_logits`` sampling, ``serve.py:29-56``). Requests join in free slots
+``sample_logits`` sampling, ``serve.py:29-56``, run on the device from each
+request's own random numbers: the logits stay there). Requests join in free slots
 (their state zeroed) and leave when they reach ``max_tokens`` or an end token;
 the last active request then moves into the freed slot, so the active
 sequences stay ``[0, n)``. Requests are independent: each one's tokens are the
@@ -32,14 +33,17 @@ import numpy as np
 import torch
 
 from .model import HipModel
+from .sample import MAX_V, sample_tokens
 
 __all__ = ["HipEngine", "HipState", "HipRwkvEngine", "HipRwkvState", "BatchScheduler", "Request",
            "sample_logits"]
 
 
-def sample_logits(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None) -> int:
+def sample_logits(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None, min_p=0.0) -> int:
     """Next token from logits (V,): argmax at temperature <= 0, else softmax
-    sampling after top-k and top-p (nucleus) filtering (serve.py:29-56)."""
+    sampling after top-k and top-p (nucleus) filtering (serve.py:29-56), then
+    of the tokens at least ``min_p`` times as probable as the best one. Draws
+    one number from ``rng``."""
     if temperature is None or temperature <= 0:
         return int(np.argmax(logits))
     z = np.asarray(logits, dtype=np.float64) / float(temperature)
@@ -58,6 +62,8 @@ def sample_logits(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None) -> int:
         z[order] = np.where(cut, -np.inf, srt)
     z = z - z.max()
     p = np.exp(z)
+    if min_p and min_p > 0:
+        p[p < min_p] = 0.0
     total = p.sum()
     if not np.isfinite(total) or total <= 0:
         return int(np.argmax(logits))
@@ -204,12 +210,23 @@ class Request:
     temperature: float = 0.0
     top_p: float = 1.0
     top_k: int = 0
+    min_p: float = 0.0
     eos: int | None = None
     seed: int | None = None
     output: list = field(default_factory=list)
     done: bool = False
     pos: int = 0                       # prompt tokens consumed
     rng: object = None
+
+    @property
+    def greedy(self) -> bool:
+        return self.temperature is None or self.temperature <= 0
+
+    @property
+    def on_device(self) -> bool:
+        """Whether the device sampler knows the request's settings (it does unless
+        top_k is negative)."""
+        return self.greedy or not self.top_k or self.top_k > 0
 
     def next_input(self) -> int:
         return int(self.prompt[self.pos]) if self.pos < len(self.prompt) else int(self.output[-1])
@@ -224,6 +241,8 @@ class BatchScheduler:
         self.waiting: list[Request] = []
         self.finished: list[Request] = []
         self.steps = 0
+        self._rows = None                  # the requests whose settings the device holds
+        self._settings = None
 
     def submit(self, prompt, max_tokens: int, **kw) -> Request:
         if len(prompt) == 0:
@@ -266,6 +285,24 @@ class BatchScheduler:
             self.finished.append(self.active[i])
         self.active = [self.active[i] for i in keep]
 
+    def _sample(self, logits, wanted):
+        """The next tokens on the device: sample_logits' rules, with one number
+        from each sampling request's own generator, as it draws them."""
+        dev = logits.device
+        if self._rows is None or len(self._rows) != len(self.active) \
+                or any(a is not b for a, b in zip(self._rows, self.active)):
+            # the settings go over only when the active requests change
+            cols = [[0.0 if r.greedy else float(r.temperature) for r in self.active],
+                    [float(r.top_p) for r in self.active], [float(r.min_p or 0.0) for r in self.active]]
+            self._settings = (torch.tensor(cols, dtype=torch.float64, device=dev),
+                              torch.tensor([min(int(r.top_k or 0), 1 << 30) for r in self.active],
+                                           dtype=torch.int32, device=dev))
+            self._rows = list(self.active)
+        u = torch.tensor([r.rng.random() if w and not r.greedy else 0.0 for r, w in zip(self.active, wanted)],
+                         dtype=torch.float64, device=dev)
+        (temperature, top_p, min_p), top_k = self._settings
+        return sample_tokens(logits, u, temperature, top_k, top_p, min_p).cpu().numpy()
+
     def step(self) -> int:
         """One iteration over every active request; returns how many stepped."""
         self._admit()
@@ -276,16 +313,22 @@ class BatchScheduler:
         toks = torch.tensor([r.next_input() for r in self.active], dtype=torch.int32, device=dev)
         logits = self.model.step_batch(toks)
         self.steps += 1
-        greedy = all(r.temperature is None or r.temperature <= 0 for r in self.active)
-        picks = logits.argmax(1).cpu().numpy() if greedy else None
-        host = None if greedy else logits.float().cpu().numpy()
+        wanted = [r.pos >= len(r.prompt) - 1 for r in self.active]     # past the prompt after this step
+        picks = host = None
+        if all(r.greedy for r in self.active):
+            picks = logits.argmax(1).cpu().numpy()
+        elif logits.is_cuda and logits.shape[1] <= MAX_V and all(r.on_device for r in self.active):
+            picks = self._sample(logits, wanted)
+        else:
+            host = logits.float().cpu().numpy()
         gone = []
         for i, r in enumerate(self.active):
             if r.pos < len(r.prompt):
                 r.pos += 1
                 if r.pos < len(r.prompt):
                     continue                   # still prefilling: logits unused
-            t = int(picks[i]) if greedy else sample_logits(host[i], r.temperature, r.top_p, r.top_k, r.rng)
+            t = int(picks[i]) if host is None else sample_logits(host[i], r.temperature, r.top_p, r.top_k, r.rng,
+                                                                 r.min_p)
             r.output.append(t)
             if len(r.output) >= r.max_tokens or (r.eos is not None and t == r.eos):
                 gone.append(i)

@@ -1,0 +1,123 @@
+"""The three operators together, as a pre-normed recurrent language model of one block
+uses them: trained (layer norm, gated delta rule, their gradients through plain torch
+layers) against the same model in 64 bits, and served (prompt, then token by token in a
+captured graph: norm, delta step, head, sampled token) against its own prompt form.
+
+Tolerances, fixed before the first run. The model's matrices are fp32 torch products of
+at most 64 terms, the operators hold fp32; a gradient passes about ten such stages, each
+off by at most some 64 2^-24 = 4e-6 of the sizes involved: 1e-4 of the largest entry.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from sunnynet_amd import runtime
+
+pytestmark = pytest.mark.gpu
+D, Hk, H, K, V, VOCAB = 48, 2, 4, 16, 24, 97
+
+
+def weights(seed=0):
+    g = torch.Generator().manual_seed(seed)
+
+    def rn(*s, std=0.2):
+        return std * torch.randn(*s, generator=g)
+
+    return {"embed": rn(VOCAB, D, std=1.0), "w1": 1 + rn(D), "b1": rn(D), "qk": rn(2 * Hk * K, D), "v": rn(H * V, D),
+            "gb": rn(2 * H, D), "out": rn(D, H * V), "w2": 1 + rn(D), "b2": rn(D)}
+
+
+def delta64(q, k, v, g, beta, s):
+    outs = []
+    for t in range(q.shape[1]):
+        qt, kt = (x[:, t].repeat_interleave(H // Hk, 1) for x in (q, k))
+        s = s * torch.exp(g[:, t])[..., None, None]
+        u = beta[:, t, :, None] * (v[:, t] - (s * kt[..., None]).sum(2))
+        s = s + kt[..., None] * u[:, :, None, :]
+        outs.append((s * qt[..., None]).sum(2) * K ** -0.5)
+    return torch.stack(outs, 1), s
+
+
+def norm64(x, w, b, eps):
+    d = x - x.mean(-1, keepdim=True)
+    return d / torch.sqrt(d.square().mean(-1, keepdim=True) + eps) * w + b
+
+
+def model(p, tokens, s0, norm, delta):
+    """tokens (B, T) -> logits (B, T, VOCAB), state."""
+    B, T = tokens.shape
+    x = p["embed"][tokens]
+    h = norm(x, p["w1"], p["b1"], 4.1e-4)
+    q, k = (h @ p["qk"].t()).view(B, T, 2, Hk, K).unbind(2)
+    k = k / k.norm(dim=-1, keepdim=True)
+    v = (h @ p["v"].t()).view(B, T, H, V)
+    g, beta = (h @ p["gb"].t()).view(B, T, 2, H).unbind(2)
+    o, s = delta(q, k, v, -torch.nn.functional.softplus(g), torch.sigmoid(beta), s0)
+    x = x + o.reshape(B, T, H * V) @ p["out"].t()
+    return norm(x, p["w2"], p["b2"], 4.1e-4) @ p["embed"].t(), s
+
+
+def loss_of(logits, targets):
+    z = logits - logits.logsumexp(-1, keepdim=True)
+    return -z.gather(-1, targets[..., None]).mean()
+
+
+def test_trained(gpu):
+    p = weights()
+    g = torch.Generator().manual_seed(1)
+    tokens = torch.randint(0, VOCAB, (3, 78), generator=g)
+    s0 = 0.1 * torch.randn(3, H, K, V, generator=g)
+    p64 = {n: t.double().requires_grad_() for n, t in p.items()}
+    lg, s = model(p64, tokens[:, :-1], s0.double(), norm64, delta64)
+    want = torch.autograd.grad(loss_of(lg, tokens[:, 1:]) + s.square().mean(), list(p64.values()))
+    pd = {n: t.cuda().requires_grad_() for n, t in p.items()}
+    td = tokens.cuda()
+    out, sd = model(pd, td[:, :-1], s0.cuda(), runtime.layer_norm, runtime.gated_delta)
+    got = torch.autograd.grad(loss_of(out, td[:, 1:]) + sd.square().mean(), list(pd.values()))
+    assert (out.double().cpu() - lg).abs().max() <= 1e-4 * lg.abs().max()
+    assert (sd.double().cpu() - s).abs().max() <= 1e-4 * s.abs().max()
+    for n, a, b in zip(p, got, want):
+        assert (a.double().cpu() - b).abs().max() <= 1e-4 * b.abs().max(), n
+
+
+def test_served(gpu):
+    """A prompt, then sampled tokens one by one in a captured graph. Feeding the whole
+    text as one prompt gives the same logits, and with them the same tokens wherever the
+    random number is not at a border of the distribution."""
+    p = {n: t.cuda() for n, t in weights(2).items()}
+    B, T, N = 4, 37, 20
+    g = torch.Generator().manual_seed(3)
+    prompt = torch.randint(0, VOCAB, (B, T), generator=g).cuda()
+    u = torch.rand(N, B, dtype=torch.float64, generator=g).cuda()
+    pick = dict(temperature=0.9, top_k=30, top_p=0.9, min_p=0.001)
+
+    def step(q, k, v, gg, beta, s):
+        return runtime.delta_step(q[:, 0], k[:, 0], v[:, 0], gg[:, 0].contiguous(), beta[:, 0].contiguous(), s)[:, None], s
+
+    logits, state = model(p, prompt, None, runtime.layer_norm, runtime.gated_delta)
+    token = runtime.sample_tokens(logits[:, -1], u[0], **pick)
+    text, every = [token.clone()], [logits[:, -1].clone()]
+    now = torch.empty_like(u[0])
+    # warm the library calls up on the side stream that the graph is captured from
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        model(p, token[:, None].long(), state.clone(), runtime.layer_norm, step)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held, _ = model(p, token[:, None].long(), state, runtime.layer_norm, step)
+        token.copy_(runtime.sample_tokens(held[:, 0], now, **pick))
+    for i in range(1, N):
+        now.copy_(u[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        text.append(token.clone())
+        every.append(held[:, 0].clone())
+    text, every = torch.stack(text, 1), torch.stack(every, 1)
+    whole, end = model(p, torch.cat([prompt, text[:, :-1].long()], 1), None, runtime.layer_norm, runtime.gated_delta)
+    assert (whole[:, T - 1:] - every).abs().max() <= 1e-4 * whole.abs().max()
+    assert (end - state).abs().max() <= 1e-4 * end.abs().max()
+    for i in range(N):
+        assert torch.equal(runtime.sample_tokens(every[:, i], u[i], **pick), text[:, i])
