@@ -37,7 +37,7 @@ constexpr int64_t kDeltaStride = 1 << 24;
 
 struct DeltaP {
     SnHipDelta d;
-    int64_t slots;          // chunk slots of all sequences
+    int64_t slots, groups;  // chunk slots of all sequences; groups of NS chunks
     int KP, VP;             // K and V padded: saved states are (KP, VP), errors (VP, 32)
     int rep;                // value heads per query and key head
     bool vec;               // every eight elements of a row of q or k are 16-byte aligned
@@ -49,20 +49,28 @@ __host__ __device__ inline int64_t delta_slots(const SnHipDelta& d) {
 __host__ __device__ inline int delta_kp(int64_t K) { return K <= 64 ? 64 : 128; }
 __host__ __device__ inline int delta_vp(int64_t V) { return (int)((V + 15) / 16 * 16); }
 
-// What the forward keeps for the backward, per slot and head: S (KP, VP) before the chunk,
-// and behind all of those E^T (VP, 32).
-__host__ __device__ inline float* delta_state(const DeltaP& a, int64_t slot, int h) {
-    return a.d.states + (slot * a.d.H + h) * (int64_t)(a.VP * a.KP);
+// The backward takes NS chunks at a time (two for 16-bit inputs, whose tiles leave LDS for
+// it; one for fp32): states are kept per such group, which halves their bytes.
+__host__ __device__ constexpr int delta_ns(int64_t dtype) { return dtype == SNHIP_F32 ? 1 : 2; }
+__host__ __device__ inline int64_t delta_groups(const SnHipDelta& d) {
+    const int64_t n = kDC * delta_ns(d.dtype);
+    return d.cu ? d.T / n + d.N : d.B * ((d.T + n - 1) / n);
 }
-__host__ __device__ inline float* delta_errors(const DeltaP& a, int64_t slot, int h) {
-    return a.d.states + a.slots * a.d.H * (int64_t)(a.VP * a.KP) + (slot * a.d.H + h) * (int64_t)(a.VP * kDC);
+// What the forward keeps for the backward, per group and head: S (KP, VP) before it, and
+// behind all of those E^T (VP, 32 NS).
+__host__ __device__ inline float* delta_state(const DeltaP& a, int64_t group, int h) {
+    return a.d.states + (group * a.d.H + h) * (int64_t)(a.VP * a.KP);
+}
+__host__ __device__ inline float* delta_errors(const DeltaP& a, int64_t group, int h) {
+    return a.d.states + a.groups * a.d.H * (int64_t)(a.VP * a.KP) +
+           (group * a.d.H + h) * (int64_t)(a.VP * kDC * delta_ns(a.d.dtype));
 }
 
 // A sequence: its first token as a row of the contiguous arrays, its batch entry and
 // first token there, its length, and the slot of its first chunk. With cu the slots of
 // a sequence begin at cu[n] / 32 + n, which leaves every sequence enough of them.
 struct DeltaSeq {
-    int64_t row, b, t0, slot;
+    int64_t row, b, t0, slot, group;
     int len;
 };
 __device__ __forceinline__ int64_t delta_edge(const SnHipDelta& d, int64_t n) {
@@ -77,33 +85,37 @@ __device__ __forceinline__ DeltaSeq delta_seq(const SnHipDelta& d, int64_t n) {
         s.b = 0;
         s.len = (int)(e > a ? e - a : 0);
         s.slot = a / kDC + n;
+        s.group = a / (kDC * delta_ns(d.dtype)) + n;
     } else {
         s.row = n * d.T;
         s.t0 = 0;
         s.b = n;
         s.len = (int)d.T;
         s.slot = n * ((d.T + kDC - 1) / kDC);
+        const int64_t c = kDC * delta_ns(d.dtype);
+        s.group = n * ((d.T + c - 1) / c);
     }
     return s;
 }
-// The sequence and chunk of a slot; false for a slot that no chunk uses.
-__device__ __forceinline__ bool delta_chunk_of(const SnHipDelta& d, int64_t slot, DeltaSeq* s, int* chunk) {
+// The sequence and chunk of a slot (C = kDC), or the sequence and group of a group's
+// number (C = kDC NS); false for one that is not used.
+template <int C> __device__ __forceinline__ bool delta_chunk_of(const SnHipDelta& d, int64_t slot, DeltaSeq* s, int* chunk) {
     int64_t n;
     if (d.cu) {
         int64_t lo = 0, hi = d.N - 1;          // the last sequence that begins at or before the slot
         while (lo < hi) {
             const int64_t mid = (lo + hi + 1) / 2;
-            if (delta_edge(d, mid) / kDC + mid <= slot) lo = mid;
+            if (delta_edge(d, mid) / C + mid <= slot) lo = mid;
             else hi = mid - 1;
         }
         n = lo;
     } else {
-        n = slot / ((d.T + kDC - 1) / kDC);
+        n = slot / ((d.T + C - 1) / C);
     }
     *s = delta_seq(d, n);
-    const int64_t c = slot - s->slot;
+    const int64_t c = slot - (C == kDC ? s->slot : s->group);
     *chunk = (int)c;
-    return c >= 0 && c * kDC < s->len;
+    return c >= 0 && c * C < s->len;
 }
 
 template <typename T>
@@ -111,11 +123,11 @@ __device__ __forceinline__ const T* delta_at(const void* p, const int64_t* st, i
     return static_cast<const T*>(p) + b * st[0] + t * st[1] + h * st[2];
 }
 
-// A (32, KP) tile of a (tokens, K) array on its way from memory to LDS, held by NTH
+// An (R, KP) tile of a (tokens, K) array on its way from memory to LDS, held by NTH
 // threads: rows from n on and columns from K on are 0.
-template <typename T, int KP, int NTH, bool VEC> struct RowsFetch {
-    static constexpr int P = ElemPlanes<T>::n, N = (kDC * KP / 8 + NTH - 1) / NTH;
-    static constexpr bool whole = kDC * KP / 8 % NTH == 0;
+template <typename T, int KP, int NTH, bool VEC, int R = kDC> struct RowsFetch {
+    static constexpr int P = ElemPlanes<T>::n, N = (R * KP / 8 + NTH - 1) / NTH;
+    static constexpr bool whole = R * KP / 8 % NTH == 0;
     Vec8<T> x[N];
     int off[N];            // of this thread's vectors in any chunk
     __device__ __forceinline__ void init(int64_t stride, int K, int tid) {
@@ -130,11 +142,11 @@ template <typename T, int KP, int NTH, bool VEC> struct RowsFetch {
 #pragma unroll
         for (int j = 0; j < N; j++) x[j] = buf_load8<T>(r, off[j], K - (tid + j * NTH) % (KP / 8) * 8, VEC);
     }
-    __device__ __forceinline__ void store(Tile<P, kDC, KP> to, int tid) const {
+    __device__ __forceinline__ void store(Tile<P, R, KP> to, int tid) const {
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const int i = tid + j * NTH, t = i / (KP / 8), c = i % (KP / 8) * 8;
-            if (whole || t < kDC) to.put8(t, c, split_raw8<T>(x[j]));
+            if (whole || t < R) to.put8(t, c, split_raw8<T>(x[j]));
         }
     }
 };

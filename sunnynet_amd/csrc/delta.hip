@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
     const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15;
     DeltaSeq s;
     int chunk;
-    if (!delta_chunk_of(d, blockIdx.x, &s, &chunk)) return;
+    if (!delta_chunk_of<kDC>(d, blockIdx.x, &s, &chunk)) return;
     const int64_t t0 = (int64_t)chunk * kDC;
     const int n = (int)(s.len - t0 < kDC ? s.len - t0 : kDC);
     const Tile<P, kDC, KP> K{sk}, Q{sq};
@@ -119,6 +119,7 @@ template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, float* send) {
     constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W;
     constexpr int LO = sizeof(T) == 4 ? 3 : 2;      // planes of the products that only reach out
+    constexpr int NS = sizeof(T) == 4 ? 1 : 2;
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, kDC, kDC> MatM;
     typedef Tile<LO, kDC, kDC> MatP;
@@ -186,8 +187,9 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
         for (int i = 0; i < 8; i++) vc[i] = float_of_bits<T>(vv[i]);
         const bool more = t0 + kDC < s.len;
         if (more) fetch(t0 + kDC);
-        if (d.states) {       // S (KP, VP) before the chunk, for the backward
-            const __amdgpu_buffer_rsrc_t st = make_rsrc(delta_state(a, s.slot + t0 / kDC, h), (uint32_t)(a.VP * KP * 4));
+        if (d.states && t0 % (kDC * NS) == 0) {       // S (KP, VP) before the group, for the backward
+            const __amdgpu_buffer_rsrc_t st =
+                make_rsrc(delta_state(a, s.group + t0 / (kDC * NS), h), (uint32_t)(a.VP * KP * 4));
             const int at = v < a.VP ? (g8 * a.VP + v) * 4 : kNowhere;
 #pragma unroll
             for (int kt = 0; kt < NK; kt++)
@@ -236,9 +238,11 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             }
         }
         if (d.states) {
-            const __amdgpu_buffer_rsrc_t re = make_rsrc(delta_errors(a, s.slot + t0 / kDC, h), (uint32_t)(a.VP * kDC * 4));
+            const __amdgpu_buffer_rsrc_t re =
+                make_rsrc(delta_errors(a, s.group + t0 / (kDC * NS), h), (uint32_t)(a.VP * kDC * NS * 4));
 #pragma unroll
-            for (int m = 0; m < 2; m++) buf_store4(re, (v * kDC + g8 + 4 * m) * 4, e[m]);
+            for (int m = 0; m < 2; m++)
+                buf_store4(re, (v * kDC * NS + t0 % (kDC * NS) + g8 + 4 * m) * 4, e[m]);
         }
         const Frag<LO> U = split8<LO>(x);
         const Frag<3> LU = split8<3>(y);
@@ -397,6 +401,7 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
         if (st[1] < 0 || st[1] >= kDeltaStride) return SNHIP_E_INVAL;
     a->d = *d;
     a->slots = delta_slots(*d);
+    a->groups = delta_groups(*d);
     a->KP = delta_kp(d->K);
     a->VP = delta_vp(d->V);
     a->rep = (int)(d->H / d->Hk);
@@ -418,7 +423,7 @@ int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d) {
     return d ? delta_slots(*d) * d->H * kDeltaChunk : 0;
 }
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d) {
-    return d ? delta_slots(*d) * d->H * delta_vp(d->V) * (kDC + (int64_t)delta_kp(d->K)) : 0;
+    return d ? delta_groups(*d) * d->H * delta_vp(d->V) * (kDC * delta_ns(d->dtype) + (int64_t)delta_kp(d->K)) : 0;
 }
 
 snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send, void* stream) {

@@ -8,7 +8,7 @@
 //   Y_ij = scale D_ij beta_j dO_i.E_j (j <= i)   Z_ij = W_i.E_j, F_ij = -D_ij beta_j Z_ij (j < i)
 //   dQ = scale G (dO S^T) + Y K
 //   dK = L beta (E dS^T) - G (W S^T) + Y^T Q + (F + F^T) K
-//   dbeta_j = E_j.dU_j - sum over i > j of Z_ij D_ij k_i.k_j
+//   dbeta_j = E_j.dU_j - sum over i > j in j's chunk of Z_ij D_ij k_i.k_j
 // and, with H = Y (q.k) + F (k.k) elementwise below the diagonal (on it a decay of 1
 // has no gradient: its two shares are left out, not cancelled),
 //   dg_t = sum over i >= t of [ sum_j H_ij - sum_j H_ji
@@ -22,21 +22,22 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a);
 
 namespace {
 
-// Per slot and head: W^T (VP, 32), dS (KP, VP) after the chunk, and (VP / 16, 32) sums of
-// E dU over 16 columns.
+// Per group of NS chunks and head: W^T (VP, 32 NS), dS (KP, VP) after the group, and
+// (VP / 16, 32 NS) sums of E dU over 16 columns.
 struct DeltaWs {
     float* w;
     float* ds;
     float* eu;
 };
-__host__ __device__ inline DeltaWs delta_ws(const DeltaP& a, float* ws, int64_t slot, int h) {
-    const int64_t i = slot * a.d.H + h, n = a.slots * a.d.H, w = kDC * a.VP, ds = (int64_t)a.VP * a.KP;
-    return {ws + i * w, ws + n * w + i * ds, ws + n * (w + ds) + i * (a.VP / 16 * kDC)};
+__host__ __device__ inline DeltaWs delta_ws(const DeltaP& a, float* ws, int64_t group, int h) {
+    const int64_t i = group * a.d.H + h, n = a.groups * a.d.H, c = kDC * delta_ns(a.d.dtype), w = c * a.VP,
+                  ds = (int64_t)a.VP * a.KP;
+    return {ws + i * w, ws + n * w + i * ds, ws + n * (w + ds) + i * (a.VP / 16 * c)};
 }
 
 template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDeltaGrad gr) {
-    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W;
+    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W, NS = sizeof(T) == 4 ? 1 : 2, C = kDC * NS;
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, kDC, kDC> Mat;
     __shared__ alignas(16) __bf16 sk[2][Rows::elems], sq[2][Rows::elems], sm[2][Mat::elems], sp[2][Mat::elems];
@@ -79,9 +80,9 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
         const __amdgpu_buffer_rsrc_t ro = rows_window(dop + t0 * d.H * V, d.H * V, n, V);
 #pragma unroll
         for (int i = 0; i < 8; i++) vv[i] = buf_load_bits<T>(ro, o_off + i * o_step);
-        const __amdgpu_buffer_rsrc_t re = make_rsrc(delta_errors(a, s.slot + t0 / kDC, h), (uint32_t)(a.VP * kDC * 4));
+        const __amdgpu_buffer_rsrc_t re = make_rsrc(delta_errors(a, s.group + t0 / C, h), (uint32_t)(a.VP * C * 4));
 #pragma unroll
-        for (int m = 0; m < 2; m++) ev[m] = buf_load4(re, (v * kDC + g8 + 4 * m) * 4);
+        for (int m = 0; m < 2; m++) ev[m] = buf_load4(re, (v * C + t0 % C + g8 + 4 * m) * 4);
     };
     auto store = [&](int b) {
         fk.store(Rows{sk[b]}, tid);
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
     for (int t0 = last, b = 0; t0 >= 0; t0 -= kDC, b ^= 1) {
         const Rows K{sk[b]}, Q{sq[b]};
         const Mat M{sm[b]}, PM{sp[b]};
-        const DeltaWs w = delta_ws(a, gr.ws, s.slot + t0 / kDC, h);
+        const DeltaWs w = delta_ws(a, gr.ws, s.group + t0 / C, h);
         const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
         float G[8], L[8], be[8], x[8], y[8], od[8];
         const f32x4 e[2] = {ev[0], ev[1]};
@@ -109,9 +110,10 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
         for (int i = 0; i < 8; i++) od[i] = float_of_bits<T>(vv[i]);
         if (t0 > 0) fetch(t0 - kDC);
         const __amdgpu_buffer_rsrc_t rds = make_rsrc(w.ds, (uint32_t)(a.VP * KP * 4)),
-                                     rw = make_rsrc(w.w, (uint32_t)(a.VP * kDC * 4)),
-                                     reu = make_rsrc(w.eu, (uint32_t)(a.VP / 16 * kDC * 4));
+                                     rw = make_rsrc(w.w, (uint32_t)(a.VP * C * 4)),
+                                     reu = make_rsrc(w.eu, (uint32_t)(a.VP / 16 * C * 4));
         const int at = v < a.VP ? (g8 * a.VP + v) * 4 : kNowhere;
+        if (NS == 1 || t0 % C || t0 == last)       // the group's last chunk
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
 #pragma unroll
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
             for (int r = 0; r < 4; r++) {
                 x[4 * m + r] = du[m][r] * be[4 * m + r];
                 const float eu = sum16(e[m][r] * du[m][r]);
-                buf_store<float>(reu, l16 == 0 ? ((v >> 4) * kDC + g8 + 4 * m + r) * 4 : kNowhere, eu);
+                buf_store<float>(reu, l16 == 0 ? ((v >> 4) * C + t0 % C + g8 + 4 * m + r) * 4 : kNowhere, eu);
             }
         }
         const Frag<3> dE = split8<3>(x);
@@ -161,7 +163,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
 #pragma unroll
         for (int m = 0; m < 2; m++) {
             const f32x4 wv = wm[m];
-            buf_store4(rw, (v * kDC + g8 + 4 * m) * 4, wv);
+            buf_store4(rw, (v * C + t0 % C + g8 + 4 * m) * 4, wv);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 buf_store<T>(rdv, o_off + (4 * m + r) * o_step, (T)wv[r]);
@@ -199,65 +201,92 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
             }
 }
 
+// The row of tile i of a lower triangle, counted by rows: 0; 1, 1; 2, 2, 2; ...
+__device__ __forceinline__ int delta_tile_row(int i) { return i < 1 ? 0 : i < 3 ? 1 : i < 6 ? 2 : 3; }
+
+// The lane's place in a phase of a loop, as a value of that phase: the addresses that it
+// makes are not carried around the loop in registers.
+struct LanePlace {
+    int lane, l16, g4, g8, blk16, blkp;
+    __device__ __forceinline__ explicit LanePlace(int l) {
+        asm volatile("" : "+v"(l));
+        lane = l & 63;
+        l16 = lane & 15;
+        g4 = lane >> 4 << 2;
+        g8 = 2 * g4;
+        blk16 = 4 * (lane & 3);
+        blkp = 8 * (lane & 3);
+    }
+};
+
 __device__ __forceinline__ float sum_groups(float x) {
     x += __shfl_xor(x, 16);
     return x + __shfl_xor(x, 32);
 }
 
-// One chunk of one query and key head: a block of KP / 16 waves runs over the value heads
-// that share it, so dq and dk are summed in registers. Per head and 64 columns of V, E, W
-// and dO go through LDS (E and W by column, as the scans leave them, read transposed), and
-// a wave owns 16 columns of K in the products with S and dS; the 32x32 matrices Y and F
-// are six tasks of a 16x16 tile each. What the next step reads is fetched into
-// registers a step ahead. Bound by the bytes of S and dS.
+// One group of NS chunks (C = 32 NS tokens, taken as one chunk) of one query and key head:
+// a block of KP / 16 waves runs over the value heads that share it, so dq and dk are summed
+// in registers. Per head and 64 columns of V, E, W and dO go through LDS (E and W by
+// column, as the scans leave them, read transposed), and a wave owns 16 columns of K in the
+// products with S and dS; Y and F are made by tiles of 16x16, a wave taking every
+// (KP / 16)-th. What the next step reads is fetched into registers a step ahead. Bound by
+// the bytes of S and dS, and by the latency of its steps.
 template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
-    constexpr int P = ElemPlanes<T>::n, VT = 64, NW = KP / 16, NTH = 64 * NW, NT = 6 / NW + 1;
-    typedef Tile<P, kDC, KP> Rows;
-    typedef Tile<3, VT, kDC> Cols;
-    typedef Tile<3, kDC, kDC> Mat;
+    constexpr int NS = sizeof(T) == 4 ? 1 : 2, C = kDC * NS, NM = 2 * NS;      // NM tiles of 16 tokens
+    constexpr int P = ElemPlanes<T>::n, VT = 64, NW = KP / 16, NTH = 64 * NW;
+    constexpr int TILES = NM * (NM + 1) / 2, NT = (2 * TILES + NW - 1) / NW;   // of Y, then of F; per wave
+    typedef Tile<P, C, KP> Rows;
+    typedef Tile<3, VT, C> Cols;
+    typedef Tile<3, C, C> Mat;
     static_assert(Cols::elems >= Mat::elems, "Y and F take the places of E and W");
     __shared__ alignas(16) __bf16 sk[Rows::elems], sq[Rows::elems], se[Cols::elems], sw[Cols::elems],
-        so[Tile<P, kDC, VT>::elems];
-    __shared__ float sv[3 * kDC], seu[kDC], kread[NW][kDC], kwrite[NW][kDC], trow[6][16], tcol[6][16], tzk[3][16], dots[NW];
-    __shared__ double sc[kDC];
+        so[Tile<P, C, VT>::elems];
+    __shared__ float sG[C], sL[C], sB[C], seu[C], kread[NW][C], kwrite[NW][C], trow[2 * TILES][16], tcol[2 * TILES][16],
+        tzk[TILES][16], dots[NW];
+    __shared__ double sc[C];
     const SnHipDelta& d = a.d;
-    const int hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g4 = (lane >> 4) * 4, g8 = 2 * g4,
-              l16 = lane & 15, blk16 = 4 * (lane & 3), blkp = 8 * (lane & 3);
+    const int hk = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15,
+              g8 = (lane >> 4) * 8;
     DeltaSeq s;
-    int chunk;
-    if (!delta_chunk_of(d, blockIdx.x, &s, &chunk)) return;
-    const int64_t t0 = (int64_t)chunk * kDC;
-    const int n = (int)(s.len - t0 < kDC ? s.len - t0 : kDC), V = (int)d.V, Kd = (int)d.K;
+    int group;
+    if (!delta_chunk_of<C>(d, blockIdx.x, &s, &group)) return;
+    const int64_t t0 = (int64_t)group * C;
+    const int n = (int)(s.len - t0 < C ? s.len - t0 : C), V = (int)d.V, Kd = (int)d.K;
     const Rows K{sk}, Q{sq};
     const Cols ET{se}, WT{sw};
-    const Tile<P, kDC, VT> DO{so};
+    const Tile<P, C, VT> DO{so};
     const Mat Y{se}, FF{sw};
-    RowsFetch<T, KP, NTH, VEC> fk, fq;
+    RowsFetch<T, KP, NTH, VEC, C> fk, fq;
     fk.init(d.k_stride[1], Kd, tid);
     fq.init(d.q_stride[1], Kd, tid);
     fk.load(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t0, hk), d.k_stride[1], n, Kd, tid);
     fq.load(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t0, hk), d.q_stride[1], n, Kd, tid);
 
-    // Fetches ahead. Tiles: 64 columns of V of E^T, then of W^T (four vectors of eight tokens
-    // a column), and dO (eight vectors a token).
-    constexpr int NEW = 512 / NTH;
+    // Fetches ahead. Tiles: 64 columns of V of E^T, then of W^T (C / 8 vectors of eight tokens
+    // a column; those of a chunk that the sequence does not reach were never written and
+    // count as 0), and dO (eight vectors a token).
+    constexpr int EV = VT * C / 8, NEW = 2 * EV / NTH, NO = (C * 8 + NTH - 1) / NTH;
     Vec8<float> pe[NEW];
-    Vec8<T> po;
+    Vec8<T> po[NO];
     const int o_step = (int)d.H * V;
     auto fetch_tiles = [&](int h, int vt) {
-        const uint32_t bytes = (uint32_t)(a.VP * kDC * 4);
+        const uint32_t bytes = (uint32_t)(a.VP * C * 4);
         const __amdgpu_buffer_rsrc_t re = make_rsrc(delta_errors(a, blockIdx.x, h), bytes),
                                      rw = make_rsrc(delta_ws(a, gr.ws, blockIdx.x, h).w, bytes);
 #pragma unroll
         for (int j = 0; j < NEW; j++) {
-            const int u = tid + j * NTH;
-            pe[j] = buf_load8<float>(u < 256 ? re : rw, (vt * kDC + (u & 255) * 8) * 4, 8, true);
+            const int u = tid + j * NTH, c = u % (C / 8) * 8;
+            const int at = (c & ~(kDC - 1)) < n ? (vt * C + u % EV * 8) * 4 : kNowhere;
+            pe[j] = buf_load8<float>(u < EV ? re : rw, at, 8, true);
         }
-        const int c = vt + (tid & 7) * 8;
         const T* op = static_cast<const T*>(gr.dout) + ((s.row + t0) * d.H + h) * (int64_t)V;
-        po = buf_load8<T>(rows_window(op, o_step, n, V),
-                          c < V && tid < 256 ? ((tid >> 3) * o_step + c) * (int)sizeof(T) : kNowhere, V - c, vec_o);
+        const __amdgpu_buffer_rsrc_t ro = rows_window(op, o_step, n, V);
+#pragma unroll
+        for (int j = 0; j < NO; j++) {
+            const int u = tid + j * NTH, c = vt + (u & 7) * 8;
+            po[j] = buf_load8<T>(ro, c < V && u < C * 8 ? ((u >> 3) * o_step + c) * (int)sizeof(T) : kNowhere, V - c, vec_o);
+        }
     };
     // States: 32 columns of V from `v0` on of S and dS, the rows of K of this wave.
     const int kc = wave * 16;
@@ -271,52 +300,64 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
     fetch_states(hk * a.rep, 0);
     fk.store(K, tid);
     fq.store(Q, tid);
-    f32x4 dq[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, dk[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    f32x4 dq[NM], dk[NM];
+#pragma unroll
+    for (int m = 0; m < NM; m++) dq[m] = dk[m] = f32x4{0, 0, 0, 0};
 
     for (int h = hk * a.rep, end = h + a.rep; h < end; h++) {
-        if (tid < 3 * kDC) sv[tid] = d.chunks[((int64_t)blockIdx.x * d.H + h) * kDeltaChunk + kDeltaG + tid];
-        if (wave == 3) {        // decays, and the parts of E dU
+        if (wave == NW - 1) {        // decays, and the parts of E dU
             const int64_t at = (s.row + t0 + lane) * d.H + h;
             double c = lane < n ? (double)delta_decay(d.g[at]) : 0.0;
 #pragma unroll
-            for (int o = 1; o < kDC; o <<= 1) {
-                const double y = __shfl_up(c, o, kDC);
-                if ((lane & 31) >= o) c += y;
+            for (int o = 1; o < C; o <<= 1) {
+                const double y = __shfl_up(c, o, C);
+                if ((lane & (C - 1)) >= o) c += y;
             }
-            if (lane < kDC) {
+            const double last = __shfl(c, C - 1, C);
+            if (lane < C) {
                 sc[lane] = c;
+                sG[lane] = expf((float)c);
+                sL[lane] = expf((float)(last - c));
+                sB[lane] = lane < n ? d.beta[at] : 0.f;
                 const float* eu = delta_ws(a, gr.ws, blockIdx.x, h).eu;
                 float t = 0.f;
-                for (int i = 0; i < a.VP / 16; i++) t += eu[i * kDC + lane];
+                if (lane < n)
+                    for (int i = 0; i < a.VP / 16; i++) t += eu[i * C + lane];
                 seu[lane] = t;
             }
         }
-        f32x4 small[NT], q1[2], k1[2], k2[2];
+        f32x4 small[NT], q1[NM], k1[NM], k2[NM];
 #pragma unroll
         for (int j = 0; j < NT; j++) small[j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int m = 0; m < 2; m++) q1[m] = k1[m] = k2[m] = f32x4{0, 0, 0, 0};
+        for (int m = 0; m < NM; m++) q1[m] = k1[m] = k2[m] = f32x4{0, 0, 0, 0};
         float ss = 0.f;
         for (int vt = 0; vt < a.VP; vt += VT) {
 #pragma unroll
             for (int j = 0; j < NEW; j++) {
-                const int u = tid + j * NTH, r = (u & 255) >> 2, c = (u & 3) * 8;
-                (u < 256 ? ET : WT).put8(r, c, split_raw8<float>(pe[j]));
+                const int u = tid + j * NTH, r = u % EV / (C / 8), c = u % (C / 8) * 8;
+                (u < EV ? ET : WT).put8(r, c, split_raw8<float>(pe[j]));
             }
-            if (tid < 256) DO.put8(tid >> 3, (tid & 7) * 8, split_raw8<T>(po));
+#pragma unroll
+            for (int j = 0; j < NO; j++) {
+                const int u = tid + j * NTH;
+                if (u < C * 8) DO.put8(u >> 3, (u & 7) * 8, split_raw8<T>(po[j]));
+            }
             barrier_lds();
             if (vt + VT < a.VP) fetch_tiles(h, vt + VT);
             else if (h + 1 < end) fetch_tiles(h + 1, 0);
             const int nv = a.VP - vt < VT ? (a.VP - vt + 31) & ~31 : VT;       // whole 32s
+            const LanePlace L(lane);
 #pragma unroll
             for (int j = 0; j < NT; j++) {
-                const int task = wave + j * NW, ti = task % 3 ? 1 : 0, tj = task % 3 == 2 ? 1 : 0;
-                if (task < 6)
+                const int task = wave + j * NW, ti = delta_tile_row(task % TILES), tj = task % TILES - ti * (ti + 1) / 2;
+                if (task < 2 * TILES)
                     for (int i = 0; i < nv; i += 32) {
-                        const Frag<3> b = ET.tfrag(i, 16 * tj + blk16, lane);
-                        small[j] = task < 3 ? mma<3>(DO.frag(16 * ti + l16, i, lane), b, small[j])
-                                            : mma<3>(WT.tfrag(i, 16 * ti + blk16, lane), b, small[j]);
+                        const Frag<3> b = ET.tfrag(i, 16 * tj + L.blk16, L.lane);
+                        small[j] = task < TILES ? mma<3>(DO.frag(16 * ti + L.l16, i, L.lane), b, small[j])
+                                                : mma<3>(WT.tfrag(i, 16 * ti + L.blk16, L.lane), b, small[j]);
                     }
+                __builtin_amdgcn_sched_barrier(0);       // reads of later tiles would need registers
             }
             for (int i = 0; i < nv; i += 32) {
 #pragma unroll
@@ -325,35 +366,43 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
                 if (vt + i + 32 < a.VP) fetch_states(h, vt + i + 32);
                 else if (h + 1 < end) fetch_states(h + 1, 0);
 #pragma unroll
-                for (int m = 0; m < 2; m++) {
-                    q1[m] = mma<3>(DO.frag(pair_row(m, l16), i, lane), b, q1[m]);
-                    k1[m] = mma<3>(WT.tfrag(i, blkp + 4 * m, lane), b, k1[m]);
-                    k2[m] = mma<3>(ET.tfrag(i, blkp + 4 * m, lane), e, k2[m]);
+                for (int m = 0; m < NM; m++) {
+                    const int r = 32 * (m >> 1), q = m & 1;
+                    q1[m] = mma<3>(DO.frag(r + pair_row(q, L.l16), i, L.lane), b, q1[m]);
+                    k1[m] = mma<3>(WT.tfrag(i, r + L.blkp + 4 * q, L.lane), b, k1[m]);
+                    k2[m] = mma<3>(ET.tfrag(i, r + L.blkp + 4 * q, L.lane), e, k2[m]);
+                    if (m & 1) __builtin_amdgcn_sched_barrier(0);
                 }
             }
             barrier_lds();
         }
         ss = sum_groups(sum16(ss));
         if (lane == 0) dots[wave] = ss;
+        // Y's upper tiles are 0
+        for (int i = tid; i < C * C / 8; i += NTH) {
+            const int row = i / (C / 8), c = i % (C / 8) * 8;
+            if (c / 16 > row / 16) Y.put8(row, c, Frag<3>{});
+        }
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            // tiles (0,0), (1,0), (1,1) of Y with its part of H, then of F with its part
-            const int task = wave + j * NW, ti = task % 3 ? 1 : 0, tj = task % 3 == 2 ? 1 : 0;
-            if (task >= 6) break;
-            const Rows A{task < 3 ? sq : sk};
+            const LanePlace L(lane);
+            // a tile of Y with its part of H, or of F with its part
+            const int task = wave + j * NW, tile = task % TILES, ti = delta_tile_row(tile), tj = tile - ti * (ti + 1) / 2;
+            if (task >= 2 * TILES) break;
+            const Rows A{task < TILES ? sq : sk};
             f32x4 qk = {0, 0, 0, 0};       // q.k, or k.k
 #pragma unroll
             for (int c = 0; c < KP; c += 32)
-                qk = mma<3>(A.frag(16 * ti + l16, c, lane), K.frag(16 * tj + l16, c, lane), qk);
-            const int col = tj * 16 + l16;
-            const float bj = sv[2 * kDC + col];
+                qk = mma<3>(A.frag(16 * ti + L.l16, c, L.lane), K.frag(16 * tj + L.l16, c, L.lane), qk);
+            const int col = tj * 16 + L.l16;
+            const float bj = sB[col];
             float hsum = 0.f, zsum = 0.f, f[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int row = 16 * ti + g4 + r;
+                const int row = 16 * ti + L.g4 + r;
                 const float D = col <= row ? expf((float)(sc[row] - sc[col])) : 0.f;
                 float e;
-                if (task < 3) {
+                if (task < TILES) {
                     const float y = (float)d.scale * D * bj * small[j][r];
                     e = col < row ? y * qk[r] : 0.f;
                     Y.put(row, col, y);
@@ -361,21 +410,21 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
                     const float zd = col < row ? D * small[j][r] : 0.f;
                     f[r] = -bj * zd;
                     e = f[r] * qk[r];
-                    zsum = fmaf(zd, qk[r], zsum);
+                    if (ti / 2 == tj / 2) zsum = fmaf(zd, qk[r], zsum);     // dU has the other chunks' part
                     if (ti != tj) {
                         FF.put(row, col, f[r]);
                         FF.put(col, row, f[r]);
                     }
                 }
                 const float er = sum16(e);
-                if (l16 == 0) trow[task][g4 + r] = er;
+                if (L.l16 == 0) trow[task][L.g4 + r] = er;
                 hsum += e;
             }
             hsum = sum_groups(hsum);
-            if (lane < 16) tcol[task][lane] = hsum;
-            if (task >= 3) {
+            if (L.lane < 16) tcol[task][lane] = hsum;
+            if (task >= TILES) {
                 zsum = sum_groups(zsum);
-                if (lane < 16) tzk[task - 3][lane] = zsum;
+                if (L.lane < 16) tzk[tile][lane] = zsum;
                 if (ti == tj) {
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
@@ -383,75 +432,91 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
                         float t = 0.f;
 #pragma unroll
                         for (int rr = 0; rr < 4; rr++) {
-                            const float x = __shfl(f[rr], (l16 >> 2) * 16 + g4 + r);
-                            if ((l16 & 3) == rr) t = x;
+                            const float x = __shfl(f[rr], (L.l16 >> 2) * 16 + L.g4 + r);
+                            if ((L.l16 & 3) == rr) t = x;
                         }
-                        FF.put(16 * ti + g4 + r, col, f[r] + t);
+                        FF.put(16 * ti + L.g4 + r, col, f[r] + t);
                     }
                 }
             }
-        }
-        if (wave == 3) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) Y.put(g4 + r, 16 + l16, 0.f);
+            __builtin_amdgcn_sched_barrier(0);
         }
         barrier_lds();
-        const Frag<P> bk = K.tfrag(0, kc + blk16, lane), bq = Q.tfrag(0, kc + blk16, lane);
+        const LanePlace L(lane);
+        Frag<P> bk[NS], bq[NS];
 #pragma unroll
-        for (int m = 0; m < 2; m++) {
+        for (int i = 0; i < NS; i++) {
+            bk[i] = K.tfrag(32 * i, kc + L.blk16, L.lane);
+            bq[i] = Q.tfrag(32 * i, kc + L.blk16, L.lane);
+        }
+#pragma unroll
+        for (int m = 0; m < NM; m++) {
+            const int b32 = 32 * (m >> 1), q = m & 1;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const int t = g8 + 4 * m + r;
-                const float qv = Q.get(t, kc + l16), kv = K.get(t, kc + l16), G = sv[t];
+                const int t = b32 + L.g8 + 4 * q + r;
+                const float qv = Q.get(t, kc + L.l16), kv = K.get(t, kc + L.l16), G = sG[t];
                 q1[m][r] *= (float)d.scale * G;
                 k1[m][r] *= -G;
-                k2[m][r] *= sv[kDC + t] * sv[2 * kDC + t];
+                k2[m][r] *= sL[t] * sB[t];
                 const float cr = sum16(fmaf(qv, q1[m][r], kv * k1[m][r])), cw = sum16(kv * k2[m][r]);
-                if (l16 == 0) {
+                if (L.l16 == 0) {
                     kread[wave][t] = cr;
                     kwrite[wave][t] = cw;
                 }
             }
-            dq[m] += mma<3>(Y.frag(pair_row(m, l16), 0, lane), bk, q1[m]);
-            const f32x4 t = mma<3>(Y.tfrag(0, blkp + 4 * m, lane), bq, k1[m] + k2[m]);
-            dk[m] += mma<3>(FF.frag(pair_row(m, l16), 0, lane), bk, t);
+            f32x4 t = k1[m] + k2[m];
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                if (32 * i <= b32) q1[m] = mma<3>(Y.frag(b32 + pair_row(q, L.l16), 32 * i, L.lane), bk[i], q1[m]);
+                if (32 * i >= b32) t = mma<3>(Y.tfrag(32 * i, b32 + L.blkp + 4 * q, L.lane), bq[i], t);
+                t = mma<3>(FF.frag(b32 + pair_row(q, L.l16), 32 * i, L.lane), bk[i], t);
+            }
+            dq[m] += q1[m];
+            dk[m] += t;
+            __builtin_amdgcn_sched_barrier(0);
         }
         barrier_lds();
-        if (tid < kDC) {
+        if (tid < C) {
             // dg_t: reads and H by later tokens, less H's columns there, and the writes of
             // earlier ones (a write's share in dc_C less its own dc is left of its token)
             const int t = tid, hi = t >> 4, lo = t & 15;
-            float dc = 0.f;
-            for (int i = 0; i < 6; i += 3)       // Y's part, F's part
-                dc += hi ? trow[i + 1][lo] + trow[i + 2][lo] - tcol[i + 2][lo]
-                         : trow[i][lo] - tcol[i][lo] - tcol[i + 1][lo];
-            const float db = seu[t] - (hi ? tzk[2][lo] : tzk[0][lo] + tzk[1][lo]);
-            float wr = 0.f, all = 0.f;
+            float dc = 0.f, db = seu[t], wr = 0.f, all = 0.f;
+            for (int i = 0; i < NM; i++) {         // tile (hi, i) of its row, (i, hi) of its column
+                if (i <= hi)
+                    dc += trow[hi * (hi + 1) / 2 + i][lo] + trow[TILES + hi * (hi + 1) / 2 + i][lo];
+                if (i >= hi) {
+                    const int c = i * (i + 1) / 2 + hi;
+                    dc -= tcol[c][lo] + tcol[TILES + c][lo];
+                    db -= tzk[c][lo];
+                }
+            }
             for (int i = 0; i < NW; i++) {
                 dc += kread[i][t];
                 wr += kwrite[i][t];
                 all += dots[i];
             }
 #pragma unroll
-            for (int o = 1; o < kDC; o <<= 1) {
-                const float x = __shfl_down(dc, o, kDC), y = __shfl_up(wr, o, kDC);
-                if (t + o < kDC) dc += x;
+            for (int o = 1; o < C; o <<= 1) {
+                const float x = __shfl_down(dc, o, C), y = __shfl_up(wr, o, C);
+                if (t + o < C) dc += x;
                 if (t >= o) wr += y;
             }
-            const float before = __shfl_up(wr, 1, kDC);
-            dc += (t ? before : 0.f) + sv[kDC - 1] * all;
+            const float before = __shfl_up(wr, 1, C);
+            dc += (t ? before : 0.f) + sG[C - 1] * all;
             if (t < n) {
                 gr.dg[(s.row + t0 + t) * d.H + h] = dc;
                 gr.dbeta[(s.row + t0 + t) * d.H + h] = db;
             }
         }
-        barrier_lds();        // sv, sc and the sums are the next head's
+        barrier_lds();        // sc and the sums are the next head's
     }
     if (kc + l16 >= Kd) return;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int64_t at = ((s.row + t0 + g8 + i) * d.Hk + hk) * (int64_t)Kd + kc + l16;
-        if (g8 + i < n) {
+    for (int i = 0; i < 4 * NM; i++) {
+        const int t = 32 * (i >> 3) + g8 + (i & 7);
+        const int64_t at = ((s.row + t0 + t) * d.Hk + hk) * (int64_t)Kd + kc + l16;
+        if (t < n) {
             static_cast<T*>(gr.dq)[at] = (T)dq[i >> 2][i & 3];
             static_cast<T*>(gr.dk)[at] = (T)dk[i >> 2][i & 3];
         }
@@ -464,7 +529,7 @@ snhip_status bwd_t(const DeltaP& a, const SnHipDeltaGrad& gr, hipStream_t st) {
     k_delta_rscan<T, KP, VEC><<<grid, 64 * kDeltaW, 0, st>>>(a, gr);
     SNHIP_CHECK(hipGetLastError());
     const bool vec_o = a.d.V % 8 == 0 && reinterpret_cast<uintptr_t>(gr.dout) % 16 == 0;
-    k_delta_local<T, KP, VEC><<<dim3((unsigned)a.slots, (unsigned)a.d.Hk), 4 * KP, 0, st>>>(a, gr, vec_o);
+    k_delta_local<T, KP, VEC><<<dim3((unsigned)a.groups, (unsigned)a.d.Hk), 4 * KP, 0, st>>>(a, gr, vec_o);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
@@ -477,7 +542,9 @@ using namespace snhip;
 extern "C" {
 
 int64_t snhip_op_delta_bwd_floats(const SnHipDelta* d) {
-    return d ? delta_slots(*d) * d->H * delta_vp(d->V) * (kDC + (int64_t)delta_kp(d->K) + kDC / 16) : 0;
+    if (!d) return 0;
+    const int64_t c = kDC * delta_ns(d->dtype);
+    return delta_groups(*d) * d->H * delta_vp(d->V) * (c + delta_kp(d->K) + c / 16);
 }
 
 snhip_status snhip_op_delta_bwd_dev(const SnHipDelta* d, const SnHipDeltaGrad* gr, void* stream) {
