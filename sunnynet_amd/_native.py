@@ -188,11 +188,17 @@ def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The current stream's handle without the Stream object around it (2 us a call less),
+# where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def on_device(device, call, *args) -> int:
     """call(*args, stream) on torch's current stream of `device`, with that device the
     current one, as the library's operators expect."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    at = device.index
+    stream = _raw_stream(at) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == at:
         return call(*args, stream)
     with torch.cuda.device(device):
         return call(*args, stream)

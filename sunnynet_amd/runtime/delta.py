@@ -34,14 +34,20 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _shapes(q, k, v, g, beta, s0, cu):
-    """(B, T, N, Hk, H, K, V) of a call, after its checks."""
-    if q.dim() != 4 or v.dim() != 4 or k.shape != q.shape:
-        raise ValueError("shape mismatch: q, k (B,T,Hk,K); v (B,T,H,V)")
-    B, T, Hk, K = q.shape
-    H, V = v.shape[2:]
-    if v.shape[:2] != (B, T) or g.shape != (B, T, H) or beta.shape != (B, T, H):
-        raise ValueError("shape mismatch: q, k (B,T,Hk,K); v (B,T,H,V); g, beta (B,T,H)")
+def _shapes(q, k, v, g, beta, s0, cu, step=False):
+    """(B, T, N, Hk, H, K, V) of a call, after its checks. step: one token, without T axes."""
+    if step:
+        (B, Hk, K), T = q.shape, 1
+        H, V = v.shape[1:]
+        if k.shape != q.shape or v.shape[0] != B or g.shape != (B, H) or beta.shape != (B, H):
+            raise ValueError("shape mismatch: q, k (B,Hk,K); v (B,H,V); g, beta (B,H)")
+    else:
+        if q.dim() != 4 or v.dim() != 4 or k.shape != q.shape:
+            raise ValueError("shape mismatch: q, k (B,T,Hk,K); v (B,T,H,V)")
+        B, T, Hk, K = q.shape
+        H, V = v.shape[2:]
+        if v.shape[:2] != (B, T) or g.shape != (B, T, H) or beta.shape != (B, T, H):
+            raise ValueError("shape mismatch: q, k (B,T,Hk,K); v (B,T,H,V); g, beta (B,T,H)")
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{H} value heads cannot share {Hk} query and key heads evenly")
     if not 1 <= K <= MAX_K or not 1 <= V <= MAX_V or H > MAX_HEADS:
@@ -66,8 +72,9 @@ def _shapes(q, k, v, g, beta, s0, cu):
         raise ValueError("at most 65535 sequences per call")
     if s0 is not None:
         _check_state(s0, (N, H, K, V), "s0")
-    ts = [t for t in (q, k, v, g, beta, s0, cu) if t is not None]
-    if not q.is_cuda or any(t.device != q.device for t in ts):
+    dev = q.device
+    if not q.is_cuda or k.device != dev or v.device != dev or g.device != dev or beta.device != dev \
+            or s0 is not None and s0.device != dev or cu is not None and cu.device != dev:
         raise ValueError("the delta rule takes tensors of one GPU")
     return B, T, N, Hk, H, K, V
 
@@ -200,9 +207,9 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
     ``send``. No autograd."""
     if q.dim() != 3 or v.dim() != 3 or k.dim() != 3 or g.dim() != 2 or beta.dim() != 2:
         raise ValueError("shape mismatch: q, k (B,Hk,K); v (B,H,V); g, beta (B,H)")
-    q, k, v, g, beta = (t.unsqueeze(1) for t in (_rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()))
-    dims = _shapes(q, k, v, g, beta, s, None)
-    B, T, N, Hk, H, K, V = dims
+    q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
+    dims = _shapes(q, k, v, g, beta, s, None, step=True)
+    B, _, N, Hk, H, K, V = dims
     if send is None:
         send = s
     elif send is not s:
@@ -212,8 +219,10 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
     out = torch.empty(B, H, V, dtype=v.dtype, device=q.device)
     if B == 0:
         return out
-    scale = K ** -0.5 if scale is None else float(scale)
-    rc = _native.on_device(q.device, _native.lib().snhip_op_delta_step_dev,
-                           _pack(q, k, v, g, beta, s, None, dims, scale), out.data_ptr(), send.data_ptr())
+    (qb, qh, _), (kb, kh, _), (vb, vh, _) = q.stride(), k.stride(), v.stride()
+    args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), s.data_ptr(), 0,
+                      qb, 0, qh, kb, 0, kh, vb, 0, vh, *dims, DTYPES[q.dtype],
+                      K ** -0.5 if scale is None else float(scale), 0, 0)
+    rc = _native.on_device(q.device, _native.lib().snhip_op_delta_step_dev, args, out.data_ptr(), send.data_ptr())
     _native.check(rc, "snhip_op_delta_step_dev")
     return out

@@ -48,11 +48,17 @@ def norm_bwd(dy, x, weight, mean, rstd, *, need=(True, True, True)):
     """Gradients of norm_fwd(..., keep=True) -> (dx, dweight, dbias), each None where
     ``need`` says so. The sums over rows run in a fixed order."""
     R, D = _check(x, weight, None)
+    if any(t is None for t in (mean, rstd)):
+        raise ValueError("mean and rstd must be norm_fwd's")
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device or not dy.is_contiguous():
         raise ValueError("dy must be contiguous and like x")
     if any(t.shape != (R,) or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous()
            for t in (mean, rstd)):
         raise ValueError("mean and rstd must be norm_fwd's")
+    return _bwd(dy, x, weight, mean, rstd, need, R, D)
+
+
+def _bwd(dy, x, weight, mean, rstd, need, R, D):
     L = _native.lib()
     dx = torch.empty_like(x) if need[0] else None
     new = torch.empty if R else torch.zeros
@@ -81,7 +87,7 @@ class LayerNorm(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
-        return *norm_bwd(dy.contiguous(), x, weight, mean, rstd, need=ctx.needs_input_grad[:3]), None
+        return *_bwd(dy.contiguous(), x, weight, mean, rstd, ctx.needs_input_grad[:3], mean.shape[0], x.shape[-1]), None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
