@@ -40,6 +40,8 @@ struct DeltaP {
     int64_t slots, groups;  // chunk slots of all sequences; groups of NS chunks
     int KP, VP;             // K and V padded: saved states are (KP, VP), errors (VP, 32)
     int rep;                // value heads per query and key head
+    int segs, seg_chunks;   // parts of a sequence that are scanned at once, and their chunks
+    float* seg_state;       // per sequence, part and head: delta_seg_floats
     bool vec;               // every eight elements of a row of q or k are 16-byte aligned
 };
 
@@ -64,6 +66,23 @@ __host__ __device__ inline float* delta_state(const DeltaP& a, int64_t group, in
 __host__ __device__ inline float* delta_errors(const DeltaP& a, int64_t group, int h) {
     return a.d.states + a.groups * a.d.H * (int64_t)(a.VP * a.KP) +
            (group * a.d.H + h) * (int64_t)(a.VP * kDC * delta_ns(a.d.dtype));
+}
+
+// Few heads and a long sequence leave the scan a handful of waves. Then the sequence is
+// scanned in parts: over a part the state is an affine map of the state before it,
+// S' = A S + B, where B is what the scan makes of S = 0 and A what it makes of S = I with
+// no values: K more columns. One pass makes A and B of all parts, a small kernel joins
+// them, and the ordinary scan runs over all parts at once from their true states. This is
+// 2 to 3 times the work. Per part and head: (KP, VP + KP) for [B A], then (KP, VP) for S.
+__host__ __device__ inline int64_t delta_seg_floats(int KP, int VP) { return (int64_t)KP * (2 * VP + KP); }
+// Waves that fill the card (256 CUs of four SIMDs), and the fewest chunks worth a part.
+constexpr int kDeltaWaves = 1024, kDeltaSegChunks = 32;
+inline int delta_segs(const SnHipDelta& d) {
+    const int64_t waves = (int64_t)d.H * d.N * (delta_vp(d.V) / 16), chunks = (d.T + kDC - 1) / kDC;
+    int64_t n = kDeltaWaves / waves;
+    if (n > chunks / kDeltaSegChunks) n = chunks / kDeltaSegChunks;
+    // below four parts the second pass and the join take what the first one gives
+    return n < 4 ? 1 : n > 16 ? 16 : (int)n;
 }
 
 // A sequence: its first token as a row of the contiguous arrays, its batch entry and

@@ -114,8 +114,10 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
 // The scan over chunks: kDeltaW waves, 16 columns of V each. Half types read the state by
 // two planes where only out (of that type) depends on it. The next chunk's tiles are
 // fetched into registers while this one is worked on, and put into the other half of LDS:
-// one barrier per chunk, no wait for memory in between.
-template <typename T, int KP, bool VEC>
+// one barrier per chunk, no wait for memory in between. PASS 0 scans whole sequences or, from
+// the states that the join left, the parts of sequences; PASS 1 makes the parts' maps:
+// columns from VP on are those of A, and there is no output.
+template <typename T, int KP, bool VEC, int PASS>
 __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, float* send) {
     constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W;
     constexpr int LO = sizeof(T) == 4 ? 3 : 2;      // planes of the products that only reach out
@@ -127,9 +129,18 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
     __shared__ alignas(16) float sv[2][3 * kDC];
     const SnHipDelta& d = a.d;
     const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g8 = (lane >> 4) * 8;
-    const DeltaSeq s = delta_seq(d, blockIdx.z);
+    const int64_t seq = blockIdx.z / a.segs;
+    const int seg = blockIdx.z % a.segs;
+    const DeltaSeq s = delta_seq(d, seq);
+    const int begin = seg * a.seg_chunks * kDC;
+    // a part that the sequence does not reach, or (for the maps) whose end is the sequence's
+    if (seg && begin >= s.len) return;
+    const bool last = a.segs == 1 || begin + a.seg_chunks * kDC >= s.len;
+    if (PASS == 1 && (last || (seg == 0 && (int)blockIdx.x * 16 * W >= a.VP))) return;      // part 0's A is not used
+    const int stop = last ? s.len : begin + a.seg_chunks * kDC;
     const int v = (blockIdx.x * W + wave) * 16 + l16, V = (int)d.V, Kd = (int)d.K;
-    const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
+    const int64_t sbase = (seq * d.H + h) * d.K * d.V;
+    float* part = a.segs > 1 ? a.seg_state + ((seq * a.segs + seg) * d.H + h) * delta_seg_floats(KP, a.VP) : nullptr;
     const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0, h / a.rep);
     const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0, h / a.rep);
     const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0, h);
@@ -141,7 +152,9 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
-            S[kt][r] = d.s0 && k < Kd && v < V ? d.s0[sbase + (int64_t)k * V + v] : 0.f;
+            if (PASS == 1 && v >= a.VP) S[kt][r] = k == v - a.VP ? 1.f : 0.f;
+            else if (seg == 0) S[kt][r] = d.s0 && k < Kd && v < V ? d.s0[sbase + (int64_t)k * V + v] : 0.f;
+            else S[kt][r] = PASS == 0 && v < a.VP ? part[(int64_t)KP * (a.VP + KP) + k * a.VP + v] : 0.f;
         }
     RowsFetch<T, KP, NTH, VEC> fk, fq;
     MatFetch<3, NTH> fm;
@@ -156,9 +169,9 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
         const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
         const __amdgpu_buffer_rsrc_t r = make_rsrc(rec + (int64_t)(t0 / kDC) * d.H * kDeltaChunk, kDeltaChunk * 4);
         fk.load(kp + t0 * d.k_stride[1], d.k_stride[1], n, Kd, tid);
-        fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, tid);
+        if (PASS == 0) fq.load(qp + t0 * d.q_stride[1], d.q_stride[1], n, Kd, tid);
         fm.load(r, 0, tid);
-        fp.load(r, kDeltaP, tid);
+        if (PASS == 0) fp.load(r, kDeltaP, tid);
 #pragma unroll
         for (int j = 0; j * NTH < 3 * kDC; j++) fv[j] = buf_load<float>(r, (kDeltaG + tid + j * NTH) * 4);
         const __amdgpu_buffer_rsrc_t rv = rows_window(vp + t0 * d.v_stride[1], d.v_stride[1], n, V);
@@ -167,27 +180,29 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
     };
     auto store = [&](int b) {
         fk.store(Rows{sk[b]}, tid);
-        fq.store(Rows{sq[b]}, tid);
         fm.store(MatM{sm[b]}, tid);
-        fp.store(MatP{sp[b]}, tid);
+        if (PASS == 0) {
+            fq.store(Rows{sq[b]}, tid);
+            fp.store(MatP{sp[b]}, tid);
+        }
 #pragma unroll
         for (int j = 0; j * NTH < 3 * kDC; j++)
             if (tid + j * NTH < 3 * kDC) sv[b][tid + j * NTH] = fv[j];
     };
-    if (s.len > 0) {
-        fetch(0);
+    if (begin < stop) {
+        fetch(begin);
         store(0);
     }
     barrier_lds();
-    for (int t0 = 0, b = 0; t0 < s.len; t0 += kDC, b ^= 1) {
+    for (int t0 = begin, b = 0; t0 < stop; t0 += kDC, b ^= 1) {
         const int n = s.len - t0 < kDC ? s.len - t0 : kDC;
         const Rows K{sk[b]}, Q{sq[b]};
         float vc[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) vc[i] = float_of_bits<T>(vv[i]);
-        const bool more = t0 + kDC < s.len;
+        const bool more = t0 + kDC < stop;
         if (more) fetch(t0 + kDC);
-        if (d.states && t0 % (kDC * NS) == 0) {       // S (KP, VP) before the group, for the backward
+        if (PASS == 0 && d.states && t0 % (kDC * NS) == 0) {       // S (KP, VP) before the group, for the backward
             const __amdgpu_buffer_rsrc_t st =
                 make_rsrc(delta_state(a, s.group + t0 / (kDC * NS), h), (uint32_t)(a.VP * KP * 4));
             const int at = v < a.VP ? (g8 * a.VP + v) * 4 : kNowhere;
@@ -208,7 +223,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             const Frag<P> kf[2] = {K.frag(pair_row(0, l16), 32 * p, lane), K.frag(pair_row(1, l16), 32 * p, lane)},
                           qf[2] = {Q.frag(pair_row(0, l16), 32 * p, lane), Q.frag(pair_row(1, l16), 32 * p, lane)};
             mma_n<3>(kf, f, ks);
-            mma_n<LO>(qf, f, o);
+            if (PASS == 0) mma_n<LO>(qf, f, o);
         }
         float G[8], L[8], be[8], x[8], y[8];
 #pragma unroll
@@ -237,7 +252,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
                 y[4 * m + r] = x[4 * m + r] * L[4 * m + r];
             }
         }
-        if (d.states) {
+        if (PASS == 0 && d.states) {
             const __amdgpu_buffer_rsrc_t re =
                 make_rsrc(delta_errors(a, s.group + t0 / (kDC * NS), h), (uint32_t)(a.VP * kDC * NS * 4));
 #pragma unroll
@@ -260,6 +275,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
 #pragma unroll
             for (int i = 0; i < 4; i++) S[k4 + i] = t[i];
         }
+        if constexpr (PASS == 0) {
         const __amdgpu_buffer_rsrc_t ro =
             rows_window(out + ((s.row + t0) * d.H + h) * (int64_t)V, d.H * (int64_t)V, n, V);
 #pragma unroll
@@ -268,10 +284,19 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
 #pragma unroll
             for (int r = 0; r < 4; r++) buf_store<T>(ro, o_off + (4 * m + r) * o_step, (T)o[m][r]);
         }
+        }
         if (more) store(b ^ 1);
         barrier_lds();
     }
-    if (send && v < V)
+    if (PASS == 1 && v < a.VP + KP)
+#pragma unroll
+        for (int kt = 0; kt < NK; kt++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
+                part[k * (a.VP + KP) + v] = S[kt][r];
+            }
+    if (PASS == 0 && last && send && v < V)
 #pragma unroll
         for (int kt = 0; kt < NK; kt++)
 #pragma unroll
@@ -279,6 +304,64 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
                 const int k = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r;
                 if (k < Kd) send[sbase + (int64_t)k * V + v] = S[kt][r];
             }
+}
+
+// Joins the parts of a sequence: S after a part is A S + B. A block owns 16 columns of S, a
+// wave of it 32 rows: its rows of A come from memory, a part ahead, and the waves hand each
+// other their rows of S through LDS. Part 0 began with the sequence's own state, so its B
+// is the state after it.
+template <int KP> __global__ __launch_bounds__(2 * KP) void k_delta_join(DeltaP a) {
+    constexpr int NP = KP / 32;
+    __shared__ alignas(16) bf16x8 sf[2][NP][3][64];
+    const SnHipDelta& d = a.d;
+    const int h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, g8 = (lane >> 4) * 8,
+              v = blockIdx.x * 16 + l16, ld = a.VP + KP, row0 = 32 * wave;
+    const DeltaSeq s = delta_seq(d, blockIdx.z);
+    const int64_t step = d.H * delta_seg_floats(KP, a.VP);
+    float* part = a.seg_state + (blockIdx.z * (int64_t)a.segs * d.H + h) * delta_seg_floats(KP, a.VP);
+    Vec8<float> na[2][NP];
+    float nb[8];
+    auto fetch = [&](const float* from, bool with_a) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) nb[i] = from[(row0 + g8 + i) * ld + v];
+        if (with_a)
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+                    na[m][p] = load_raw8(from + (row0 + pair_row(m, l16)) * ld + a.VP + 32 * p + g8, 8, true);
+    };
+    fetch(part, false);
+    for (int seg = 0; seg + 1 < a.segs && (seg + 1) * a.seg_chunks * kDC < s.len; seg++, part += step) {
+        f32x4 t[2] = {{nb[0], nb[1], nb[2], nb[3]}, {nb[4], nb[5], nb[6], nb[7]}};
+        Frag<3> fa[2][NP];
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+            for (int p = 0; p < NP; p++) fa[m][p] = split_raw8<float>(na[m][p]);
+        const bool more = seg + 2 < a.segs && (seg + 2) * a.seg_chunks * kDC < s.len;
+        if (more) fetch(part + step, true);
+        if (seg)
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                Frag<3> f;
+#pragma unroll
+                for (int i = 0; i < 3; i++) f.p[i] = sf[seg & 1][p][i][lane];
+#pragma unroll
+                for (int m = 0; m < 2; m++) t[m] = mma<3>(fa[m][p], f, t[m]);
+            }
+        float* next = part + step + (int64_t)KP * ld;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            x[i] = t[i >> 2][i & 3];
+            next[(row0 + g8 + i) * a.VP + v] = x[i];
+        }
+        const Frag<3> f = split8<3>(x);
+#pragma unroll
+        for (int i = 0; i < 3; i++) sf[(seg + 1) & 1][wave][i][lane] = f.p[i];
+        barrier_lds();
+    }
 }
 
 // Token by token. A wave owns 32 columns of V of one sequence and head: lane (kg, vg)
@@ -382,8 +465,14 @@ template <typename T, int KP, bool VEC>
 snhip_status fwd_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
     k_delta_prep<T, KP, VEC><<<dim3((unsigned)a.slots, (unsigned)a.d.H), 256, 0, st>>>(a);
     SNHIP_CHECK(hipGetLastError());
-    const dim3 grid((unsigned)((a.VP / 16 + kDeltaW - 1) / kDeltaW), (unsigned)a.d.H, (unsigned)a.d.N);
-    k_delta_scan<T, KP, VEC><<<grid, 64 * kDeltaW, 0, st>>>(a, (T*)out, send);
+    const unsigned H = (unsigned)a.d.H, N = (unsigned)a.d.N, per = 16 * kDeltaW;
+    if (a.segs > 1) {
+        k_delta_scan<T, KP, VEC, 1><<<dim3((a.VP + KP + per - 1) / per, H, N * a.segs), 64 * kDeltaW, 0, st>>>(a, nullptr, nullptr);
+        SNHIP_CHECK(hipGetLastError());
+        k_delta_join<KP><<<dim3(a.VP / 16, H, N), 2 * KP, 0, st>>>(a);
+        SNHIP_CHECK(hipGetLastError());
+    }
+    k_delta_scan<T, KP, VEC, 0><<<dim3((a.VP + per - 1) / per, H, N * a.segs), 64 * kDeltaW, 0, st>>>(a, (T*)out, send);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
@@ -402,6 +491,10 @@ snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
     a->d = *d;
     a->slots = delta_slots(*d);
     a->groups = delta_groups(*d);
+    a->segs = delta_segs(*d);
+    a->seg_chunks = (int)(((d->T + kDC - 1) / kDC + a->segs - 1) / a->segs);
+    if (d->dtype != SNHIP_F32) a->seg_chunks += a->seg_chunks & 1;      // whole groups of the backward
+    a->seg_state = d->chunks + delta_slots(*d) * d->H * kDeltaChunk;
     a->KP = delta_kp(d->K);
     a->VP = delta_vp(d->V);
     a->rep = (int)(d->H / d->Hk);
@@ -420,7 +513,10 @@ using namespace snhip;
 extern "C" {
 
 int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d) {
-    return d ? delta_slots(*d) * d->H * kDeltaChunk : 0;
+    if (!d) return 0;
+    const int64_t segs = delta_segs(*d);
+    return delta_slots(*d) * d->H * kDeltaChunk +
+           (segs > 1 ? d->N * segs * d->H * delta_seg_floats(delta_kp(d->K), delta_vp(d->V)) : 0);
 }
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d) {
     return d ? delta_groups(*d) * d->H * delta_vp(d->V) * (kDC * delta_ns(d->dtype) + (int64_t)delta_kp(d->K)) : 0;

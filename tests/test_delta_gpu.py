@@ -186,6 +186,47 @@ def test_packed_sequences_equal_their_own_calls(gpu, dtype):
             assert torch.equal(p[0], q[i] if m == "s0" else q[0, a:e]), m
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(1, 4100, 1, 1, 8, 5), (1, 5003, 1, 2, 65, 40), (2, 4200, 1, 1, 128, 20)], ids=str)
+def test_long_sequences_in_parts(gpu, shape, dtype):
+    """Few heads and thousands of tokens: the sequence is scanned in parts that are joined.
+    A part's map is one more product of K terms than the scan's own, once a part."""
+    close.dtype = dtype
+    x = inputs(*shape, dtype, seed=21)
+    x["g"] *= 0.01                         # states that reach through several parts
+    x64 = as64(x, True)
+    ro, rs = ref(*x64)
+    leaf = [x[n].requires_grad_() for n in NAMES]
+    out, send = runtime.gated_delta(*leaf)
+    close("out", out, ro, shape[4])
+    close("send", send, rs, shape[4])
+    with torch.no_grad():
+        plain = runtime.gated_delta(*leaf)
+    assert torch.equal(plain[0], out) and torch.equal(plain[1], send)
+    gen = torch.Generator().manual_seed(22)
+    do, ds = torch.randn(ro.shape, generator=gen).to(dtype), torch.randn(rs.shape, generator=gen)
+    want = torch.autograd.grad((ro, rs), x64, (do.double(), ds.double()))
+    got = torch.autograd.grad((out, send), leaf, (do.cuda(), ds.cuda()))
+    for n, a, b in zip(NAMES, got, want):
+        close("d" + n, a, b, shape[4], True)
+
+
+def test_long_packed_sequences_in_parts(gpu):
+    close.dtype = F32
+    lens = [3000, 1, 4000, 0, 700, 2500]
+    x = inputs(1, sum(lens), 1, 2, 24, 16, F32, N=len(lens), seed=23)
+    x["g"] *= 0.01
+    edges = torch.tensor([0] + lens).cumsum(0)
+    out, send = runtime.gated_delta(**x, cu_seqlens=edges.int().cuda())
+    for i, n in enumerate(lens):
+        a, e = int(edges[i]), int(edges[i + 1])
+        one = {m: (x[m][:, a:e] if m != "s0" else x[m][i:i + 1]) for m in NAMES}
+        ro, rs = ref(*as64(one))
+        if n:
+            close("out", out[:, a:e], ro, 24)
+        close("send", send[i:i + 1], rs, 24)
+
+
 def test_edges_outside_the_rows_are_clamped(gpu):
     x = inputs(1, 50, 1, 1, 16, 16, F32, N=2)
     for edges, same in (([-5, 20, 1000], [0, 20, 50]), ([0, 50, 50], [0, 50, 50])):
