@@ -42,9 +42,10 @@ extern "C" {
  * decreases is refused by nothing and gives unspecified results (in bounds).
  *
  * Ranges: 1 <= K <= 128, 1 <= V <= 4096, H a multiple of Hk, H <= 65535, N <= 65535,
- * B T < 2^31. g <= 0 is meant (a decay); -inf forgets the state exactly, other
+ * B T < 2^31, H K, H V and every token stride below 2^24 (strides not negative). g <= 0 is meant (a decay); -inf forgets the state exactly, other
  * values are clamped at -200, where exp(g) is 0 in fp32. Non-finite values reach
- * the results of their sequence and head only, as NaN. */
+ * the results of their sequence and head (in gradients of q and k: of the heads that
+ * share theirs) only, as NaN, from the chunk of 32 tokens that holds them on. */
 typedef struct SnHipDelta {
     const void* q;
     const void* k;
@@ -61,7 +62,8 @@ typedef struct SnHipDelta {
     double scale;
     float* chunks;              /* workspace: snhip_op_delta_chunk_floats floats  */
     float* states;              /* snhip_op_delta_state_floats floats, written by
-                                   the forward for the backward; NULL: not kept   */
+                                   the forward for the backward; NULL: not kept.
+                                   Both workspaces 16-byte aligned                */
 } SnHipDelta;
 
 /* Floats of the two workspaces of a call (the other fields of d are not read). */
@@ -69,7 +71,7 @@ int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d);
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d);
 
 /* out and send (NULL: not wanted). T >= 1, N >= 1. Calls of at most
- * 16 tokens without cu and without states need no workspace (chunks NULL). */
+ * 12 tokens without cu and without states need no workspace (chunks NULL). */
 snhip_status snhip_op_delta_fwd_dev(const SnHipDelta* d, void* out, float* send, void* stream);
 
 /* One or a few tokens: the same recurrence token by token, at any T and without
@@ -80,7 +82,8 @@ snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send
  * dout (B,T,H,V) contiguous, of the inputs' type; dsend (N,H,K,V) or NULL (zeros).
  * dq, dk (B,T,Hk,K), dv (B,T,H,V) contiguous, of the inputs' type, dq and dk summed
  * over the value heads that share them; dg, dbeta (B,T,H) fp32; ds0 (N,H,K,V) fp32
- * or NULL. ws: snhip_op_delta_bwd_floats floats. Sums run in a fixed order. */
+ * or NULL. ws: snhip_op_delta_bwd_floats floats, 16-byte aligned. Sums run in a fixed
+ * order. */
 typedef struct SnHipDeltaGrad {
     const void* dout;
     const float* dsend;

@@ -319,7 +319,7 @@ template <int KP> __global__ __launch_bounds__(2 * KP) void k_delta_join(DeltaP 
     const DeltaSeq s = delta_seq(d, blockIdx.z);
     const int64_t step = d.H * delta_seg_floats(KP, a.VP);
     float* part = a.seg_state + (blockIdx.z * (int64_t)a.segs * d.H + h) * delta_seg_floats(KP, a.VP);
-    Vec8<float> na[2][NP];
+    Vec8<float> na[2][NP] = {};
     float nb[8];
     auto fetch = [&](const float* from, bool with_a) {
 #pragma unroll
@@ -367,42 +367,55 @@ template <int KP> __global__ __launch_bounds__(2 * KP) void k_delta_join(DeltaP 
 // Token by token. A wave owns 32 columns of V of one sequence and head: lane (kg, vg)
 // holds rows kg RPT .. + RPT - 1 and four columns, all in registers from one read of the
 // state to one write. q.S' = a q.S + (q.k) u, so one pass over the state gives both
-// read-outs. Bound by the state's bytes.
-template <typename T, int RPT>
+// read-outs. Bound by the state's bytes; for one sequence by the latency of its reads, so
+// all of them are on their way before the first is used. FOUR: V is a multiple of four.
+template <typename T, int RPT, bool VEC, bool FOUR>
 __global__ __launch_bounds__(64) void k_delta_step(DeltaP a, T* out, const float* s0, float* send) {
     const SnHipDelta& d = a.d;
-    const int h = blockIdx.y, lane = threadIdx.x, kg = lane >> 3, k0 = kg * RPT;
+    const int h = blockIdx.y, lane = threadIdx.x, kg = lane >> 3, k0 = kg * RPT, E = (int)sizeof(T);
     const int V = (int)d.V, Kd = (int)d.K, v0 = blockIdx.x * 32 + (lane & 7) * 4;
     const DeltaSeq s = delta_seq(d, blockIdx.z);
     const int64_t sbase = ((int64_t)blockIdx.z * d.H + h) * d.K * d.V;
-    const bool whole = (V & 3) == 0 && v0 < V;       // four columns at a 16-byte address
+    Vec8<T> nq[RPT / 8], nk[RPT / 8];
+    unsigned nv[4];
+    float ng, nb;
+    auto fetch = [&](int t) {
+        const __amdgpu_buffer_rsrc_t rq = rows_window(delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t, h / a.rep), 0, 1, Kd),
+                                     rk = rows_window(delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t, h / a.rep), 0, 1, Kd),
+                                     rv = rows_window(delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t, h), 0, 1, V);
+        const int64_t row = (s.row + t) * d.H + h;
+        ng = d.g[row];
+        nb = d.beta[row];
+#pragma unroll
+        for (int i = 0; i < RPT / 8; i++) {
+            nq[i] = buf_load8<T>(rq, (k0 + 8 * i) * E, Kd - k0 - 8 * i, VEC);
+            nk[i] = buf_load8<T>(rk, (k0 + 8 * i) * E, Kd - k0 - 8 * i, VEC);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) nv[j] = buf_load_bits<T>(rv, (v0 + j) * E);
+    };
+    if (s.len > 0) fetch(0);
+    // rows from K on lie past the state's bytes, and read as 0; so does a state that is not there
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(s0 ? s0 + sbase : nullptr, s0 ? (uint32_t)(Kd * V * 4) : 0u);
+    auto place = [&](int i, int j) { return v0 + j < V ? ((k0 + i) * V + v0 + j) * 4 : kNowhere; };
     f32x4 S[RPT];
 #pragma unroll
     for (int i = 0; i < RPT; i++) {
-        S[i] = f32x4{0, 0, 0, 0};
-        const int k = k0 + i;
-        if (!s0 || k >= Kd) continue;
-        const float* p = s0 + sbase + (int64_t)k * V + v0;
-        if (whole) {
-            S[i] = *reinterpret_cast<const f32x4*>(p);
+        if constexpr (FOUR) {
+            S[i] = buf_load4(rs, place(i, 0));
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (v0 + j < V) S[i][j] = p[j];
+            for (int j = 0; j < 4; j++) S[i][j] = buf_load<float>(rs, place(i, j));
         }
     }
     for (int t = 0; t < s.len; t++) {
-        const T* qp = delta_at<T>(d.q, d.q_stride, s.b, s.t0 + t, h / a.rep);
-        const T* kp = delta_at<T>(d.k, d.k_stride, s.b, s.t0 + t, h / a.rep);
-        const T* vp = delta_at<T>(d.v, d.v_stride, s.b, s.t0 + t, h);
-        const int64_t row = (s.row + t) * d.H + h;
-        const float al = expf(d.g[row]), be = d.beta[row];
-        float q[RPT], k[RPT];
+        float q[RPT], k[RPT], vv[4];
 #pragma unroll
-        for (int i = 0; i < RPT; i += 8) {
-            load8(qp + k0 + i, Kd - k0 - i, a.vec, q + i);
-            load8(kp + k0 + i, Kd - k0 - i, a.vec, k + i);
-        }
+        for (int i = 0; i < RPT; i++) q[i] = (float)nq[i / 8][i % 8], k[i] = (float)nk[i / 8][i % 8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) vv[j] = float_of_bits<T>(nv[j]);
+        const float al = expf(ng), be = nb;
+        if (t + 1 < s.len) fetch(t + 1);
         f32x4 sk = {0, 0, 0, 0}, sq = {0, 0, 0, 0};
         float qk = 0.f;
 #pragma unroll
@@ -424,12 +437,11 @@ __global__ __launch_bounds__(64) void k_delta_step(DeltaP a, T* out, const float
             }
         }
         f32x4 u;
+        const __amdgpu_buffer_rsrc_t ro = rows_window(out + ((s.row + t) * d.H + h) * (int64_t)V, 0, 1, V);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float vv = v0 + j < V ? (float)vp[v0 + j] : 0.f;
-            u[j] = be * (vv - al * sk[j]);
-            const float o = (float)d.scale * (al * sq[j] + qk * u[j]);
-            if (kg == 0 && v0 + j < V) out[row * V + v0 + j] = (T)o;
+            u[j] = be * (vv[j] - al * sk[j]);
+            buf_store<T>(ro, kg == 0 ? (v0 + j) * E : kNowhere, (T)((float)d.scale * (al * sq[j] + qk * u[j])));
         }
 #pragma unroll
         for (int i = 0; i < RPT; i++)
@@ -437,26 +449,23 @@ __global__ __launch_bounds__(64) void k_delta_step(DeltaP a, T* out, const float
             for (int j = 0; j < 4; j++) S[i][j] = fmaf(k[i], u[j], al * S[i][j]);
     }
     if (!send) return;
+    const __amdgpu_buffer_rsrc_t rt = make_rsrc(send + sbase, (uint32_t)(Kd * V * 4));
 #pragma unroll
     for (int i = 0; i < RPT; i++) {
-        const int k = k0 + i;
-        if (k >= Kd) continue;
-        float* p = send + sbase + (int64_t)k * V + v0;
-        if (whole) {
-            *reinterpret_cast<f32x4*>(p) = S[i];
+        if constexpr (FOUR) {
+            buf_store4(rt, place(i, 0), S[i]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (v0 + j < V) p[j] = S[i][j];
+            for (int j = 0; j < 4; j++) buf_store<float>(rt, place(i, j), S[i][j]);
         }
     }
 }
 
-template <typename T>
+template <typename T, int KP, bool VEC>
 snhip_status step_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
     const dim3 grid((unsigned)((a.d.V + 31) / 32), (unsigned)a.d.H, (unsigned)a.d.N);
-    if (a.KP == 64) k_delta_step<T, 8><<<grid, 64, 0, st>>>(a, (T*)out, a.d.s0, send);
-    else k_delta_step<T, 16><<<grid, 64, 0, st>>>(a, (T*)out, a.d.s0, send);
+    if (a.d.V % 4 == 0) k_delta_step<T, KP / 8, VEC, true><<<grid, 64, 0, st>>>(a, (T*)out, a.d.s0, send);
+    else k_delta_step<T, KP / 8, VEC, false><<<grid, 64, 0, st>>>(a, (T*)out, a.d.s0, send);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
@@ -526,9 +535,9 @@ snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send
     DeltaP a;
     const snhip_status rc = delta_args(d, &a);
     if (rc != SNHIP_OK || !out || !send) return SNHIP_E_INVAL;
-    if (d->dtype == SNHIP_F32) return step_t<float>(a, out, send, as_stream(stream));
-    if (d->dtype == SNHIP_BF16) return step_t<__bf16>(a, out, send, as_stream(stream));
-    return step_t<_Float16>(a, out, send, as_stream(stream));
+    return delta_pick(a, [&](auto t, auto kp, auto vec) {
+        return step_t<decltype(t), decltype(kp)::value, decltype(vec)::value>(a, out, send, as_stream(stream));
+    });
 }
 
 snhip_status snhip_op_delta_fwd_dev(const SnHipDelta* d, void* out, float* send, void* stream) {
@@ -537,10 +546,10 @@ snhip_status snhip_op_delta_fwd_dev(const SnHipDelta* d, void* out, float* send,
     if (rc != SNHIP_OK || !out) return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);
     if (!d->chunks) {
-        if (d->cu || d->states || d->T > 16) return SNHIP_E_INVAL;
-        if (d->dtype == SNHIP_F32) return step_t<float>(a, out, send, st);
-        if (d->dtype == SNHIP_BF16) return step_t<__bf16>(a, out, send, st);
-        return step_t<_Float16>(a, out, send, st);
+        if (d->cu || d->states || d->T > kDeltaStepTokens) return SNHIP_E_INVAL;
+        return delta_pick(a, [&](auto t, auto kp, auto vec) {
+            return step_t<decltype(t), decltype(kp)::value, decltype(vec)::value>(a, out, send, st);
+        });
     }
     return delta_pick(a, [&](auto t, auto kp, auto vec) {
         return fwd_t<decltype(t), decltype(kp)::value, decltype(vec)::value>(a, out, send, st);

@@ -18,6 +18,7 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native
 
@@ -25,7 +26,7 @@ __all__ = ["GatedDelta", "delta_bwd", "delta_fwd", "delta_step", "gated_delta"]
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_K, MAX_V, MAX_HEADS, MAX_STRIDE = 128, 4096, 65535, 1 << 24
-STEP_TOKENS = 16               # at most this many tokens run token by token
+STEP_TOKENS = 12               # at most this many tokens run token by token
 _ARGS = struct.Struct("7P9q8qd2P")     # SnHipDelta
 _GRAD = struct.Struct("9P")            # SnHipDeltaGrad
 
@@ -106,6 +107,10 @@ def delta_fwd(q, k, v, g, beta, s0=None, *, scale=None, cu_seqlens=None, keep=Fa
     ``saved``: what delta_bwd needs (``keep``), else None. ``scale``: K ** -0.5 if None."""
     q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
     dims = _shapes(q, k, v, g, beta, s0, cu_seqlens)
+    return _fwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, keep)
+
+
+def _fwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, keep):
     B, T, N, Hk, H, K, V = dims
     scale = K ** -0.5 if scale is None else float(scale)
     new = torch.empty if cu_seqlens is None else torch.zeros
@@ -135,14 +140,18 @@ def delta_bwd(q, k, v, g, beta, s0, saved, dout, dsend=None, *, scale=None, cu_s
     q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
     dims = _shapes(q, k, v, g, beta, s0, cu_seqlens)
     B, T, N, Hk, H, K, V = dims
-    scale = K ** -0.5 if scale is None else float(scale)
     if dout.shape != (B, T, H, V) or dout.dtype != v.dtype or dout.device != q.device:
         raise ValueError("dout must be (B,T,H,V), of the inputs' type and device")
     if dsend is not None:
         _check_state(dsend, (N, H, K, V), "dsend")
         if dsend.device != q.device:
             raise ValueError("the delta rule takes tensors of one GPU")
-    dout = dout.contiguous()
+    return _bwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, saved, dout.contiguous(), dsend, need_ds0)
+
+
+def _bwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, saved, dout, dsend, need_ds0):
+    B, T, N, Hk, H, K, V = dims
+    scale = K ** -0.5 if scale is None else float(scale)
     new = torch.empty if cu_seqlens is None else torch.zeros
     dq, dk = (new(B, T, Hk, K, dtype=q.dtype, device=q.device) for _ in range(2))
     dv = new(B, T, H, V, dtype=q.dtype, device=q.device)
@@ -171,29 +180,27 @@ class GatedDelta(torch.autograd.Function):
     def forward(ctx, q, k, v, g, beta, s0, scale, cu_seqlens):
         q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
         s0 = None if s0 is None else s0.contiguous()
-        keep = any(ctx.needs_input_grad)
-        out, send, saved = delta_fwd(q, k, v, g, beta, s0, scale=scale, cu_seqlens=cu_seqlens, keep=keep)
-        if keep:
-            ctx.save_for_backward(q, k, v, g, beta, s0, cu_seqlens, *saved)
-            ctx.scale = scale
-            ctx.set_materialize_grads(False)
+        dims = _shapes(q, k, v, g, beta, s0, cu_seqlens)
+        out, send, saved = _fwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, True)
+        ctx.save_for_backward(q, k, v, g, beta, s0, cu_seqlens, *saved)
+        ctx.scale, ctx.dims = scale, dims
+        ctx.set_materialize_grads(False)
         return out, send
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dsend):
         q, k, v, g, beta, s0, cu, *saved = ctx.saved_tensors
-        if dout is None:
-            dout = torch.zeros(*v.shape, dtype=v.dtype, device=v.device)
+        dout = torch.zeros(v.shape, dtype=v.dtype, device=v.device) if dout is None else dout.contiguous()
         if dsend is not None:
             dsend = dsend.contiguous()
-        grads = delta_bwd(q, k, v, g, beta, s0, saved, dout, dsend, scale=ctx.scale, cu_seqlens=cu,
-                          need_ds0=ctx.needs_input_grad[5])
+        grads = _bwd(q, k, v, g, beta, s0, cu, ctx.dims, ctx.scale, saved, dout, dsend, ctx.needs_input_grad[5])
         return *grads, None, None
 
 
 def gated_delta(q, k, v, g, beta, s0=None, *, scale=None, cu_seqlens=None):
     """(out, send) of the gated delta rule under autograd (shapes: delta_fwd). Without
-    a gradient to keep anything for, calls of up to 16 tokens run token by token."""
+    a gradient to keep anything for, calls of up to 12 tokens run token by token."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, s0)):
         return GatedDelta.apply(q, k, v, g, beta, s0, scale, cu_seqlens)
     if s0 is not None:

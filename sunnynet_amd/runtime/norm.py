@@ -5,6 +5,7 @@ divided by ``sqrt(var + eps)``, times a gain, plus a centre.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _native
 from .delta import DTYPES, _ptr
@@ -79,12 +80,12 @@ class LayerNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         x = x.contiguous()
         weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-        y, mean, rstd = norm_fwd(x, weight, bias, eps, keep=any(ctx.needs_input_grad))
-        if mean is not None:
-            ctx.save_for_backward(x, weight, mean, rstd)
+        y, mean, rstd = norm_fwd(x, weight, bias, eps, keep=True)
+        ctx.save_for_backward(x, weight, mean, rstd)
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         return *_bwd(dy.contiguous(), x, weight, mean, rstd, ctx.needs_input_grad[:3], mean.shape[0], x.shape[-1]), None
