@@ -30,6 +30,8 @@ constexpr int kDC = 32;                            // tokens per chunk
 // and beta (32 each).
 constexpr int kDeltaP = 1536, kDeltaG = 3072, kDeltaChunk = 3168;
 
+// Tokens of a call: positions inside a sequence, and a part's end past it, fit 32 bits.
+constexpr int64_t kDeltaTokens = (1 << 30) - 1;
 // The longest call that runs token by token without workspaces. 12 heads of 64, one
 // sequence: 11.5 us token by token and 11.8 in chunks at 12 tokens; 64 sequences of 16
 // heads of 128: 46 and 78 us (57 and 78 at 16).

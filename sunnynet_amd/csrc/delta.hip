@@ -492,9 +492,11 @@ snhip_status fwd_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
 snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
     if (!d || !d->q || !d->k || !d->v || !d->g || !d->beta) return SNHIP_E_INVAL;
     if (d->B < 1 || d->T < 1 || d->N < 1 || d->N > 65535 || d->H < 1 || d->H > 65535 || d->Hk < 1 ||
-        d->H % d->Hk || d->K < 1 || d->K > 128 || d->V < 1 || d->V > 4096 || d->T > INT32_MAX / d->B ||
+        d->H % d->Hk || d->K < 1 || d->K > 128 || d->V < 1 || d->V > 4096 || d->T > kDeltaTokens / d->B ||
         (d->cu ? d->B != 1 : d->N != d->B) || d->H * d->V >= kDeltaStride || d->H * d->K >= kDeltaStride || d->dtype < SNHIP_F32 || d->dtype > SNHIP_F16)
         return SNHIP_E_INVAL;
+    for (const void* w : {(const void*)d->chunks, (const void*)d->states})
+        if (reinterpret_cast<uintptr_t>(w) % 16) return SNHIP_E_INVAL;
     for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride})
         if (st[1] < 0 || st[1] >= kDeltaStride) return SNHIP_E_INVAL;
     a->d = *d;

@@ -551,7 +551,7 @@ snhip_status snhip_op_delta_bwd_dev(const SnHipDelta* d, const SnHipDeltaGrad* g
     DeltaP a;
     const snhip_status rc = delta_args(d, &a);
     if (rc != SNHIP_OK || !gr || !d->chunks || !d->states || !gr->dout || !gr->dq || !gr->dk || !gr->dv ||
-        !gr->dg || !gr->dbeta || !gr->ws)
+        !gr->dg || !gr->dbeta || !gr->ws || reinterpret_cast<uintptr_t>(gr->ws) % 16)
         return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);
     return delta_pick(a, [&](auto t, auto kp, auto vec) {

@@ -56,8 +56,8 @@ def _shapes(q, k, v, g, beta, s0, cu, step=False):
                          f"got K = {K}, V = {V}, {H} heads")
     if H * max(K, V) >= MAX_STRIDE:
         raise ValueError(f"H * K and H * V must be below {MAX_STRIDE}")
-    if B * T >= 1 << 31:
-        raise ValueError("B * T must be below 2^31")
+    if B * T >= 1 << 30:
+        raise ValueError("B * T must be below 2^30")
     if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("q, k and v must be float32, bfloat16 or float16, all three the same")
     if g.dtype != torch.float32 or beta.dtype != torch.float32:
@@ -214,6 +214,9 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
     ``send``. No autograd."""
     if q.dim() != 3 or v.dim() != 3 or k.dim() != 3 or g.dim() != 2 or beta.dim() != 2:
         raise ValueError("shape mismatch: q, k (B,Hk,K); v (B,H,V); g, beta (B,H)")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or beta.requires_grad or s.requires_grad):
+        raise RuntimeError("delta_step keeps nothing for a backward pass: call gated_delta, or use torch.no_grad()")
     q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
     dims = _shapes(q, k, v, g, beta, s, None, step=True)
     B, _, N, Hk, H, K, V = dims

@@ -24,6 +24,8 @@ def _setting(x, name, B, device, dtype):
         return None, x
     if x.shape != (B,) or x.device != device or x.dtype.is_complex or x.dtype == torch.bool:
         raise ValueError(f"{name} must be a number or a vector of one number per row on the logits' device")
+    if x.dtype == torch.int64 and dtype == torch.int32:
+        x = x.clamp(max=MAX_V)             # as large as any row: no filter, and not another number in 32 bits
     return x.to(dtype).contiguous(), 0
 
 

@@ -332,6 +332,47 @@ def test_prompt_then_steps_equal_one_prompt(gpu):
     close("send", s, rs, 64)
 
 
+def test_views_that_the_kernels_do_not_take_are_copied(gpu):
+    """Expanded axes (stride 0) are read in place; a token stride of 2^24 is copied."""
+    x = inputs(2, 40, 1, 2, 16, 16, F32, seed=30)
+    same = dict(x, q=x["q"][:, :1].expand(-1, 40, -1, -1), k=x["k"][:1].expand(2, -1, -1, -1))
+    want = runtime.gated_delta(**{n: t.clone() for n, t in same.items()})
+    got = runtime.gated_delta(**same)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    far = torch.zeros(2, 3, 1 << 24, dtype=F16, device="cuda")
+    half = {n: t[:, :3].half() if n in "qkv" else t[:, :3].contiguous() if n != "s0" else t for n, t in x.items()}
+    far[:, :, :16] = half["q"][:, :, 0]
+    view = far[:, :, None, :16]
+    assert view.stride(1) == 1 << 24
+    a, b = runtime.gated_delta(**half), runtime.gated_delta(**dict(half, q=view))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_second_derivatives_are_refused(gpu):
+    x = inputs(1, 20, 1, 1, 8, 8, F32)
+    leaf = [x[n].requires_grad_() for n in NAMES]
+    out, _ = runtime.gated_delta(*leaf)
+    grad, = torch.autograd.grad(out.sum(), leaf[:1], create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams share nothing: each has the results of a call alone."""
+    xs = [inputs(2, 300, 1, 2, 64, 64, BF16, seed=40 + i) for i in range(2)]
+    want = [runtime.gated_delta(**x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(3):
+        got = []
+        for st, x in zip(streams, xs):
+            with torch.cuda.stream(st):
+                got.append(runtime.gated_delta(**x))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_no_tokens_and_no_sequences(gpu):
     x = inputs(2, 0, 1, 2, 8, 8, F32)
     out, send = runtime.gated_delta(**x)

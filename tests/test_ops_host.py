@@ -51,6 +51,15 @@ def test_delta_step_refuses():
             runtime.delta_step(y["q"], y["k"], y["v"], y["g"], y["beta"], y["s0"])
 
 
+def test_delta_step_refuses_a_tape():
+    x = {n: t[:, 0] if n != "s0" else t for n, t in good().items()}
+    x["v"].requires_grad_()
+    with pytest.raises(RuntimeError, match="gated_delta"):
+        runtime.delta_step(x["q"], x["k"], x["v"], x["g"], x["beta"], x["s0"])
+    with torch.no_grad(), pytest.raises(ValueError, match="one GPU"):
+        runtime.delta_step(x["q"], x["k"], x["v"], x["g"], x["beta"], x["s0"])
+
+
 def test_norm_refuses():
     x, w = torch.zeros(4, 8), torch.ones(8)
     for args, what in (((x, torch.ones(7)), "length D"), ((x, w.half()), "float32"), ((x.double(),), "float32"),
@@ -83,7 +92,7 @@ def test_c_calls_refuse():
     bad = [dict(q=0), dict(dims=(0, T, 0, Hk, H, K, V)), dict(dims=(B, 0, B, Hk, H, K, V)),
            dict(dims=(B, T, B + 1, Hk, H, K, V)), dict(dims=(B, T, B, 3, H, K, V)),
            dict(dims=(B, T, B, Hk, H, 129, V)), dict(dims=(B, T, B, Hk, H, K, 4097)),
-           dict(dims=(B, T, B, Hk, H, 0, V)), dict(dims=(2, 1 << 30, 2, Hk, H, K, V)),
+           dict(dims=(B, T, B, Hk, H, 0, V)), dict(dims=(2, 1 << 29, 2, Hk, H, K, V)), dict(dims=(1, 1 << 30, 1, Hk, H, K, V)),
            dict(dims=(B, T, 3, Hk, H, K, V), cu=P), dict(dims=(65536, 1, 65536, Hk, H, K, V)), dict(dtype=3),
            dict(dtype=-1)]
     grads = delta._GRAD.pack(*[P] * 9)
@@ -93,6 +102,12 @@ def test_c_calls_refuse():
         assert L.snhip_op_delta_step_dev(a, P, P, None) == -1, b
         assert L.snhip_op_delta_bwd_dev(a, grads, None) == -1, b
     assert L.snhip_op_delta_fwd_dev(_delta(), None, P, None) == -1
+    assert L.snhip_op_delta_fwd_dev(_delta(chunks=P + 4), P, P, None) == -1          # workspaces 16-byte aligned
+    assert L.snhip_op_delta_fwd_dev(_delta(states=P + 8), P, P, None) == -1
+    assert L.snhip_op_delta_bwd_dev(_delta(states=P), delta._GRAD.pack(*[P] * 8, P + 4), None) == -1
+    wide = delta._ARGS.pack(P, P, P, P, P, 0, 0, *([1, 1 << 24, 1] * 3), B, T, B, Hk, H, K, V, 0, 1.0, P, 0)
+    back = delta._ARGS.pack(P, P, P, P, P, 0, 0, *([1, -1, 1] * 3), B, T, B, Hk, H, K, V, 0, 1.0, P, 0)
+    assert L.snhip_op_delta_fwd_dev(wide, P, P, None) == -1 and L.snhip_op_delta_fwd_dev(back, P, P, None) == -1
     assert L.snhip_op_delta_fwd_dev(None, P, P, None) == -1
     assert L.snhip_op_delta_step_dev(_delta(), P, None, None) == -1
     # without a workspace only short calls

@@ -73,7 +73,7 @@ MIXES = [(1.0, 0, 1.0, 0.0), (0.7, 40, 1.0, 0.0), (0.9, 0, 0.9, 0.0), (1.3, 0, 1
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("V", [1, 2, 63, 64, 65, 1000, 1025, 4096, 12000, 32000, 65536, 151001])
+@pytest.mark.parametrize("V", [1, 2, 3, 4, 5, 63, 64, 65, 1000, 1025, 4096, 12000, 32000, 65536, 151001])
 def test_sample(gpu, V, dtype):
     rng = np.random.default_rng(V)
     B = 5 if V > 50000 else 12
@@ -155,6 +155,13 @@ def test_strides_and_types_of_settings(gpu):
     for view in (wide[:, 3:503], wide[::2], wide.t()[:10], wide[:1].expand(10, 700), wide[0:10, 5:6]):
         want = runtime.sample_tokens(view.contiguous(), u[:view.shape[0]], 0.7, 30, 0.9)
         assert torch.equal(runtime.sample_tokens(view, u[:view.shape[0]], 0.7, 30, 0.9), want)
+    for dt in (torch.bfloat16, torch.float16):                   # rows at odd addresses
+        half = wide.to(dt)
+        for view in (half[:, 1:698], half.reshape(-1)[3:3 + 9 * 701].view(9, 701), half[1::3, 7:]):
+            want = runtime.sample_tokens(view.contiguous(), u[:view.shape[0]], 0.7, 30, 0.9)
+            assert torch.equal(runtime.sample_tokens(view, u[:view.shape[0]], 0.7, 30, 0.9), want)
+    big = torch.full((10,), (1 << 32) + 5, dtype=torch.int64, device="cuda")      # above every V: no filter
+    assert torch.equal(runtime.sample_tokens(wide, u, 1.5, big), runtime.sample_tokens(wide, u, 1.5))
     f = u.float()
     assert torch.equal(runtime.sample_tokens(wide, f), runtime.sample_tokens(wide, f.double()))
     a = runtime.sample_tokens(wide, u, torch.full((10,), 0.5).cuda(), torch.full((10,), 3).cuda(), 0.75, 0.125)
