@@ -237,7 +237,8 @@ __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaG
     constexpr int P = ElemPlanes<T>::n, VT = 64, NW = KP / 16, NTH = 64 * NW;
     constexpr int TILES = NM * (NM + 1) / 2, NT = (2 * TILES + NW - 1) / NW;   // of Y, then of F; per wave
     typedef Tile<P, C, KP> Rows;
-    typedef Tile<3, VT, C> Cols;
+    // C = 32: rows of 64 bytes; C = 64: of 192, where LDS holds that beside the 16-bit tiles
+    typedef Tile<3, VT, C, NS == 1 ? 0 : P == 1 ? 32 : 8> Cols;
     typedef Tile<3, C, C> Mat;
     static_assert(Cols::elems >= Mat::elems, "Y and F take the places of E and W");
     __shared__ alignas(16) __bf16 sk[Rows::elems], sq[Rows::elems], se[Cols::elems], sw[Cols::elems],

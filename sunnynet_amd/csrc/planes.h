@@ -90,9 +90,10 @@ __device__ __forceinline__ void mma_n(const Frag<NA> (&a)[N], const Frag<NB>& b,
 __device__ __forceinline__ int pair_row(int m, int i) { return 8 * (i >> 2) + 4 * m + (i & 3); }
 
 // A tile of P planes of R rows and C columns in LDS. Rows are padded by 16 bytes, which
-// spreads a product's 16 rows over the banks.
-template <int P, int R, int C> struct Tile {
-    static constexpr int ld = C + 8;
+// spreads the 16 rows of a frag over the banks; a tile that is only read transposed does
+// better with rows 64 bytes apart modulo 256, which spreads the four rows of a tfrag.
+template <int P, int R, int C, int PAD = 8> struct Tile {
+    static constexpr int ld = C + PAD;
     static constexpr int elems = P * R * ld;
     __bf16* s;
     __device__ __forceinline__ __bf16* at(int p, int r, int c) const { return s + (p * R + r) * ld + c; }
