@@ -57,11 +57,14 @@ __host__ __device__ inline int64_t delta_slots(const SnHipDelta& d) {
 __host__ __device__ inline int delta_kp(int64_t K) { return K <= 64 ? 64 : 128; }
 __host__ __device__ inline int delta_vp(int64_t V) { return (int)((V + 15) / 16 * 16); }
 
-// The backward takes NS chunks at a time (two for 16-bit inputs, whose tiles leave LDS for
-// it; one for fp32): states are kept per such group, which halves their bytes.
-__host__ __device__ constexpr int delta_ns(int64_t dtype) { return dtype == SNHIP_F32 ? 1 : 2; }
+// The backward takes NS chunks at a time, and states are kept per such group. Two halve the
+// bytes of the states: forward and backward of 8 x 2048 tokens, 16 heads of 128 in bf16,
+// take 1.13 ms with two and 1.38 with one. Heads of up to 64 have a quarter of those bytes,
+// and their tiles of one chunk leave room for more blocks on a CU (0.67 ms with one, 0.77
+// with two); three planes of fp32 leave no room for two.
+__host__ __device__ constexpr int delta_ns(int64_t dtype, int64_t K) { return dtype == SNHIP_F32 || K <= 64 ? 1 : 2; }
 __host__ __device__ inline int64_t delta_groups(const SnHipDelta& d) {
-    const int64_t n = kDC * delta_ns(d.dtype);
+    const int64_t n = kDC * delta_ns(d.dtype, d.K);
     return d.cu ? d.T / n + d.N : d.B * ((d.T + n - 1) / n);
 }
 // What the forward keeps for the backward, per group and head: S (KP, VP) before it, and
@@ -71,7 +74,7 @@ __host__ __device__ inline float* delta_state(const DeltaP& a, int64_t group, in
 }
 __host__ __device__ inline float* delta_errors(const DeltaP& a, int64_t group, int h) {
     return a.d.states + a.groups * a.d.H * (int64_t)(a.VP * a.KP) +
-           (group * a.d.H + h) * (int64_t)(a.VP * kDC * delta_ns(a.d.dtype));
+           (group * a.d.H + h) * (int64_t)(a.VP * kDC * delta_ns(a.d.dtype, a.d.K));
 }
 
 // Few heads and a long sequence leave the scan a handful of waves. Then the sequence is
@@ -110,14 +113,14 @@ __device__ __forceinline__ DeltaSeq delta_seq(const SnHipDelta& d, int64_t n) {
         s.b = 0;
         s.len = (int)(e > a ? e - a : 0);
         s.slot = a / kDC + n;
-        s.group = a / (kDC * delta_ns(d.dtype)) + n;
+        s.group = a / (kDC * delta_ns(d.dtype, d.K)) + n;
     } else {
         s.row = n * d.T;
         s.t0 = 0;
         s.b = n;
         s.len = (int)d.T;
         s.slot = n * ((d.T + kDC - 1) / kDC);
-        const int64_t c = kDC * delta_ns(d.dtype);
+        const int64_t c = kDC * delta_ns(d.dtype, d.K);
         s.group = n * ((d.T + c - 1) / c);
     }
     return s;

@@ -121,7 +121,7 @@ template <typename T, int KP, bool VEC, int PASS>
 __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, float* send) {
     constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W;
     constexpr int LO = sizeof(T) == 4 ? 3 : 2;      // planes of the products that only reach out
-    constexpr int NS = sizeof(T) == 4 ? 1 : 2;
+    constexpr int NS = sizeof(T) == 4 || KP == 64 ? 1 : 2;
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, kDC, kDC> MatM;
     typedef Tile<LO, kDC, kDC> MatP;
@@ -530,7 +530,7 @@ int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d) {
            (segs > 1 ? d->N * segs * d->H * delta_seg_floats(delta_kp(d->K), delta_vp(d->V)) : 0);
 }
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d) {
-    return d ? delta_groups(*d) * d->H * delta_vp(d->V) * (kDC * delta_ns(d->dtype) + (int64_t)delta_kp(d->K)) : 0;
+    return d ? delta_groups(*d) * d->H * delta_vp(d->V) * (kDC * delta_ns(d->dtype, d->K) + (int64_t)delta_kp(d->K)) : 0;
 }
 
 snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send, void* stream) {

@@ -30,14 +30,14 @@ struct DeltaWs {
     float* eu;
 };
 __host__ __device__ inline DeltaWs delta_ws(const DeltaP& a, float* ws, int64_t group, int h) {
-    const int64_t i = group * a.d.H + h, n = a.groups * a.d.H, c = kDC * delta_ns(a.d.dtype), w = c * a.VP,
+    const int64_t i = group * a.d.H + h, n = a.groups * a.d.H, c = kDC * delta_ns(a.d.dtype, a.d.K), w = c * a.VP,
                   ds = (int64_t)a.VP * a.KP;
     return {ws + i * w, ws + n * w + i * ds, ws + n * (w + ds) + i * (a.VP / 16 * c)};
 }
 
 template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDeltaGrad gr) {
-    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W, NS = sizeof(T) == 4 ? 1 : 2, C = kDC * NS;
+    constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W, NS = sizeof(T) == 4 || KP == 64 ? 1 : 2, C = kDC * NS;
     typedef Tile<P, kDC, KP> Rows;
     typedef Tile<3, kDC, kDC> Mat;
     __shared__ alignas(16) __bf16 sk[2][Rows::elems], sq[2][Rows::elems], sm[2][Mat::elems], sp[2][Mat::elems];
@@ -233,7 +233,7 @@ __device__ __forceinline__ float sum_groups(float x) {
 // the bytes of S and dS, and by the latency of its steps.
 template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
-    constexpr int NS = sizeof(T) == 4 ? 1 : 2, C = kDC * NS, NM = 2 * NS;      // NM tiles of 16 tokens
+    constexpr int NS = sizeof(T) == 4 || KP == 64 ? 1 : 2, C = kDC * NS, NM = 2 * NS;      // NM tiles of 16 tokens
     constexpr int P = ElemPlanes<T>::n, VT = 64, NW = KP / 16, NTH = 64 * NW;
     constexpr int TILES = NM * (NM + 1) / 2, NT = (2 * TILES + NW - 1) / NW;   // of Y, then of F; per wave
     typedef Tile<P, C, KP> Rows;
@@ -544,7 +544,7 @@ extern "C" {
 
 int64_t snhip_op_delta_bwd_floats(const SnHipDelta* d) {
     if (!d) return 0;
-    const int64_t c = kDC * delta_ns(d->dtype);
+    const int64_t c = kDC * delta_ns(d->dtype, d->K);
     return delta_groups(*d) * d->H * delta_vp(d->V) * (c + delta_kp(d->K) + c / 16);
 }
 
