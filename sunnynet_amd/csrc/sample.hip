@@ -219,7 +219,7 @@ __device__ __forceinline__ void end_bin(bool by_sum, u64 limit, unsigned count, 
 struct Cut {
     float x;
     int end;
-    __device__ __forceinline__ bool keeps(int i, float y) const { return y > x || (y == x && i < end); }
+    __device__ __forceinline__ bool keeps(int i, float y) const { return (y > x) | ((y == x) & (i < end)); }
 };
 
 // The first index at which the running total of val(i, x) over indices exceeds
@@ -229,10 +229,10 @@ template <typename D, typename F, typename G> __device__ __forceinline__ int fin
     __syncthreads();
     if (tid == 0) s.pick = s.bin = -1;
     row.each_slab([&](int j, int i, f32x4 x) {
-        u64 t = 0;
+        u64 v[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) t += val(i + e, x[e]);
-        t = wave_sum(t);
+        for (int e = 0; e < 4; e++) v[e] = val(i + e, x[e]);
+        const u64 t = wave_sum(v[0] + v[1] + (v[2] + v[3]));
         if (lane == 0) s.group[j][wave] = t;
     });
     __syncthreads();
@@ -485,13 +485,18 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
     }
     if (some_p) {
         u64 t = 0;
-        row.each([&](int, float x) {
-            const int i = bin_of(x);
-            if (i < kBins && x >= cut.x) {
-                const u64 y = w(x, s);
-                t += y;
-                atomicAdd(&s.count[i], 1u);
-                atomicAdd(&s.sum[i], y);
+        row.each_slab([&](int, int, f32x4 x) {
+            u64 y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = w(x[e], s);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = bin_of(x[e]);
+                if (i < kBins && x[e] >= cut.x) {
+                    t += y[e];
+                    atomicAdd(&s.count[i], 1u);
+                    atomicAdd(&s.sum[i], y[e]);
+                }
             }
         });
         t = wave_sum(t);
@@ -544,10 +549,11 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
             cut = cut_by_keys(row, w, s.low_key, s.high_key, true, limit, s.above_count, above, s);
         }
     }
+    // weights first, choices after: a branch per token would wait for the table token by token
     auto kept = [&](int i, float x) -> u64 {
-        if (!cut.keeps(i, x)) return 0;
         const double y = w.real(x, s);
-        return y < w.low ? 0 : w.whole(y);
+        const u64 n = w.whole(y);
+        return (cut.keeps(i, x) & !(y < w.low)) ? n : 0;
     };
     const int pick = find_index(row, s, kept, point_of);
     if (pick < 0) return first_max();
