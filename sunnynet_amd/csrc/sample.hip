@@ -2,8 +2,8 @@
 //
 // With m the largest logit, token i weighs exp((x_i - m) / T). The filters keep, in the
 // descending order of the logits, a prefix each: top-k by count, top-p by share, min-p by
-// weight. So a row needs no sort: it needs the place at which a prefix ends. A block holds
-// its row in registers (rows of up to 65536; longer ones are read again) and
+// weight. So a row needs no sort: it needs the place at which a prefix ends. A block has a
+// row, which it reads again in each pass (from L2: the first pass has brought it there), and
 //   - counts, or sums, the row into 2048 bins of equal width of (m - x) / T in LDS, down to
 //     where weights are 0, and finds the bin in which the prefix ends;
 //   - takes that bin's few tokens (for top-k all tokens from it up, if few) into a list and
@@ -17,6 +17,10 @@
 // the LDS atomics nor the division of the row change a result, and the rounding of a
 // weight (2^-42 of the largest for 2^20 tokens, 2^-47 for 32000) is far below what a sum
 // of 32-bit floats would leave.
+//
+// With few rows the time is that of one block's passes, not of memory: a pass takes about
+// 0.5 us per 4,096 tokens, 1 us where it computes weights. 64 rows of 32000: 7 us for the
+// largest logit alone, 16 us without filters, 15 us with top-k 40, 33 us with top-p 0.9.
 #include "common.h"
 #include "planes.h"
 #include "snhip_ops.h"
@@ -24,9 +28,8 @@
 namespace snhip {
 namespace {
 
-constexpr int kBins = 2048, kThreads = 1024, kWaves = kThreads / 64;
-constexpr int kSlab = 4 * kThreads;          // tokens of one pass: four neighbours a thread
-constexpr int kSlabs = (1 << 20) / kSlab;
+constexpr int kBins = 2048;
+constexpr int kGroup = 256;                  // neighbouring tokens of a wave: four a lane
 constexpr int kList = 256;
 constexpr float kRange = 44.f;               // exp(-44) is 0 in the scaled weights
 typedef unsigned long long u64;
@@ -44,18 +47,18 @@ struct Shared {
     u64 sum[kBins];                // of bins; the groups' sums at the end
     unsigned count[kBins];
     double exp2[128];              // 2^(j / 128)
-    u64 wsum[kWaves];
-    unsigned wcount[kWaves];
+    u64 wsum[16];
+    unsigned wcount[16];
     float lx[kList];               // the list: logits, indices, weights
     int li[kList];
     u64 lw[kList];
-    float wmax[kWaves];
-    int windex[kWaves];
+    float wmax[16];
+    int windex[16];
     unsigned listed, low_key, high_key;
     int bin, pick;
     u64 above_sum, total;
     unsigned above_count;
-    u64 group[kSlabs][kWaves];     // kept weight of 256 neighbouring tokens
+    u64 group[(1 << 20) / kGroup];        // kept weight of kGroup neighbouring tokens
 };
 
 // exp((x - m) / T) 2^bits, in 64 bits: 2^(n / 128) from the table, the rest (below
@@ -99,24 +102,25 @@ __device__ __forceinline__ u64 wave_sum(u64 x) {
     return t;
 }
 
-// A row, read where it is used: a slab of kSlab tokens at a time, the next one on its way
+// A row, read where it is used: a slab of 4 TH tokens at a time, the next one on its way
 // (a row of 65536 fp32 is 256 KB, in L2 after the first pass; held in registers it made
 // every pass spill). A thread has four neighbouring tokens of a slab, from first(j) on. In
 // the last, partial slab that is at most V - 4, so that every read is of four tokens inside
 // the row; those that a neighbour has already, and whole reads past the end, count as -inf.
 // Rows of fewer than four tokens (ONE) are read one by one.
-template <typename T, bool ONE> struct RowData {
+template <typename T, bool ONE, int TH> struct RowData {
+    static constexpr int threads = TH, waves = TH / 64, slab = 4 * TH;
     typedef T T4 __attribute__((ext_vector_type(4)));
     const T* p;
     int V, full, slabs;            // whole slabs, and all
     __device__ __forceinline__ void init(const T* at, int n) {
         p = at;
         V = n;
-        full = V / kSlab;
-        slabs = (V + kSlab - 1) / kSlab;
+        full = V / slab;
+        slabs = (V + slab - 1) / slab;
     }
     __device__ __forceinline__ int first(int j) const {
-        const int i = j * kSlab + 4 * (int)threadIdx.x;
+        const int i = j * slab + 4 * (int)threadIdx.x;
         return ONE || i < V - 4 ? i : V - 4;
     }
     __device__ __forceinline__ T4 fetch(int i) const {
@@ -131,7 +135,7 @@ template <typename T, bool ONE> struct RowData {
         }
     }
     __device__ __forceinline__ f32x4 load(int j) const {
-        const int want = j * kSlab + 4 * (int)threadIdx.x, i = first(j);
+        const int want = j * slab + 4 * (int)threadIdx.x, i = first(j);
         const T4 t = fetch(i);
         f32x4 v;
 #pragma unroll
@@ -144,8 +148,8 @@ template <typename T, bool ONE> struct RowData {
             int i = 4 * (int)threadIdx.x;
             T4 t = fetch(i);
 #pragma unroll 1
-            for (int j = 0; j < full; j++, i += kSlab) {
-                const T4 next = fetch(j + 1 < full ? i + kSlab : i);
+            for (int j = 0; j < full; j++, i += slab) {
+                const T4 next = fetch(j + 1 < full ? i + slab : i);
                 f32x4 v;
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = (float)t[e];
@@ -164,8 +168,8 @@ template <typename T, bool ONE> struct RowData {
     }
 };
 
-__device__ __forceinline__ void clear_bins(Shared& s) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) {
+template <int TH> __device__ __forceinline__ void clear_bins(Shared& s) {
+    for (int i = threadIdx.x; i < kBins; i += TH) {
         s.sum[i] = 0;
         s.count[i] = 0;
     }
@@ -180,13 +184,21 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
 // The last used bin before which fewer than `limit` tokens lie (or, by sum, a weight of
 // at most `limit`), counting from (count, sum) above the first bin. -1: no bin is used.
 // Leaves the bin and what lies above it in s.
-__device__ __forceinline__ void end_bin(bool by_sum, u64 limit, unsigned count, u64 sum, Shared& s) {
+template <int TH> __device__ __forceinline__ void end_bin(bool by_sum, u64 limit, unsigned count, u64 sum, Shared& s) {
+    constexpr int NB = kBins / TH, NW = TH / 64;          // bins of a thread
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __syncthreads();
-    const unsigned c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
-    const u64 s0 = s.sum[2 * tid], s1 = s.sum[2 * tid + 1];
-    unsigned c = c0 + c1;
-    u64 t = s0 + s1;
+    unsigned ci[NB], c = 0;
+    u64 ti[NB], t = 0;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        ci[i] = s.count[NB * tid + i];
+        ti[i] = s.sum[NB * tid + i];
+        c += ci[i];
+        t += ti[i];
+    }
+    const unsigned mine_c = c;
+    const u64 mine_t = t;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const unsigned y = __shfl_up(c, o);
@@ -196,20 +208,26 @@ __device__ __forceinline__ void end_bin(bool by_sum, u64 limit, unsigned count, 
     if (lane == 63) s.wcount[wave] = c, s.wsum[wave] = t;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) {
+    for (int w = 0; w < NW; w++) {
         c += w < wave ? s.wcount[w] : 0;
         t += w < wave ? s.wsum[w] : 0;
     }
-    c += count - (c0 + c1);            // above the first of this thread's two bins
-    t += sum - (s0 + s1);
-    const bool a0 = c0 && (by_sum ? t <= limit : c < limit);
-    const bool a1 = c1 && (by_sum ? t + s0 <= limit : c + c0 < limit);
-    const int mine = a1 ? 2 * tid + 1 : a0 ? 2 * tid : -1;
+    c += count - mine_c;               // above the first of this thread's bins
+    t += sum - mine_t;
+    int mine = -1;
+    unsigned above_c = 0;
+    u64 above_t = 0;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        if (ci[i] && (by_sum ? t <= limit : c < limit)) mine = NB * tid + i, above_c = c, above_t = t;
+        c += ci[i];
+        t += ti[i];
+    }
     if (mine >= 0) atomicMax(&s.bin, mine);
     __syncthreads();
     if (mine >= 0 && mine == s.bin) {
-        s.above_count = a1 ? c + c0 : c;
-        s.above_sum = a1 ? t + s0 : t;
+        s.above_count = above_c;
+        s.above_sum = above_t;
     }
     __syncthreads();
 }
@@ -233,12 +251,12 @@ template <typename D, typename F, typename G> __device__ __forceinline__ int fin
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = val(i + e, x[e]);
         const u64 t = wave_sum(v[0] + v[1] + (v[2] + v[3]));
-        if (lane == 0) s.group[j][wave] = t;
+        if (lane == 0) s.group[j * D::waves + wave] = t;
     });
     __syncthreads();
     // wave 0 walks the groups, 64 at a time
-    const u64* g = &s.group[0][0];
-    const int n = row.slabs * kWaves;
+    const u64* g = s.group;
+    const int n = row.slabs * D::waves;
     if (wave == 0) {
         u64 before = 0, total = 0;
         for (int i = lane; i < n; i += 64) total += g[i];
@@ -268,9 +286,9 @@ template <typename D, typename F, typename G> __device__ __forceinline__ int fin
     __syncthreads();
     const int at = s.bin;
     const u64 point = point_of(s.total);
-    if (at >= 0 && wave == at % kWaves) {
-        const f32x4 x = row.load(at / kWaves);
-        const int i = row.first(at / kWaves);
+    if (at >= 0 && wave == at % D::waves) {
+        const f32x4 x = row.load(at / D::waves);
+        const int i = row.first(at / D::waves);
         u64 w[4], t = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) t += w[e] = val(i + e, x[e]);
@@ -303,7 +321,7 @@ __device__ __forceinline__ Cut cut_by_keys(D& row, const Weights& w, unsigned lo
         int shift = 0;
         while ((span >> shift) >= kBins) shift++;
         __syncthreads();
-        clear_bins(s);
+        clear_bins<D::threads>(s);
         __syncthreads();
         row.each([&](int i, float x) {
             const unsigned k = sort_key(x);
@@ -313,7 +331,7 @@ __device__ __forceinline__ Cut cut_by_keys(D& row, const Weights& w, unsigned lo
                 if (by_sum) atomicAdd(&s.sum[b], w(x, s));
             }
         });
-        end_bin(by_sum, limit, count, sum, s);
+        end_bin<D::threads>(by_sum, limit, count, sum, s);
         count = s.above_count;
         sum = s.above_sum;
         high -= (unsigned)s.bin << shift;
@@ -338,8 +356,8 @@ __device__ __forceinline__ Cut cut_by_keys(D& row, const Weights& w, unsigned lo
 // The block's threads in groups of equal size, one group per listed token.
 struct ListView {
     int n, per, me;                // listed tokens, threads a group, this group's token
-    __device__ __forceinline__ explicit ListView(int n_) : n(n_) {
-        per = n <= 64 ? 16 : n <= 128 ? 8 : 4;
+    __device__ __forceinline__ ListView(int n_, int threads) : n(n_) {
+        per = threads / (n <= 64 ? 64 : n <= 128 ? 128 : kList);
         me = (int)threadIdx.x / per;
     }
     __device__ __forceinline__ bool first() const { return me < n && (int)threadIdx.x % per == 0; }
@@ -352,21 +370,21 @@ struct ListView {
         return t;
     }
 };
-static_assert(kThreads >= 4 * kList, "a group of threads for every listed token");
-
-template <typename T, bool ONE>
-__global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens) {
+template <typename T, bool ONE, int TH>
+__global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
+    constexpr int NW = TH / 64;
+    static_assert(TH >= kList && NW <= 16);
     __shared__ Shared s;
     const int64_t b = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    RowData<T, ONE> row;
+    RowData<T, ONE, TH> row;
     row.init(static_cast<const T*>(a.logits) + b * a.stride, (int)a.V);
     const double temperature = a.temperature ? a.temperature[b] : a.temperature0;
     const double top_p = a.top_p ? a.top_p[b] : a.top_p0, min_p = a.min_p ? a.min_p[b] : a.min_p0;
     const int64_t top_k = a.top_k ? a.top_k[b] : a.top_k0;
     const double u = a.u[b];
     if (tid < 128) s.exp2[tid] = exp2((double)tid / 128.);
-    clear_bins(s);
+    clear_bins<TH>(s);
 
     // the largest logit; a NaN makes it NaN
     float m = -INFINITY;
@@ -380,7 +398,7 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
     if (lane == 0) s.wmax[wave] = m;
     __syncthreads();
     m = s.wmax[0];
-    for (int w = 1; w < kWaves; w++) m = s.wmax[w] > m || s.wmax[w] != s.wmax[w] ? s.wmax[w] : m;
+    for (int w = 1; w < NW; w++) m = s.wmax[w] > m || s.wmax[w] != s.wmax[w] ? s.wmax[w] : m;
     // written so that one NaN wins: a NaN m compares false, and a later number does not replace it
     const double zmax = (double)m / temperature;
     auto first_max = [&] {
@@ -395,7 +413,7 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
         __syncthreads();
         if (lane == 0) s.windex[wave] = at;
         __syncthreads();
-        for (int w = 0; w < kWaves; w++) at = at < s.windex[w] ? at : s.windex[w];
+        for (int w = 0; w < NW; w++) at = at < s.windex[w] ? at : s.windex[w];
         if (tid == 0) tokens[b] = at;
     };
     if (!(temperature > 0.) || !(fabs(zmax) < INFINITY)) return first_max();
@@ -420,7 +438,7 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
             const int i = bin_of(x);
             if (i < kBins) atomicAdd(&s.count[i], 1u);
         });
-        end_bin(false, (u64)top_k, 0, 0, s);
+        end_bin<TH>(false, (u64)top_k, 0, 0, s);
         const int last = s.bin;
         const unsigned above = s.above_count, in = s.count[last];
         const bool all = above + in <= (unsigned)kList;          // every candidate fits the list
@@ -438,7 +456,7 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
         __syncthreads();
         if (all) {
             // the rest on the list alone: a group of threads per token
-            const ListView list((int)s.listed);
+            const ListView list((int)s.listed, TH);
             const int n = list.n, me = list.me;
             const float x = me < n ? s.lx[me] : 0.f;
             const int at = me < n ? s.li[me] : 0;
@@ -467,7 +485,7 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
             if (tid == 0) tokens[b] = s.pick;
             return;
         } else if (in <= (unsigned)kList) {
-            const ListView list((int)s.listed);
+            const ListView list((int)s.listed, TH);
             const int n = list.n, me = list.me;
             const float x = me < n ? s.lx[me] : 0.f;
             const unsigned rank = above + list.sum<unsigned>([&](int j) -> unsigned { return s.lx[j] > x; });
@@ -480,7 +498,7 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
             cut = cut_by_keys(row, w, s.low_key, s.high_key, false, (u64)top_k, above, 0, s);
         }
         __syncthreads();
-        clear_bins(s);
+        clear_bins<TH>(s);
         __syncthreads();
     }
     if (some_p) {
@@ -503,9 +521,9 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
         if (lane == 0) s.wsum[wave] = t;
         __syncthreads();
         t = 0;
-        for (int i = 0; i < kWaves; i++) t += s.wsum[i];
+        for (int i = 0; i < NW; i++) t += s.wsum[i];
         const u64 limit = (u64)(top_p * (double)t);
-        end_bin(true, limit, 0, 0, s);
+        end_bin<TH>(true, limit, 0, 0, s);
         const int last = s.bin;
         const u64 above = s.above_sum;
         const unsigned in = s.count[last];
@@ -523,7 +541,7 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
         __syncthreads();
         if (in <= (unsigned)kList) {
             // in order, the last token before which the sum is within the limit
-            const ListView list((int)s.listed);
+            const ListView list((int)s.listed, TH);
             const int n = list.n, me = list.me;
             const float x = me < n ? s.lx[me] : 0.f;
             const int at = me < n ? s.li[me] : 0;
@@ -561,8 +579,14 @@ __global__ __launch_bounds__(kThreads) void k_sample(SnHipSample a, int* tokens)
 }
 
 template <typename T> void sample_t(const SnHipSample& a, int* tokens, hipStream_t st) {
-    if (a.V < 4) k_sample<T, true><<<(unsigned)a.B, kThreads, 0, st>>>(a, tokens);
-    else k_sample<T, false><<<(unsigned)a.B, kThreads, 0, st>>>(a, tokens);
+    // A row of 16 waves is done sooner, two rows of 8 waves share a CU's LDS and registers:
+    // 8 for more rows than CUs (top-p 0.9, 512 rows of 12000: 27 us against 39; of 65536: 108
+    // against 126) and for short rows, whose barriers weigh more (one row of 1000: 10.2
+    // against 11.9); 16 otherwise (64 rows of 32000: 33 against 37; of 8000: 17 both).
+    const unsigned B = (unsigned)a.B;
+    if (a.V < 4) k_sample<T, true, 512><<<B, 512, 0, st>>>(a, tokens);
+    else if (B > 256 || a.V <= 8192) k_sample<T, false, 512><<<B, 512, 0, st>>>(a, tokens);
+    else k_sample<T, false, 1024><<<B, 1024, 0, st>>>(a, tokens);
 }
 
 }  // namespace
