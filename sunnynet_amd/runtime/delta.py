@@ -123,9 +123,9 @@ def _fwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, keep):
     chunks = states = None
     if keep or cu_seqlens is not None or T > STEP_TOKENS:
         sizes = _pack(q, k, v, g, beta, s0, cu_seqlens, dims, scale)
-        chunks = torch.empty(L.snhip_op_delta_chunk_floats(sizes), device=q.device)
+        chunks = torch.empty(L.snhip_op_delta_chunk_floats(sizes), dtype=torch.float32, device=q.device)
         if keep:
-            states = torch.empty(L.snhip_op_delta_state_floats(sizes), device=q.device)
+            states = torch.empty(L.snhip_op_delta_state_floats(sizes), dtype=torch.float32, device=q.device)
     rc = _native.on_device(q.device, L.snhip_op_delta_fwd_dev,
                            _pack(q, k, v, g, beta, s0, cu_seqlens, dims, scale, chunks, states), out.data_ptr(),
                            send.data_ptr())
@@ -146,6 +146,12 @@ def delta_bwd(q, k, v, g, beta, s0, saved, dout, dsend=None, *, scale=None, cu_s
         _check_state(dsend, (N, H, K, V), "dsend")
         if dsend.device != q.device:
             raise ValueError("the delta rule takes tensors of one GPU")
+    if B * T and N:
+        L, sizes = _native.lib(), _pack(q, k, v, g, beta, s0, cu_seqlens, dims, 1.0)
+        sizes = L.snhip_op_delta_chunk_floats(sizes), L.snhip_op_delta_state_floats(sizes)
+        if not saved or any(t is None or t.shape != (n,) or t.dtype != torch.float32 or t.device != q.device
+                            or not t.is_contiguous() for t, n in zip(saved, sizes)):
+            raise ValueError("saved must be delta_fwd's, of the same shapes, with keep=True")
     return _bwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, saved, dout.contiguous(), dsend, need_ds0)
 
 
@@ -155,8 +161,8 @@ def _bwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, saved, dout, dsend, need
     new = torch.empty if cu_seqlens is None else torch.zeros
     dq, dk = (new(B, T, Hk, K, dtype=q.dtype, device=q.device) for _ in range(2))
     dv = new(B, T, H, V, dtype=q.dtype, device=q.device)
-    dg, db = (new(B, T, H, device=q.device) for _ in range(2))
-    ds0 = torch.empty(N, H, K, V, device=q.device) if need_ds0 else None
+    dg, db = (new(B, T, H, dtype=torch.float32, device=q.device) for _ in range(2))
+    ds0 = torch.empty(N, H, K, V, dtype=torch.float32, device=q.device) if need_ds0 else None
     if B * T == 0 or N == 0:
         if need_ds0:
             ds0.zero_() if dsend is None else ds0.copy_(dsend)
@@ -164,7 +170,7 @@ def _bwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, saved, dout, dsend, need
     L = _native.lib()
     chunks, states = saved
     args = _pack(q, k, v, g, beta, s0, cu_seqlens, dims, scale, chunks, states)
-    ws = torch.empty(L.snhip_op_delta_bwd_floats(args), device=q.device)
+    ws = torch.empty(L.snhip_op_delta_bwd_floats(args), dtype=torch.float32, device=q.device)
     grads = _GRAD.pack(dout.data_ptr(), _ptr(dsend), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(),
                        db.data_ptr(), _ptr(ds0), ws.data_ptr())
     rc = _native.on_device(q.device, L.snhip_op_delta_bwd_dev, args, grads)

@@ -37,7 +37,7 @@ def norm_fwd(x, weight=None, bias=None, eps=1e-5, *, keep=False):
     with ``keep``, else None. weight, bias: (D) float32 or None."""
     R, D = _check(x, weight, bias)
     y = torch.empty_like(x)
-    mean, rstd = (torch.empty(R, device=x.device) for _ in range(2)) if keep else (None, None)
+    mean, rstd = (torch.empty(R, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
     if R:
         rc = _native.on_device(x.device, _native.lib().snhip_op_norm_fwd_dev, x.data_ptr(), _ptr(weight), _ptr(bias),
                                y.data_ptr(), _ptr(mean), _ptr(rstd), R, D, eps, DTYPES[x.dtype])
@@ -63,9 +63,11 @@ def _bwd(dy, x, weight, mean, rstd, need, R, D):
     L = _native.lib()
     dx = torch.empty_like(x) if need[0] else None
     new = torch.empty if R else torch.zeros
-    dw, db = (new(D, device=x.device) if n else None for n in need[1:])
+    dw, db = (new(D, dtype=torch.float32, device=x.device) if n else None for n in need[1:])
     if R and any(need):
-        ws = torch.empty(L.snhip_op_norm_bwd_floats(R, D), device=x.device) if need[1] or need[2] else None
+        ws = None
+        if need[1] or need[2]:
+            ws = torch.empty(L.snhip_op_norm_bwd_floats(R, D), dtype=torch.float32, device=x.device)
         rc = _native.on_device(x.device, L.snhip_op_norm_bwd_dev, dy.data_ptr(), x.data_ptr(), _ptr(weight),
                                mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), R, D,
                                DTYPES[x.dtype])

@@ -121,3 +121,40 @@ def test_served(gpu):
     assert (end - state).abs().max() <= 1e-4 * end.abs().max()
     for i in range(N):
         assert torch.equal(runtime.sample_tokens(every[:, i], u[i], **pick), text[:, i])
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_the_default_type_changes_nothing(gpu, default):
+    """Workspaces, statistics and gradients of decays are fp32 whatever torch's default is."""
+    gen = torch.Generator().manual_seed(3)
+
+    def rn(*s):
+        return torch.randn(*s, generator=gen, dtype=torch.float32).cuda()
+
+    q, k, v = rn(2, 77, 2, 16), rn(2, 77, 2, 16) / 4, rn(2, 77, 4, 24)
+    leaves = [q, k, v, -rn(2, 77, 4).abs(), torch.sigmoid(rn(2, 77, 4)), rn(2, 4, 16, 24), rn(24), rn(24)]
+    seed = rn(2, 77, 4, 24)
+
+    def run():
+        own = [t.clone().requires_grad_() for t in leaves]
+        out, send = runtime.gated_delta(*own[:6])
+        y = runtime.layer_norm(out, *own[6:])
+        return y, send, *torch.autograd.grad([y, send], own, [seed, leaves[5]])
+
+    want = run()
+    try:
+        torch.set_default_dtype(default)
+        have = run()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    for a, b in zip(have, want):
+        assert a.dtype == torch.float32 and torch.equal(a, b)
+
+
+def test_what_the_forward_kept_for_other_shapes_is_refused(gpu):
+    x = [torch.zeros(1, 40, 2, 16, device="cuda") for _ in range(3)]
+    g, beta = torch.zeros(2, 1, 40, 2, device="cuda")
+    short = runtime.delta_fwd(*(t[:, :20] for t in x), g[:, :20], beta[:, :20], keep=True)[2]
+    for saved in (short, None, (None, None)):
+        with pytest.raises(ValueError, match="saved"):
+            runtime.delta_bwd(*x, g, beta, None, saved, x[2])
