@@ -193,11 +193,15 @@ def stream_handle(device=None) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def raw_stream(device) -> int:
+    """The handle of torch's current stream of `device`; 0 is the default stream."""
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def on_device(device, call, *args) -> int:
     """call(*args, stream) on torch's current stream of `device`, with that device the
     current one, as the library's operators expect."""
-    at = device.index
-    stream = _raw_stream(at) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    at, stream = device.index, raw_stream(device)
     if torch.cuda.current_device() == at:
         return call(*args, stream)
     with torch.cuda.device(device):

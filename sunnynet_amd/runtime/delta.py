@@ -31,6 +31,27 @@ _ARGS = struct.Struct("7P9q8qd2P")     # SnHipDelta
 _GRAD = struct.Struct("9P")            # SnHipDeltaGrad
 
 
+def note_leaves(ctx, device):
+    """Torch makes a leaf's gradient node on the stream that first uses the leaf, keeps it
+    while a graph of it lives, and waits on that stream in every backward pass through it.
+    Inside a capture no wait on the default stream is possible, and the process ends at it:
+    nodes that are seen on the default stream are marked, and a capture that meets a marked
+    one is refused."""
+    if device.type != "cuda":
+        return                 # refused later
+    on_default = not _native.raw_stream(device)        # which cannot be captured
+    if not on_default and not torch.cuda.is_current_stream_capturing():
+        return
+    for node, _ in ctx.next_functions:
+        if node is None or node.name() != "torch::autograd::AccumulateGrad":
+            continue
+        if on_default:
+            node.metadata["snhip_default_stream"] = True
+        elif "snhip_default_stream" in node.metadata:
+            raise RuntimeError("a graph of these leaves, made on the default stream, is still alive: delete its "
+                               "outputs before capturing, or make it on another stream")
+
+
 def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
@@ -184,6 +205,7 @@ class GatedDelta(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, s0, scale, cu_seqlens):
+        note_leaves(ctx, q.device)
         q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
         s0 = None if s0 is None else s0.contiguous()
         dims = _shapes(q, k, v, g, beta, s0, cu_seqlens)
@@ -206,7 +228,8 @@ class GatedDelta(torch.autograd.Function):
 
 def gated_delta(q, k, v, g, beta, s0=None, *, scale=None, cu_seqlens=None):
     """(out, send) of the gated delta rule under autograd (shapes: delta_fwd). Without
-    a gradient to keep anything for, calls of up to 12 tokens run token by token."""
+    a gradient to keep anything for, calls of up to 12 tokens run token by token. A capture
+    may hold this and its backward pass; see note_leaves for the one that is refused."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, s0)):
         return GatedDelta.apply(q, k, v, g, beta, s0, scale, cu_seqlens)
     if s0 is not None:

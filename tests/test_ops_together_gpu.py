@@ -158,3 +158,64 @@ def test_what_the_forward_kept_for_other_shapes_is_refused(gpu):
     for saved in (short, None, (None, None)):
         with pytest.raises(ValueError, match="saved"):
             runtime.delta_bwd(*x, g, beta, None, saved, x[2])
+
+
+def test_training_in_a_graph(gpu):
+    """Forward and autograd's backward captured after a pass on a side stream whose outputs
+    are still alive; replays against eager passes over copies of the leaves."""
+    gen = torch.Generator().manual_seed(5)
+
+    def leaves():
+        r = [torch.randn(*s, generator=gen).cuda() for s in
+             [(2, 70, 2, 16), (2, 70, 2, 16), (2, 70, 4, 24), (2, 70, 4), (2, 70, 4), (2, 4, 16, 24), (24,), (24,)]]
+        return [r[0], r[1] / 4, r[2], -r[3].abs(), torch.sigmoid(r[4]), *r[5:]]
+
+    def run(t):
+        out, send = runtime.gated_delta(*t[:6])
+        y = runtime.layer_norm(out, *t[6:])
+        torch.autograd.backward([y, send], [dy, ds])
+        return y, send
+
+    dy, ds = torch.randn(2, 70, 4, 24, generator=gen).cuda(), torch.randn(2, 4, 16, 24, generator=gen).cuda()
+    held = [t.requires_grad_() for t in leaves()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        warm = run(held)
+    torch.cuda.current_stream().wait_stream(side)
+    for t in held:
+        t.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = run(held)
+    for _ in range(3):
+        new = [t.requires_grad_() for t in leaves()]
+        with torch.no_grad():
+            for t, n in zip(held, new):
+                t.copy_(n)
+        graph.replay()
+        want = run(new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert all(torch.equal(a.grad, b.grad) for a, b in zip(held, new))
+    del warm
+
+
+def test_a_capture_beside_a_living_eager_graph_is_refused(gpu):
+    x = torch.randn(3, 24, device="cuda", requires_grad=True)
+    q, k, v = (torch.randn(1, 40, 2, 16, device="cuda", requires_grad=True) for _ in range(3))
+    g, beta = -torch.rand(1, 40, 2, device="cuda"), torch.rand(1, 40, 2, device="cuda")
+    calls = [lambda: runtime.layer_norm(x), lambda: runtime.gated_delta(q, k, v, g, beta)[0]]
+    for call in calls:
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="still alive"):
+                call()
+            torch.zeros(1, device="cuda")
+        want = torch.autograd.grad(alive.sum(), x if call is calls[0] else q)[0]
+        assert torch.isfinite(want).all()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
