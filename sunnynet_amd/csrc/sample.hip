@@ -20,7 +20,7 @@
 //
 // With few rows the time is that of one block's passes, not of HBM: per 4,096 fp32 tokens
 // a pass takes 0.24 us to read them (70 GB/s, one CU's share of L2; more slabs on their way
-// at once change nothing), 0.4 to count them, 1.2 to weigh them (instruction issue). 64 rows of 32000: 7 us for the
+// at once change nothing), 0.4 to count them, 1.1 to weigh them (instruction issue). 64 rows of 32000: 7 us for the
 // largest logit alone, 16 us without filters, 15 us with top-k 40, 33 us with top-p 0.9.
 #include "common.h"
 #include "planes.h"
@@ -32,6 +32,7 @@ namespace {
 constexpr int kBins = 2048;
 constexpr int kGroup = 256;                  // neighbouring tokens of a wave: four a lane
 constexpr int kList = 256;
+constexpr int kFracs = 128;                  // of 16 with a polynomial of degree 6: 25.1 us, not 24.4, for 65536
 constexpr float kRange = 44.f;               // exp(-44) is 0 in the scaled weights
 typedef unsigned long long u64;
 
@@ -47,7 +48,7 @@ __device__ __forceinline__ float key_logit(unsigned k) {
 struct Shared {
     u64 sum[kBins];                // of bins; the groups' sums at the end
     unsigned count[kBins];
-    double exp2[128];              // 2^(j / 128)
+    double exp2[kFracs];           // 2^(j / kFracs + bits)
     u64 wsum[16];
     unsigned wcount[16];
     float lx[kList];               // the list: logits, indices, weights
@@ -62,20 +63,19 @@ struct Shared {
     u64 group[(1 << 20) / kGroup];        // kept weight of kGroup neighbouring tokens
 };
 
-// exp((x - m) / T) 2^bits, in 64 bits: 2^(n / 128) from the table, the rest (below
-// 2^-8 log 2) by its Taylor polynomial of degree 4, 1e-15 of the value. n comes from
-// adding 1.5 2^52, whose last bits it is; the power of two is added to the exponent's bits
-// (the value stays above 2^-72).
+// exp((x - m) / T) 2^bits, in 64 bits: 2^(n / kFracs + bits) from the table, the rest (below
+// log 2 / (2 kFracs)) by its Taylor polynomial of degree 4, 1e-15 of the value. n comes from
+// adding 1.5 2^52, whose last bits it is; its power of two is added to the exponent's bits.
+// Below 2^-70 the value stays 2^-70, which rounds to the whole number 0.
 struct Weights {
-    double m, step, low;           // step: 128 / (T log 2)
-    int bits;
+    double m, step, low;           // step: kFracs / (T log 2)
     __device__ __forceinline__ double real(float x, const Shared& s) const {
-        const double t = ((double)x - m) * step, c = 0x1.8p52;
-        const double q = t + c, r = (t - (q - c)) * (0.69314718055994530942 / 128.);
+        constexpr double c = 0x1.8p52, l = 0.69314718055994530942 / kFracs;
+        const double t = fmax(((double)x - m) * step, -kFracs * 70.), q = t + c, r = t - (q - c);
         const int i = (int)(unsigned)__double_as_longlong(q);
-        const double p = fma(r, fma(r, fma(r, fma(r, 1. / 24., 1. / 6.), 0.5), 1.), 1.);
-        const double w = __longlong_as_double(__double_as_longlong(s.exp2[i & 127] * p) + ((long long)((i >> 7) + bits) << 52));
-        return t > -128. * 70. ? w : 0.;
+        const double p = fma(r, fma(r, fma(r, fma(r, l * l * l * l / 24., l * l * l / 6.), l * l / 2.), l), 1.);
+        const double w = s.exp2[i & (kFracs - 1)] * p;
+        return __hiloint2double(__double2hiint(w) + ((i & -kFracs) * ((1 << 20) / kFracs)), __double2loint(w));
     }
     // Rounded to a whole number (below 2^52), by adding 2^52.
     __device__ __forceinline__ u64 whole(double w) const {
@@ -384,7 +384,10 @@ __global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
     const double top_p = a.top_p ? a.top_p[b] : a.top_p0, min_p = a.min_p ? a.min_p[b] : a.min_p0;
     const int64_t top_k = a.top_k ? a.top_k[b] : a.top_k0;
     const double u = a.u[b];
-    if (tid < 128) s.exp2[tid] = exp2((double)tid / 128.);
+    int bits = 0;                  // a row's sum of weights of up to 2^bits stays below 2^62
+    while ((1 << bits) < row.V) bits++;
+    bits = 62 - bits < 51 ? 62 - bits : 51;
+    if (tid < kFracs) s.exp2[tid] = ldexp(exp2((double)tid / kFracs), bits);
     clear_bins<TH>(s);
 
     // the largest logit; a NaN makes it NaN
@@ -423,12 +426,9 @@ __global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
         return total && point >= total ? total - 1 : point;
     };
     Weights w;
-    int bits = 0;
-    while ((1 << bits) < row.V) bits++;
-    w.bits = 62 - bits < 51 ? 62 - bits : 51;
     w.m = (double)m;
-    w.step = fmin(128. / (0.69314718055994530942 * temperature), 1e300);
-    w.low = min_p * ldexp(1., w.bits);
+    w.step = fmin(kFracs / (0.69314718055994530942 * temperature), 1e300);
+    w.low = min_p * ldexp(1., bits);
     const float per = (float)fmin((double)kBins / ((double)kRange * temperature), 1e30);
     auto bin_of = [&](float x) { return (int)fminf((m - x) * per, 2.f * kBins); };     // kBins and up: weight 0
 
