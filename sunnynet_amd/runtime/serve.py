@@ -210,13 +210,13 @@ class Request:
     temperature: float = 0.0
     top_p: float = 1.0
     top_k: int = 0
-    min_p: float = 0.0
     eos: int | None = None
     seed: int | None = None
     output: list = field(default_factory=list)
     done: bool = False
     pos: int = 0                       # prompt tokens consumed
     rng: object = None
+    min_p: float = 0.0
 
     @property
     def greedy(self) -> bool:
@@ -227,6 +227,13 @@ class Request:
         """Whether the device sampler knows the request's settings (it does unless
         top_k is negative)."""
         return self.greedy or not self.top_k or self.top_k > 0
+
+    @property
+    def settings(self) -> tuple:
+        """(temperature, top_p, min_p, top_k) as the device sampler takes them."""
+        if self.greedy:
+            return 0.0, 1.0, 0.0, 0
+        return float(self.temperature), float(self.top_p), float(self.min_p or 0.0), min(int(self.top_k or 0), 1 << 30)
 
     def next_input(self) -> int:
         return int(self.prompt[self.pos]) if self.pos < len(self.prompt) else int(self.output[-1])
@@ -241,8 +248,7 @@ class BatchScheduler:
         self.waiting: list[Request] = []
         self.finished: list[Request] = []
         self.steps = 0
-        self._rows = None                  # the requests whose settings the device holds
-        self._settings = None
+        self._held = self._settings = None     # settings of the rows, here and on the device
 
     def submit(self, prompt, max_tokens: int, **kw) -> Request:
         if len(prompt) == 0:
@@ -289,17 +295,14 @@ class BatchScheduler:
         """The next tokens on the device: sample_logits' rules, with one number
         from each sampling request's own generator, as it draws them."""
         dev = logits.device
-        if self._rows is None or len(self._rows) != len(self.active) \
-                or any(a is not b for a, b in zip(self._rows, self.active)):
-            # the settings go over only when the active requests change
-            cols = [[0.0 if r.greedy else float(r.temperature) for r in self.active],
-                    [float(r.top_p) for r in self.active], [float(r.min_p or 0.0) for r in self.active]]
+        held = [r.settings for r in self.active]
+        if held != self._held:             # they go over only when one of them changes
+            *cols, top_k = zip(*held)
             self._settings = (torch.tensor(cols, dtype=torch.float64, device=dev),
-                              torch.tensor([min(int(r.top_k or 0), 1 << 30) for r in self.active],
-                                           dtype=torch.int32, device=dev))
-            self._rows = list(self.active)
-        u = torch.tensor([r.rng.random() if w and not r.greedy else 0.0 for r, w in zip(self.active, wanted)],
-                         dtype=torch.float64, device=dev)
+                              torch.tensor(top_k, dtype=torch.int32, device=dev))
+            self._held = held
+        u = torch.tensor([(r.rng or np.random.default_rng()).random() if w and not r.greedy else 0.0
+                          for r, w in zip(self.active, wanted)], dtype=torch.float64, device=dev)
         (temperature, top_p, min_p), top_k = self._settings
         return sample_tokens(logits, u, temperature, top_k, top_p, min_p).cpu().numpy()
 

@@ -77,6 +77,32 @@ def test_settings_the_device_does_not_know_stay_on_the_host(gpu, tmp_path, monke
     serve_all(tmp_path, [dict()])                                  # greedy requests alone
 
 
+def test_settings_changed_between_steps(gpu, tmp_path):
+    """A request's settings hold from the next step on, and a greedy one's filters are not read."""
+    path = tmp_path / "m.bin"
+    path.write_bytes(pack_sunny_blob(init_sunnynet(TINY, 0)))
+    c = TINY
+    m = Recorder(HipModel(path, c.vocab_size, c.dim, c.inner, c.rank, c.taps, c.layers, max_batch=3))
+    sch = BatchScheduler(m)
+    reqs = [sch.submit([5], 24, seed=1, temperature=3.0), sch.submit([6], 24, seed=2, temperature=0.0, top_p=None),
+            sch.submit([7], 24, seed=3, temperature=1.0, top_k=9)]
+    gens = [np.random.default_rng(s) for s in (1, 2, 3)]
+    for step in range(24):
+        if step == 8:
+            reqs[0].top_k, reqs[2].temperature = 2, 0.01
+        if step == 16:
+            reqs[0].temperature, reqs[2].top_p, reqs[2].temperature = 0.0, 0.3, 5.0
+        sch.step()
+        for row, r, gen in zip(m.seen[-1], reqs, gens):
+            assert r.output[step] == sample_logits(row, r.temperature, r.top_p, r.top_k, gen, r.min_p)
+    m.close()
+
+
+def test_fields_keep_their_places():
+    r = serve.Request([1], 2, 0.5, 0.9, 3, 7, 11)
+    assert (r.temperature, r.top_p, r.top_k, r.eos, r.seed, r.min_p) == (0.5, 0.9, 3, 7, 11, 0.0)
+
+
 def test_min_p_of_the_host_sampler():
     z = np.log(np.array([0.5, 0.3, 0.15, 0.05]))
     draws = {sample_logits(z, 1.0, 1.0, 0, np.random.default_rng(i), 0.4) for i in range(50)}
