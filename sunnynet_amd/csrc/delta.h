@@ -181,14 +181,18 @@ template <typename T, int KP, int NTH, bool VEC, int R = kDC> struct RowsFetch {
 };
 
 // The first Q planes of a (32, 32) matrix of a chunk's record (at float `at`), likewise.
+// The matrix's place is part of the vector offset, which the hardware checks against the
+// record; threads past the planes fetch nothing.
 template <int Q, int NTH> struct MatFetch {
     static constexpr int N = (Q * 128 + NTH - 1) / NTH;
     static constexpr bool whole = Q * 128 % NTH == 0;
     bf16x8 x[N];
+    // Of vector i, in bytes from the record's start.
+    static constexpr int offset(int i, int at) { return whole || i < Q * 128 ? at * 4 + i * 16 : kNowhere; }
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rec, int at, int tid) {
 #pragma unroll
         for (int j = 0; j < N; j++)
-            x[j] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rec, (tid + j * NTH) * 16, at * 4, 0));
+            x[j] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rec, offset(tid + j * NTH, at), 0, 0));
     }
     __device__ __forceinline__ void store(Tile<Q, kDC, kDC> to, int tid) const {
 #pragma unroll
