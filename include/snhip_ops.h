@@ -66,7 +66,8 @@ typedef struct SnHipDelta {
                                    Both workspaces 16-byte aligned                */
 } SnHipDelta;
 
-/* Floats of the two workspaces of a call (the other fields of d are not read). */
+/* Floats of the two workspaces of a call (the other fields of d are not read); 0 for
+ * sizes outside the ranges. */
 int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d);
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d);
 
@@ -82,7 +83,7 @@ snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send
  * dout (B,T,H,V) contiguous, of the inputs' type; dsend (N,H,K,V) or NULL (zeros).
  * dq, dk (B,T,Hk,K), dv (B,T,H,V) contiguous, of the inputs' type, dq and dk summed
  * over the value heads that share them; dg, dbeta (B,T,H) fp32; ds0 (N,H,K,V) fp32
- * or NULL. ws: snhip_op_delta_bwd_floats floats, 16-byte aligned. Sums run in a fixed
+ * or NULL. ws: snhip_op_delta_bwd_floats floats (0 outside the ranges), 16-byte aligned. Sums run in a fixed
  * order. */
 typedef struct SnHipDeltaGrad {
     const void* dout;

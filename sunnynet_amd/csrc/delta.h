@@ -51,6 +51,14 @@ struct DeltaP {
     bool vec;               // every eight elements of a row of q or k are 16-byte aligned
 };
 
+// Whether a call's sizes and type are in the documented ranges.
+inline bool delta_in_range(const SnHipDelta& d) {
+    return d.B >= 1 && d.T >= 1 && d.N >= 1 && d.N <= 65535 && d.H >= 1 && d.H <= 65535 && d.Hk >= 1 &&
+           d.H % d.Hk == 0 && d.K >= 1 && d.K <= 128 && d.V >= 1 && d.V <= 4096 && d.T <= kDeltaTokens / d.B &&
+           (d.cu ? d.B == 1 : d.N == d.B) && d.H * d.V < kDeltaStride && d.H * d.K < kDeltaStride &&
+           d.dtype >= SNHIP_F32 && d.dtype <= SNHIP_F16;
+}
+
 __host__ __device__ inline int64_t delta_slots(const SnHipDelta& d) {
     return d.cu ? d.T / kDC + d.N : d.B * ((d.T + kDC - 1) / kDC);
 }

@@ -499,10 +499,7 @@ snhip_status fwd_t(const DeltaP& a, void* out, float* send, hipStream_t st) {
 // Checks d and fills in what the kernels derive from it.
 snhip_status delta_args(const SnHipDelta* d, DeltaP* a) {
     if (!d || !d->q || !d->k || !d->v || !d->g || !d->beta) return SNHIP_E_INVAL;
-    if (d->B < 1 || d->T < 1 || d->N < 1 || d->N > 65535 || d->H < 1 || d->H > 65535 || d->Hk < 1 ||
-        d->H % d->Hk || d->K < 1 || d->K > 128 || d->V < 1 || d->V > 4096 || d->T > kDeltaTokens / d->B ||
-        (d->cu ? d->B != 1 : d->N != d->B) || d->H * d->V >= kDeltaStride || d->H * d->K >= kDeltaStride || d->dtype < SNHIP_F32 || d->dtype > SNHIP_F16)
-        return SNHIP_E_INVAL;
+    if (!delta_in_range(*d)) return SNHIP_E_INVAL;
     for (const void* w : {(const void*)d->chunks, (const void*)d->states})
         if (reinterpret_cast<uintptr_t>(w) % 16) return SNHIP_E_INVAL;
     for (const int64_t* st : {d->q_stride, d->k_stride, d->v_stride})
@@ -532,13 +529,14 @@ using namespace snhip;
 extern "C" {
 
 int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d) {
-    if (!d) return 0;
+    if (!d || !delta_in_range(*d)) return 0;
     const int64_t segs = delta_segs(*d);
     return delta_slots(*d) * d->H * kDeltaChunk +
            (segs > 1 ? d->N * segs * d->H * delta_seg_floats(delta_kp(d->K), delta_vp(d->V)) : 0);
 }
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d) {
-    return d ? delta_groups(*d) * d->H * delta_vp(d->V) * (kDC * delta_ns(d->dtype, d->K) + (int64_t)delta_kp(d->K)) : 0;
+    if (!d || !delta_in_range(*d)) return 0;
+    return delta_groups(*d) * d->H * delta_vp(d->V) * (kDC * delta_ns(d->dtype, d->K) + (int64_t)delta_kp(d->K));
 }
 
 snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send, void* stream) {

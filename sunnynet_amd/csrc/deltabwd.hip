@@ -548,7 +548,7 @@ using namespace snhip;
 extern "C" {
 
 int64_t snhip_op_delta_bwd_floats(const SnHipDelta* d) {
-    if (!d) return 0;
+    if (!d || !delta_in_range(*d)) return 0;
     const int64_t c = kDC * delta_ns(d->dtype, d->K);
     return delta_groups(*d) * d->H * delta_vp(d->V) * (c + delta_kp(d->K) + c / 16);
 }
