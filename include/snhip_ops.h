@@ -42,10 +42,12 @@ extern "C" {
  * decreases is refused by nothing and gives unspecified results (in bounds).
  *
  * Ranges: 1 <= K <= 128, 1 <= V <= 4096, H a multiple of Hk, H <= 65535, N <= 65535,
- * B T < 2^30, H K, H V and every token stride below 2^24 (strides not negative). g <= 0 is meant (a decay); -inf forgets the state exactly, other
- * values are clamped at -200, where exp(g) is 0 in fp32. Non-finite values reach
- * the results of their sequence and head (in gradients of q and k: of the heads that
- * share theirs) only, as NaN, from the chunk of 32 tokens that holds them on. */
+ * B T < 2^30, H K, H V and every token stride below 2^24 (strides not negative); with
+ * workspaces fewer than 2^23 chunks of 32 tokens (B ceil(T / 32), with cu T / 32 + N).
+ * g <= 0 is meant (a decay); -inf forgets the state exactly, other values are clamped
+ * at -200, where exp(g) is 0 in fp32. Non-finite values reach the results of their
+ * sequence and head (in gradients of q and k: of the heads that share theirs) only, as
+ * NaN, from the chunk of 32 tokens that holds them on. */
 typedef struct SnHipDelta {
     const void* q;
     const void* k;

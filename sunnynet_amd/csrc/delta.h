@@ -32,6 +32,9 @@ constexpr int kDeltaP = 3 * kDC * kDC / 2, kDeltaG = 2 * kDeltaP, kDeltaChunk = 
 
 // Tokens of a call: positions inside a sequence, and a part's end past it, fit 32 bits.
 constexpr int64_t kDeltaTokens = (1 << 30) - 1;
+// Chunks of a call: the kernels launch up to 512 threads for each, in one dimension of a
+// grid that holds fewer than 2^32.
+constexpr int64_t kDeltaSlots = (1 << 23) - 1;
 // The longest call that runs token by token without workspaces. 12 heads of 64, one
 // sequence: 11.5 us token by token and 11.8 in chunks at 12 tokens; 64 sequences of 16
 // heads of 128: 46 and 78 us (57 and 78 at 16).

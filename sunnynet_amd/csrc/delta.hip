@@ -529,13 +529,13 @@ using namespace snhip;
 extern "C" {
 
 int64_t snhip_op_delta_chunk_floats(const SnHipDelta* d) {
-    if (!d || !delta_in_range(*d)) return 0;
+    if (!d || !delta_in_range(*d) || delta_slots(*d) > kDeltaSlots) return 0;
     const int64_t segs = delta_segs(*d);
     return delta_slots(*d) * d->H * kDeltaChunk +
            (segs > 1 ? d->N * segs * d->H * delta_seg_floats(delta_kp(d->K), delta_vp(d->V)) : 0);
 }
 int64_t snhip_op_delta_state_floats(const SnHipDelta* d) {
-    if (!d || !delta_in_range(*d)) return 0;
+    if (!d || !delta_in_range(*d) || delta_slots(*d) > kDeltaSlots) return 0;
     return delta_groups(*d) * d->H * delta_vp(d->V) * (kDC * delta_ns(d->dtype, d->K) + (int64_t)delta_kp(d->K));
 }
 
@@ -559,6 +559,7 @@ snhip_status snhip_op_delta_fwd_dev(const SnHipDelta* d, void* out, float* send,
             return step_t<decltype(t), decltype(kp)::value, decltype(vec)::value>(a, out, send, st);
         });
     }
+    if (a.slots > kDeltaSlots) return SNHIP_E_INVAL;
     return delta_pick(a, [&](auto t, auto kp, auto vec) {
         return fwd_t<decltype(t), decltype(kp)::value, decltype(vec)::value>(a, out, send, st);
     });

@@ -548,7 +548,7 @@ using namespace snhip;
 extern "C" {
 
 int64_t snhip_op_delta_bwd_floats(const SnHipDelta* d) {
-    if (!d || !delta_in_range(*d)) return 0;
+    if (!d || !delta_in_range(*d) || delta_slots(*d) > kDeltaSlots) return 0;
     const int64_t c = kDC * delta_ns(d->dtype, d->K);
     return delta_groups(*d) * d->H * delta_vp(d->V) * (c + delta_kp(d->K) + c / 16);
 }
@@ -556,7 +556,7 @@ int64_t snhip_op_delta_bwd_floats(const SnHipDelta* d) {
 snhip_status snhip_op_delta_bwd_dev(const SnHipDelta* d, const SnHipDeltaGrad* gr, void* stream) {
     DeltaP a;
     const snhip_status rc = delta_args(d, &a);
-    if (rc != SNHIP_OK || !gr || !d->chunks || !d->states || !gr->dout || !gr->dq || !gr->dk || !gr->dv ||
+    if (rc != SNHIP_OK || a.slots > kDeltaSlots || !gr || !d->chunks || !d->states || !gr->dout || !gr->dq || !gr->dk || !gr->dv ||
         !gr->dg || !gr->dbeta || !gr->ws || reinterpret_cast<uintptr_t>(gr->ws) % 16)
         return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);

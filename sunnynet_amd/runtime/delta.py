@@ -92,6 +92,8 @@ def _shapes(q, k, v, g, beta, s0, cu, step=False):
         N = cu.shape[0] - 1
     if N > 65535:
         raise ValueError("at most 65535 sequences per call")
+    if not step and (B * -(-T // 32) if cu is None else T // 32 + N) >= 1 << 23:
+        raise ValueError("fewer than 2^23 chunks of 32 tokens per call")
     if s0 is not None:
         _check_state(s0, (N, H, K, V), "s0")
     dev = q.device
