@@ -248,9 +248,15 @@ snhip_status norm_fwd_t(const void* x, const float* w, const float* b, void* y, 
     const bool vec = D % 8 == 0 && aligned(x) && aligned(y) && aligned(w) && aligned(b);
     return norm_shape(D, [&](auto nv, auto wpr) -> snhip_status {
         constexpr int NV = decltype(nv)::value, WPR = decltype(wpr)::value, RPB = norm_waves(WPR) / WPR;
-        k_norm_fwd<T, NV, WPR><<<(unsigned)((R + RPB - 1) / RPB), 64 * norm_waves(WPR), 0, st>>>(
-            (const T*)x, w, b, (T*)y, mean, rstd, R, (int)D, eps, vec);
-        SNHIP_CHECK(hipGetLastError());
+        // a grid holds fewer than 2^32 threads: more rows go in several launches
+        constexpr int64_t most = (int64_t)RPB << 21;
+        for (int64_t r = 0; r < R; r += most) {
+            const int64_t n = R - r < most ? R - r : most;
+            k_norm_fwd<T, NV, WPR><<<(unsigned)((n + RPB - 1) / RPB), 64 * norm_waves(WPR), 0, st>>>(
+                (const T*)x + r * D, w, b, (T*)y + r * D, mean ? mean + r : nullptr, rstd ? rstd + r : nullptr, n,
+                (int)D, eps, vec);
+            SNHIP_CHECK(hipGetLastError());
+        }
         return SNHIP_OK;
     });
 }
