@@ -579,15 +579,28 @@ __global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
     if (tid == 0) tokens[b] = pick;
 }
 
-template <typename T> void sample_t(const SnHipSample& a, int* tokens, hipStream_t st) {
+template <typename T> snhip_status sample_t(const SnHipSample& all, int* tokens, hipStream_t st) {
     // A row of 16 waves is done sooner, two rows of 8 waves share a CU's LDS and registers:
     // 8 for more rows than CUs (top-p 0.9, 512 rows of 12000: 27 us against 39; of 65536: 108
     // against 126) and for short rows, whose barriers weigh more (one row of 1000: 10.2
     // against 11.9); 16 otherwise (64 rows of 32000: 33 against 37; of 8000: 17 both).
-    const unsigned B = (unsigned)a.B;
-    if (a.V < 4) k_sample<T, true, 512><<<B, 512, 0, st>>>(a, tokens);
-    else if (B > 256 || a.V <= 8192) k_sample<T, false, 512><<<B, 512, 0, st>>>(a, tokens);
-    else k_sample<T, false, 1024><<<B, 1024, 0, st>>>(a, tokens);
+    // A grid holds fewer than 2^32 threads: more rows go in several launches.
+    constexpr int64_t most = 1 << 22;
+    for (int64_t r = 0; r < all.B; r += most) {
+        SnHipSample a = all;
+        const unsigned B = (unsigned)(all.B - r < most ? all.B - r : most);
+        a.logits = static_cast<const T*>(all.logits) + r * all.stride;
+        a.u += r;
+        if (a.temperature) a.temperature += r;
+        if (a.top_k) a.top_k += r;
+        if (a.top_p) a.top_p += r;
+        if (a.min_p) a.min_p += r;
+        if (a.V < 4) k_sample<T, true, 512><<<B, 512, 0, st>>>(a, tokens + r);
+        else if (B > 256 || a.V <= 8192) k_sample<T, false, 512><<<B, 512, 0, st>>>(a, tokens + r);
+        else k_sample<T, false, 1024><<<B, 1024, 0, st>>>(a, tokens + r);
+        SNHIP_CHECK(hipGetLastError());
+    }
+    return SNHIP_OK;
 }
 
 }  // namespace
@@ -600,9 +613,7 @@ extern "C" snhip_status snhip_op_sample_dev(const SnHipSample* s, int32_t* token
         s->stride < 0 || s->dtype < SNHIP_F32 || s->dtype > SNHIP_F16)
         return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);
-    if (s->dtype == SNHIP_F32) sample_t<float>(*s, tokens, st);
-    else if (s->dtype == SNHIP_BF16) sample_t<__bf16>(*s, tokens, st);
-    else sample_t<_Float16>(*s, tokens, st);
-    SNHIP_CHECK(hipGetLastError());
-    return SNHIP_OK;
+    if (s->dtype == SNHIP_F32) return sample_t<float>(*s, tokens, st);
+    if (s->dtype == SNHIP_BF16) return sample_t<__bf16>(*s, tokens, st);
+    return sample_t<_Float16>(*s, tokens, st);
 }
