@@ -18,6 +18,7 @@ from __future__ import annotations
 import struct
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _native
@@ -50,6 +51,13 @@ def note_leaves(ctx, device):
         elif "snhip_default_stream" in node.metadata:
             raise RuntimeError("a graph of these leaves, made on the default stream, is still alive: delete its "
                                "outputs before capturing, or make it on another stream")
+
+
+def refuse_tangents(name, *tensors):
+    """Forward-mode derivatives are not there, and a result without one would count as
+    constant. Dual tensors need no requires_grad, and carry their tangents under no_grad."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode derivative")
 
 
 def _ptr(t):
@@ -231,7 +239,9 @@ class GatedDelta(torch.autograd.Function):
 def gated_delta(q, k, v, g, beta, s0=None, *, scale=None, cu_seqlens=None):
     """(out, send) of the gated delta rule under autograd (shapes: delta_fwd). Without
     a gradient to keep anything for, calls of up to 12 tokens run token by token. A capture
-    may hold this and its backward pass; see note_leaves for the one that is refused."""
+    may hold this and its backward pass; see note_leaves for the one that is refused.
+    Forward-mode and second derivatives are refused."""
+    refuse_tangents("gated_delta", q, k, v, g, beta, s0)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, s0)):
         return GatedDelta.apply(q, k, v, g, beta, s0, scale, cu_seqlens)
     if s0 is not None:
@@ -248,6 +258,7 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
                                     or beta.requires_grad or s.requires_grad):
         raise RuntimeError("delta_step keeps nothing for a backward pass: call gated_delta, or use torch.no_grad()")
+    refuse_tangents("delta_step", q, k, v, g, beta, s)
     q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
     dims = _shapes(q, k, v, g, beta, s, None, step=True)
     B, _, N, Hk, H, K, V = dims

@@ -8,7 +8,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _native
-from .delta import DTYPES, _ptr, note_leaves
+from .delta import DTYPES, _ptr, note_leaves, refuse_tangents
 
 __all__ = ["LayerNorm", "layer_norm", "norm_bwd", "norm_fwd"]
 
@@ -98,7 +98,9 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis, under
     autograd: x (..., D) float32, bfloat16 or float16, weight and bias (D) float32 or
     None. Statistics and sums are float32. A capture may hold this and its backward pass;
-    see note_leaves for the one that is refused."""
+    see note_leaves for the one that is refused. Forward-mode and second derivatives are
+    refused."""
+    refuse_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         return LayerNorm.apply(x, weight, bias, float(eps))
     weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
