@@ -277,4 +277,5 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
                       K ** -0.5 if scale is None else float(scale), 0, 0)
     rc = _native.on_device(q.device, _native.lib().snhip_op_delta_step_dev, args, out.data_ptr(), send.data_ptr())
     _native.check(rc, "snhip_op_delta_step_dev")
+    torch.autograd.graph.increment_version(send)       # a graph that saved the old state refuses this one
     return out

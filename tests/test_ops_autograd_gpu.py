@@ -1,0 +1,35 @@
+"""The operators inside other graphs, on the GPU."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from sunnynet_amd import runtime
+
+pytestmark = pytest.mark.gpu
+
+
+def step_args(dev):
+    gen = torch.Generator(dev).manual_seed(1)
+
+    def rn(*s):
+        return torch.randn(*s, generator=gen, device=dev)
+
+    return [rn(2, 1, 8), rn(2, 1, 8), rn(2, 2, 6), -rn(2, 2).abs(), torch.sigmoid(rn(2, 2))], rn(2, 2, 8, 6)
+
+
+@pytest.mark.parametrize("apart", [False, True], ids=["in_place", "send"])
+def test_a_graph_that_saved_the_state_refuses_a_stepped_one(gpu, apart):
+    """w's gradient needs the state that the forward read: once delta_step has written over it,
+    the backward pass is an error and no wrong number."""
+    args, s = step_args(gpu)
+    kept = torch.zeros_like(s) if apart else s
+    w = torch.ones_like(s).requires_grad_()
+    read = (kept * w).sum()
+    runtime.delta_step(*args, s, send=kept)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        read.backward()
+    again = (kept * w).sum()                # the new state, read after the step
+    want = kept.clone()
+    again.backward()
+    assert torch.equal(w.grad, want)
