@@ -194,4 +194,5 @@ def step(a: torch.Tensor, b: torch.Tensor, s: torch.Tensor, gated: bool = False)
     else:
         rc = L.snhip_abi_recur_step(a.data_ptr(), b.data_ptr(), s.data_ptr(), B, N, g)
     _native.check(rc, "snhip_abi_recur_step")
+    torch.autograd.graph.increment_version(s)          # a graph that saved the old state refuses this one
     return s
