@@ -36,13 +36,3 @@ def test_tangents_are_refused_not_dropped(grad):
                     call(args)
         with pytest.raises(NotImplementedError, match=name):
             torch.func.jvp(lambda x: call([x, *args[1:]]), (args[0],), (args[0],))
-
-
-def test_a_graph_that_saved_the_state_refuses_a_stepped_one():
-    """The step of the plain recurrence writes s in place behind a raw pointer."""
-    a, b, s = torch.rand(2, 8), torch.rand(2, 8), torch.rand(2, 8)
-    w = torch.ones(2, 8, requires_grad=True)
-    read = (s * w).sum()
-    runtime.step(a, b, s)
-    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
-        read.backward()

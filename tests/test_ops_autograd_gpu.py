@@ -33,3 +33,14 @@ def test_a_graph_that_saved_the_state_refuses_a_stepped_one(gpu, apart):
     want = kept.clone()
     again.backward()
     assert torch.equal(w.grad, want)
+
+
+@pytest.mark.parametrize("where", ["cpu", "cuda"])
+def test_the_plain_recurrence_counts_as_modifying_its_state(gpu, where):
+    """The step of the plain recurrence writes s in place behind a raw pointer."""
+    a, b, s = (torch.rand(2, 8, device=where) for _ in range(3))
+    w = torch.ones(2, 8, device=where, requires_grad=True)
+    read = (s * w).sum()
+    runtime.step(a, b, s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        read.backward()
