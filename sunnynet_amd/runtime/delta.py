@@ -256,9 +256,10 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
     if q.dim() != 3 or v.dim() != 3 or k.dim() != 3 or g.dim() != 2 or beta.dim() != 2:
         raise ValueError("shape mismatch: q, k (B,Hk,K); v (B,H,V); g, beta (B,H)")
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
-                                    or beta.requires_grad or s.requires_grad):
+                                    or beta.requires_grad or s.requires_grad
+                                    or send is not None and send.requires_grad):
         raise RuntimeError("delta_step keeps nothing for a backward pass: call gated_delta, or use torch.no_grad()")
-    refuse_tangents("delta_step", q, k, v, g, beta, s)
+    refuse_tangents("delta_step", q, k, v, g, beta, s, send)
     q, k, v, g, beta = _rows(q), _rows(k), _rows(v), g.contiguous(), beta.contiguous()
     dims = _shapes(q, k, v, g, beta, s, None, step=True)
     B, _, N, Hk, H, K, V = dims

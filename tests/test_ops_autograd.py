@@ -36,3 +36,14 @@ def test_tangents_are_refused_not_dropped(grad):
                     call(args)
         with pytest.raises(NotImplementedError, match=name):
             torch.func.jvp(lambda x: call([x, *args[1:]]), (args[0],), (args[0],))
+
+
+def test_a_tracked_send_is_refused():
+    """Writing a tensor that autograd tracks would leave its history wrong."""
+    args = delta_args(True)
+    with pytest.raises(RuntimeError, match="gated_delta"):
+        runtime.delta_step(*args, send=torch.zeros_like(args[5]).requires_grad_())
+    with torch.no_grad(), pytest.raises(ValueError, match="one GPU"):
+        runtime.delta_step(*args, send=torch.zeros_like(args[5]).requires_grad_())
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="delta_step"):
+        runtime.delta_step(*args, send=forward_ad.make_dual(torch.zeros_like(args[5]), torch.ones_like(args[5])))
