@@ -78,7 +78,8 @@ int64_t snhip_op_delta_state_floats(const SnHipDelta* d);
 snhip_status snhip_op_delta_fwd_dev(const SnHipDelta* d, void* out, float* send, void* stream);
 
 /* One or a few tokens: the same recurrence token by token, at any T and without
- * workspaces. send may be s0 (updated in place) and must be given. */
+ * workspaces. send must be given; it may be s0 (updated in place), but not overlap it
+ * otherwise. */
 snhip_status snhip_op_delta_step_dev(const SnHipDelta* d, void* out, float* send, void* stream);
 
 /* Gradients: d as in the forward call, with the chunks and states that it wrote.

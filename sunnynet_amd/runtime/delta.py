@@ -269,6 +269,8 @@ def delta_step(q, k, v, g, beta, s, *, scale=None, send=None):
         _check_state(send, (N, H, K, V), "send")
         if send.device != q.device:
             raise ValueError("the delta rule takes tensors of one GPU")
+        if 0 < abs(send.data_ptr() - s.data_ptr()) < s.numel() * 4:
+            raise ValueError("send must be s or lie apart from it")
     out = torch.empty(B, H, V, dtype=v.dtype, device=q.device)
     if B == 0:
         return out

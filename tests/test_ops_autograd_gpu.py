@@ -44,3 +44,17 @@ def test_the_plain_recurrence_counts_as_modifying_its_state(gpu, where):
     runtime.step(a, b, s)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         read.backward()
+
+
+def test_a_send_that_overlaps_the_state_is_refused(gpu):
+    """Heads are read and written in no order, so only the same place or another one will do."""
+    args, s = step_args(gpu)
+    both = torch.zeros(2, *s.shape, device=gpu)
+    both[0] = s
+    flat = both.view(-1)
+    with pytest.raises(ValueError, match="apart"):
+        runtime.delta_step(*args, both[0], send=flat[1:1 + s.numel()].view(s.shape))
+    same = both[0].clone()
+    out = runtime.delta_step(*args, both[0], send=both[1])
+    assert torch.equal(runtime.delta_step(*args, both[0], send=flat[:s.numel()].view(s.shape)), out)
+    assert torch.equal(both[0], both[1]) and not torch.equal(both[0], same)
