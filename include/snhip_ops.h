@@ -148,6 +148,9 @@ typedef struct SnHipSample {
     int64_t dtype;
 } SnHipSample;
 snhip_status snhip_op_sample_dev(const SnHipSample* s, int32_t* tokens, void* stream);
+/* The same, and in drew (B, NULL: not wanted) 1 where u chose the token, 0 where the row
+ * gave its first maximal logit. */
+snhip_status snhip_op_sample_drew_dev(const SnHipSample* s, int32_t* tokens, int32_t* drew, void* stream);
 
 #ifdef __cplusplus
 }

@@ -132,6 +132,7 @@ _SIGS = {
     "snhip_op_norm_bwd_floats": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64]),
     "snhip_op_norm_bwd_dev": (I32, [V, V, V, V, V, V, V, V, V, ctypes.c_int64, ctypes.c_int64, I32, V]),
     "snhip_op_sample_dev": (I32, [CP, V, V]),
+    "snhip_op_sample_drew_dev": (I32, [CP, V, V, V]),
     "snhip_refmath_host": (I32, [V, V, V, I32]),
     "snhip_refmath_dev": (I32, [V, V, V, I32, V]),
 }

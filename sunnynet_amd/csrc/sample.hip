@@ -372,7 +372,7 @@ struct ListView {
     }
 };
 template <typename T, bool ONE, int TH>
-__global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
+__global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens, int* drew) {
     constexpr int NW = TH / 64;
     static_assert(TH >= kList && NW <= 16);
     __shared__ Shared s;
@@ -418,7 +418,16 @@ __global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
         if (lane == 0) s.windex[wave] = at;
         __syncthreads();
         for (int w = 0; w < NW; w++) at = at < s.windex[w] ? at : s.windex[w];
-        if (tid == 0) tokens[b] = at;
+        if (tid == 0) {
+            tokens[b] = at;
+            if (drew) drew[b] = 0;
+        }
+    };
+    auto chosen = [&](int at) {
+        if (tid == 0) {
+            tokens[b] = at;
+            if (drew) drew[b] = 1;
+        }
     };
     if (!(temperature > 0.) || !(fabs(zmax) < INFINITY)) return first_max();
     auto point_of = [&](u64 total) -> u64 {
@@ -483,8 +492,7 @@ __global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
             if (list.first() && mine && before <= point && point < before + mine) s.pick = at;
             __syncthreads();
             if (s.pick < 0) return first_max();        // min-p leaves nothing
-            if (tid == 0) tokens[b] = s.pick;
-            return;
+            return chosen(s.pick);
         } else if (in <= (unsigned)kList) {
             const ListView list((int)s.listed, TH);
             const int n = list.n, me = list.me;
@@ -576,10 +584,10 @@ __global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens) {
     };
     const int pick = find_index(row, s, kept, point_of);
     if (pick < 0) return first_max();
-    if (tid == 0) tokens[b] = pick;
+    chosen(pick);
 }
 
-template <typename T> snhip_status sample_t(const SnHipSample& all, int* tokens, hipStream_t st) {
+template <typename T> snhip_status sample_t(const SnHipSample& all, int* tokens, int* drew, hipStream_t st) {
     // A row of 16 waves is done sooner, two rows of 8 waves share a CU's LDS and registers:
     // 8 for more rows than CUs (top-p 0.9, 512 rows of 12000: 27 us against 39; of 65536: 108
     // against 126) and for short rows, whose barriers weigh more (one row of 1000: 10.2
@@ -595,9 +603,10 @@ template <typename T> snhip_status sample_t(const SnHipSample& all, int* tokens,
         if (a.top_k) a.top_k += r;
         if (a.top_p) a.top_p += r;
         if (a.min_p) a.min_p += r;
-        if (a.V < 4) k_sample<T, true, 512><<<B, 512, 0, st>>>(a, tokens + r);
-        else if (B > 256 || a.V <= 8192) k_sample<T, false, 512><<<B, 512, 0, st>>>(a, tokens + r);
-        else k_sample<T, false, 1024><<<B, 1024, 0, st>>>(a, tokens + r);
+        int* told = drew ? drew + r : nullptr;
+        if (a.V < 4) k_sample<T, true, 512><<<B, 512, 0, st>>>(a, tokens + r, told);
+        else if (B > 256 || a.V <= 8192) k_sample<T, false, 512><<<B, 512, 0, st>>>(a, tokens + r, told);
+        else k_sample<T, false, 1024><<<B, 1024, 0, st>>>(a, tokens + r, told);
         SNHIP_CHECK(hipGetLastError());
     }
     return SNHIP_OK;
@@ -608,12 +617,20 @@ template <typename T> snhip_status sample_t(const SnHipSample& all, int* tokens,
 
 using namespace snhip;
 
-extern "C" snhip_status snhip_op_sample_dev(const SnHipSample* s, int32_t* tokens, void* stream) {
+extern "C" {
+
+snhip_status snhip_op_sample_drew_dev(const SnHipSample* s, int32_t* tokens, int32_t* drew, void* stream) {
     if (!s || !s->logits || !s->u || !tokens || s->B < 1 || s->B > INT32_MAX || s->V < 1 || s->V > (1 << 20) ||
         s->stride < 0 || s->dtype < SNHIP_F32 || s->dtype > SNHIP_F16)
         return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);
-    if (s->dtype == SNHIP_F32) return sample_t<float>(*s, tokens, st);
-    if (s->dtype == SNHIP_BF16) return sample_t<__bf16>(*s, tokens, st);
-    return sample_t<_Float16>(*s, tokens, st);
+    if (s->dtype == SNHIP_F32) return sample_t<float>(*s, tokens, drew, st);
+    if (s->dtype == SNHIP_BF16) return sample_t<__bf16>(*s, tokens, drew, st);
+    return sample_t<_Float16>(*s, tokens, drew, st);
 }
+
+snhip_status snhip_op_sample_dev(const SnHipSample* s, int32_t* tokens, void* stream) {
+    return snhip_op_sample_drew_dev(s, tokens, nullptr, stream);
+}
+
+}  // extern "C"

@@ -29,7 +29,7 @@ def _setting(x, name, B, device, dtype):
     return x.to(dtype).contiguous(), 0
 
 
-def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, drew=False):
     """logits (B, V) float32, bfloat16 or float16 (rows contiguous, any row stride), u (B)
     float64 or float32 in [0, 1) -> tokens (B) int32 on the device, without a host
     synchronization. Each setting is one number or a vector of B. Per row:
@@ -42,7 +42,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     * min_p keeps weights of at least min_p (the largest weight is 1);
     * the token is the first whose running share of what is kept exceeds u.
 
-    A row whose weights have no finite positive sum gives its first maximal logit."""
+    A row whose weights have no finite positive sum gives its first maximal logit. With
+    ``drew`` the result is (2, B): the tokens, and 1 where u chose the row's token, else 0."""
     if logits.dim() != 2 or not 1 <= logits.shape[1] <= MAX_V:
         raise ValueError(f"logits must be (B, V) with V from 1 to {MAX_V}")
     B, V = logits.shape
@@ -56,7 +57,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < 0:
         logits = logits.contiguous()
     dev = logits.device
-    tokens = torch.empty(B, dtype=torch.int32, device=dev)
+    tokens = torch.empty((2, B) if drew else B, dtype=torch.int32, device=dev)
     if B == 0:
         return tokens
     f64 = torch.float64
@@ -67,6 +68,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     m, m0 = _setting(min_p, "min_p", B, dev, f64)
     args = _ARGS.pack(logits.data_ptr(), u.data_ptr(), *(0 if x is None else x.data_ptr() for x in (t, k, p, m)),
                       float(t0), float(p0), float(m0), int(k0), B, V, logits.stride(0), DTYPES[logits.dtype])
-    rc = _native.on_device(dev, _native.lib().snhip_op_sample_dev, args, tokens.data_ptr())
-    _native.check(rc, "snhip_op_sample_dev")
+    rc = _native.on_device(dev, _native.lib().snhip_op_sample_drew_dev, args, tokens.data_ptr(),
+                           tokens[1].data_ptr() if drew else None)
+    _native.check(rc, "snhip_op_sample_drew_dev")
     return tokens

@@ -43,7 +43,8 @@ def sample_logits(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None, min_p=0
     """Next token from logits (V,): argmax at temperature <= 0, else softmax
     sampling after top-k and top-p (nucleus) filtering (serve.py:29-56), then
     of the tokens at least ``min_p`` times as probable as the best one. Draws
-    one number from ``rng``."""
+    one number from ``rng``, or none where no finite distribution is left (the
+    argmax then)."""
     if temperature is None or temperature <= 0:
         return int(np.argmax(logits))
     z = np.asarray(logits, dtype=np.float64) / float(temperature)
@@ -69,6 +70,14 @@ def sample_logits(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None, min_p=0
         return int(np.argmax(logits))
     rng = rng or np.random.default_rng()
     return int(rng.choice(z.size, p=p / total))
+
+
+def _give_back(rng):
+    """Take back the one number drawn last from a PCG64 generator."""
+    bits = rng.bit_generator
+    state = bits.state
+    bits.advance((1 << 128) - 1)               # its period less one; drops the held half word
+    bits.state = {**state, "state": bits.state["state"]}
 
 
 class HipState:
@@ -225,8 +234,10 @@ class Request:
     @property
     def on_device(self) -> bool:
         """Whether the device sampler knows the request's settings (it does unless
-        top_k is negative)."""
-        return self.greedy or not self.top_k or self.top_k > 0
+        top_k is negative) and its generator (submit's kind can take a number back)."""
+        return self.greedy or ((not self.top_k or self.top_k > 0) and
+                               (self.rng is None or isinstance(getattr(self.rng, "bit_generator", None),
+                                                               np.random.PCG64)))
 
     @property
     def settings(self) -> tuple:
@@ -293,7 +304,8 @@ class BatchScheduler:
 
     def _sample(self, logits, wanted):
         """The next tokens on the device: sample_logits' rules, with one number
-        from each sampling request's own generator, as it draws them."""
+        from each sampling request's own generator, as it draws them: a row without
+        a distribution draws none."""
         dev = logits.device
         held = [r.settings for r in self.active]
         if held != self._held:             # they go over only when one of them changes
@@ -301,10 +313,15 @@ class BatchScheduler:
             self._settings = (torch.tensor(cols, dtype=torch.float64, device=dev),
                               torch.tensor(top_k, dtype=torch.int32, device=dev))
             self._held = held
-        u = torch.tensor([(r.rng or np.random.default_rng()).random() if w and not r.greedy else 0.0
-                          for r, w in zip(self.active, wanted)], dtype=torch.float64, device=dev)
+        draws = [w and not r.greedy for r, w in zip(self.active, wanted)]
+        u = torch.tensor([(r.rng or np.random.default_rng()).random() if d else 0.0
+                          for r, d in zip(self.active, draws)], dtype=torch.float64, device=dev)
         (temperature, top_p, min_p), top_k = self._settings
-        return sample_tokens(logits, u, temperature, top_k, top_p, min_p).cpu().numpy()
+        picks, drew = sample_tokens(logits, u, temperature, top_k, top_p, min_p, True).cpu().numpy()
+        for r, d, used in zip(self.active, draws, drew):
+            if d and not used and r.rng is not None:
+                _give_back(r.rng)
+        return picks
 
     def step(self) -> int:
         """One iteration over every active request; returns how many stepped."""

@@ -27,3 +27,18 @@ def test_more_rows_than_a_grid_holds(gpu):
         assert torch.equal(runtime.sample_tokens(x[part], u[part], t[part], k[part], p[part], m[part]), got[part])
     greedy = runtime.sample_tokens(x, u, 0.0)
     assert torch.equal(greedy.long(), x.float().argmax(1))
+
+
+def test_whether_u_chose_the_token(gpu):
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[0.0, 1, 2, 3, -inf], [nan, 1, 2, 3, 4], [1, inf, 0, 0, 0], [-inf] * 5, [1, 2, 3, 4, 5]], device=gpu)
+    u = torch.full((5,), 0.3, device=gpu)
+    t = torch.tensor([1.0, 1, 1, 1, 0], device=gpu)
+    for more in ((0, 1.0, 0.0), (2, 1.0, 0.0), (0, 0.9, 0.0), (2, 0.9, 0.1)):
+        both = runtime.sample_tokens(x, u, t, *more, drew=True)
+        assert both.shape == (2, 5) and both[1].tolist() == [1, 0, 0, 0, 0]
+        assert torch.equal(both[0], runtime.sample_tokens(x, u, t, *more))
+        assert both[0, 1:].tolist() == [0, 1, 0, 4]
+    for k in (0, 2):                       # min-p above every weight leaves nothing
+        assert runtime.sample_tokens(x[:1], u[:1], 1.0, k, 1.0, 2.0, drew=True).tolist() == [[3], [0]]
+    assert runtime.sample_tokens(x[:0], u[:0], drew=True).shape == (2, 0)
