@@ -212,6 +212,9 @@ class HipRwkvEngine:
             state.shift.copy_(sh)
 
 
+_GREEDY = 0.0, 1.0, 0.0, 0
+
+
 @dataclass
 class Request:
     prompt: list
@@ -235,15 +238,15 @@ class Request:
     def on_device(self) -> bool:
         """Whether the device sampler knows the request's settings (it does unless
         top_k is negative) and its generator (submit's kind can take a number back)."""
-        return self.greedy or ((not self.top_k or self.top_k > 0) and
-                               (self.rng is None or isinstance(getattr(self.rng, "bit_generator", None),
-                                                               np.random.PCG64)))
+        bits = getattr(self.rng, "bit_generator", None)
+        return self.greedy or ((not self.top_k or self.top_k > 0)
+                               and (self.rng is None or isinstance(bits, np.random.PCG64)))
 
     @property
     def settings(self) -> tuple:
         """(temperature, top_p, min_p, top_k) as the device sampler takes them."""
         if self.greedy:
-            return 0.0, 1.0, 0.0, 0
+            return _GREEDY
         return float(self.temperature), float(self.top_p), float(self.min_p or 0.0), min(int(self.top_k or 0), 1 << 30)
 
     def next_input(self) -> int:
@@ -302,18 +305,17 @@ class BatchScheduler:
             self.finished.append(self.active[i])
         self.active = [self.active[i] for i in keep]
 
-    def _sample(self, logits, wanted):
-        """The next tokens on the device: sample_logits' rules, with one number
-        from each sampling request's own generator, as it draws them: a row without
-        a distribution draws none."""
+    def _sample(self, logits, on_host, draws):
+        """The next tokens of the rows that are not sampled on the host, on the device:
+        sample_logits' rules, with one number from the own generator of each request
+        that draws, as it draws them: a row without a distribution draws none."""
         dev = logits.device
-        held = [r.settings for r in self.active]
+        held = [_GREEDY if h else r.settings for r, h in zip(self.active, on_host)]
         if held != self._held:             # they go over only when one of them changes
             *cols, top_k = zip(*held)
             self._settings = (torch.tensor(cols, dtype=torch.float64, device=dev),
                               torch.tensor(top_k, dtype=torch.int32, device=dev))
             self._held = held
-        draws = [w and not r.greedy for r, w in zip(self.active, wanted)]
         u = torch.tensor([(r.rng or np.random.default_rng()).random() if d else 0.0
                           for r, d in zip(self.active, draws)], dtype=torch.float64, device=dev)
         (temperature, top_p, min_p), top_k = self._settings
@@ -334,21 +336,25 @@ class BatchScheduler:
         logits = self.model.step_batch(toks)
         self.steps += 1
         wanted = [r.pos >= len(r.prompt) - 1 for r in self.active]     # past the prompt after this step
-        picks = host = None
-        if all(r.greedy for r in self.active):
+        greedy = [r.greedy for r in self.active]
+        picks, on_host = None, [False] * n
+        if all(greedy):
             picks = logits.argmax(1).cpu().numpy()
-        elif logits.is_cuda and logits.shape[1] <= MAX_V and all(r.on_device for r in self.active):
-            picks = self._sample(logits, wanted)
-        else:
-            host = logits.float().cpu().numpy()
+        else:                              # a row goes by its own settings, whatever its neighbours ask for
+            device = logits.is_cuda and logits.shape[1] <= MAX_V
+            on_host = [not (g or device and r.on_device) for r, g in zip(self.active, greedy)]
+            if any(on_host):
+                host = logits.float().cpu().numpy()
+                on_host = [h or g for h, g in zip(on_host, greedy)]
+            if not all(on_host):
+                picks = self._sample(logits, on_host, [w and not (h or g) for w, h, g in zip(wanted, on_host, greedy)])
         gone = []
         for i, r in enumerate(self.active):
             if r.pos < len(r.prompt):
                 r.pos += 1
                 if r.pos < len(r.prompt):
                     continue                   # still prefilling: logits unused
-            t = int(picks[i]) if host is None else sample_logits(host[i], r.temperature, r.top_p, r.top_k, r.rng,
-                                                                 r.min_p)
+            t = sample_logits(host[i], r.temperature, r.top_p, r.top_k, r.rng, r.min_p) if on_host[i] else int(picks[i])
             r.output.append(t)
             if len(r.output) >= r.max_tokens or (r.eos is not None and t == r.eos):
                 gone.append(i)

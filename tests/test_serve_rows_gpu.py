@@ -73,3 +73,27 @@ def test_other_generators_sample_on_the_host(gpu):
     sch.run()
     for i, (r, g) in enumerate(zip(reqs, gens)):
         assert r.output == [sample_logits(steps[t, i].astype(np.float32), 1.0, rng=g) for t in range(6)]
+
+
+def test_neighbours_do_not_move_a_row_to_the_host(gpu, monkeypatch):
+    """Equal logits at the nucleus' border go by index on the device and in no fixed order on the
+    host: a request's tokens are its own whether or not a neighbour's settings need the host."""
+    rng = np.random.default_rng(3)
+    tied = np.round(rng.standard_normal((40, 3, 300)))
+    own = [dict(temperature=1.0, top_p=0.5), dict(temperature=1.3, top_p=0.6)]
+    out = []
+    for other in (dict(temperature=1.0), dict(temperature=1.0, top_k=-3)):
+        sch = BatchScheduler(Given(tied, gpu))
+        reqs = [sch.submit([1], 40, seed=i, **s) for i, s in enumerate([*own, other])]
+        sch.run()
+        out.append([r.output for r in reqs])
+    assert out[0][:2] == out[1][:2]
+    gen = np.random.default_rng(2)         # the neighbour itself is sampled on the host
+    assert out[1][2] == [sample_logits(tied[t, 2].astype(np.float32), 1.0, 1.0, -3, gen) for t in range(40)]
+
+
+def test_a_batch_of_rows_for_both(gpu):
+    rng = np.random.default_rng(4)
+    serve(2 * rng.standard_normal((12, 5, 90)), [dict(temperature=1.0, top_k=-5), dict(), dict(temperature=0.7, top_k=9),
+                                                 dict(temperature=1.1, top_p=0.8), dict(temperature=0.5, top_k=-1)], gpu,
+          prompts=[1, 3, 1, 7, 4])
