@@ -338,7 +338,9 @@ class BatchScheduler:
         wanted = [r.pos >= len(r.prompt) - 1 for r in self.active]     # past the prompt after this step
         greedy = [r.greedy for r in self.active]
         picks, on_host = None, [False] * n
-        if all(greedy):
+        if not any(wanted):                # prompts only: no token is chosen, nothing waits for the logits
+            pass
+        elif all(greedy):
             picks = logits.argmax(1).cpu().numpy()
         else:                              # a row goes by its own settings, whatever its neighbours ask for
             device = logits.is_cuda and logits.shape[1] <= MAX_V

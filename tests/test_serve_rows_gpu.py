@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from sunnynet_amd.runtime import serve as serve_module
 from sunnynet_amd.runtime.serve import BatchScheduler, sample_logits
 
 pytestmark = pytest.mark.gpu
@@ -97,3 +98,13 @@ def test_a_batch_of_rows_for_both(gpu):
     serve(2 * rng.standard_normal((12, 5, 90)), [dict(temperature=1.0, top_k=-5), dict(), dict(temperature=0.7, top_k=9),
                                                  dict(temperature=1.1, top_p=0.8), dict(temperature=0.5, top_k=-1)], gpu,
           prompts=[1, 3, 1, 7, 4])
+
+
+def test_steps_inside_prompts_choose_nothing(gpu, monkeypatch):
+    """Steps that leave every request inside its prompt do not sample or copy logits."""
+    calls = []
+    plain = serve_module.sample_tokens
+    monkeypatch.setattr(serve_module, "sample_tokens", lambda *a: calls.append(a[0].shape[0]) or plain(*a))
+    rng = np.random.default_rng(6)
+    serve(rng.standard_normal((8, 2, 30)), [dict(temperature=1.0), dict(temperature=0.5, top_k=4)], gpu, prompts=[5, 7])
+    assert len(calls) == 4                 # from the fifth step on
