@@ -27,6 +27,7 @@ ones it would produce alone.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -236,10 +237,11 @@ class Request:
 
     @property
     def on_device(self) -> bool:
-        """Whether the device sampler knows the request's settings (it does unless
-        top_k is negative) and its generator (submit's kind can take a number back)."""
-        bits = getattr(self.rng, "bit_generator", None)
-        return self.greedy or ((not self.top_k or self.top_k > 0)
+        """Whether the device sampler knows the request's settings (a finite temperature
+        and a top_k that is a whole number from 0 on, or None) and its generator (submit's
+        kind can take a number back)."""
+        k, bits = self.top_k, getattr(self.rng, "bit_generator", None)
+        return self.greedy or ((not k or isinstance(k, (int, np.integer)) and k > 0) and math.isfinite(self.temperature)
                                and (self.rng is None or isinstance(bits, np.random.PCG64)))
 
     @property

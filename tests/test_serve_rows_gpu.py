@@ -108,3 +108,14 @@ def test_steps_inside_prompts_choose_nothing(gpu, monkeypatch):
     rng = np.random.default_rng(6)
     serve(rng.standard_normal((8, 2, 30)), [dict(temperature=1.0), dict(temperature=0.5, top_k=4)], gpu, prompts=[5, 7])
     assert len(calls) == 4                 # from the fifth step on
+
+
+@pytest.mark.filterwarnings("ignore::RuntimeWarning")
+def test_settings_that_only_the_host_knows(gpu):
+    """top_k that is no whole number, and temperatures that are not finite."""
+    rng = np.random.default_rng(7)
+    steps = rng.standard_normal((7, 6, 60))
+    steps[2, 3, 10:] = -INF                # at an infinite temperature no distribution, by the host's rule
+    settings = [dict(temperature=1.0, top_k=INF), dict(temperature=1.0, top_k=np.int64(5)), dict(temperature=INF),
+                dict(temperature=INF, top_p=0.5), dict(temperature=NAN), dict(temperature=0.9, top_k=None)]
+    serve(steps, settings, gpu)
