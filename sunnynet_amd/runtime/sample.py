@@ -24,8 +24,9 @@ def _setting(x, name, B, device, dtype):
         return None, x
     if x.shape != (B,) or x.device != device or x.dtype.is_complex or x.dtype == torch.bool:
         raise ValueError(f"{name} must be a number or a vector of one number per row on the logits' device")
-    if x.dtype == torch.int64 and dtype == torch.int32:
-        x = x.clamp(max=MAX_V)             # as large as any row: no filter, and not another number in 32 bits
+    if dtype == torch.int32 and x.dtype not in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        # to what filters alike, so that 32 bits do not make another number of it
+        x = (x.double().nan_to_num(0) if x.is_floating_point() else x.to(torch.int64)).clamp(0, MAX_V)
     return x.to(dtype).contiguous(), 0
 
 
@@ -67,7 +68,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, dre
     p, p0 = _setting(top_p, "top_p", B, dev, f64)
     m, m0 = _setting(min_p, "min_p", B, dev, f64)
     args = _ARGS.pack(logits.data_ptr(), u.data_ptr(), *(0 if x is None else x.data_ptr() for x in (t, k, p, m)),
-                      float(t0), float(p0), float(m0), int(k0), B, V, logits.stride(0), DTYPES[logits.dtype])
+                      float(t0), float(p0), float(m0), min(max(int(k0), 0), MAX_V), B, V, logits.stride(0), DTYPES[logits.dtype])
     rc = _native.on_device(dev, _native.lib().snhip_op_sample_drew_dev, args, tokens.data_ptr(),
                            tokens[1].data_ptr() if drew else None)
     _native.check(rc, "snhip_op_sample_drew_dev")

@@ -42,3 +42,22 @@ def test_whether_u_chose_the_token(gpu):
     for k in (0, 2):                       # min-p above every weight leaves nothing
         assert runtime.sample_tokens(x[:1], u[:1], 1.0, k, 1.0, 2.0, drew=True).tolist() == [[3], [0]]
     assert runtime.sample_tokens(x[:0], u[:0], drew=True).shape == (2, 0)
+
+
+def test_top_k_by_row_of_other_types(gpu):
+    """Numbers that 32 bits do not hold filter as they are: none below 1, none from V on."""
+    gen = torch.Generator(gpu).manual_seed(4)
+    x = torch.randn(6, 900, device=gpu, generator=gen)
+    u = torch.rand(6, dtype=torch.float64, device=gpu, generator=gen)
+    none, five = runtime.sample_tokens(x, u, 1.5), runtime.sample_tokens(x, u, 1.5, 5)
+    assert not torch.equal(none, five)
+    far = [-(1 << 32) + 5, (1 << 32) + 5, -(1 << 62), 1 << 62, -1, 0]
+    assert torch.equal(runtime.sample_tokens(x, u, 1.5, torch.tensor(far, device=gpu)), none)
+    for dt in (torch.float32, torch.float64):
+        far = torch.tensor([-1e30, 1e30, float("inf"), -float("inf"), float("nan"), 0.0], dtype=dt, device=gpu)
+        assert torch.equal(runtime.sample_tokens(x, u, 1.5, far), none)
+    for dt in (torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.float16, torch.float64):
+        k = torch.full((6,), 5, dtype=dt, device=gpu)
+        assert torch.equal(runtime.sample_tokens(x, u, 1.5, k), five)
+    assert torch.equal(runtime.sample_tokens(x, u, 1.5, 10 ** 30), none)
+    assert torch.equal(runtime.sample_tokens(x, u, 1.5, -10 ** 30), none)
