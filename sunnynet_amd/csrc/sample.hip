@@ -438,8 +438,9 @@ __global__ __launch_bounds__(TH) void k_sample(SnHipSample a, int* tokens, int* 
     w.m = (double)m;
     w.step = fmin(kFracs / (0.69314718055994530942 * temperature), 1e300);
     w.low = min_p * ldexp(1., bits);
-    const float per = (float)fmin((double)kBins / ((double)kRange * temperature), 1e30);
-    auto bin_of = [&](float x) { return (int)fminf((m - x) * per, 2.f * kBins); };     // kBins and up: weight 0
+    // in halves, whose difference is finite for any two finite logits
+    const float per = (float)fmin(2. * kBins / ((double)kRange * temperature), 1e30), half = 0.5f * m;
+    auto bin_of = [&](float x) { return (int)fminf(fmaf(x, -0.5f, half) * per, 2.f * kBins); };     // kBins and up: weight 0
 
     Cut cut{-INFINITY, INT32_MAX};
     const bool some_k = top_k > 0 && top_k < row.V, some_p = top_p > 0. && top_p < 1.;

@@ -2,6 +2,7 @@
 limits, and settings far from 1."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
@@ -61,3 +62,38 @@ def test_top_k_by_row_of_other_types(gpu):
         assert torch.equal(runtime.sample_tokens(x, u, 1.5, k), five)
     assert torch.equal(runtime.sample_tokens(x, u, 1.5, 10 ** 30), none)
     assert torch.equal(runtime.sample_tokens(x, u, 1.5, -10 ** 30), none)
+
+
+def pick(row, u, t, k, p, m):
+    """The definition for one row of float64 (temperature > 0)."""
+    z = row / t
+    w = np.exp(z - z.max())
+    if 0 < k < z.size:
+        w[z < np.sort(z)[-k]] = 0.0
+    if 0 < p < 1:
+        order = np.argsort(-z, kind="stable")
+        ws = w[order]
+        cut = np.cumsum(ws) - ws > p * ws.sum()
+        cut[0] = False
+        w[order[cut]] = 0.0
+    w[w < m] = 0.0
+    c = np.cumsum(w) / w.sum()
+    return int(np.searchsorted(c, u, side="right")), np.abs(c - u).min()
+
+
+def test_logits_further_apart_than_fp32_reaches(gpu):
+    """Differences of two finite logits that are infinite in fp32, at a temperature that makes
+    them ordinary. Random numbers nearer than 1e-9 to a border are left out."""
+    rng = np.random.default_rng(5)
+    x = torch.tensor(rng.uniform(-3.4e38, 3.4e38, (40, 700)), dtype=torch.float32)
+    rows, tested = x.double().numpy(), 0
+    for t in (1e38, 4e37, 3e39):
+        for k, p, m in ((0, 1.0, 0.0), (600, 1.0, 0.0), (0, 0.97, 0.0), (650, 0.9, 0.01), (120, 1.0, 0.0)):
+            u = rng.random(40)
+            got = runtime.sample_tokens(x.to(gpu), torch.tensor(u).to(gpu), t, k, p, m).tolist()
+            for i in range(40):
+                want, near = pick(rows[i], u[i], t, k, p, m)
+                if near > 1e-9:
+                    assert got[i] == want, (t, k, p, m, i)
+                    tested += 1
+    assert tested > 590
