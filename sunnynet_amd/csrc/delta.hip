@@ -114,8 +114,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
     }
 }
 
-// The scan over chunks: kDeltaW waves, 16 columns of V each. Half types read the state by
-// two planes where only out (of that type) depends on it. The next chunk's tiles are
+// The scan over chunks: kDeltaW waves, 16 columns of V each. The next chunk's tiles are
 // fetched into registers while this one is worked on, and put into the other half of LDS:
 // one barrier per chunk, no wait for memory in between. Bound by the chain of a chunk's
 // products (each waits for the one before), of which a SIMD has one to three waves to
@@ -126,12 +125,10 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
 template <typename T, int KP, bool VEC, int PASS>
 __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, float* send) {
     constexpr int P = ElemPlanes<T>::n, NK = KP / 16, W = kDeltaW, NTH = 64 * W;
-    constexpr int LO = sizeof(T) == 4 ? 3 : 2;      // planes of the products that only reach out
     constexpr int NS = sizeof(T) == 4 || KP == 64 ? 1 : 2;
     typedef Tile<P, kDC, KP> Rows;
-    typedef Tile<3, kDC, kDC> MatM;
-    typedef Tile<LO, kDC, kDC> MatP;
-    __shared__ alignas(16) __bf16 sk[2][Rows::elems], sq[2][Rows::elems], sm[2][MatM::elems], sp[2][MatP::elems];
+    typedef Tile<3, kDC, kDC> Mat;
+    __shared__ alignas(16) __bf16 sk[2][Rows::elems], sq[2][Rows::elems], sm[2][Mat::elems], sp[2][Mat::elems];
     __shared__ alignas(16) float sv[2][3 * kDC];
     const SnHipDelta& d = a.d;
     const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, g8 = (lane >> 4) * 8;
@@ -163,8 +160,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             else S[kt][r] = PASS == 0 && v < a.VP ? part[(int64_t)KP * (a.VP + KP) + k * a.VP + v] : 0.f;
         }
     RowsFetch<T, KP, NTH, VEC> fk, fq;
-    MatFetch<3, NTH> fm;
-    MatFetch<LO, NTH> fp;
+    MatFetch<3, NTH> fm, fp;
     float fv[(3 * kDC + NTH - 1) / NTH];
     unsigned vv[8];
     fk.init(d.k_stride[1], Kd, tid);
@@ -186,10 +182,10 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
     };
     auto store = [&](int b) {
         fk.store(Rows{sk[b]}, tid);
-        fm.store(MatM{sm[b]}, tid);
+        fm.store(Mat{sm[b]}, tid);
         if (PASS == 0) {
             fq.store(Rows{sq[b]}, tid);
-            fp.store(MatP{sp[b]}, tid);
+            fp.store(Mat{sp[b]}, tid);
         }
 #pragma unroll
         for (int j = 0; j * NTH < 3 * kDC; j++)
@@ -229,7 +225,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             const Frag<P> kf[2] = {K.frag(pair_row(0, l16), 32 * p, lane), K.frag(pair_row(1, l16), 32 * p, lane)},
                           qf[2] = {Q.frag(pair_row(0, l16), 32 * p, lane), Q.frag(pair_row(1, l16), 32 * p, lane)};
             mma_n<3>(kf, f, ks);
-            if (PASS == 0) mma_n<LO>(qf, f, o);
+            if (PASS == 0) mma_n<3>(qf, f, o);
         }
         float G[8], L[8], be[8], x[8], y[8];
 #pragma unroll
@@ -246,7 +242,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             o[i >> 2][i & 3] *= (float)d.scale * G[i];
         }
         const Frag<3> X = split8<3>(x);
-        const MatM M{sm[b]};
+        const Mat M{sm[b]};
         const Frag<3> mf[2] = {M.frag(pair_row(0, l16), 0, lane), M.frag(pair_row(1, l16), 0, lane)};
         f32x4 e[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
         mma_n<3>(mf, X, e);
@@ -265,7 +261,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             for (int m = 0; m < 2; m++)
                 buf_store4(re, (v * kDC * NS + t0 % (kDC * NS) + g8 + 4 * m) * 4, e[m]);
         }
-        const Frag<LO> U = split8<LO>(x);
+        const Frag<3> U = split8<3>(x);
         const Frag<3> LU = split8<3>(y);
         const float decay = sv[b][kDC - 1];
 #pragma unroll
@@ -286,7 +282,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             rows_window(out + ((s.row + t0) * d.H + h) * (int64_t)V, d.H * (int64_t)V, n, V);
 #pragma unroll
         for (int m = 0; m < 2; m++) {
-            o[m] = mma<LO>(MatP{sp[b]}.frag(pair_row(m, l16), 0, lane), U, o[m]);
+            o[m] = mma<3>(Mat{sp[b]}.frag(pair_row(m, l16), 0, lane), U, o[m]);
 #pragma unroll
             for (int r = 0; r < 4; r++) buf_store<T>(ro, o_off + (4 * m + r) * o_step, (T)o[m][r]);
         }
