@@ -332,7 +332,7 @@ template <int KP> __global__ __launch_bounds__(2 * KP) void k_delta_join(DeltaP 
             for (int m = 0; m < 2; m++)
 #pragma unroll
                 for (int p = 0; p < NP; p++)
-                    na[m][p] = load_raw8(from + (row0 + pair_row(m, l16)) * ld + a.VP + 32 * p + g8, 8, true);
+                    na[m][p] = load_floats8(from + (row0 + pair_row(m, l16)) * ld + a.VP + 32 * p + g8);
     };
     fetch(part, false);
     for (int seg = 0; seg + 1 < a.segs && (seg + 1) * a.seg_chunks * kDC < s.len; seg++, part += step) {

@@ -147,22 +147,10 @@ template <int P, int R, int C, int PAD = 8> struct Tile {
 
 template <typename T> using Vec8 = T __attribute__((ext_vector_type(8)));
 
-// Eight consecutive elements from `src`, of which the first `n` exist (the rest are 0).
-// vec: the address is 16-byte aligned.
-template <typename T> __device__ __forceinline__ Vec8<T> load_raw8(const T* src, int n, bool vec) {
-    Vec8<T> x;
-    if (vec && n >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
-            x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-        } else {
-            x = *reinterpret_cast<const Vec8<T>*>(src);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = i < n ? src[i] : (T)0.f;
-    }
-    return x;
+// Eight consecutive floats from a 16-byte aligned address.
+__device__ __forceinline__ Vec8<float> load_floats8(const float* src) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // A window of n rows of `len` elements, `stride` elements apart, as a buffer: an offset

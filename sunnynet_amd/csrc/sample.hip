@@ -46,7 +46,7 @@ __device__ __forceinline__ float key_logit(unsigned k) {
 }
 
 struct Shared {
-    u64 sum[kBins];                // of bins; the groups' sums at the end
+    u64 sum[kBins];                // of bins
     unsigned count[kBins];
     double exp2[kFracs];           // 2^(j / kFracs + bits)
     u64 wsum[16];

@@ -97,3 +97,59 @@ def test_logits_further_apart_than_fp32_reaches(gpu):
                     assert got[i] == want, (t, k, p, m, i)
                     tested += 1
     assert tested > 590
+
+
+LONG = [(1.0, 0, 1.0, 0.0), (0.7, 40, 0.95, 0.0), (0.9, 0, 0.9, 0.02), (1.2, 700, 0.8, 0.0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V", [8193, 12000, 65537])
+def test_many_long_rows(gpu, V, dtype):
+    """More than 256 rows of more than 8192 logits: rows of 8 waves, against the definition and
+    against calls of fewer rows, which have 16."""
+    rng = np.random.default_rng(V)
+    for B in (257, 512):
+        x = torch.tensor(2.5 * rng.standard_normal((B, V)), dtype=torch.float32).to(dtype)
+        rows, u, dev = x[:6].double().numpy(), rng.random(B), x.to(gpu)
+        for mix in LONG:
+            near = [pick(rows[i], u[i], *mix) for i in range(6)]
+            got = runtime.sample_tokens(dev, torch.tensor(u).to(gpu), *mix)
+            for i, (want, gap) in enumerate(near):
+                if gap > V * 2.0 ** -45:               # the weights' rounding at this V: below 2^-46 each
+                    assert int(got[i]) == want, (mix, i)
+            half = [runtime.sample_tokens(dev[s], torch.tensor(u[s]).to(gpu), *mix)
+                    for s in (slice(0, 200), slice(200, 400), slice(400, B)) if s.start < B]
+            assert torch.equal(torch.cat(half), got)
+
+
+@pytest.mark.parametrize("V", [(1 << 20) - 1, 1 << 20])
+def test_the_longest_rows(gpu, V):
+    """Weights are whole multiples of 2^-42 of the largest, so shares are off by less than
+    V 2^-43, and with the total's own rounding less than V 2^-42: random numbers and nuclei
+    nearer than that to a border are moved."""
+    rng = np.random.default_rng(V)
+    x = torch.tensor(6 * rng.standard_normal(V), dtype=torch.float32)
+    row, near = x.double().numpy(), V * 2.0 ** -42
+    for t, k, p, m in ((1.0, 0, 1.0, 0.0), (0.8, 5000, 1.0, 0.0), (0.9, 0, 0.6, 0.0), (1.0, 200, 0.9, 1e-3)):
+        if p < 1:
+            z = np.sort(row)[::-1] / t
+            w = np.exp(z - z[0])
+            if k:
+                w = w[:k]
+            edge = np.cumsum(w) / w.sum()
+            while np.abs(edge - p).min() < near:
+                p += 1e-4
+        u, want = [], []
+        while len(u) < 300:
+            c = rng.random()
+            if len(u) < 3:
+                tok, gap = pick(row, c, t, k, p, m)
+                if gap < near:
+                    continue
+                want.append(tok)
+            u.append(c)
+        u = torch.tensor(u, dtype=torch.float64).to(gpu)
+        few = runtime.sample_tokens(x.to(gpu)[None].expand(3, V), u[:3], t, k, p, m)
+        many = runtime.sample_tokens(x.to(gpu)[None].expand(300, V), u, t, k, p, m)
+        assert few.tolist() == want and torch.equal(many[:3], few)
+        assert torch.equal(many[-3:], runtime.sample_tokens(x.to(gpu)[None].expand(3, V), u[-3:], t, k, p, m))
