@@ -130,8 +130,10 @@ snhip_status snhip_op_norm_bwd_dev(const void* dy, const void* x, const float* w
  *   the token is the first one up to which the remaining weights sum to more than u
  *   of their total.
  * A row whose weights have no finite positive sum (an infinite or NaN maximum) gives
- * its first maximal logit. Weights are summed as whole numbers (of 2^-42 at
- * V = 2^20, 2^-47 at 32000), so a token does not depend on an order of summation. tokens (B) int32.
+ * its first maximal logit. Weights are summed as whole numbers of 2^-b of the largest,
+ * b = min(51, 62 - ceil(log2 V)) (42 at V = 2^20, 47 at 32000), so a token does not depend
+ * on an order of summation, and differs from that of exact weights only where u or a
+ * nucleus' end is within V 2^-b of a border, as a share. tokens (B) int32.
  * 1 <= V <= 2^20, B < 2^31. */
 typedef struct SnHipSample {
     const void* logits;

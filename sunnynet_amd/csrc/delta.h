@@ -35,9 +35,9 @@ constexpr int64_t kDeltaTokens = (1 << 30) - 1;
 // Chunks of a call: the kernels launch up to 512 threads for each, in one dimension of a
 // grid that holds fewer than 2^32.
 constexpr int64_t kDeltaSlots = (1 << 23) - 1;
-// The longest call that runs token by token without workspaces. 12 heads of 64, one
-// sequence: 11.5 us token by token and 11.8 in chunks at 12 tokens; 64 sequences of 16
-// heads of 128: 46 and 78 us (57 and 78 at 16).
+// The longest call that runs token by token without workspaces. 12 tokens, calls with their
+// host work: one sequence, 12 heads of 64 in fp32, 13.2 us token by token and 18.7 in chunks;
+// 64 sequences, 16 heads of 128 in bf16, 45 and 78 (57 and 78 at 16 tokens).
 constexpr int kDeltaStepTokens = 12;
 // Waves of a block of the scans, 16 columns of V each.
 constexpr int kDeltaW = 4;
@@ -47,7 +47,7 @@ constexpr int64_t kDeltaStride = 1 << 24;
 struct DeltaP {
     SnHipDelta d;
     int64_t slots, groups;  // chunk slots of all sequences; groups of NS chunks
-    int KP, VP;             // K and V padded: saved states are (KP, VP), errors (VP, 32)
+    int KP, VP;             // K and V padded: saved states are (KP, VP), errors (VP, 32 NS)
     int rep;                // value heads per query and key head
     int segs, seg_chunks;   // parts of a sequence that are scanned at once, and their chunks
     float* seg_state;       // per sequence, part and head: delta_seg_floats
@@ -70,8 +70,8 @@ __host__ __device__ inline int delta_vp(int64_t V) { return (int)((V + 15) / 16 
 
 // The backward takes NS chunks at a time, and states are kept per such group. Two halve the
 // bytes of the states: forward and backward of 8 x 2048 tokens, 16 heads of 128 in bf16,
-// take 1.13 ms with two and 1.38 with one. Heads of up to 64 have a quarter of those bytes,
-// and their tiles of one chunk leave room for more blocks on a CU (0.67 ms with one, 0.77
+// take 1.05 ms with two and 1.35 with one. Heads of up to 64 have a quarter of those bytes,
+// and their tiles of one chunk leave room for more blocks on a CU (0.65 ms with one, 0.73
 // with two); three planes of fp32 leave no room for two.
 __host__ __device__ constexpr int delta_ns(int64_t dtype, int64_t K) { return dtype == SNHIP_F32 || K <= 64 ? 1 : 2; }
 __host__ __device__ inline int64_t delta_groups(const SnHipDelta& d) {
@@ -102,7 +102,7 @@ inline int delta_segs(const SnHipDelta& d) {
     int64_t n = kDeltaWaves / waves;
     if (n > chunks / kDeltaSegChunks) n = chunks / kDeltaSegChunks;
     // Below four parts the second pass and the join take what the first one gives. 16384
-    // tokens, 16 heads of 128 in fp16: 1,612 us in one part, 531 in eight.
+    // tokens, 16 heads of 128 in fp16: 1,776 us in one part, 537 in eight.
     return n < 4 ? 1 : n > 16 ? 16 : (int)n;
 }
 

@@ -10,7 +10,7 @@ namespace {
 // A = N diag(beta), goes by halves: its two diagonal 16x16 blocks by forward substitution,
 // a column per lane, then M10 = -M11 A10 M00. M and P are left as the planes in which the
 // scans multiply them. Bound by the latency of its steps, hidden by the blocks of a CU:
-// 49.5 us for 8 x 2048 tokens, 16 heads of 128 in bf16 (4.8 TB/s of what its blocks read
+// 50 us for 8 x 2048 tokens, 16 heads of 128 in bf16 (4.7 TB/s of what its blocks read
 // and write).
 template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void k_delta_prep(DeltaP a) {
 // fetched into registers while this one is worked on, and put into the other half of LDS:
 // one barrier per chunk, no wait for memory in between. Bound by the chain of a chunk's
 // products (each waits for the one before), of which a SIMD has one to three waves to
-// overlap: 8 x 2048 tokens, 16 heads of 128 in bf16 take 173 us, 270 with the states and
+// overlap: 8 x 2048 tokens, 16 heads of 128 in bf16 take 217 us, 286 with the states and
 // errors kept for the backward. PASS 0 scans whole sequences or, from
 // the states that the join left, the parts of sequences; PASS 1 makes the parts' maps:
 // columns from VP on are those of A, and there is no output.

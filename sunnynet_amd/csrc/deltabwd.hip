@@ -235,7 +235,8 @@ __device__ __forceinline__ float sum_groups(float x) {
 // products with S and dS; Y and F are made by tiles of 16x16, a wave taking every
 // (KP / 16)-th. What the next step reads is fetched into registers a step ahead. Bound by
 // the bytes of S and dS, and by the latency of its steps (one block of eight waves on a CU
-// waits in 60 % of its cycles): 510 us for 8 x 2048 tokens, 16 heads of 128 in bf16.
+// waits in 60 % of its cycles; in 16 bits with K > 64 it has all 256 registers and spills 7):
+// 510 us for 8 x 2048 tokens, 16 heads of 128 in bf16.
 template <typename T, int KP, bool VEC>
 __global__ __launch_bounds__(4 * KP, 2) void k_delta_local(DeltaP a, SnHipDeltaGrad gr, bool vec_o) {
     constexpr int NS = sizeof(T) == 4 || KP == 64 ? 1 : 2, C = kDC * NS, NM = 2 * NS;      // NM tiles of 16 tokens

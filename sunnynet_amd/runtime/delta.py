@@ -214,7 +214,10 @@ def _bwd(q, k, v, g, beta, s0, cu_seqlens, dims, scale, saved, dout, dsend, need
 
 class GatedDelta(torch.autograd.Function):
     """The gated delta rule under autograd: (out, send) of delta_fwd, gradients of
-    delta_bwd. Keeps the chunks' states, K V fp32 values per 32 tokens and head."""
+    delta_bwd. Keeps the forward's two workspaces, in fp32 per head: a state (K to 64 or
+    128, V to a multiple of 16) for every 32 tokens (64 in 16 bits with K > 64), V errors
+    a token and 99 floats a token of chunk matrices; a long sequence of few heads also its
+    parts' maps (snhip_op_delta_chunk_floats and snhip_op_delta_state_floats say how many)."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, s0, scale, cu_seqlens):

@@ -34,7 +34,7 @@ def _check(x, w, b):
 
 def norm_fwd(x, weight=None, bias=None, eps=1e-5, *, keep=False):
     """x (..., D) -> (y, mean, rstd): y of x's type; the row statistics in float32
-    with ``keep``, else None. weight, bias: (D) float32 or None."""
+    with ``keep``, else None. weight, bias: (D) float32 or None. Without autograd."""
     R, D = _check(x, weight, bias)
     y = torch.empty_like(x)
     mean, rstd = (torch.empty(R, dtype=torch.float32, device=x.device) for _ in range(2)) if keep else (None, None)
