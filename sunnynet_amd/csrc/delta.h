@@ -191,10 +191,11 @@ template <typename T, int KP, int NTH, bool VEC, int R = kDC> struct RowsFetch {
     }
 };
 
-// The first Q planes of a (32, 32) matrix of a chunk's record (at float `at`), likewise.
+// The three planes of a (32, 32) matrix of a chunk's record (at float `at`), likewise.
 // The matrix's place is part of the vector offset, which the hardware checks against the
 // record; threads past the planes fetch nothing.
-template <int Q, int NTH> struct MatFetch {
+template <int NTH> struct MatFetch {
+    static constexpr int Q = 3;
     static constexpr int N = (Q * 128 + NTH - 1) / NTH;
     static constexpr bool whole = Q * 128 % NTH == 0;
     bf16x8 x[N];

@@ -160,7 +160,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_scan(DeltaP a, T* out, f
             else S[kt][r] = PASS == 0 && v < a.VP ? part[(int64_t)KP * (a.VP + KP) + k * a.VP + v] : 0.f;
         }
     RowsFetch<T, KP, NTH, VEC> fk, fq;
-    MatFetch<3, NTH> fm, fp;
+    MatFetch<NTH> fm, fp;
     float fv[(3 * kDC + NTH - 1) / NTH];
     unsigned vv[8];
     fk.init(d.k_stride[1], Kd, tid);

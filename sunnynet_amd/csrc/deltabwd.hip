@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * kDeltaW) void k_delta_rscan(DeltaP a, SnHipDel
             S[kt][r] = gr.dsend && k < Kd && v < V ? gr.dsend[sbase + (int64_t)k * V + v] : 0.f;
         }
     RowsFetch<T, KP, NTH, VEC> fk, fq;
-    MatFetch<3, NTH> fm, fp;
+    MatFetch<NTH> fm, fp;
     float fv[(3 * kDC + NTH - 1) / NTH];
     unsigned vv[8];
     f32x4 ev[2];
