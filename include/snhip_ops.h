@@ -102,6 +102,63 @@ typedef struct SnHipDeltaGrad {
 int64_t snhip_op_delta_bwd_floats(const SnHipDelta* d);
 snhip_status snhip_op_delta_bwd_dev(const SnHipDelta* d, const SnHipDeltaGrad* gr, void* stream);
 
+/* ------------------------------------------------------ linear attention
+ * With a decay for each head. Per sequence and value head h, with a = exp(g):
+ *   S_t = a_t S_{t-1} + k_t v_t^T          (K, V)
+ *   out_t = scale S_t^T q_t
+ * Layouts, types, sequences, non-finite values and ranges as for the gated delta rule, but:
+ * g is (B,T,H), or with head_g (H): one decay for all tokens of a head; H K and H V are
+ * below 2^23; chunks are of up to 64 tokens and their number is not bounded; no call has
+ * to have a workspace unless snhip_op_linear_parts_floats says so. */
+typedef struct SnHipLinear {
+    const void* q;
+    const void* k;
+    const void* v;
+    const float* g;
+    const float* s0;            /* NULL: zeros                                    */
+    const int32_t* cu;          /* NULL: B sequences of T tokens                  */
+    int64_t q_stride[3];        /* batch, token, head                             */
+    int64_t k_stride[3];
+    int64_t v_stride[3];
+    int64_t B, T, N, Hk, H, K, V;
+    int64_t dtype;              /* SNHIP_F32 / BF16 / F16                         */
+    int64_t head_g;             /* 1: g (and dg) is (H)                           */
+    double scale;
+    float* parts;               /* workspace of snhip_op_linear_parts_floats
+                                   floats, 16-byte aligned: the states in the
+                                   middle of long sequences, which the backward
+                                   call reads                                     */
+} SnHipLinear;
+
+/* Floats of the workspace of a call (d's arrays are not read, but whether cu is NULL is);
+ * 0: none is needed, or the sizes are outside the ranges. */
+int64_t snhip_op_linear_parts_floats(const SnHipLinear* d);
+/* out and send (NULL: not wanted). T >= 1, N >= 1. */
+snhip_status snhip_op_linear_fwd_dev(const SnHipLinear* d, void* out, float* send, void* stream);
+/* The same token by token, without cu and without a workspace: for one or a few tokens.
+ * send must be given; it may be s0 (updated in place), but not overlap it otherwise. */
+snhip_status snhip_op_linear_step_dev(const SnHipLinear* d, void* out, float* send, void* stream);
+
+/* Gradients: d as in the forward call, with the parts that it wrote. dout (B,T,H,V)
+ * contiguous, of the inputs' type; dsend (N,H,K,V) or NULL (zeros), and with it send, the
+ * forward's. dq, dk (B,T,Hk,K), dv (B,T,H,V) contiguous, of the inputs' type, dq and dk
+ * summed over the value heads that share them; dg fp32 as g; ds0 (N,H,K,V) fp32 or NULL.
+ * ws: snhip_op_linear_bwd_floats floats (0 outside the ranges), 16-byte aligned. Sums run
+ * in a fixed order. */
+typedef struct SnHipLinearGrad {
+    const void* dout;
+    const float* dsend;
+    const float* send;
+    void* dq;
+    void* dk;
+    void* dv;
+    float* dg;
+    float* ds0;
+    float* ws;
+} SnHipLinearGrad;
+int64_t snhip_op_linear_bwd_floats(const SnHipLinear* d);
+snhip_status snhip_op_linear_bwd_dev(const SnHipLinear* d, const SnHipLinearGrad* gr, void* stream);
+
 /* ------------------------------------------------------------ layer norm
  * y = (x - mean) rstd w + b per row of D values, rstd = 1 / sqrt(var + eps), var
  * over D. x, y (R, D) contiguous of one element type; w, b (D) fp32 or NULL (ones,

@@ -133,6 +133,11 @@ _SIGS = {
     "snhip_op_norm_bwd_dev": (I32, [V, V, V, V, V, V, V, V, V, ctypes.c_int64, ctypes.c_int64, I32, V]),
     "snhip_op_sample_dev": (I32, [CP, V, V]),
     "snhip_op_sample_drew_dev": (I32, [CP, V, V, V]),
+    "snhip_op_linear_parts_floats": (ctypes.c_int64, [CP]),
+    "snhip_op_linear_fwd_dev": (I32, [CP, V, V, V]),
+    "snhip_op_linear_step_dev": (I32, [CP, V, V, V]),
+    "snhip_op_linear_bwd_floats": (ctypes.c_int64, [CP]),
+    "snhip_op_linear_bwd_dev": (I32, [CP, CP, V]),
     "snhip_refmath_host": (I32, [V, V, V, I32]),
     "snhip_refmath_dev": (I32, [V, V, V, I32, V]),
 }
