@@ -174,6 +174,42 @@ snhip_status snhip_op_norm_bwd_dev(const void* dy, const void* x, const float* w
                                    const float* rstd, void* dx, float* dw, float* db, float* ws, int64_t R,
                                    int64_t D, int32_t dtype, void* stream);
 
+/* ------------------------------------------------------------- embedding
+ * y_i = scale table[id_i]: table (R, D) and y (n, D) contiguous of one element type, ids
+ * int32 or (wide) int64. An id outside [0, R) gives a row of zeros. 1 <= n < 2^31,
+ * 1 <= R <= 2^28, 1 <= D <= 2^20. */
+snhip_status snhip_op_embed_fwd_dev(const void* table, const void* ids, int32_t wide, void* y, int64_t n,
+                                    int64_t R, int64_t D, float scale, int32_t dtype, void* stream);
+/* dtable (R, D), all of it written: scale times the sum of dy's rows of each id, in fp32
+ * in the batch's order (in groups of a fixed division: the same call gives the same
+ * bits), rounded once; rows that no id names are 0. Ids outside [0, R) are left out. ws:
+ * snhip_op_embed_bwd_bytes bytes (0 outside the ranges), 16-byte aligned. */
+int64_t snhip_op_embed_bwd_bytes(int64_t n, int64_t R, int64_t D, int32_t dtype);
+snhip_status snhip_op_embed_bwd_dev(const void* dy, const void* ids, int32_t wide, void* dtable, void* ws,
+                                    int64_t n, int64_t R, int64_t D, float scale, int32_t dtype, void* stream);
+
+/* -------------------------------------------------------------- clipping
+ * The common norm of `count` tensors, norm = sqrt(sum of all x^2), and
+ * y = x min(1, max_norm / (norm + 1e-6)) for each: elements contiguous, each tensor of
+ * its own type. x, y, n, dtype: HOST arrays of `count`, read before the call returns;
+ * y[i] is x[i] or lies apart from every x and other y (overlaps are refused; y NULL: the
+ * norm alone). Squares are summed in 64 bits in a fixed order, the factor is fp32 and a
+ * product is rounded once. Where the factor is 1, tensors in place are not touched. A norm
+ * that is infinite makes finite values 0 and others NaN, one that is NaN makes all NaN.
+ * norm: one fp32 on the device. ws: snhip_op_clip_doubles doubles, on the device.
+ * 0 <= n[i] < 2^36, count < 2^20. */
+typedef struct SnHipClip {
+    const void* const* x;
+    void* const* y;             /* NULL: the norm alone                           */
+    const int64_t* n;           /* elements                                       */
+    const int32_t* dtype;       /* SNHIP_F32 / BF16 / F16                         */
+    int64_t count;
+    double max_norm;
+    double* ws;
+} SnHipClip;
+int64_t snhip_op_clip_doubles(int64_t count);
+snhip_status snhip_op_clip_dev(const SnHipClip* c, float* norm, void* stream);
+
 /* -------------------------------------------------------------- sampling
  * The next token of every row of logits (B, V), rows `stride` elements apart, from
  * one random number u in [0, 1) per row. Row settings come from the arrays (B), or,

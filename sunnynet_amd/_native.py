@@ -138,6 +138,13 @@ _SIGS = {
     "snhip_op_linear_step_dev": (I32, [CP, V, V, V]),
     "snhip_op_linear_bwd_floats": (ctypes.c_int64, [CP]),
     "snhip_op_linear_bwd_dev": (I32, [CP, CP, V]),
+    "snhip_op_embed_fwd_dev": (I32, [V, V, I32, V, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
+                                     I32, V]),
+    "snhip_op_embed_bwd_bytes": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, I32]),
+    "snhip_op_embed_bwd_dev": (I32, [V, V, I32, V, V, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_float,
+                                     I32, V]),
+    "snhip_op_clip_doubles": (ctypes.c_int64, [ctypes.c_int64]),
+    "snhip_op_clip_dev": (I32, [CP, V, V]),
     "snhip_refmath_host": (I32, [V, V, V, I32]),
     "snhip_refmath_dev": (I32, [V, V, V, I32, V]),
 }

@@ -14,15 +14,18 @@ from __future__ import annotations
 import torch
 
 from .. import _native
+from .clip import clip_grad_norm, grad_norm
 from .delta import GatedDelta, delta_bwd, delta_fwd, delta_step, gated_delta
+from .embed import Embed, embed, embed_bwd, embed_fwd
 from .linear import LinearAttention, linear_attention, linear_bwd, linear_fwd, linear_step
 from .norm import LayerNorm, layer_norm, norm_bwd, norm_fwd
 from .sample import sample_tokens
 
-__all__ = ["FMA", "GATED", "CoreFused", "GatedDelta", "GatedScan", "LayerNorm", "LinearAttention", "core_bwd",
-           "core_forward", "core_fwd", "delta_bwd", "delta_fwd", "delta_step", "gated_delta", "gated_scan",
-           "layer_norm", "linear_attention", "linear_bwd", "linear_fwd", "linear_step", "load_runtime",
-           "norm_bwd", "norm_fwd", "runtime_available", "sample_tokens", "scan", "scan_bwd", "step"]
+__all__ = ["CoreFused", "Embed", "FMA", "GATED", "GatedDelta", "GatedScan", "LayerNorm", "LinearAttention",
+           "clip_grad_norm", "core_bwd", "core_forward", "core_fwd", "delta_bwd", "delta_fwd", "delta_step",
+           "embed", "embed_bwd", "embed_fwd", "gated_delta", "gated_scan", "grad_norm", "layer_norm",
+           "linear_attention", "linear_bwd", "linear_fwd", "linear_step", "load_runtime", "norm_bwd",
+           "norm_fwd", "runtime_available", "sample_tokens", "scan", "scan_bwd", "step"]
 
 FMA = 0
 GATED = 1

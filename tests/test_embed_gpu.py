@@ -1,0 +1,106 @@
+"""The embedding lookup and the table's gradient (runtime.embed) against 64 bits.
+
+Tolerances: a lookup is one fp32 product and one rounding to T, 2^-24 + finfo(T).eps / 2 of
+the value, fixed before the first run; and the factor is an fp32 number, rounded from the
+caller's: with |scale' - scale| <= 2^-24 |scale| the product is scale x (1 + a)(1 + b), |a|,
+|b| <= 2^-24, so off by at most 2 2^-24 + 2^-48 (1.7, the tests' factor, is no fp32 number),
+and with the rounding to T less than 2 2^-24 + finfo(T).eps / 2 + 2^-32. Below T's smallest
+normal number its numbers are a fixed distance apart, smallest_normal finfo(T).eps (2^-24 in
+fp16, where sums that cancel reach it), and a rounding is off by half of that. A row of the gradient is a sum of m fp32 terms, each
+addition off by 2^-24 of what is summed so far: m 2^-24 of the sum of the terms' sizes, then
+the same two roundings.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from sunnynet_amd import runtime
+
+pytestmark = pytest.mark.gpu
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def text(n, R, seed, spread=3.0):
+    """Ids of which few are frequent; spread 0: all of them id 0."""
+    u = torch.rand(n, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)
+    return ((R * u ** spread).long().clamp(0, R - 1) if spread else torch.zeros(n, dtype=torch.int64))
+
+
+def check(table, ids, scale, dy, dtype):
+    leaf = table.clone().requires_grad_()
+    y = runtime.embed(leaf, ids, scale)
+    (grad,) = torch.autograd.grad(y, leaf, dy)
+    t, i, g = table.double().cpu(), ids.cpu().flatten().long(), dy.double().cpu().flatten(0, -2)
+    R, D = t.shape
+    live = (i >= 0) & (i < R)
+    want = torch.zeros(i.numel(), D, dtype=torch.float64)
+    want[live] = scale * t[i[live]]
+    half = torch.finfo(dtype).eps / 2 * (dtype != F32) + (2 + 2.0 ** -8) * 2.0 ** -24
+    least = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    got = y.detach().double().cpu().flatten(0, -2)
+    assert y.shape == (*ids.shape, D) and y.dtype == dtype
+    assert ((got - want).abs() <= half * want.abs() + least).all()
+    total, size = (torch.zeros(R, D, dtype=torch.float64) for _ in range(2))
+    total.index_add_(0, i[live], g[live])
+    size.index_add_(0, i[live], g[live].abs())
+    m = torch.bincount(i[live], minlength=R)[:, None]
+    room = half * (scale * total).abs() + abs(scale) * m * 2.0 ** -24 * size * (1 + half) + least
+    assert grad.shape == (R, D) and grad.dtype == dtype
+    assert ((grad.double().cpu() - scale * total).abs() <= room).all()
+    assert not grad.cpu()[m[:, 0] == 0].any()
+    (again,) = torch.autograd.grad(runtime.embed(leaf, ids, scale), leaf, dy)
+    assert torch.equal(again, grad)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("n, R, D, spread", [
+    (1, 1, 1, 1), (1, 5000, 64, 1), (7, 3, 5, 1), (64, 65536, 768, 1), (333, 12000, 200, 3), (2048, 100, 39, 2),
+    (2049, 1023, 40, 3), (5000, 1024, 1000, 3), (9001, 70000, 24, 4), (4096, 1 << 20, 8, 1), (3000, 50, 1600, 0),
+    (20000, 7, 17, 2), (40000, 300, 64, 5),
+])
+def test_against_64_bits(gpu, n, R, D, spread, dtype):
+    g = torch.Generator().manual_seed(n)
+    table = torch.randn(R, D, generator=g).to(dtype).cuda()
+    dy = torch.randn(n, D, generator=g).to(dtype).cuda()
+    check(table, text(n, R, n, spread).cuda(), 1.7, dy, dtype)
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32], ids=["int64", "int32"])
+def test_ids_of_no_row(gpu, kind):
+    """Padding and ids past the table: zeros and no gradient; (B, T) ids."""
+    ids = text(600, 90, 1, 1).view(20, 30).to(kind)
+    ids[:, 25:] = -1
+    ids[3, 4], ids[5, 6] = 90, torch.iinfo(kind).max
+    ids[7, 8] = torch.iinfo(kind).min
+    table, dy = torch.randn(90, 56).cuda(), torch.randn(20, 30, 56).cuda()
+    check(table, ids.cuda(), 1.0, dy, F32)
+    check(table, torch.full((50,), -1, dtype=kind).cuda(), 1.0, dy.flatten(0, 1)[:50].contiguous(), F32)
+
+
+def test_views_and_nothing(gpu):
+    """Tables and gradients that begin off 16 bytes, non-contiguous ones, no ids at all."""
+    flat = torch.randn(40 * 24 + 3).cuda()
+    ids = text(100, 40, 2).cuda()
+    check(flat[3:].view(40, 24), ids, 2.0, torch.randn(100, 24).cuda(), F32)
+    check(flat[:960].view(24, 40).t(), ids, 2.0, torch.randn(24, 100).cuda().t(), F32)
+    leaf = flat[:960].view(40, 24).clone().requires_grad_()
+    y = runtime.embed(leaf, ids[:0])
+    assert y.shape == (0, 24)
+    (grad,) = torch.autograd.grad(y, leaf, torch.empty(0, 24).cuda())
+    assert grad.shape == leaf.shape and not grad.any()
+
+
+def test_values_that_are_not_finite(gpu):
+    """They stay with their id."""
+    table, ids = torch.ones(6, 32).cuda(), torch.tensor([0, 1, 1, 4, 4, 5] * 20).cuda()
+    dy = torch.ones(120, 32).cuda()
+    dy[4, 3], dy[8, 0] = float("nan"), float("inf")
+    grad = runtime.embed_bwd(dy, ids, 6)
+    want = torch.zeros(6, 32)
+    want[[0, 5]], want[[1, 4]] = 20.0, 40.0
+    want[4, 3], want[1, 0] = float("nan"), float("inf")
+    assert torch.allclose(grad.cpu(), want, rtol=0, atol=0, equal_nan=True)
+    table[2, 2] = float("nan")
+    assert not runtime.embed(table, ids).isnan().any()
+    assert runtime.embed(table, torch.tensor([2]).cuda()).isnan().sum() == 1
