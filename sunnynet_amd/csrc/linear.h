@@ -118,7 +118,7 @@ struct LinPass {
     LinRows A, B, C, X;     // X: with which y is multiplied for the decay's gradient
     int rows, cols;         // A's and C's columns
     bool turned;
-    bool vec;               // every eight elements of a row of A, B and C are 16-byte aligned
+    bool vec;               // every eight elements of a row of A, B, C and X are 16-byte aligned (X's too)
     const float* begin;     // (N,H,K,V) the state at the sequence's (backward: last) first token, or null
     float* end;             // (N,H,K,V) the state after all tokens, or null
     float* parts;           // (slots,H,K,V): of every part the state it begins with (STATE: writes its own sum)
@@ -126,7 +126,8 @@ struct LinPass {
     void* y;                // T (B,T,H / y_rep,cols), or fp32 per slice (y_f32)
     int y_rep;
     bool y_f32;
-    float* dot;             // (4 blocks of rows, B T, H): a wave's part of X_i.y_i without the token's own share
+    bool y_vec;             // every four elements of a row of y are aligned
+    float* dot;             // (4 blocks of rows, H, B T): a wave's part of X_i.y_i without the token's own share
 };
 
 

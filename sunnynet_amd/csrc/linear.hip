@@ -138,8 +138,10 @@ __global__ __launch_bounds__(256) void k_lin_dg(LinShape d, const float* dots, i
         double e = 0.;
         const int64_t row = (s.row + t) * d.H + h;
         if (t >= begin)
-            for (int w = 0; w < waves; w++)
-                e += (double)dots[w * all * d.H + row] - (double)dots[(waves + w) * all * d.H + row];
+            for (int w = 0; w < waves; w++) {
+                const float* x = dots + (w * d.H + h) * all + s.row + t;
+                e += (double)x[0] - (double)x[waves * d.H * all];
+            }
         for (int o = 1; o < 64; o <<= 1) {
             const double z = __shfl_up(e, o);
             if (lane >= o) e += z;
@@ -224,6 +226,11 @@ int64_t lin_slices(const SnHipLinear& d) { return d.H / d.Hk * lin_row_blocks(d)
 bool aligned8(const void* p, const int64_t* st, int64_t cols, int64_t dtype) {
     const int64_t step = dtype == SNHIP_F32 ? 4 : 8;      // elements of 16 bytes
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && st[0] % step == 0 && st[1] % step == 0 && st[2] % step == 0 && cols % 8 == 0;
+}
+
+// Whether every four elements of rows of `cols` are aligned.
+bool lin_four(const void* p, int64_t cols, int64_t dtype) {
+    return cols % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (dtype == SNHIP_F32 ? 16 : 8) == 0;
 }
 
 LinRows rows_of(const void* p, const int64_t* st, int64_t rep) { return {p, {st[0], st[1], st[2]}, (int)rep}; }
@@ -330,6 +337,7 @@ snhip_status snhip_op_linear_fwd_dev(const SnHipLinear* d, void* out, float* sen
     a.decay = d->parts + s.slots * s.H * s.K * s.V;
     a.y = out;
     a.y_rep = 1;
+    a.y_vec = lin_four(out, d->V, d->dtype);
     if (s.split) {
         snhip_status rc = lin_run_any(*d, s, a, false, 2, st);
         if (rc == SNHIP_OK) rc = lin_join(s, false, d->parts, d->s0, st);
@@ -365,6 +373,7 @@ snhip_status snhip_op_linear_bwd_dev(const SnHipLinear* d, const SnHipLinearGrad
     a.parts = parts;
     a.decay = parts + s.slots * s.H * s.K * s.V;
     a.y = gr->dv;
+    a.y_vec = lin_four(gr->dv, d->V, d->dtype);
     snhip_status rc = SNHIP_OK;
     if (s.split) {
         rc = lin_run_any(*d, s, a, true, 2, st);
@@ -383,6 +392,7 @@ snhip_status snhip_op_linear_bwd_dev(const SnHipLinear* d, const SnHipLinearGrad
         b.y_rep = (int)rep;
         b.y_f32 = slices > 1;
         b.y = slices > 1 ? slice : y;
+        b.y_vec = lin_four(b.y, d->K, slices > 1 ? SNHIP_F32 : d->dtype);
         b.dot = dot;
         snhip_status r = lin_run_any(*d, s, b, rev, 1, st);
         if (r != SNHIP_OK || slices == 1) return r;

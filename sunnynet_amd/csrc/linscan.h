@@ -48,6 +48,8 @@ template <typename T, int R, int W> struct LinFetch {
     }
 };
 
+__device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
+
 // Values of a fragment, its planes added from the smallest.
 template <int P> __device__ __forceinline__ void join8(const Frag<P>& f, float* x) {
 #pragma unroll
@@ -55,6 +57,61 @@ template <int P> __device__ __forceinline__ void join8(const Frag<P>& f, float* 
         x[i] = (float)f.p[P - 1][i];
 #pragma unroll
         for (int p = P - 2; p >= 0; p--) x[i] += (float)f.p[p][i];
+    }
+}
+
+template <int P> __device__ __forceinline__ void join4(const Frag<P>& f, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[i] = (float)f.p[P - 1][i];
+#pragma unroll
+        for (int p = P - 2; p >= 0; p--) x[i] += (float)f.p[p][i];
+    }
+}
+
+// acc[m][n] += a[n] b[m] (mma): N M products next to each other, none of which waits for another.
+template <int LIM, int N, int M, int NA, int NB>
+__device__ __forceinline__ void mma_nm(const Frag<NA> (&a)[N], const Frag<NB> (&b)[M], f32x4 (&acc)[M][N]) {
+#pragma unroll
+    for (int s = LIM - 1; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < NA; i++) {
+            const int j = s - i;
+            if (j >= 0 && j < NB)
+#pragma unroll
+                for (int m = 0; m < M; m++)
+#pragma unroll
+                    for (int n = 0; n < N; n++)
+                        acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n].p[i], b[m].p[j], acc[m][n], 0, 0, 0);
+        }
+}
+
+// Four neighbouring elements from `off`, of which the first n exist. vec: aligned, all exist.
+template <typename T> __device__ __forceinline__ void buf_load4e(__amdgpu_buffer_rsrc_t r, int off, int n, bool vec, float* x) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4 v = buf_load4(r, off);
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = v[i];
+        } else {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            const T4 v = __builtin_bit_cast(T4, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+#pragma unroll
+            for (int i = 0; i < 4; i++) x[i] = (float)v[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = (float)buf_load<T>(r, i < n ? off + i * (int)sizeof(T) : kNowhere);
+    }
+}
+template <typename T> __device__ __forceinline__ void buf_store4e(__amdgpu_buffer_rsrc_t r, int off, int n, bool vec, f32x4 x) {
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (vec) {
+        if constexpr (sizeof(T) == 4) buf_store4(r, off, x);
+        else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, __builtin_convertvector(x, T4)), r, off, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) buf_store<T>(r, i < n ? off + i * (int)sizeof(T) : kNowhere, (T)x[i]);
     }
 }
 
@@ -66,7 +123,7 @@ __device__ __forceinline__ int lin_tile_row(int i) { return i < 1 ? 0 : i < 3 ? 
 // tiles are fetched into registers while this one is worked on.
 template <typename T, int DP, int NC, bool REV, bool DOT, bool STATE>
 __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinShape d, LinPass a) {
-    constexpr int P = ElemPlanes<T>::n, C = LinChunk<T>::n, NB = C / 32, NK = DP / 16, W = 64 * NC, E = (int)sizeof(T);
+    constexpr int P = ElemPlanes<T>::n, C = LinChunk<T>::n, NB = C / 32, NT = C / 16, NK = DP / 16, W = 64 * NC, E = (int)sizeof(T);
     typedef Tile<P, C, DP> Rows;
     typedef Tile<P, C, W> Cols;
     typedef Tile<3, C, C> Mat;
@@ -118,7 +175,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
     const T* ap = STATE ? nullptr : lin_at<T>(a.A, q.b, q.t0, h) + r0;
     const T* bp = lin_at<T>(a.B, q.b, q.t0, h) + r0;
     const T* cp = lin_at<T>(a.C, q.b, q.t0, h) + col_block * W;
-    const T* xp = DOT ? lin_at<T>(a.X, q.b, q.t0, h) : nullptr;
+    const T* xp = DOT ? lin_at<T>(a.X, q.b, q.t0, h) + col_block * W : nullptr;
     auto fetch = [&](int t0) {
         const int n = q.len - t0 < C ? q.len - t0 : C;
         if (!STATE) fa.load(ap + t0 * a.A.st[1], a.A.st[1], n, rows, a.vec, tid);
@@ -131,7 +188,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         fb.store(Bt, tid);
         fc.store(Ct, tid);
         if (wave == 0) {
-            double c = (double)lin_decay(fg);
+            double c = (double)lin_decay(fg) * 1.4426950408889634074;         // powers of two from here on
 #pragma unroll
             for (int o = 1; o < C; o <<= 1) {
                 const double y = __shfl_up(c, o);
@@ -140,7 +197,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
             const double end = __shfl(c, C - 1);
             if (lane < C) {
                 s.c[lane] = c;
-                const float in = expf((float)c), out = expf((float)(end - c));
+                const float in = exp2_of(c), out = exp2_of(end - c);
                 s.row[lane] = REV ? out : d.scale * in;
                 s.upd[lane] = REV ? d.scale * in : out;
             }
@@ -168,13 +225,11 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         l16 = lane & 15;
         g8 = (lane >> 4) * 8;
         const double c_end = s.c[C - 1];
-        const float decay = expf((float)c_end);
+        const float decay = exp2_of(c_end);
         total += c_end;
-        f32x4 y[NC][NB][2];
+        f32x4 y[NT][NC];       // y[t][c][r] is token 16 t + l16 of column 16 c + 4 (lane / 16) + r
         if constexpr (!STATE) {
             // P, made transposed: a lane has four neighbouring columns of one row
-            constexpr int NT = C / 16;
-#pragma unroll
             for (int t = wave; t < NT * (NT + 1) / 2; t += 4) {
                 const int hi = lin_tile_row(t), lo = t - hi * (hi + 1) / 2, ti = REV ? lo : hi, tj = REV ? hi : lo;
                 f32x4 acc = {0, 0, 0, 0};
@@ -188,7 +243,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                 for (int r = 0; r < 4; r++) {
                     const int j = j0 + r;
                     const double gap = REV ? s.c[j] - ci_ : ci_ - s.c[j];
-                    x[r] = (REV ? j >= i : j <= i) ? d.scale * expf((float)gap) * acc[r] : 0.f;
+                    x[r] = (REV ? j >= i : j <= i) ? d.scale * exp2_of(gap) * acc[r] : 0.f;
                     if (DOT && j == i) {
                         sdiag[i] = x[r];
                         x[r] = 0.f;
@@ -206,14 +261,15 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                 }
             }
 #pragma unroll
-            for (int c = 0; c < NC; c++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int m = 0; m < 2; m++) y[c][b][m] = {0, 0, 0, 0};
+                for (int c = 0; c < NC; c++) y[t][c] = {0, 0, 0, 0};
 #pragma unroll
             for (int p = 0; p < DP / 32; p++) {
                 Frag<3> f[NC];
+                Frag<P> af[NT];
+#pragma unroll
+                for (int t = 0; t < NT; t++) af[t] = A.frag(16 * t + l16, 32 * p, lane);
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
                     float x[8];
@@ -221,22 +277,14 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                     for (int r = 0; r < 4; r++) x[r] = S[c][2 * p][r], x[4 + r] = S[c][2 * p + 1][r];
                     f[c] = split8<3>(x);
                 }
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const Frag<P> af[2] = {A.frag(32 * b + pair_row(0, l16), 32 * p, lane),
-                                           A.frag(32 * b + pair_row(1, l16), 32 * p, lane)};
-#pragma unroll
-                    for (int c = 0; c < NC; c++) mma_n<3>(af, f[c], y[c][b]);
-                }
+                mma_nm<3>(f, af, y);
             }
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int t = 0; t < NT; t++) {
+                const float f = s.row[16 * t + l16];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float f = s.row[32 * b + g8 + i];
-#pragma unroll
-                    for (int c = 0; c < NC; c++) y[c][b][i >> 2][i & 3] *= f;
-                }
+                for (int c = 0; c < NC; c++) y[t][c] *= f;
+            }
         }
 #pragma unroll
         for (int c = 0; c < NC; c++)
@@ -268,69 +316,84 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                 }
             }
         }
-        unsigned xv[DOT ? NC * NB * 8 : 1];
+        // what the dots take: X, and C of the token itself, whose share is added after them
+        const int j4 = wave * 16 * NC + (lane >> 4) * 4;       // this lane's first column in C
+        float xv[DOT ? NT : 1][NC][4];
+        Frag<P> own[DOT ? NT : 1][NC];
         if constexpr (DOT) {
-            const __amdgpu_buffer_rsrc_t r = rows_window(xp + t0 * a.X.st[1], a.X.st[1], n, a.cols);
-            const int step = (int)a.X.st[1] * E;
+            const __amdgpu_buffer_rsrc_t r = rows_window(xp + t0 * a.X.st[1], a.X.st[1], n, cols);
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int c = 0; c < NC; c++) {
-                    const int j = c0 + 16 * c + l16, off = j < a.cols ? (32 * b + g8) * step + j * E : kNowhere;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) xv[(b * NC + c) * 8 + i] = buf_load_bits<T>(r, off + i * step);
+                    const int j = j4 + 16 * c;
+                    buf_load4e<T>(r, j < cols ? ((16 * t + l16) * (int)a.X.st[1] + j) * E : kNowhere, cols - j, a.vec, xv[t][c]);
                 }
+        }
+        if constexpr (DOT) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int p = 0; p < P; p++)
+                        *reinterpret_cast<bf16x4*>(&own[t][c].p[p]) = *reinterpret_cast<const bf16x4*>(Ct.at(p, 16 * t + l16, j4 + 16 * c));
         }
         barrier_lds();
         if (more) store();                     // only P is read from here on
         if constexpr (!STATE) {
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int jb = 0; jb < NB; jb++) {
 #pragma unroll
-                for (int jb = REV ? b : 0; jb < (REV ? NB : b + 1); jb++) {
-                    const Frag<3> pf[2] = {Pm.frag(32 * b + pair_row(0, l16), 32 * jb, lane),
-                                           Pm.frag(32 * b + pair_row(1, l16), 32 * jb, lane)};
+                for (int t2 = 0; t2 < NT; t2 += 2) {
+                    if (REV ? t2 > 2 * jb : t2 < 2 * jb) continue;
+                    const Frag<3> pf[2] = {Pm.frag(16 * t2 + l16, 32 * jb, lane), Pm.frag(16 * t2 + 16 + l16, 32 * jb, lane)};
+                    f32x4 o[2][NC];
 #pragma unroll
-                    for (int c = 0; c < NC; c++) mma_n<3>(pf, cf[jb][c], y[c][b]);
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) o[m][c] = y[t2 + m][c];
+                    mma_nm<3>(cf[jb], pf, o);
+#pragma unroll
+                    for (int m = 0; m < 2; m++)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) y[t2 + m][c] = o[m][c];
                 }
+            }
             if constexpr (DOT) {
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    float own[NC][8];
+                for (int t = 0; t < NT; t++) {
+                    const float w = sdiag[16 * t + l16];
+                    float e = 0.f;
 #pragma unroll
-                    for (int c = 0; c < NC; c++) join8(cf[b][c], own[c]);
+                    for (int c = 0; c < NC; c++) {
+                        float o[4];
+                        join4(own[t][c], o);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int t = 32 * b + g8 + i;
-                        float e = 0.f;
-#pragma unroll
-                        for (int c = 0; c < NC; c++) {
-                            f32x4& o = y[c][b][i >> 2];
-                            e = fmaf(float_of_bits<T>(xv[(b * NC + c) * 8 + i]), o[i & 3], e);
-                            o[i & 3] = fmaf(sdiag[t], own[c][i], o[i & 3]);
+                        for (int r = 0; r < 4; r++) {
+                            e = fmaf(xv[t][c][r], y[t][c][r], e);
+                            y[t][c][r] = fmaf(w, o[r], y[t][c][r]);
                         }
-                        e = sum16(e);
-                        if (l16 == 0 && t < n)
-                            a.dot[((row_block * 4 + wave) * (d.B * d.T) + q.row + t0 + t) * d.H + h] = e;
                     }
+                    e += __shfl_xor(e, 16);
+                    e += __shfl_xor(e, 32);
+                    if (lane < 16 && 16 * t + lane < n)
+                        a.dot[((int64_t)(row_block * 4 + wave) * d.H + h) * (d.B * d.T) + q.row + t0 + 16 * t + lane] = e;
                 }
             }
             const int64_t HY = d.H / a.y_rep, row = q.row + t0;
             const int64_t slice = a.y_f32 ? ((int64_t)row_block * a.y_rep + h % a.y_rep) * (d.B * d.T) : 0;
-            const int64_t at = ((slice + row) * HY + h / a.y_rep) * a.cols;
-            const int64_t step = HY * a.cols;
+            const int64_t step = HY * a.cols, at = ((slice + row) * HY + h / a.y_rep) * a.cols + col_block * W;
             auto put = [&](auto zero) {
                 typedef decltype(zero) U;
-                const __amdgpu_buffer_rsrc_t ry = rows_window(static_cast<const U*>(a.y) + at, step, n, a.cols);
+                const __amdgpu_buffer_rsrc_t ry = rows_window(static_cast<const U*>(a.y) + at, step, n, cols);
 #pragma unroll
-                for (int b = 0; b < NB; b++)
+                for (int t = 0; t < NT; t++)
 #pragma unroll
                     for (int c = 0; c < NC; c++) {
-                        const int j = c0 + 16 * c + l16;
-                        const int off = j < a.cols ? ((32 * b + g8) * (int)step + j) * (int)sizeof(U) : kNowhere;
-#pragma unroll
-                        for (int i = 0; i < 8; i++)
-                            buf_store<U>(ry, off + i * (int)step * (int)sizeof(U), (U)y[c][b][i >> 2][i & 3]);
+                        const int j = j4 + 16 * c;
+                        const int off = j < cols ? ((16 * t + l16) * (int)step + j) * (int)sizeof(U) : kNowhere;
+                        buf_store4e<U>(ry, off, cols - j, a.y_vec, y[t][c]);
                     }
             };
             if (a.y_f32) put(0.f);
@@ -343,7 +406,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         each_state([&](int n, int kt, int r, int64_t at, bool in) {
             if (in) to[at] = S[n][kt][r];
         });
-        if (tid == 0 && blockIdx.z == 0) a.decay[(int64_t)blockIdx.x * d.H + h] = expf((float)total);
+        if (tid == 0 && blockIdx.z == 0) a.decay[(int64_t)blockIdx.x * d.H + h] = exp2_of(total);
     } else if (last_run && a.end) {
         float* to = a.end + (seq * d.H + h) * kv;
         each_state([&](int n, int kt, int r, int64_t at, bool in) {
