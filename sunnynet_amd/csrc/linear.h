@@ -34,6 +34,7 @@ namespace snhip {
 
 constexpr int64_t kLinTokens = (1 << 30) - 1;      // positions fit 32 bits
 constexpr int64_t kLinStride = 1 << 24;            // token strides: offsets inside a chunk fit 32 bits
+constexpr int kLinWaves = 4;                       // of a block, and so the parts of a dot
 constexpr int kLinRows = 128;                      // contracted rows of a block: all of K, or of a block of V
 constexpr int kLinStepTokens = 12;                 // the longest call that may run token by token
 
@@ -50,6 +51,7 @@ struct LinShape {
     int per_seq;            // parts of a sequence, without cu
     bool head_g;            // g is (H), not (B,T,H)
     bool split;             // more parts than one per sequence can be
+    bool narrow;            // blocks of 64 columns, not 128
     float scale;
 };
 
@@ -127,7 +129,7 @@ struct LinPass {
     int y_rep;
     bool y_f32;
     bool y_vec;             // every four elements of a row of y are aligned
-    float* dot;             // (4 blocks of rows, H, B T): a wave's part of X_i.y_i without the token's own share
+    float* dot;             // (blocks of rows, blocks of columns, waves, H, B T): a wave's part of X_i.y_i without the token's own share
 };
 
 

@@ -83,21 +83,25 @@ __global__ __launch_bounds__(64) void k_lin_step(LinShape d, LinRows q, LinRows 
     }
 }
 
-// Joins the parts of a sequence, a thread per element of the state: the parts' own sums
+// Joins the parts of a sequence, a thread per element of the state, or four of them: the parts' own sums
 // become the states that they begin with (REV: end with, from the last part back).
-template <bool REV> __global__ __launch_bounds__(256) void k_lin_join(LinShape d, float* parts, const float* decay, const float* begin) {
-    const int64_t kv = d.K * d.V, i = blockIdx.x * (int64_t)256 + threadIdx.x, h = blockIdx.y, seq = blockIdx.z;
+template <typename F, bool REV>
+__global__ __launch_bounds__(256) void k_lin_join(LinShape d, float* all, const float* decay, const float* begin) {
+    const int64_t kv = d.K * d.V / (sizeof(F) / 4), i = blockIdx.x * (int64_t)256 + threadIdx.x, h = blockIdx.y, seq = blockIdx.z;
     if (i >= kv) return;
+    F* const parts = reinterpret_cast<F*>(all);
     const LinSeq s = lin_seq(d, seq);
     const int np = (s.len + d.part - 1) / d.part;
-    float run = begin ? begin[(seq * d.H + h) * kv + i] : 0.f;
-    auto at = [&](int p) { return ((s.slot + (REV ? np - 1 - p : p)) * d.H + h) * kv + i; };
-    auto factor = [&](int p) { return decay[(s.slot + (REV ? np - 1 - p : p)) * d.H + h]; };
-    float own = np > 1 ? parts[at(0)] : 0.f;
+    F run = {};
+    if (begin) run = reinterpret_cast<const F*>(begin)[(seq * d.H + h) * kv + i];
+    auto slot = [&](int p) { return (s.slot + (REV ? np - 1 - p : p)) * d.H + h; };
+    F own = {};
+    if (np > 1) own = parts[slot(0) * kv + i];
     for (int p = 0; p + 1 < np; p++) {
-        const float next = p + 2 < np ? parts[at(p + 1)] : 0.f;
-        run = fmaf(factor(p), run, own);
-        parts[at(p + 1)] = run;
+        F next = {};
+        if (p + 2 < np) next = parts[slot(p + 1) * kv + i];
+        run = run * decay[slot(p)] + own;
+        parts[slot(p + 1) * kv + i] = run;
         own = next;
     }
 }
@@ -130,8 +134,15 @@ __global__ __launch_bounds__(256) void k_lin_dg(LinShape d, const float* dots, i
         return (sw[0] + sw[1]) + (sw[2] + sw[3]);
     };
     double carry = 0., total = 0.;
-    if (x)
-        for (int64_t i = tid; i < kv; i += 256) carry += (double)x[i] * (double)y[i];
+    if (x && kv % 4 == 0 && (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % 16 == 0) {
+#pragma unroll 4
+        for (int i = 4 * tid; i < (int)kv; i += 1024) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(x + i), b = *reinterpret_cast<const f32x4*>(y + i);
+            carry += ((double)a[0] * b[0] + (double)a[1] * b[1]) + ((double)a[2] * b[2] + (double)a[3] * b[3]);
+        }
+    } else if (x) {
+        for (int i = tid; i < (int)kv; i += 256) carry += (double)x[i] * (double)y[i];
+    }
     carry = block_sum(carry);
     for (int t0 = stop; t0 > begin; t0 -= 256) {           // thread 0 the last token
         const int t = t0 - 1 - tid;
@@ -198,11 +209,13 @@ bool lin_in_range(const SnHipLinear& d) {
            d.dtype >= SNHIP_F32 && d.dtype <= SNHIP_F16;
 }
 
-// Blocks that fill the card (256 CUs, two each), and the fewest tokens worth a part.
+// Blocks that fill the card (a CU each), and the fewest tokens worth a part.
 constexpr int64_t kLinBlocks = 512, kLinPart = 256;
 
 void lin_shape(const SnHipLinear& d, LinShape* s) {
-    const int64_t tokens = d.B * d.T, blocks = d.H * ((d.V + 127) / 128);
+    const int64_t tokens = d.B * d.T;
+    s->narrow = false;
+    const int64_t blocks = d.H * (s->narrow ? (d.V + 63) / 64 : (d.V + 127) / 128);
     int64_t part = tokens * blocks / kLinBlocks;
     part = ((part < kLinPart ? kLinPart : part) + 63) / 64 * 64;
     if (part > d.T) part = (d.T + 63) / 64 * 64;
@@ -219,8 +232,15 @@ void lin_shape(const SnHipLinear& d, LinShape* s) {
 
 int64_t parts_floats(const LinShape& s) { return s.split ? (s.slots * s.H * (s.K * s.V + 1) + 3) / 4 * 4 : 0; }
 
+// The parts' sums of the decay's gradient, in 64 bits.
+int64_t lin_sums_floats(const LinShape& s) { return (2 * s.slots * s.H + 3) / 4 * 4; }
+
 // Slices of dq and dk: value heads that share a head, blocks of 128 columns of V.
 int64_t lin_row_blocks(const SnHipLinear& d) { return (d.V + kLinRows - 1) / kLinRows; }
+// Parts of a dot of X and y: waves of all blocks of K's columns, for each block of V's rows.
+int64_t lin_dots(const SnHipLinear& d, const LinShape& s) {
+    return kLinWaves * lin_row_blocks(d) * (s.narrow ? (d.K + 63) / 64 : 1);
+}
 int64_t lin_slices(const SnHipLinear& d) { return d.H / d.Hk * lin_row_blocks(d); }
 
 bool aligned8(const void* p, const int64_t* st, int64_t cols, int64_t dtype) {
@@ -242,10 +262,13 @@ snhip_status lin_run_any(const SnHipLinear& d, const LinShape& s, const LinPass&
 }
 
 snhip_status lin_join(const LinShape& s, bool rev, float* parts, const float* begin, hipStream_t st) {
-    const dim3 grid((unsigned)((s.K * s.V + 255) / 256), (unsigned)s.H, (unsigned)s.N);
     const float* decay = parts + s.slots * s.H * s.K * s.V;
-    if (rev) k_lin_join<true><<<grid, 256, 0, st>>>(s, parts, decay, begin);
-    else k_lin_join<false><<<grid, 256, 0, st>>>(s, parts, decay, begin);
+    const bool four = s.K * s.V % 4 == 0 && reinterpret_cast<uintptr_t>(begin) % 16 == 0;
+    const dim3 grid((unsigned)((s.K * s.V / (four ? 4 : 1) + 255) / 256), (unsigned)s.H, (unsigned)s.N);
+    if (four && rev) k_lin_join<f32x4, true><<<grid, 256, 0, st>>>(s, parts, decay, begin);
+    else if (four) k_lin_join<f32x4, false><<<grid, 256, 0, st>>>(s, parts, decay, begin);
+    else if (rev) k_lin_join<float, true><<<grid, 256, 0, st>>>(s, parts, decay, begin);
+    else k_lin_join<float, false><<<grid, 256, 0, st>>>(s, parts, decay, begin);
     SNHIP_CHECK(hipGetLastError());
     return SNHIP_OK;
 }
@@ -309,7 +332,7 @@ int64_t snhip_op_linear_bwd_floats(const SnHipLinear* d) {
     LinShape s;
     lin_shape(*d, &s);
     const int64_t tokens = d->B * d->T, slices = lin_slices(*d);
-    return 2 * s.slots * s.H + parts_floats(s) + 8 * lin_row_blocks(*d) * tokens * d->H +
+    return lin_sums_floats(s) + parts_floats(s) + 2 * lin_dots(*d, s) * tokens * d->H +
            (slices > 1 ? slices * tokens * d->Hk * d->K : 0);
 }
 
@@ -352,11 +375,12 @@ snhip_status snhip_op_linear_bwd_dev(const SnHipLinear* d, const SnHipLinearGrad
         (gr->dsend && !gr->send) || (s.split && !d->parts) || reinterpret_cast<uintptr_t>(gr->ws) % 16)
         return SNHIP_E_INVAL;
     const hipStream_t st = as_stream(stream);
-    const int64_t rep = d->H / d->Hk, tokens = d->B * d->T, blocks = lin_row_blocks(*d), slices = lin_slices(*d);
+    const int64_t rep = d->H / d->Hk, tokens = d->B * d->T, slices = lin_slices(*d);
     double* const sums = reinterpret_cast<double*>(gr->ws);
-    float* const parts = gr->ws + 2 * s.slots * s.H;
+    float* const parts = gr->ws + lin_sums_floats(s);
     float* const dots = parts + parts_floats(s);
-    float* const slice = dots + 8 * blocks * tokens * d->H;
+    const int64_t waves = lin_dots(*d, s);
+    float* const slice = dots + 2 * waves * tokens * d->H;
     const int64_t dout_st[3] = {d->T * d->H * d->V, d->H * d->V, d->V};
     const LinRows q = rows_of(d->q, d->q_stride, rep), k = rows_of(d->k, d->k_stride, rep), v = rows_of(d->v, d->v_stride, 1),
                   o = rows_of(gr->dout, dout_st, 1);
@@ -402,9 +426,9 @@ snhip_status snhip_op_linear_bwd_dev(const SnHipLinear* d, const SnHipLinearGrad
                                         : add_t<_Float16>(s, slice, y, n, slices, per, st);
     };
     if (rc == SNHIP_OK) rc = turned(o, v, k, q, d->s0, d->parts, dots, gr->dq, false);
-    if (rc == SNHIP_OK) rc = turned(v, o, q, k, gr->dsend, parts, dots + 4 * blocks * tokens * d->H, gr->dk, true);
+    if (rc == SNHIP_OK) rc = turned(v, o, q, k, gr->dsend, parts, dots + waves * tokens * d->H, gr->dk, true);
     if (rc != SNHIP_OK) return rc;
-    k_lin_dg<<<dim3((unsigned)s.slots, (unsigned)s.H), 256, 0, st>>>(s, dots, (int)(4 * blocks), d->parts, parts, gr->send,
+    k_lin_dg<<<dim3((unsigned)s.slots, (unsigned)s.H), 256, 0, st>>>(s, dots, (int)waves, d->parts, parts, gr->send,
                                                                     gr->dsend, gr->dg, sums);
     SNHIP_CHECK(hipGetLastError());
     if (s.head_g) {

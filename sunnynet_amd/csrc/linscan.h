@@ -15,12 +15,55 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 
-// An (R, W) tile of a (tokens, columns) array on its way from memory to LDS, held by 256
+// A tile of P planes of R rows and C columns in LDS without padding (planes.h has one with):
+// the 16-byte units of a row are permuted by an exclusive or with bits of the row, chosen so
+// that both ways of reading spread over the banks. The 16 rows of a frag meet 16 different
+// units, and the four rows that a transposing read takes at once lie four units apart.
+template <int P, int R, int C> struct SwTile {
+    static constexpr int elems = P * R * C, U = C / 8, G = 16 / U;         // units of a row, rows of 256 bytes
+    static_assert(U == 16 || U == 8 || U == 4);
+    __bf16* s;
+    static __device__ __forceinline__ int mix(int r) {
+        const int x = r / G;
+        return U == 16 ? (x & 3) << 2 | (x >> 2 & 3) : U == 8 ? (x & 1) << 2 | (x >> 1 & 3) : x & 3;
+    }
+    __device__ __forceinline__ __bf16* at(int p, int r, int c) const {
+        return s + (p * R + r) * C + (((c >> 3) ^ mix(r)) << 3) + (c & 7);
+    }
+    // Row r0 + lane % 16 (r0 a multiple of 16), columns c0..c0 + 31 as the contraction.
+    __device__ __forceinline__ Frag<P> frag(int r0, int c0, int lane) const {
+        Frag<P> f;
+#pragma unroll
+        for (int p = 0; p < P; p++)
+            f.p[p] = *reinterpret_cast<const bf16x8*>(s + (p * R + r0) * C + (lane & 15) * C +
+                                                      (((c0 >> 3) + (lane >> 4)) ^ mix(lane & 15)) * 8);
+        return f;
+    }
+    // Rows r0..r0 + 31 as the contraction (r0 a multiple of 32); the lane fetches its row's
+    // four columns from `block` on, see planes.h.
+    __device__ __forceinline__ Frag<P> tfrag(int r0, int block, int lane) const {
+        Frag<P> f;
+        const int r = 8 * (lane >> 4) + ((lane >> 2) & 3), u = block >> 3, e = block & 7;
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            const bf16x4 lo = Tile<P, R, C>::tread(s + (p * R + r0) * C + r * C + (u ^ mix(r)) * 8 + e),
+                         hi = Tile<P, R, C>::tread(s + (p * R + r0 + 4) * C + r * C + (u ^ mix(r + 4)) * 8 + e);
+            f.p[p] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        return f;
+    }
+    __device__ __forceinline__ void put8(int r, int c, const Frag<P>& f) const {
+#pragma unroll
+        for (int p = 0; p < P; p++) *reinterpret_cast<bf16x8*>(at(p, r, c)) = f.p[p];
+    }
+};
+
+// An (R, W) tile of a (tokens, columns) array on its way from memory to LDS, held by NTH
 // threads: tokens from n on and columns from `cols` on are 0 (a stride below `cols` would let
 // the window alone hand out other rows).
-template <typename T, int R, int W> struct LinFetch {
-    static constexpr int P = ElemPlanes<T>::n, N = R * W / 8 / 256;
-    static_assert(R * W / 8 % 256 == 0);
+template <typename T, int R, int W, int NTH> struct LinFetch {
+    static constexpr int N = (R * W / 8 + NTH - 1) / NTH;
+    static constexpr bool whole = R * W / 8 % NTH == 0;
     Vec8<T> x[N];
     __device__ __forceinline__ void load(const T* src, int64_t stride, int n, int cols, bool vec, int tid) {
         const __amdgpu_buffer_rsrc_t r = rows_window(src, stride, n, cols);
@@ -28,62 +71,58 @@ template <typename T, int R, int W> struct LinFetch {
         if (vec) {
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                const int i = tid + j * 256, t = i / (W / 8), c = i % (W / 8) * 8;
-                x[j] = buf_load8<T>(r, t < n && c < cols ? (t * step + c) * (int)sizeof(T) : kNowhere, 8, true);
+                const int i = tid + j * NTH, t = i / (W / 8), c = i % (W / 8) * 8;
+                x[j] = buf_load8<T>(r, t < n && (whole || t < R) && c < cols ? (t * step + c) * (int)sizeof(T) : kNowhere, 8, true);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                const int i = here(tid) + j * 256, t = i / (W / 8), c = i % (W / 8) * 8;
-                x[j] = buf_load8<T>(r, (t * step + c) * (int)sizeof(T), t < n ? cols - c : 0, false);
+                const int i = here(tid) + j * NTH, t = i / (W / 8), c = i % (W / 8) * 8;
+                x[j] = buf_load8<T>(r, (t * step + c) * (int)sizeof(T), t < n && (whole || t < R) ? cols - c : 0, false);
             }
         }
     }
     template <typename Tl> __device__ __forceinline__ void store(Tl to, int tid) const {
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int i = tid + j * 256;
-            to.put8(i / (W / 8), i % (W / 8) * 8, split_raw8<T>(x[j]));
+            const int i = tid + j * NTH;
+            if (whole || i < R * W / 8) to.put8(i / (W / 8), i % (W / 8) * 8, split_raw8<T>(x[j]));
         }
     }
 };
 
 __device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// Values of a fragment, its planes added from the smallest.
-template <int P> __device__ __forceinline__ void join8(const Frag<P>& f, float* x) {
+// Value e of a fragment, its planes added from the smallest.
+template <int P> __device__ __forceinline__ float value_of(const Frag<P>& f, int e) {
+    float x = (float)f.p[P - 1][e];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        x[i] = (float)f.p[P - 1][i];
+    for (int p = P - 2; p >= 0; p--) x += (float)f.p[p][e];
+    return x;
+}
+// Values e and e + 1 of a fragment: eight bits a plane by truncation, which makes three planes
+// exact, and the bits of a plane one instruction's to pack (a rounding one takes longer).
+__device__ __forceinline__ void split2(float x, float y, Frag<3>& f, int e) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    unsigned u = __float_as_uint(x), v = __float_as_uint(y);
 #pragma unroll
-        for (int p = P - 2; p >= 0; p--) x[i] += (float)f.p[p][i];
+    for (int p = 0; p < 3; p++) {
+        const bf16x2 h = __builtin_bit_cast(bf16x2, __builtin_amdgcn_perm(v, u, 0x07060302));
+        f.p[p][e] = h[0];
+        f.p[p][e + 1] = h[1];
+        u = __float_as_uint(__uint_as_float(u) - __uint_as_float(u & 0xffff0000u));
+        v = __float_as_uint(__uint_as_float(v) - __uint_as_float(v & 0xffff0000u));
     }
 }
-
-template <int P> __device__ __forceinline__ void join4(const Frag<P>& f, float* x) {
+// f(plane of three, plane of the other) for the plane pairs of a product of fp32 precision
+// (planes.h), the smallest first.
+template <int PAIRS, typename F> __device__ __forceinline__ void each_product(F f) {
+    constexpr int P = PAIRS == 3 ? 1 : PAIRS == 5 ? 2 : 3;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        x[i] = (float)f.p[P - 1][i];
+    for (int s = 2; s >= 0; s--)
 #pragma unroll
-        for (int p = P - 2; p >= 0; p--) x[i] += (float)f.p[p][i];
-    }
-}
-
-// acc[m][n] += a[n] b[m] (mma): N M products next to each other, none of which waits for another.
-template <int LIM, int N, int M, int NA, int NB>
-__device__ __forceinline__ void mma_nm(const Frag<NA> (&a)[N], const Frag<NB> (&b)[M], f32x4 (&acc)[M][N]) {
-#pragma unroll
-    for (int s = LIM - 1; s >= 0; s--)
-#pragma unroll
-        for (int i = 0; i < NA; i++) {
-            const int j = s - i;
-            if (j >= 0 && j < NB)
-#pragma unroll
-                for (int m = 0; m < M; m++)
-#pragma unroll
-                    for (int n = 0; n < N; n++)
-                        acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[n].p[i], b[m].p[j], acc[m][n], 0, 0, 0);
-        }
+        for (int i = 0; i < 3; i++)
+            if (s - i >= 0 && s - i < P) f(i, s - i);
 }
 
 // Four neighbouring elements from `off`, of which the first n exist. vec: aligned, all exist.
@@ -123,10 +162,11 @@ __device__ __forceinline__ int lin_tile_row(int i) { return i < 1 ? 0 : i < 3 ? 
 // tiles are fetched into registers while this one is worked on.
 template <typename T, int DP, int NC, bool REV, bool DOT, bool STATE>
 __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinShape d, LinPass a) {
-    constexpr int P = ElemPlanes<T>::n, C = LinChunk<T>::n, NB = C / 32, NT = C / 16, NK = DP / 16, W = 64 * NC, E = (int)sizeof(T);
-    typedef Tile<P, C, DP> Rows;
-    typedef Tile<P, C, W> Cols;
-    typedef Tile<3, C, C> Mat;
+    constexpr int P = ElemPlanes<T>::n, C = LinChunk<T>::n, NB = C / 32, NT = C / 16, NK = DP / 16, NW = kLinWaves, W = 64 * NC, PAIRS = P == 1 ? 3 : P == 2 ? 5 : 6,
+                  NTH = 256, E = (int)sizeof(T);
+    typedef SwTile<P, C, DP> Rows;
+    typedef SwTile<P, C, W> Cols;
+    typedef SwTile<3, C, C> Mat;
     __shared__ alignas(16) __bf16 sa[STATE ? 8 : Rows::elems], sb[Rows::elems], sc[Cols::elems], sp[STATE ? 8 : Mat::elems];
     __shared__ struct { double c[C]; float row[C], upd[C]; } s;      // a chunk's running sums, row factors and weights
     __shared__ float sdiag[DOT ? C : 1];
@@ -150,40 +190,51 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
 
     // place of row i, column j of this block's S in a (K, V) state
     const int r0 = row_block * kLinRows, c0 = col_block * W + wave * 16 * NC;
-    const int64_t rs = a.turned ? 1 : d.V, cs = a.turned ? d.V : 1, kv = d.K * d.V;
+    f32x4 S[NC][NK];       // S[c][2 p + e][r] is row 32 p + g8 + 4 e + r of column 16 c + l16
+    const int64_t kv = d.K * d.V;
+    const int rs = (a.turned ? 1 : (int)d.V) * 4, cs = (a.turned ? (int)d.V : 1) * 4;
     auto each_state = [&](auto f) {
+        const int g = here(g8), j0 = c0 + here(l16);
 #pragma unroll
-        for (int n = 0; n < NC; n++)
+        for (int c = 0; c < NC; c++) {
+            const int j = j0 + 16 * c, at = (r0 + g) * rs + j * cs;
 #pragma unroll
             for (int kt = 0; kt < NK; kt++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int i = (kt >> 1) * 32 + g8 + 4 * (kt & 1) + r, j = c0 + 16 * n + l16;
-                    f(n, kt, r, (r0 + i) * rs + j * cs, i < rows && j < a.cols);
+                    const int i = (kt >> 1) * 32 + 4 * (kt & 1) + r;
+                    f(S[c][kt], r, g + i < rows && j < a.cols ? at + i * rs : kNowhere);
                 }
+        }
     };
-    f32x4 S[NC][NK];       // S[n][2 p + e][r] is row 32 p + g8 + 4 e + r of column 16 n + l16
+    auto state_at = [&](const float* p, int64_t n) {
+        return make_rsrc(p ? p + (n * d.H + h) * kv : nullptr, p ? (uint32_t)kv * 4u : 0u);
+    };
     {
-        const float* from = first_run ? (a.begin ? a.begin + (seq * d.H + h) * kv : nullptr)
-                                      : a.parts + ((int64_t)blockIdx.x * d.H + h) * kv;
-        if (STATE) from = nullptr;
-        each_state([&](int n, int kt, int r, int64_t at, bool in) { S[n][kt][r] = from && in ? from[at] : 0.f; });
+        const float* const from = STATE ? nullptr : first_run ? a.begin : a.parts;
+        const __amdgpu_buffer_rsrc_t st = state_at(from, first_run ? seq : (int64_t)blockIdx.x);
+        each_state([&](f32x4& x, int r, int at) { x[r] = buf_load<float>(st, at); });
     }
-    LinFetch<T, C, DP> fa, fb;
-    LinFetch<T, C, W> fc;
+    LinFetch<T, C, DP, NTH> fa, fb;
+    LinFetch<T, C, W, NTH> fc;
     float fg = 0.f;
     const T* ap = STATE ? nullptr : lin_at<T>(a.A, q.b, q.t0, h) + r0;
     const T* bp = lin_at<T>(a.B, q.b, q.t0, h) + r0;
     const T* cp = lin_at<T>(a.C, q.b, q.t0, h) + col_block * W;
     const T* xp = DOT ? lin_at<T>(a.X, q.b, q.t0, h) + col_block * W : nullptr;
+    // rows of y lie `step` elements apart, the sequence's first at y_at
+    const int step = (int)(d.H / a.y_rep) * a.cols;
+    const int64_t slice = a.y_f32 ? ((int64_t)row_block * a.y_rep + h % a.y_rep) * (d.B * d.T) : 0;
+    const int64_t y_at = (slice + q.row) * step + h / a.y_rep * a.cols + col_block * W;
     auto fetch = [&](int t0) {
-        const int n = q.len - t0 < C ? q.len - t0 : C;
+        const int n = q.len - t0 < C ? q.len - t0 : C, tid = here((int)threadIdx.x), lane = tid & 63;
         if (!STATE) fa.load(ap + t0 * a.A.st[1], a.A.st[1], n, rows, a.vec, tid);
         fb.load(bp + t0 * a.B.st[1], a.B.st[1], n, rows, a.vec, tid);
         fc.load(cp + t0 * a.C.st[1], a.C.st[1], n, cols, a.vec, tid);
         if (wave == 0) fg = lane < n ? d.g[d.head_g ? h : (q.row + t0 + lane) * d.H + h] : 0.f;
     };
     auto store = [&]() {
+        const int tid = here((int)threadIdx.x), lane = tid & 63;
         if (!STATE) fa.store(A, tid);
         fb.store(Bt, tid);
         fc.store(Ct, tid);
@@ -204,7 +255,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         }
     };
     if constexpr (!STATE) {                    // the tiles beside the diagonal that products of 32 read
-        for (int i = tid; i < 3 * C * C / 8; i += 256) {
+        for (int i = tid; i < 3 * C * C / 8; i += NTH) {
             const int p = i / (C * C / 8), k = i % (C * C / 8);
             *reinterpret_cast<bf16x8*>(Pm.at(p, k / (C / 8), k % (C / 8) * 8)) = bf16x8{};
         }
@@ -220,7 +271,6 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
     for (int ci = 0; ci < n_chunks; ci++) {
         const int t0 = chunk_at(ci), n = q.len - t0 < C ? q.len - t0 : C;
         const bool more = ci + 1 < n_chunks;
-        if (more) fetch(chunk_at(ci + 1));
         lane = here(lane);
         l16 = lane & 15;
         g8 = (lane >> 4) * 8;
@@ -228,23 +278,40 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         const float decay = exp2_of(c_end);
         total += c_end;
         f32x4 y[NT][NC];       // y[t][c][r] is token 16 t + l16 of column 16 c + 4 (lane / 16) + r
+        Frag<P> cf[NB][NC];    // C by columns, and its rows times the weights, which S takes up
+        Frag<3> u[2][NC];
+        constexpr int STEPS = 4 * NC;          // pairs of values of a step's operands
+        auto columns_of = [&](int b) {
+#pragma unroll
+            for (int c = 0; c < NC; c++) cf[b][c] = Ct.tfrag(32 * b, wave * 16 * NC + 16 * c + 4 * (lane & 3), lane);
+        };
+        auto weigh = [&](int b, int i) {       // pair i of the operand
+            const int c = i >> 2, e = 2 * (i & 3);
+            const float2 w = *reinterpret_cast<const float2*>(&s.upd[32 * b + g8 + e]);
+            split2(value_of(cf[b][c], e) * w.x, value_of(cf[b][c], e + 1) * w.y, u[b & 1][c], e);
+        };
         if constexpr (!STATE) {
-            // P, made transposed: a lane has four neighbouring columns of one row
-            for (int t = wave; t < NT * (NT + 1) / 2; t += 4) {
+            // P, made transposed: a lane has four neighbouring columns of one row. A wave makes
+            // every fourth tile; where there is none left, the last once more (the same values).
+            constexpr int TILES = NT * (NT + 1) / 2;
+#pragma unroll
+            for (int k = 0; k < TILES; k += NW) {
+                const int t = wave + k < TILES ? wave + k : TILES - 1;
                 const int hi = lin_tile_row(t), lo = t - hi * (hi + 1) / 2, ti = REV ? lo : hi, tj = REV ? hi : lo;
+                const int i = 16 * ti + l16, j0 = 16 * tj + (lane >> 4) * 4;
                 f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
-                for (int p = 0; p < DP; p += 32)
-                    acc = mma<3>(Bt.frag(16 * tj + l16, p, lane), A.frag(16 * ti + l16, p, lane), acc);
-                const int i = 16 * ti + l16, j0 = 16 * tj + (lane >> 4) * 4;
+                for (int p = 0; p < DP; p += 32) acc = mma<3>(Bt.frag(16 * tj, p, lane), A.frag(16 * ti, p, lane), acc);
                 const double ci_ = s.c[i];
+                double cj[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) cj[r] = s.c[j0 + r];
                 float x[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int j = j0 + r;
-                    const double gap = REV ? s.c[j] - ci_ : ci_ - s.c[j];
-                    x[r] = (REV ? j >= i : j <= i) ? d.scale * exp2_of(gap) * acc[r] : 0.f;
-                    if (DOT && j == i) {
+                    const float w = d.scale * exp2_of(REV ? cj[r] - ci_ : ci_ - cj[r]) * acc[r];
+                    x[r] = (REV ? j0 + r >= i : j0 + r <= i) ? w : 0.f;
+                    if (DOT && j0 + r == i) {
                         sdiag[i] = x[r];
                         x[r] = 0.f;
                     }
@@ -264,56 +331,89 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
             for (int t = 0; t < NT; t++)
 #pragma unroll
                 for (int c = 0; c < NC; c++) y[t][c] = {0, 0, 0, 0};
+            // Written in the order in which it is to run: the next step's operands are made
+            // between this step's products.
+            Frag<3> f[2][NC];
+            Frag<P> af[2][NT];
+            auto rows_of_a = [&](int p) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) af[p & 1][t] = A.frag(16 * t, 32 * p, lane);
+            };
+            auto planes_of = [&](int p, int i) {
+                const int c = i >> 2, e = 2 * (i & 3);
+                const f32x4& x = S[c][2 * p + (e >> 2)];
+                split2(x[e & 3], x[(e & 3) + 1], f[p & 1][c], e);
+            };
+            rows_of_a(0);
+#pragma unroll
+            for (int i = 0; i < STEPS; i++) planes_of(0, i);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int p = 0; p < DP / 32; p++) {
-                Frag<3> f[NC];
-                Frag<P> af[NT];
+                if (p + 1 < DP / 32) rows_of_a(p + 1);
+                else columns_of(0);
+                int m = 0;
+                each_product<PAIRS>([&](int i, int j) {
 #pragma unroll
-                for (int t = 0; t < NT; t++) af[t] = A.frag(16 * t + l16, 32 * p, lane);
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    float x[8];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) x[r] = S[c][2 * p][r], x[4 + r] = S[c][2 * p + 1][r];
-                    f[c] = split8<3>(x);
-                }
-                mma_nm<3>(f, af, y);
+                        for (int c = 0; c < NC; c++) {
+                            y[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[p & 1][c].p[i], af[p & 1][t].p[j], y[t][c], 0, 0, 0);
+                            constexpr int each = PAIRS * NT * NC / STEPS;
+                            if (m % each == each - 1) {
+                                if (p + 1 < DP / 32) planes_of(p + 1, m / each);
+                                else weigh(0, m / each);
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                            m++;
+                        }
+                });
             }
+        } else {
+            columns_of(0);
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const float f = s.row[16 * t + l16];
-#pragma unroll
-                for (int c = 0; c < NC; c++) y[t][c] *= f;
-            }
+            for (int i = 0; i < STEPS; i++) weigh(0, i);
         }
+        if (more) fetch(chunk_at(ci + 1));
+        Frag<P> bf[2][2];
+        auto columns_of_b = [&](int i) {       // step i: 32 rows of S, of 32 tokens
+            const int b = i / (NK / 2), k2 = i % (NK / 2) * 2;
 #pragma unroll
-        for (int c = 0; c < NC; c++)
-#pragma unroll
-            for (int kt = 0; kt < NK; kt++) S[c][kt] *= decay;
-        Frag<P> cf[NB][NC];
+            for (int e = 0; e < 2; e++) bf[i & 1][e] = Bt.tfrag(32 * b, 16 * k2 + 8 * (lane & 3) + 4 * e, lane);
+        };
+        columns_of_b(0);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            Frag<3> u[NC];
+            if (b + 1 < NB) columns_of(b + 1);
+            int m = 0;
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                cf[b][c] = Ct.tfrag(32 * b, wave * 16 * NC + 16 * c + 4 * (lane & 3), lane);
-                float x[8];
-                join8(cf[b][c], x);
+            for (int k = 0; k < NK / 2; k++) {
+                const int i = b * (NK / 2) + k;
+                if (i + 1 < NB * NK / 2) columns_of_b(i + 1);
+                if (b == 0)
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] *= s.upd[32 * b + g8 + i];
-                u[c] = split8<3>(x);
-            }
+                    for (int c = 0; c < NC; c++) S[c][2 * k] *= decay, S[c][2 * k + 1] *= decay;
+                each_product<PAIRS>([&](int pj, int pi) {          // u's plane pj, B's pi
 #pragma unroll
-            for (int k2 = 0; k2 < NK; k2 += 2) {
-                const Frag<P> bf[2] = {Bt.tfrag(32 * b, 16 * k2 + 8 * (lane & 3), lane),
-                                       Bt.tfrag(32 * b, 16 * k2 + 8 * (lane & 3) + 4, lane)};
+                    for (int e = 0; e < 2; e++)
 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    f32x4 t[2] = {S[c][k2], S[c][k2 + 1]};
-                    mma_n<3>(bf, u[c], t);
-                    S[c][k2] = t[0];
-                    S[c][k2 + 1] = t[1];
-                }
+                        for (int c = 0; c < NC; c++) {
+                            f32x4& x = S[c][2 * k + e];
+                            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[i & 1][e].p[pi], u[b & 1][c].p[pj], x, 0, 0, 0);
+                            constexpr int all = PAIRS * NK * NC, each = all / STEPS;
+                            if (m % each == each - 1) {
+                                if (b + 1 < NB) weigh(b + 1, m / each);
+                                else if constexpr (!STATE)
+                                    if (m / each < NT) {
+                                        const float r = s.row[16 * (m / each) + l16];
+#pragma unroll
+                                        for (int q = 0; q < NC; q++) y[m / each][q] *= r;
+                                    }
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                            m++;
+                        }
+                });
             }
         }
         // what the dots take: X, and C of the token itself, whose share is added after them
@@ -328,62 +428,47 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                 for (int c = 0; c < NC; c++) {
                     const int j = j4 + 16 * c;
                     buf_load4e<T>(r, j < cols ? ((16 * t + l16) * (int)a.X.st[1] + j) * E : kNowhere, cols - j, a.vec, xv[t][c]);
-                }
-        }
-        if constexpr (DOT) {
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int c = 0; c < NC; c++)
 #pragma unroll
                     for (int p = 0; p < P; p++)
-                        *reinterpret_cast<bf16x4*>(&own[t][c].p[p]) = *reinterpret_cast<const bf16x4*>(Ct.at(p, 16 * t + l16, j4 + 16 * c));
+                        *reinterpret_cast<bf16x4*>(&own[t][c].p[p]) = *reinterpret_cast<const bf16x4*>(Ct.at(p, 16 * t + l16, j));
+                }
         }
         barrier_lds();
         if (more) store();                     // only P is read from here on
         if constexpr (!STATE) {
 #pragma unroll
-            for (int jb = 0; jb < NB; jb++) {
+            for (int jb = 0; jb < NB; jb++)
 #pragma unroll
                 for (int t2 = 0; t2 < NT; t2 += 2) {
                     if (REV ? t2 > 2 * jb : t2 < 2 * jb) continue;
-                    const Frag<3> pf[2] = {Pm.frag(16 * t2 + l16, 32 * jb, lane), Pm.frag(16 * t2 + 16 + l16, 32 * jb, lane)};
-                    f32x4 o[2][NC];
+                    const Frag<3> pf[2] = {Pm.frag(16 * t2, 32 * jb, lane), Pm.frag(16 * t2 + 16, 32 * jb, lane)};
+                    each_product<PAIRS>([&](int pj, int pi) {      // P's plane pj, C's pi
 #pragma unroll
-                    for (int m = 0; m < 2; m++)
+                        for (int m = 0; m < 2; m++)
 #pragma unroll
-                        for (int c = 0; c < NC; c++) o[m][c] = y[t2 + m][c];
-                    mma_nm<3>(cf[jb], pf, o);
-#pragma unroll
-                    for (int m = 0; m < 2; m++)
-#pragma unroll
-                        for (int c = 0; c < NC; c++) y[t2 + m][c] = o[m][c];
+                            for (int c = 0; c < NC; c++)
+                                y[t2 + m][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(cf[jb][c].p[pi], pf[m].p[pj], y[t2 + m][c], 0, 0, 0);
+                    });
                 }
-            }
             if constexpr (DOT) {
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     const float w = sdiag[16 * t + l16];
                     float e = 0.f;
 #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-                        float o[4];
-                        join4(own[t][c], o);
+                    for (int c = 0; c < NC; c++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
                             e = fmaf(xv[t][c][r], y[t][c][r], e);
-                            y[t][c][r] = fmaf(w, o[r], y[t][c][r]);
+                            y[t][c][r] = fmaf(w, value_of(own[t][c], r), y[t][c][r]);
                         }
-                    }
                     e += __shfl_xor(e, 16);
                     e += __shfl_xor(e, 32);
                     if (lane < 16 && 16 * t + lane < n)
-                        a.dot[((int64_t)(row_block * 4 + wave) * d.H + h) * (d.B * d.T) + q.row + t0 + 16 * t + lane] = e;
+                        a.dot[((int64_t)((row_block * ncol + col_block) * NW + wave) * d.H + h) * (d.B * d.T) + q.row + t0 + 16 * t + lane] = e;
                 }
             }
-            const int64_t HY = d.H / a.y_rep, row = q.row + t0;
-            const int64_t slice = a.y_f32 ? ((int64_t)row_block * a.y_rep + h % a.y_rep) * (d.B * d.T) : 0;
-            const int64_t step = HY * a.cols, at = ((slice + row) * HY + h / a.y_rep) * a.cols + col_block * W;
+            const int64_t at = y_at + t0 * (int64_t)step;
             auto put = [&](auto zero) {
                 typedef decltype(zero) U;
                 const __amdgpu_buffer_rsrc_t ry = rows_window(static_cast<const U*>(a.y) + at, step, n, cols);
@@ -392,7 +477,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
 #pragma unroll
                     for (int c = 0; c < NC; c++) {
                         const int j = j4 + 16 * c;
-                        const int off = j < cols ? ((16 * t + l16) * (int)step + j) * (int)sizeof(U) : kNowhere;
+                        const int off = j < cols ? ((16 * t + l16) * step + j) * (int)sizeof(U) : kNowhere;
                         buf_store4e<U>(ry, off, cols - j, a.y_vec, y[t][c]);
                     }
             };
@@ -401,27 +486,20 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         }
         barrier_lds();
     }
-    if (STATE) {
-        float* to = a.parts + ((int64_t)blockIdx.x * d.H + h) * kv;
-        each_state([&](int n, int kt, int r, int64_t at, bool in) {
-            if (in) to[at] = S[n][kt][r];
-        });
-        if (tid == 0 && blockIdx.z == 0) a.decay[(int64_t)blockIdx.x * d.H + h] = exp2_of(total);
-    } else if (last_run && a.end) {
-        float* to = a.end + (seq * d.H + h) * kv;
-        each_state([&](int n, int kt, int r, int64_t at, bool in) {
-            if (in) to[at] = S[n][kt][r];
-        });
+    if (STATE || (last_run && a.end)) {
+        const __amdgpu_buffer_rsrc_t st = state_at(STATE ? a.parts : a.end, STATE ? (int64_t)blockIdx.x : seq);
+        each_state([&](f32x4& x, int r, int at) { buf_store<float>(st, at, x[r]); });
     }
+    if (STATE && tid == 0 && blockIdx.z == 0) a.decay[(int64_t)blockIdx.x * d.H + h] = exp2_of(total);
 }
 
 template <typename T> snhip_status lin_run(const LinShape& d, const LinPass& a, bool rev, int kind, hipStream_t st) {
     auto go = [&](auto dp, auto nc, auto back, auto dot, auto state) -> snhip_status {
-        constexpr int W = 64 * decltype(nc)::value;
-        const int64_t z = (int64_t)((a.cols + W - 1) / W) * ((a.rows + kLinRows - 1) / kLinRows);
+        constexpr int NC = decltype(nc)::value;
+        const int64_t z = (int64_t)((a.cols + 64 * NC - 1) / (64 * NC)) * ((a.rows + kLinRows - 1) / kLinRows);
         const dim3 grid((unsigned)d.slots, (unsigned)d.H, (unsigned)z);
-        k_lin<T, decltype(dp)::value, decltype(nc)::value, decltype(back)::value, decltype(dot)::value,
-              decltype(state)::value><<<grid, 256, 0, st>>>(d, a);
+        k_lin<T, decltype(dp)::value, NC, decltype(back)::value, decltype(dot)::value, decltype(state)::value>
+            <<<grid, 256, 0, st>>>(d, a);
         SNHIP_CHECK(hipGetLastError());
         return SNHIP_OK;
     };
@@ -435,7 +513,7 @@ template <typename T> snhip_status lin_run(const LinShape& d, const LinPass& a, 
     auto by_dir = [&](auto dp, auto nc) {
         return rev ? by_kind(dp, nc, std::true_type()) : by_kind(dp, nc, std::false_type());
     };
-    auto by_cols = [&](auto dp) { return a.cols <= 64 ? by_dir(dp, one()) : by_dir(dp, two()); };
+    auto by_cols = [&](auto dp) { return a.cols <= 64 || d.narrow ? by_dir(dp, one()) : by_dir(dp, two()); };
     return a.rows <= 64 ? by_cols(std::integral_constant<int, 64>()) : by_cols(std::integral_constant<int, 128>());
 }
 
