@@ -15,6 +15,24 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 
+// Running sums over lanes: within rows of 16 by shifts, then the rows before.
+template <int CTRL> __device__ __forceinline__ double add_shifted(double x) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), CTRL, 0xf, 0xf, true),
+              hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), CTRL, 0xf, 0xf, true);
+    return x + __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double lane_value(double x, int l) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(x), l), __builtin_amdgcn_readlane(__double2loint(x), l));
+}
+__device__ __forceinline__ double running_sum(double x, int lane) {
+    x = add_shifted<0x111>(x);
+    x = add_shifted<0x112>(x);
+    x = add_shifted<0x114>(x);
+    x = add_shifted<0x118>(x);
+    const double a = lane_value(x, 15), b = a + lane_value(x, 31), c = b + lane_value(x, 47);
+    return x + (lane < 16 ? 0. : lane < 32 ? a : lane < 48 ? b : c);
+}
+
 // A tile of P planes of R rows and C columns in LDS without padding (planes.h has one with):
 // the 16-byte units of a row are permuted by an exclusive or with bits of the row, chosen so
 // that both ways of reading spread over the banks. The 16 rows of a frag meet 16 different
@@ -62,23 +80,23 @@ template <int P, int R, int C> struct SwTile {
 // threads: tokens from n on and columns from `cols` on are 0 (a stride below `cols` would let
 // the window alone hand out other rows).
 template <typename T, int R, int W, int NTH> struct LinFetch {
-    static constexpr int N = (R * W / 8 + NTH - 1) / NTH;
-    static constexpr bool whole = R * W / 8 % NTH == 0;
+    static constexpr int N = R * W / 8 / NTH;
+    static_assert(R * W / 8 % NTH == 0);
     Vec8<T> x[N];
     __device__ __forceinline__ void load(const T* src, int64_t stride, int n, int cols, bool vec, int tid) {
         const __amdgpu_buffer_rsrc_t r = rows_window(src, stride, n, cols);
         const int step = (int)stride;
         if (vec) {
+            const int t0 = tid / (W / 8), c = tid % (W / 8) * 8, off = (t0 * step + c) * (int)sizeof(T);
+            constexpr int more = NTH / (W / 8);            // rows from one vector of a thread to the next
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const int i = tid + j * NTH, t = i / (W / 8), c = i % (W / 8) * 8;
-                x[j] = buf_load8<T>(r, t < n && (whole || t < R) && c < cols ? (t * step + c) * (int)sizeof(T) : kNowhere, 8, true);
-            }
+            for (int j = 0; j < N; j++)
+                x[j] = buf_load8<T>(r, t0 + j * more < n && c < cols ? off + j * more * step * (int)sizeof(T) : kNowhere, 8, true);
         } else {
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 const int i = here(tid) + j * NTH, t = i / (W / 8), c = i % (W / 8) * 8;
-                x[j] = buf_load8<T>(r, (t * step + c) * (int)sizeof(T), t < n && (whole || t < R) ? cols - c : 0, false);
+                x[j] = buf_load8<T>(r, (t * step + c) * (int)sizeof(T), t < n ? cols - c : 0, false);
             }
         }
     }
@@ -86,7 +104,7 @@ template <typename T, int R, int W, int NTH> struct LinFetch {
 #pragma unroll
         for (int j = 0; j < N; j++) {
             const int i = tid + j * NTH;
-            if (whole || i < R * W / 8) to.put8(i / (W / 8), i % (W / 8) * 8, split_raw8<T>(x[j]));
+            to.put8(i / (W / 8), i % (W / 8) * 8, split_raw8<T>(x[j]));
         }
     }
 };
@@ -239,13 +257,9 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         fb.store(Bt, tid);
         fc.store(Ct, tid);
         if (wave == 0) {
-            double c = (double)lin_decay(fg) * 1.4426950408889634074;         // powers of two from here on
-#pragma unroll
-            for (int o = 1; o < C; o <<= 1) {
-                const double y = __shfl_up(c, o);
-                if (lane >= o) c += y;
-            }
-            const double end = __shfl(c, C - 1);
+            // powers of two from here on
+            const double c = running_sum(lane < C ? (double)lin_decay(fg) * 1.4426950408889634074 : 0., lane),
+                         end = lane_value(c, C - 1);
             if (lane < C) {
                 s.c[lane] = c;
                 const float in = exp2_of(c), out = exp2_of(end - c);
@@ -381,7 +395,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
 #pragma unroll
             for (int e = 0; e < 2; e++) bf[i & 1][e] = Bt.tfrag(32 * b, 16 * k2 + 8 * (lane & 3) + 4 * e, lane);
         };
-        columns_of_b(0);
+        if (!DOT) columns_of_b(0);             // with the dots' registers a step ahead is too much
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             if (b + 1 < NB) columns_of(b + 1);
@@ -389,7 +403,8 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
 #pragma unroll
             for (int k = 0; k < NK / 2; k++) {
                 const int i = b * (NK / 2) + k;
-                if (i + 1 < NB * NK / 2) columns_of_b(i + 1);
+                if (DOT) columns_of_b(i);
+                else if (i + 1 < NB * NK / 2) columns_of_b(i + 1);
                 if (b == 0)
 #pragma unroll
                     for (int c = 0; c < NC; c++) S[c][2 * k] *= decay, S[c][2 * k + 1] *= decay;
@@ -416,10 +431,21 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                 });
             }
         }
-        // what the dots take: X, and C of the token itself, whose share is added after them
         const int j4 = wave * 16 * NC + (lane >> 4) * 4;       // this lane's first column in C
+        Frag<P> own[DOT ? NT : 1][NC];         // C of the token itself, whose share is added after the dots
+        if constexpr (DOT) {
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int p = 0; p < P; p++)
+                        *reinterpret_cast<bf16x4*>(&own[t][c].p[p]) = *reinterpret_cast<const bf16x4*>(Ct.at(p, 16 * t + l16, j4 + 16 * c));
+        }
+        barrier_lds();
+        if (more) store();                     // only P is read from here on
+        __builtin_amdgcn_sched_barrier(0);
         float xv[DOT ? NT : 1][NC][4];
-        Frag<P> own[DOT ? NT : 1][NC];
         if constexpr (DOT) {
             const __amdgpu_buffer_rsrc_t r = rows_window(xp + t0 * a.X.st[1], a.X.st[1], n, cols);
 #pragma unroll
@@ -428,13 +454,8 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                 for (int c = 0; c < NC; c++) {
                     const int j = j4 + 16 * c;
                     buf_load4e<T>(r, j < cols ? ((16 * t + l16) * (int)a.X.st[1] + j) * E : kNowhere, cols - j, a.vec, xv[t][c]);
-#pragma unroll
-                    for (int p = 0; p < P; p++)
-                        *reinterpret_cast<bf16x4*>(&own[t][c].p[p]) = *reinterpret_cast<const bf16x4*>(Ct.at(p, 16 * t + l16, j));
                 }
         }
-        barrier_lds();
-        if (more) store();                     // only P is read from here on
         if constexpr (!STATE) {
 #pragma unroll
             for (int jb = 0; jb < NB; jb++)
@@ -473,13 +494,12 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                 typedef decltype(zero) U;
                 const __amdgpu_buffer_rsrc_t ry = rows_window(static_cast<const U*>(a.y) + at, step, n, cols);
 #pragma unroll
-                for (int t = 0; t < NT; t++)
+                for (int c = 0; c < NC; c++) {
+                    const int j = j4 + 16 * c, off = j < cols ? (l16 * step + j) * (int)sizeof(U) : kNowhere;
 #pragma unroll
-                    for (int c = 0; c < NC; c++) {
-                        const int j = j4 + 16 * c;
-                        const int off = j < cols ? ((16 * t + l16) * step + j) * (int)sizeof(U) : kNowhere;
-                        buf_store4e<U>(ry, off, cols - j, a.y_vec, y[t][c]);
-                    }
+                    for (int t = 0; t < NT; t++)           // what is added to kNowhere stays outside
+                        buf_store4e<U>(ry, off + 16 * t * step * (int)sizeof(U), cols - j, a.y_vec, y[t][c]);
+                }
             };
             if (a.y_f32) put(0.f);
             else put(T(0.f));
