@@ -9,6 +9,8 @@
 // running count; a block sums the squares of its pieces in 64 bits (a square of fp32 does
 // not overflow there) into one partial sum, and the blocks of the second kernel each add
 // all partial sums again in the same order, which is cheaper than a launch between the two.
+// The second kernels go through the pieces backwards: what the first ones read last is still
+// in the last-level cache (256 MB).
 #include <algorithm>
 #include <vector>
 
@@ -69,9 +71,11 @@ template <typename T> __device__ __forceinline__ void clip_scale(const T* x, T* 
     });
 }
 
-// f(tensor, its piece) for the pieces of this block.
-template <typename F> __device__ __forceinline__ void clip_pieces(const ClipTable& t, F f) {
-    for (int p = blockIdx.x; p < t.first[t.count]; p += gridDim.x) {
+// f(tensor, its piece) for the pieces of this block, from the first or from the last.
+template <bool BACK, typename F> __device__ __forceinline__ void clip_pieces(const ClipTable& t, F f) {
+    const int all = t.first[t.count];
+    for (int i = blockIdx.x; i < all; i += gridDim.x) {
+        const int p = BACK ? all - 1 - i : i;
         int lo = 0, hi = t.count - 1;          // the last tensor that begins at or before p
         while (lo < hi) {
             const int mid = (lo + hi + 1) / 2;
@@ -92,7 +96,7 @@ __device__ __forceinline__ double clip_block_sum(double v) {
 
 __global__ __launch_bounds__(256) void k_clip_sum(ClipTable t, double* partial) {
     double s = 0.;
-    clip_pieces(t, [&](int i, int64_t piece) {
+    clip_pieces<false>(t, [&](int i, int64_t piece) {
         if (t.dtype[i] == SNHIP_F32) s += clip_squares(static_cast<const float*>(t.x[i]), t.n[i], piece);
         else if (t.dtype[i] == SNHIP_BF16) s += clip_squares(static_cast<const __bf16*>(t.x[i]), t.n[i], piece);
         else s += clip_squares(static_cast<const _Float16*>(t.x[i]), t.n[i], piece);
@@ -116,7 +120,7 @@ __global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const double* p
     const double n = clip_norm(partial, partials), f = max_norm / (n + 1e-6);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const float factor = f >= 1. ? 1.f : (float)f;         // NaN stays
-    clip_pieces(t, [&](int i, int64_t piece) {
+    clip_pieces<true>(t, [&](int i, int64_t piece) {
         if (factor == 1.f && t.x[i] == t.y[i]) return;
         if (t.dtype[i] == SNHIP_F32) clip_scale(static_cast<const float*>(t.x[i]), static_cast<float*>(t.y[i]), t.n[i], piece, factor);
         else if (t.dtype[i] == SNHIP_BF16)
@@ -158,39 +162,37 @@ snhip_status clip_run(const SnHipClip& c, float* norm, hipStream_t st) {
             (c.n[i] && (!c.x[i] || (c.y && !c.y[i]))))
             return SNHIP_E_INVAL;
     if (c.y && clip_overlaps(c)) return SNHIP_E_INVAL;
-    int64_t partials = 0, at = 0;
-    ClipTable t;
-    // fills t with tensors from `at` on; false: none is left
-    auto next = [&]() {
-        t.count = 0;
-        t.first[0] = 0;
-        for (; at < c.count && t.count < kClipTensors; at++) {
-            const int64_t pieces = (c.n[at] + kClipPiece - 1) / kClipPiece;
-            if (!pieces) continue;
-            t.x[t.count] = c.x[at];
-            t.y[t.count] = c.y ? c.y[at] : nullptr;
-            t.n[t.count] = c.n[at];
-            t.dtype[t.count] = (unsigned char)c.dtype[at];
-            t.first[t.count + 1] = t.first[t.count] + (int)pieces;
-            t.count++;
+    std::vector<ClipTable> tables;
+    for (int64_t at = 0; at < c.count; at++) {
+        const int64_t pieces = (c.n[at] + kClipPiece - 1) / kClipPiece;
+        if (!pieces) continue;
+        if (tables.empty() || tables.back().count == kClipTensors) {
+            tables.emplace_back();
+            tables.back().count = tables.back().first[0] = 0;
         }
-        return t.count > 0;
-    };
-    auto grid = [&]() { return (unsigned)std::min<int64_t>(t.first[t.count], kClipBlocks); };
-    while (next()) {
-        k_clip_sum<<<grid(), 256, 0, st>>>(t, c.ws + partials);
+        ClipTable& t = tables.back();
+        t.x[t.count] = c.x[at];
+        t.y[t.count] = c.y ? c.y[at] : nullptr;
+        t.n[t.count] = c.n[at];
+        t.dtype[t.count] = (unsigned char)c.dtype[at];
+        t.first[t.count + 1] = t.first[t.count] + (int)pieces;
+        t.count++;
+    }
+    auto grid = [&](const ClipTable& t) { return (unsigned)std::min<int64_t>(t.first[t.count], kClipBlocks); };
+    int64_t partials = 0;
+    for (const ClipTable& t : tables) {
+        k_clip_sum<<<grid(t), 256, 0, st>>>(t, c.ws + partials);
         SNHIP_CHECK(hipGetLastError());
-        partials += grid();
+        partials += grid(t);
     }
     if (!c.y || !partials) {
         k_clip_norm<<<1, 256, 0, st>>>(c.ws, partials, norm);
         SNHIP_CHECK(hipGetLastError());
-        return SNHIP_OK;
-    }
-    at = 0;
-    for (float* first = norm; next(); first = nullptr) {
-        k_clip_scale<<<grid(), 256, 0, st>>>(t, c.ws, partials, c.max_norm, first);
-        SNHIP_CHECK(hipGetLastError());
+    } else {
+        for (size_t i = tables.size(); i-- > 0;) {
+            k_clip_scale<<<grid(tables[i]), 256, 0, st>>>(tables[i], c.ws, partials, c.max_norm, i ? nullptr : norm);
+            SNHIP_CHECK(hipGetLastError());
+        }
     }
     return SNHIP_OK;
 }

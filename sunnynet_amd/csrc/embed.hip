@@ -26,8 +26,9 @@
 namespace snhip {
 namespace {
 
-constexpr int kEmbedTiles = 128;          // at most so many tiles, of at least kEmbedTile tokens
-constexpr int kEmbedTile = 2048, kEmbedBits = 10, kEmbedBins = 1 << kEmbedBits;
+// At most so many tiles, of at least so many tokens; up to how many one block sorts alone.
+constexpr int kEmbedTiles = 128, kEmbedTile = 1024, kEmbedAlone = 4096;
+constexpr int kEmbedBits = 10, kEmbedBins = 1 << kEmbedBits, kEmbedWaves = 8;
 
 template <typename T> constexpr int kLane = 16 / (int)sizeof(T);      // columns of a lane
 
@@ -93,35 +94,43 @@ __global__ __launch_bounds__(1024) void k_embed_count(EmbedP a) {
 }
 
 // Puts a tile's tokens in the places that passes p0 to p1 - 1 give them (more than one only
-// where the tile is all there is: then its own counts are all counts).
-__global__ __launch_bounds__(1024) void k_embed_sort(EmbedP a, int p0, int p1) {
-    __shared__ int next[16][kEmbedBins];       // of a wave: its tokens of a digit, then the place of the next
-    __shared__ int wsum[16];
+// where the tile is all there is: then its own counts are all counts). A thread has PER
+// neighbouring digits.
+template <int PER> __global__ __launch_bounds__(64 * kEmbedWaves) void k_embed_sort(EmbedP a, int p0, int p1) {
+    constexpr int NW = kEmbedWaves, NTH = 64 * NW, BINS = PER * NTH;
+    __shared__ int next[NW][BINS];             // of a wave: its tokens of a digit, then the place of the next
+    __shared__ int wsum[NW];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = 1 << a.bits;
     const int64_t t0 = blockIdx.x * (int64_t)a.tile, t1 = t0 + a.tile < a.n ? t0 + a.tile : a.n;
-    const int64_t per = (a.tile + 1023) / 1024 * 64, w0 = t0 + wave * per, w1 = w0 + per < t1 ? w0 + per : t1;
+    const int64_t per = (a.tile + NTH - 1) / NTH * 64, w0 = t0 + wave * per, w1 = w0 + per < t1 ? w0 + per : t1;
     for (int p = p0; p < p1; p++) {
         const int shift = p * a.bits;
         const unsigned* const from = a.key[(p + 1) & 1];
         const int* const from_at = a.at[(p + 1) & 1];
         auto key_of = [&](int64_t i) { return p ? from[i] : embed_key(a, i); };
-        for (int i = tid; i < 16 * kEmbedBins; i += 1024) next[0][i] = 0;
+        for (int i = tid; i < NW * BINS; i += NTH) next[0][i] = 0;
         __syncthreads();
         for (int64_t i = w0 + lane; i < w1; i += 64) atomicAdd(&next[wave][(key_of(i) >> shift) & (bins - 1)], 1);
         __syncthreads();
-        // where this tile's tokens of digit `tid` begin: after all smaller digits and earlier tiles
-        int before = 0, all = 0;
-        if (tid < bins) {
-            if (a.tiles == 1)
-                for (int w = 0; w < 16; w++) all += next[w][tid];
-            else
+        // where this tile's tokens of a digit begin: after all smaller digits and earlier tiles
+        int before[PER] = {}, all[PER] = {}, sum = 0;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int b = tid * PER + j;
+            if (a.tiles == 1) {
+#pragma unroll
+                for (int w = 0; w < NW; w++) all[j] += next[w][b];
+            } else if (b < bins) {
+#pragma unroll 8
                 for (int t = 0; t < a.tiles; t++) {
-                    const int c = a.count[((int64_t)p * a.tiles + t) * bins + tid];
-                    before += t < (int)blockIdx.x ? c : 0;
-                    all += c;
+                    const int c = a.count[((int64_t)p * a.tiles + t) * bins + b];
+                    before[j] += t < (int)blockIdx.x ? c : 0;
+                    all[j] += c;
                 }
+            }
+            sum += all[j];
         }
-        int run = all;
+        int run = sum;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const int y = __shfl_up(run, o);
@@ -129,15 +138,19 @@ __global__ __launch_bounds__(1024) void k_embed_sort(EmbedP a, int p0, int p1) {
         }
         if (lane == 63) wsum[wave] = run;
         __syncthreads();
-        int place = before + run - all;
-        for (int w = 0; w < wave; w++) place += wsum[w];
-        if (tid < bins)
+        int first = run - sum;
+        for (int w = 0; w < wave; w++) first += wsum[w];
 #pragma unroll
-            for (int w = 0; w < 16; w++) {
-                const int c = next[w][tid];
-                next[w][tid] = place;
+        for (int j = 0; j < PER; j++) {
+            int place = first + before[j];
+            first += all[j];
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                const int c = next[w][tid * PER + j];
+                next[w][tid * PER + j] = place;
                 place += c;
             }
+        }
         __syncthreads();
         unsigned* const key = a.key[p & 1];
         int* const at = a.at[p & 1];
@@ -264,18 +277,18 @@ __global__ __launch_bounds__(256) void k_embed_grad(EmbedP a, const T* dy, T* ou
     flush(i1 < a.n && key[i1] == now);
 }
 
-// Adds the partial sums of the runs that begin in a group and end in a later one.
+// Adds the partial sums of the runs that begin in a group and end in a later one: a block
+// for a group and 64 lanes of columns, a wave every fourth of the groups.
 template <typename T, bool VEC> __global__ __launch_bounds__(256) void k_embed_join(EmbedP a, T* out, int slices) {
     constexpr int L = kLane<T>, U = 8;
+    __shared__ float part[3][64][L + 1];
     const unsigned* const key = a.key[(a.passes - 1) & 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t task = blockIdx.x * (int64_t)4 + wave, g = task / slices, end = (g + 1) * a.group;
+    const int64_t g = blockIdx.x / slices, i0 = g * a.group, end = i0 + a.group;
     if (end >= a.n) return;
     const unsigned k = key[end - 1];
-    const int64_t i0 = g * a.group;
-    if (key[end] != k || k >= (unsigned)a.R || (i0 > 0 && key[i0 - 1] == k && key[i0] == k)) return;
-    const int64_t c = (task % slices) * 64 * L + lane * L;
-    if (c >= a.D) return;
+    if (key[end] != k || k >= (unsigned)a.R || (i0 > 0 && key[i0 - 1] == k)) return;
+    const int64_t c = (blockIdx.x % slices) * 64 * L + lane * L;
     const int n = (int)(a.D - c < L ? a.D - c : L);
     int64_t lo = end, hi = a.n;                  // the run's end
     while (lo < hi) {
@@ -284,19 +297,28 @@ template <typename T, bool VEC> __global__ __launch_bounds__(256) void k_embed_j
         else hi = mid;
     }
     const int64_t last = (lo - 1) / a.group;
-    float sum[L];
-    embed_load<float, L, true>(a.part + (g * 2 + 1) * a.ld + c, L, sum);
-    for (int64_t q = g + 1; q <= last; q += U) {
-        float x[U][L];
+    float sum[L] = {};
+    if (c < a.D) {
+        if (wave == 0) embed_load<float, L, true>(a.part + (g * 2 + 1) * a.ld + c, L, sum);
+        for (int64_t q = g + 1 + wave; q <= last; q += 4 * U) {
+            float x[U][L];
 #pragma unroll
-        for (int u = 0; u < U; u++) embed_load<float, L, true>(a.part + (q + u <= last ? q + u : last) * 2 * a.ld + c, L, x[u]);
+            for (int u = 0; u < U; u++) embed_load<float, L, true>(a.part + (q + 4 * u <= last ? q + 4 * u : last) * 2 * a.ld + c, L, x[u]);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (q + u > last) continue;
+            for (int u = 0; u < U; u++) {
+                if (q + 4 * u > last) continue;
 #pragma unroll
-            for (int e = 0; e < L; e++) sum[e] += x[u][e];
+                for (int e = 0; e < L; e++) sum[e] += x[u][e];
+            }
         }
     }
+    if (wave)
+#pragma unroll
+        for (int e = 0; e < L; e++) part[wave - 1][lane][e] = sum[e];
+    __syncthreads();
+    if (wave || c >= a.D) return;
+#pragma unroll
+    for (int e = 0; e < L; e++) sum[e] = (sum[e] + part[0][lane][e]) + (part[1][lane][e] + part[2][lane][e]);
     embed_store<T, L, VEC>(out + (int64_t)k * a.D + c, n, sum, a.scale);
 }
 
@@ -313,7 +335,7 @@ int64_t embed_plan(EmbedP* a, const void* ids, bool wide, int64_t n, int64_t R, 
     a->wide = wide;
     a->n = n, a->R = R, a->D = D;
     a->scale = scale;
-    int64_t tiles = (n + kEmbedTile - 1) / kEmbedTile;
+    int64_t tiles = n <= kEmbedAlone ? 1 : (n + kEmbedTile - 1) / kEmbedTile;
     if (tiles > kEmbedTiles) tiles = kEmbedTiles;
     a->tile = (int)((n + tiles - 1) / tiles);
     a->tiles = (int)((n + a->tile - 1) / a->tile);
@@ -322,9 +344,12 @@ int64_t embed_plan(EmbedP* a, const void* ids, bool wide, int64_t n, int64_t R, 
     a->passes = (bits + kEmbedBits - 1) / kEmbedBits;
     a->bits = (bits + a->passes - 1) / a->passes;
     const int64_t lanes = 64 * (dtype == SNHIP_F32 ? 4 : 8), slices = (D + lanes - 1) / lanes;
-    // Enough waves to fill the card, and runs as long as they may be.
+    // Enough waves to fill the card, and runs as long as they may be; past 2^23 groups and
+    // slices longer ones, so that a grid (of fewer than 2^32 threads) holds them.
     int64_t group = n * slices / 4096;
-    a->group = (int)(group < 8 ? 8 : group > 64 ? 64 : group);
+    group = group < 8 ? 8 : group > 64 ? 64 : group;
+    if (n * slices / group >= 1 << 23) group = (n * slices >> 22) + 1;
+    a->group = (int)group;
     a->groups = (n + a->group - 1) / a->group;
     a->ld = (D + 7) / 8 * 8;
     int64_t at = 0;
@@ -358,13 +383,12 @@ template <typename T> snhip_status embed_fwd_t(const EmbedP& a, const void* tabl
 template <typename T> snhip_status embed_bwd_t(const EmbedP& a, const void* dy, void* out, bool vec, hipStream_t st) {
     const int64_t lanes = 64 * kLane<T>, slices = (a.D + lanes - 1) / lanes, tasks = (a.groups * slices + 3) / 4,
                   blocks = tasks + (a.R + 63) / 64;
-    if (blocks >= 1 << 24) return SNHIP_E_INVAL;           // a grid holds fewer than 2^32 threads
     if (vec) k_embed_grad<T, true><<<(unsigned)blocks, 256, 0, st>>>(a, (const T*)dy, (T*)out, (int)slices, tasks);
     else k_embed_grad<T, false><<<(unsigned)blocks, 256, 0, st>>>(a, (const T*)dy, (T*)out, (int)slices, tasks);
     SNHIP_CHECK(hipGetLastError());
     if (a.groups > 1) {
-        if (vec) k_embed_join<T, true><<<(unsigned)tasks, 256, 0, st>>>(a, (T*)out, (int)slices);
-        else k_embed_join<T, false><<<(unsigned)tasks, 256, 0, st>>>(a, (T*)out, (int)slices);
+        if (vec) k_embed_join<T, true><<<(unsigned)(a.groups * slices), 256, 0, st>>>(a, (T*)out, (int)slices);
+        else k_embed_join<T, false><<<(unsigned)(a.groups * slices), 256, 0, st>>>(a, (T*)out, (int)slices);
         SNHIP_CHECK(hipGetLastError());
     }
     return SNHIP_OK;
@@ -402,16 +426,17 @@ snhip_status snhip_op_embed_bwd_dev(const void* dy, const void* ids, int32_t wid
     EmbedP a;
     embed_plan(&a, ids, wide != 0, n, R, D, scale, dtype, static_cast<char*>(ws));
     const hipStream_t st = as_stream(stream);
+    auto sort = [&](int p0, int p1) {
+        if (a.bits < kEmbedBits) k_embed_sort<1><<<(unsigned)a.tiles, 64 * kEmbedWaves, 0, st>>>(a, p0, p1);
+        else k_embed_sort<2><<<(unsigned)a.tiles, 64 * kEmbedWaves, 0, st>>>(a, p0, p1);
+        return hipGetLastError();
+    };
     if (a.tiles == 1) {
-        k_embed_sort<<<1, 1024, 0, st>>>(a, 0, a.passes);
-        SNHIP_CHECK(hipGetLastError());
+        SNHIP_CHECK(sort(0, a.passes));
     } else {
         k_embed_count<<<(unsigned)a.tiles, 1024, 0, st>>>(a);
         SNHIP_CHECK(hipGetLastError());
-        for (int p = 0; p < a.passes; p++) {
-            k_embed_sort<<<(unsigned)a.tiles, 1024, 0, st>>>(a, p, p + 1);
-            SNHIP_CHECK(hipGetLastError());
-        }
+        for (int p = 0; p < a.passes; p++) SNHIP_CHECK(sort(p, p + 1));
     }
     const bool vec = embed_vec(dy, dtable, D, dtype);
     return dtype == SNHIP_F32    ? embed_bwd_t<float>(a, dy, dtable, vec, st)

@@ -23,25 +23,29 @@ _dtype = attrgetter("dtype")
 
 def _addresses(tensors, what):
     """(addresses, sizes, kinds, device index) of a list of tensors, after its checks."""
-    where = {t.get_device() for t in tensors}
+    try:
+        where = set(map(torch.Tensor.get_device, tensors))
+    except TypeError:
+        raise ValueError("the gradients must be tensors: leave out parameters without one") from None
     if len(where) > 1 or -1 in where:
         raise ValueError(f"{what} must be tensors of one GPU")
-    try:
+    dtypes = set(map(_dtype, tensors))
+    if not dtypes <= DTYPES.keys():
+        raise ValueError(f"{what} must be float32, bfloat16 or float16")
+    if len(dtypes) == 1:
+        kinds = array("i", [DTYPES[dtypes.pop()]]) * len(tensors)
+    else:
         kinds = array("i", [DTYPES[d] for d in map(_dtype, tensors)])
-    except KeyError:
-        raise ValueError(f"{what} must be float32, bfloat16 or float16") from None
     if not all(map(torch.Tensor.is_contiguous, tensors)):
         raise ValueError(f"{what} must be contiguous")
-    sizes = array("q", map(torch.Tensor.numel, tensors))
-    return array("Q", map(torch.Tensor.data_ptr, tensors)), sizes, kinds, where.pop() if where else None
+    sizes = array("q", [*map(torch.Tensor.numel, tensors)])
+    return array("Q", [*map(torch.Tensor.data_ptr, tensors)]), sizes, kinds, where.pop() if where else None
 
 
 def _run(tensors, max_norm, out):
     tensors = list(tensors)
     if len(tensors) >= MAX_TENSORS:
         raise ValueError(f"fewer than {MAX_TENSORS} tensors per call")
-    if any(t is None for t in tensors):
-        raise ValueError("the gradients must be tensors: leave out parameters without one")
     x, sizes, kinds, at = _addresses(tensors, "the gradients")
     if at is None:
         raise ValueError("no gradients")
@@ -87,9 +91,8 @@ def clip_grad_norm(grads, max_norm, *, out=None):
     grads = list(grads)
     if out is not None:
         out = list(out)
-    for t in grads if out is None else out:
-        if t is not None and t.requires_grad and t.is_leaf:
-            raise RuntimeError("a leaf that requires a gradient cannot be written in place")
+    if any(t is not None and t.requires_grad and t.is_leaf for t in (grads if out is None else out)):
+        raise RuntimeError("a leaf that requires a gradient cannot be written in place")
     norm = _run(grads, max_norm, grads if out is None else out)
     torch.autograd.graph.increment_version(grads if out is None else out)      # a graph that saved one refuses it
     return norm
