@@ -10,7 +10,8 @@
 // not overflow there) into one partial sum, and the blocks of the second kernel each add
 // all partial sums again in the same order, which is cheaper than a launch between the two.
 // The second kernels go through the pieces backwards: what the first ones read last is still
-// in the last-level cache (256 MB).
+// in the last-level cache (256 MB), and what they write is kept out of it (102 M fp32: 249 us
+// with ordinary stores, 238 so; bf16 135 and 114).
 #include <algorithm>
 #include <vector>
 
@@ -64,7 +65,7 @@ template <typename T> __device__ __forceinline__ void clip_scale(const T* x, T* 
             T8 o;
 #pragma unroll
             for (int e = 0; e < 8; e++) o[e] = (T)(v[e] * factor);
-            *reinterpret_cast<T8*>(y + i) = o;
+            __builtin_nontemporal_store(o, reinterpret_cast<T8*>(y + i));
         } else {
             for (int e = 0; e < m; e++) y[i + e] = (T)(v[e] * factor);
         }

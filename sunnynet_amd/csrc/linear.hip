@@ -209,12 +209,14 @@ bool lin_in_range(const SnHipLinear& d) {
            d.dtype >= SNHIP_F32 && d.dtype <= SNHIP_F16;
 }
 
-// Blocks that fill the card (a CU each), and the fewest tokens worth a part.
-constexpr int64_t kLinBlocks = 512, kLinPart = 256;
+// Blocks that fill the card (two a CU), and the fewest tokens worth a part: 3 x 333 tokens of 5
+// heads, all kernels of a training pass, 100 us with 64, 133 with 128, 210 with 256.
+constexpr int64_t kLinBlocks = 512, kLinPart = 64;
 
 void lin_shape(const SnHipLinear& d, LinShape* s) {
     const int64_t tokens = d.B * d.T;
-    s->narrow = false;
+    // Blocks of 64 columns where even the shortest parts leave CUs idle: 16 us less of those 100.
+    s->narrow = tokens * d.H * ((d.V + 127) / 128) / kLinPart < 256;
     const int64_t blocks = d.H * (s->narrow ? (d.V + 63) / 64 : (d.V + 127) / 128);
     int64_t part = tokens * blocks / kLinBlocks;
     part = ((part < kLinPart ? kLinPart : part) + 63) / 64 * 64;
