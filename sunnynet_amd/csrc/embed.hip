@@ -220,24 +220,18 @@ __global__ __launch_bounds__(256) void k_embed_grad(EmbedP a, const T* dy, T* ou
     const unsigned* const key = a.key[(a.passes - 1) & 1];
     const int* const at = a.at[(a.passes - 1) & 1];
     if (blockIdx.x >= fill) {
-        __shared__ unsigned used[2];
         const int64_t r0 = (blockIdx.x - fill) * 64;
-        if (threadIdx.x < 2) used[threadIdx.x] = 0;
-        int64_t lo = 0, hi = a.n;                // the first token with an id of r0 or more
+        // a lane looks for its row's first token among the sorted ones: no run is walked, however long
+        int64_t lo = 0, hi = a.n;
         while (lo < hi) {
             const int64_t mid = (lo + hi) / 2;
-            if (key[mid] < (unsigned)r0) lo = mid + 1;
+            if (key[mid] < (unsigned)r0 + lane) lo = mid + 1;
             else hi = mid;
         }
-        __syncthreads();
-        for (int64_t i = lo + threadIdx.x; i < a.n && key[i] < (unsigned)r0 + 64u; i += 256) {
-            const unsigned k = key[i] - (unsigned)r0;
-            if (i == lo || key[i - 1] != key[i]) atomicOr(&used[k >> 5], 1u << (k & 31));
-        }
-        __syncthreads();
+        const unsigned long long used = __ballot(lo < a.n && key[lo] == (unsigned)r0 + lane);
         const float zero[L] = {};
         for (int r = wave; r < 64 && r0 + r < a.R; r += 4)
-            if (!(used[r >> 5] >> (r & 31) & 1))
+            if (!(used >> r & 1))
                 for (int64_t c = lane * L; c < a.D; c += 64 * L)
                     embed_store<T, L, VEC>(out + (r0 + r) * a.D + c, (int)(a.D - c < L ? a.D - c : L), zero, 0.f);
         return;
@@ -248,6 +242,7 @@ __global__ __launch_bounds__(256) void k_embed_grad(EmbedP a, const T* dy, T* ou
     const int n = (int)(a.D - c < L ? a.D - c : L);
     float sum[L] = {};
     unsigned now = key[i0];
+    if (now >= (unsigned)a.R) return;                   // as all after it: tokens of no row
     bool open = i0 > 0 && key[i0 - 1] == now;           // the run began before this group
     auto flush = [&](bool goes_on) {
         if (now < (unsigned)a.R && c < a.D) {

@@ -36,7 +36,6 @@ constexpr int64_t kLinTokens = (1 << 30) - 1;      // positions fit 32 bits
 constexpr int64_t kLinStride = 1 << 24;            // token strides: offsets inside a chunk fit 32 bits
 constexpr int kLinWaves = 4;                       // of a block, and so the parts of a dot
 constexpr int kLinRows = 128;                      // contracted rows of a block: all of K, or of a block of V
-constexpr int kLinStepTokens = 12;                 // the longest call that may run token by token
 
 // Tokens of a chunk: three planes of fp32 leave no room for more than 32.
 template <typename T> struct LinChunk { static constexpr int n = sizeof(T) == 4 ? 32 : 64; };

@@ -43,7 +43,6 @@ def _addresses(tensors, what):
 
 
 def _run(tensors, max_norm, out):
-    tensors = list(tensors)
     if len(tensors) >= MAX_TENSORS:
         raise ValueError(f"fewer than {MAX_TENSORS} tensors per call")
     x, sizes, kinds, at = _addresses(tensors, "the gradients")
@@ -74,8 +73,9 @@ def _run(tensors, max_norm, out):
 def grad_norm(grads):
     """The norm of all elements of the gradients (contiguous float32, bfloat16 or float16
     tensors of one GPU, each of its own type) -> float32 scalar on the device. Squares are
-    summed in 64 bits in a fixed order: the same calls give the same bits."""
-    return _run(grads, 0.0, None)
+    summed in 64 bits in a fixed order: the same calls give the same bits. Not
+    differentiable."""
+    return _run(list(grads), 0.0, None)
 
 
 @torch.no_grad()

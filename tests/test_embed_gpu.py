@@ -78,6 +78,18 @@ def test_ids_of_no_row(gpu, kind):
     check(table, torch.full((50,), -1, dtype=kind).cuda(), 1.0, dy.flatten(0, 1)[:50].contiguous(), F32)
 
 
+@pytest.mark.parametrize("n", [700, 6000])
+@pytest.mark.parametrize("R", [64, 101, 4097])
+def test_padded_batches(gpu, n, R):
+    """Long runs of padding behind the last row's tokens, beside rows of one token, and padding alone."""
+    ids = text(n, R, n, 1)
+    ids[n // 3:] = -1
+    ids[0] = R - 1
+    table, dy = torch.randn(R, 40).cuda(), torch.randn(n, 40).cuda()
+    check(table, ids.cuda(), 1.0, dy, F32)
+    check(table, torch.full((n,), R, dtype=torch.int32).cuda(), 1.0, dy, F32)
+
+
 def test_views_and_nothing(gpu):
     """Tables and gradients that begin off 16 bytes, non-contiguous ones, no ids at all."""
     flat = torch.randn(40 * 24 + 3).cuda()
