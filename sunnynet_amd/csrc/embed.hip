@@ -44,7 +44,7 @@ struct EmbedP {
     int passes, bits;           // of a digit
     unsigned* key[2];           // sorted ids (R: none), and their tokens
     int* at[2];
-    int* count;                 // (passes, tiles, 2^bits)
+    int* count;                 // (tiles, 2^bits), of the pass that runs
     float* part;                // (groups, 2, ld): sums of the runs that a group shares with its neighbours
     int64_t ld;                 // D up to a multiple of 8
     int group;                  // sorted tokens of a wave
@@ -83,18 +83,17 @@ __global__ __launch_bounds__(256) void k_embed(EmbedP a, const T* table, T* y, i
     }
 }
 
-// Counts the first pass' digits of a tile and clears the later passes' counts.
-__global__ __launch_bounds__(1024) void k_embed_count(EmbedP a) {
+// Counts a pass' digits of a tile.
+__global__ __launch_bounds__(1024) void k_embed_count(EmbedP a, int p) {
     __shared__ int bin[kEmbedBins];
-    const int tid = threadIdx.x, bins = 1 << a.bits;
+    const int tid = threadIdx.x, bins = 1 << a.bits, shift = p * a.bits;
+    const unsigned* const from = a.key[(p + 1) & 1];
     if (tid < bins) bin[tid] = 0;
     __syncthreads();
     const int64_t t0 = blockIdx.x * (int64_t)a.tile, t1 = t0 + a.tile < a.n ? t0 + a.tile : a.n;
-    for (int64_t i = t0 + tid; i < t1; i += 1024) atomicAdd(&bin[embed_key(a, i) & (bins - 1)], 1);
+    for (int64_t i = t0 + tid; i < t1; i += 1024) atomicAdd(&bin[((p ? from[i] : embed_key(a, i)) >> shift) & (bins - 1)], 1);
     __syncthreads();
-    if (tid < bins)
-        for (int p = 0; p < a.passes; p++)
-            a.count[((int64_t)p * a.tiles + blockIdx.x) * bins + tid] = p ? 0 : bin[tid];
+    if (tid < bins) a.count[(int64_t)blockIdx.x * bins + tid] = bin[tid];
 }
 
 // Puts a tile's tokens in the places that passes p0 to p1 - 1 give them (more than one only
@@ -127,7 +126,7 @@ template <int PER> __global__ __launch_bounds__(64 * kEmbedWaves) void k_embed_s
             } else if (b < bins) {
 #pragma unroll 8
                 for (int t = 0; t < a.tiles; t++) {
-                    const int c = a.count[((int64_t)p * a.tiles + t) * bins + b];
+                    const int c = a.count[(int64_t)t * bins + b];
                     before[j] += t < (int)blockIdx.x ? c : 0;
                     all[j] += c;
                 }
@@ -176,8 +175,6 @@ template <int PER> __global__ __launch_bounds__(64 * kEmbedWaves) void k_embed_s
             if (live) {
                 key[to] = k;
                 at[to] = token;
-                if (a.tiles > 1 && p + 1 < a.passes)
-                    atomicAdd(&a.count[((int64_t)(p + 1) * a.tiles + to / a.tile) * bins + ((k >> (shift + a.bits)) & (bins - 1))], 1);
             }
         }
         __syncthreads();
@@ -362,7 +359,7 @@ int64_t embed_plan(EmbedP* a, const void* ids, bool wide, int64_t n, int64_t R, 
         a->key[i] = reinterpret_cast<unsigned*>(take(4 * n));
         a->at[i] = reinterpret_cast<int*>(take(4 * n));
     }
-    a->count = reinterpret_cast<int*>(take(a->tiles > 1 ? (int64_t)a->passes * a->tiles * (4 << a->bits) : 0));
+    a->count = reinterpret_cast<int*>(take(a->tiles > 1 ? (int64_t)a->tiles * (4 << a->bits) : 0));
     return at;
 }
 
@@ -433,9 +430,11 @@ snhip_status snhip_op_embed_bwd_dev(const void* dy, const void* ids, int32_t wid
     if (a.tiles == 1) {
         SNHIP_CHECK(sort(0, a.passes));
     } else {
-        k_embed_count<<<(unsigned)a.tiles, 1024, 0, st>>>(a);
-        SNHIP_CHECK(hipGetLastError());
-        for (int p = 0; p < a.passes; p++) SNHIP_CHECK(sort(p, p + 1));
+        for (int p = 0; p < a.passes; p++) {
+            k_embed_count<<<(unsigned)a.tiles, 1024, 0, st>>>(a, p);
+            SNHIP_CHECK(hipGetLastError());
+            SNHIP_CHECK(sort(p, p + 1));
+        }
     }
     const bool vec = embed_vec(dy, dtable, D, dtype);
     return dtype == SNHIP_F32    ? embed_bwd_t<float>(a, dy, dtable, vec, st)
