@@ -12,15 +12,17 @@
 // The sort goes by digits of up to 10 bits, the lowest first, two passes up to 2^20 rows. In
 // a pass a block ranks one tile of the tokens: it counts its waves' digits in LDS, adds what
 // the tiles and digits before it count, and a wave then walks its tokens 64 at a time,
-// ranking equal digits by ballots. The digits of the next pass are counted as the tokens
-// are put down, by integer atomics, whose order does not matter.
+// ranking equal digits by ballots. Each pass' digits are counted by a launch of their own: by
+// atomics beside the pass before it took 10 us more where an id is frequent.
 // A wave then takes some neighbouring sorted tokens and 16 bytes a lane of the columns, sums
 // runs of one id in fp32 and writes the rows that lie inside it; runs that go on in a
 // neighbour's tokens are left as partial sums, which k_embed_join adds in order. Rows that
 // no token names are cleared by blocks of their own beside these.
-// 32768 tokens of text, a table of 32000 x 1024 in bf16: count 3 us, two passes of 12.4 (the
-// latency of their steps), sums 36 (3.7 TB/s), joins 10; up to 4096 tokens one block sorts
-// alone: 15 us for 2331.
+// Rows of up to half a wave's columns share a wave (524288 tokens of 64 in bf16: 200 us
+// without, 129 so), and a wave joins a group's run by itself unless it is long (204 -> 95 us there
+// for ids that are all alike often).
+// 32768 tokens of text, a table of 32000 x 1024 in bf16: two passes of 4 us to count and 8 (the
+// latency of their steps), sums 25, joins 10; up to 4096 tokens one block sorts alone.
 #include <type_traits>
 
 #include "common.h"
@@ -49,6 +51,7 @@ struct EmbedP {
     int64_t ld;                 // D up to a multiple of 8
     int group;                  // sorted tokens of a wave
     int64_t groups;
+    int lanes;                  // log2 of the lanes that a group's columns take (64: or more)
     float scale;
 };
 
@@ -208,12 +211,14 @@ template <typename T, int L, bool VEC> __device__ __forceinline__ void embed_sto
     }
 }
 
-// Blocks before `fill`: four waves, a group of sorted tokens and 64 lanes of columns each.
-// The others clear the unused ones of 64 rows each.
-template <typename T, bool VEC>
+// Blocks before `fill`: four waves, a group of sorted tokens and 64 lanes of columns each,
+// or with NARROW rows several groups. The others clear the unused ones of 64 rows each.
+template <typename T, bool VEC, bool NARROW>
 __global__ __launch_bounds__(256) void k_embed_grad(EmbedP a, const T* dy, T* out, int slices, int64_t fill) {
     constexpr int L = kLane<T>, U = 8;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lg = NARROW ? a.lanes : 6, subs = 64 >> lg;      // groups of a wave
+    const int lane = threadIdx.x & 63, sub = NARROW ? lane >> lg : 0, own = NARROW ? lane & ((1 << lg) - 1) : lane;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned* const key = a.key[(a.passes - 1) & 1];
     const int* const at = a.at[(a.passes - 1) & 1];
     if (blockIdx.x >= fill) {
@@ -227,15 +232,15 @@ __global__ __launch_bounds__(256) void k_embed_grad(EmbedP a, const T* dy, T* ou
         }
         const unsigned long long used = __ballot(lo < a.n && key[lo] == (unsigned)r0 + lane);
         const float zero[L] = {};
-        for (int r = wave; r < 64 && r0 + r < a.R; r += 4)
+        for (int r = wave * subs + sub; r < 64 && r0 + r < a.R; r += 4 * subs)
             if (!(used >> r & 1))
-                for (int64_t c = lane * L; c < a.D; c += 64 * L)
+                for (int64_t c = own * L; c < a.D; c += 64 * L)
                     embed_store<T, L, VEC>(out + (r0 + r) * a.D + c, (int)(a.D - c < L ? a.D - c : L), zero, 0.f);
         return;
     }
-    const int64_t task = blockIdx.x * (int64_t)4 + wave, g = task / slices;
+    const int64_t task = blockIdx.x * (int64_t)4 + wave, g = NARROW ? task * subs + sub : task / slices;
     if (g >= a.groups) return;
-    const int64_t c = (task % slices) * 64 * L + lane * L, i0 = g * a.group, i1 = i0 + a.group < a.n ? i0 + a.group : a.n;
+    const int64_t c = (NARROW ? 0 : task % slices * 64 * L) + own * L, i0 = g * a.group, i1 = i0 + a.group < a.n ? i0 + a.group : a.n;
     const int n = (int)(a.D - c < L ? a.D - c : L);
     float sum[L] = {};
     unsigned now = key[i0];
@@ -273,49 +278,86 @@ __global__ __launch_bounds__(256) void k_embed_grad(EmbedP a, const T* dy, T* ou
     flush(i1 < a.n && key[i1] == now);
 }
 
-// Adds the partial sums of the runs that begin in a group and end in a later one: a block
-// for a group and 64 lanes of columns, a wave every fourth of the groups.
-template <typename T, bool VEC> __global__ __launch_bounds__(256) void k_embed_join(EmbedP a, T* out, int slices) {
+// Adds the partial sums of the runs that begin in a group and end in a later one, for 64
+// lanes of columns (NARROW: lanes that are left share the groups): a wave for a group whose run
+// ends within a step of loads, then all four of the block's for a longer one, in turn.
+template <typename T, bool VEC, bool NARROW> __global__ __launch_bounds__(256) void k_embed_join(EmbedP a, T* out, int slices) {
     constexpr int L = kLane<T>, U = 8;
     __shared__ float part[3][64][L + 1];
+    __shared__ int runs[4];                    // of a wave's group: groups that its run goes on in, where they are many
     const unsigned* const key = a.key[(a.passes - 1) & 1];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t g = blockIdx.x / slices, i0 = g * a.group, end = i0 + a.group;
-    if (end >= a.n) return;
-    const unsigned k = key[end - 1];
-    if (key[end] != k || k >= (unsigned)a.R || (i0 > 0 && key[i0 - 1] == k)) return;
-    const int64_t c = (blockIdx.x % slices) * 64 * L + lane * L;
+    const int lg = NARROW ? a.lanes : 6, subs = 64 >> lg, lane = threadIdx.x & 63;
+    const int sub = NARROW ? lane >> lg : 0, own = NARROW ? lane & ((1 << lg) - 1) : lane;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t g0 = blockIdx.x / slices * 4, c = (blockIdx.x % slices) * 64 * L + own * L;
     const int n = (int)(a.D - c < L ? a.D - c : L);
-    int64_t lo = end, hi = a.n;                  // the run's end
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        if (key[mid] <= k) lo = mid + 1;
-        else hi = mid;
-    }
-    const int64_t last = (lo - 1) / a.group;
-    float sum[L] = {};
-    if (c < a.D) {
-        if (wave == 0) embed_load<float, L, true>(a.part + (g * 2 + 1) * a.ld + c, L, sum);
-        for (int64_t q = g + 1 + wave; q <= last; q += 4 * U) {
-            float x[U][L];
+    auto id_of = [&](int64_t g) { return key[(g + 1) * a.group - 1]; };          // of a group's last token
+    // how many groups after g the run of g's last token goes on in
+    auto length = [&](int64_t g) {
+        const int64_t i0 = g * a.group;
+        if (i0 + a.group >= a.n) return 0;
+        const unsigned k = id_of(g);
+        if (key[i0 + a.group] != k || k >= (unsigned)a.R || (i0 > 0 && key[i0 - 1] == k)) return 0;
+        auto in = [&](int64_t j) { return (g + j) * a.group < a.n && key[(g + j) * a.group] == k; };
+        int64_t lo = 1, hi = 2;                // in(lo), by doubling not in(hi)
+        while (in(hi)) lo = hi, hi *= 2;
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (in(mid)) lo = mid;
+            else hi = mid;
+        }
+        return (int)lo;
+    };
+    float sum[L];
+    auto add = [&](int64_t g, int m, int w, int waves) {       // this wave's share of m groups after g, and g's own
+        const int step = waves * subs;
 #pragma unroll
-            for (int u = 0; u < U; u++) embed_load<float, L, true>(a.part + (q + 4 * u <= last ? q + 4 * u : last) * 2 * a.ld + c, L, x[u]);
+        for (int e = 0; e < L; e++) sum[e] = 0.f;
+        if (c < a.D) {
+            if (w == 0 && sub == 0) embed_load<float, L, true>(a.part + (g * 2 + 1) * a.ld + c, L, sum);
+            for (int q = 1 + w * subs + sub; q <= m; q += step * U) {
+                float x[U][L];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (q + 4 * u > last) continue;
+                for (int u = 0; u < U; u++)
+                    embed_load<float, L, true>(a.part + (g + (q + step * u <= m ? q + step * u : m)) * 2 * a.ld + c, L, x[u]);
 #pragma unroll
-                for (int e = 0; e < L; e++) sum[e] += x[u][e];
+                for (int u = 0; u < U; u++) {
+                    if (q + step * u > m) continue;
+#pragma unroll
+                    for (int e = 0; e < L; e++) sum[e] += x[u][e];
+                }
             }
         }
+        if (NARROW)
+            for (int o = 1 << lg; o < 64; o <<= 1)
+#pragma unroll
+                for (int e = 0; e < L; e++) sum[e] += __shfl_xor(sum[e], o);
+    };
+    auto put = [&](int64_t g) {
+        if (sub == 0 && c < a.D) embed_store<T, L, VEC>(out + (int64_t)id_of(g) * a.D + c, n, sum, a.scale);
+    };
+    const int m = length(g0 + wave);
+    const bool alone = m <= subs * U;
+    if (m > 0 && alone) {
+        add(g0 + wave, m, 0, 1);
+        put(g0 + wave);
     }
-    if (wave)
-#pragma unroll
-        for (int e = 0; e < L; e++) part[wave - 1][lane][e] = sum[e];
+    if (lane == 0) runs[wave] = alone ? 0 : m;
     __syncthreads();
-    if (wave || c >= a.D) return;
+    for (int r = 0; r < 4; r++) {
+        if (!runs[r]) continue;
+        add(g0 + r, runs[r], wave, 4);
+        if (wave)
 #pragma unroll
-    for (int e = 0; e < L; e++) sum[e] = (sum[e] + part[0][lane][e]) + (part[1][lane][e] + part[2][lane][e]);
-    embed_store<T, L, VEC>(out + (int64_t)k * a.D + c, n, sum, a.scale);
+            for (int e = 0; e < L; e++) part[wave - 1][lane][e] = sum[e];
+        __syncthreads();
+        if (!wave) {
+#pragma unroll
+            for (int e = 0; e < L; e++) sum[e] = (sum[e] + part[0][lane][e]) + (part[1][lane][e] + part[2][lane][e]);
+            put(g0 + r);
+        }
+        __syncthreads();
+    }
 }
 
 constexpr int64_t kEmbedRows = 1 << 28, kEmbedCols = 1 << 20, kEmbedTokens = INT32_MAX;
@@ -339,10 +381,12 @@ int64_t embed_plan(EmbedP* a, const void* ids, bool wide, int64_t n, int64_t R, 
     while (R >> bits) bits++;                    // of R itself, which stands for no row
     a->passes = (bits + kEmbedBits - 1) / kEmbedBits;
     a->bits = (bits + a->passes - 1) / a->passes;
-    const int64_t lanes = 64 * (dtype == SNHIP_F32 ? 4 : 8), slices = (D + lanes - 1) / lanes;
+    const int64_t lane = dtype == SNHIP_F32 ? 4 : 8, lanes = 64 * lane, slices = (D + lanes - 1) / lanes;
+    a->lanes = 6;
+    while (a->lanes > 0 && D <= lane << (a->lanes - 1)) a->lanes--;
     // Enough waves to fill the card, and runs as long as they may be; past 2^23 groups and
     // slices longer ones, so that a grid (of fewer than 2^32 threads) holds them.
-    int64_t group = n * slices / 4096;
+    int64_t group = (n * slices >> (6 - a->lanes)) / 4096;
     group = group < 8 ? 8 : group > 64 ? 64 : group;
     if (n * slices / group >= 1 << 23) group = (n * slices >> 22) + 1;
     a->group = (int)group;
@@ -377,17 +421,22 @@ template <typename T> snhip_status embed_fwd_t(const EmbedP& a, const void* tabl
 }
 
 template <typename T> snhip_status embed_bwd_t(const EmbedP& a, const void* dy, void* out, bool vec, hipStream_t st) {
-    const int64_t lanes = 64 * kLane<T>, slices = (a.D + lanes - 1) / lanes, tasks = (a.groups * slices + 3) / 4,
-                  blocks = tasks + (a.R + 63) / 64;
-    if (vec) k_embed_grad<T, true><<<(unsigned)blocks, 256, 0, st>>>(a, (const T*)dy, (T*)out, (int)slices, tasks);
-    else k_embed_grad<T, false><<<(unsigned)blocks, 256, 0, st>>>(a, (const T*)dy, (T*)out, (int)slices, tasks);
-    SNHIP_CHECK(hipGetLastError());
-    if (a.groups > 1) {
-        if (vec) k_embed_join<T, true><<<(unsigned)(a.groups * slices), 256, 0, st>>>(a, (T*)out, (int)slices);
-        else k_embed_join<T, false><<<(unsigned)(a.groups * slices), 256, 0, st>>>(a, (T*)out, (int)slices);
+    const int64_t lanes = 64 * kLane<T>, slices = (a.D + lanes - 1) / lanes, subs = 64 >> a.lanes,
+                  tasks = ((a.groups + subs - 1) / subs * slices + 3) / 4, blocks = tasks + (a.R + 63) / 64;
+    auto go = [&](auto v, auto narrow) -> snhip_status {
+        constexpr bool VEC = decltype(v)::value, NARROW = decltype(narrow)::value;
+        k_embed_grad<T, VEC, NARROW><<<(unsigned)blocks, 256, 0, st>>>(a, (const T*)dy, (T*)out, (int)slices, tasks);
         SNHIP_CHECK(hipGetLastError());
-    }
-    return SNHIP_OK;
+        if (a.groups > 1) {
+            k_embed_join<T, VEC, NARROW><<<(unsigned)((a.groups + 3) / 4 * slices), 256, 0, st>>>(a, (T*)out, (int)slices);
+            SNHIP_CHECK(hipGetLastError());
+        }
+        return SNHIP_OK;
+    };
+    typedef std::true_type yes;
+    typedef std::false_type no;
+    if (a.lanes < 6) return vec ? go(yes(), yes()) : go(no(), yes());
+    return vec ? go(yes(), no()) : go(no(), no());
 }
 
 }  // namespace
