@@ -128,3 +128,36 @@ def test_captured(gpu):
         zs = [torch.empty_like(x) for x in xs]
         assert torch.equal(runtime.clip_grad_norm(xs, 3.0, out=zs), norm)
         assert all(torch.equal(a, b) for a, b in zip(ys, zs))
+
+
+def test_one_tensor_twice(gpu):
+    """Counts twice in a norm; as two gradients to scale, or as two places, it is refused."""
+    x, y = tensors([3000], 6)[0], tensors([3000], 7)[0]
+    assert abs(float(runtime.grad_norm([x, x, y])) - norm64([x, x, y])) <= (2.0 ** -24 + 2.0 ** -40) * norm64([x, x, y])
+    kept = x.clone()
+    for grads, out in (([x, x], None), ([x, x[10:20]], None), ([x, y], [y, x]), ([x], [x.view(-1)[0:0].new_empty(0)]),
+                       ([x[:2000]], [x[1000:]]), ([y, y], [x, x])):
+        with pytest.raises(ValueError):
+            runtime.clip_grad_norm(grads, 1.0, out=out)
+    assert torch.equal(x, kept)
+    a, b = torch.empty_like(x), torch.empty_like(x)
+    check([x, x], 1.0, [a, b], runtime.clip_grad_norm([x, x], 1.0, out=[a, b]))
+
+
+def test_two_streams_at_once(gpu):
+    xs = [tensors([300000, 17, 9000], s, (BF16, F32)) for s in (8, 9)]
+    want = []
+    for x in xs:
+        ys = [torch.empty_like(t) for t in x]
+        want.append((runtime.clip_grad_norm(x, 2.0, out=ys), ys))
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for i, (x, st) in enumerate(zip(xs, streams)):
+            with torch.cuda.stream(st):
+                ys = [t.clone() for t in x]
+                got.append((i, runtime.clip_grad_norm(ys, 2.0), ys))
+    torch.cuda.synchronize()
+    for i, norm, ys in got:
+        assert torch.equal(norm, want[i][0]) and all(torch.equal(a, b) for a, b in zip(ys, want[i][1]))

@@ -116,3 +116,45 @@ def test_values_that_are_not_finite(gpu):
     table[2, 2] = float("nan")
     assert not runtime.embed(table, ids).isnan().any()
     assert runtime.embed(table, torch.tensor([2]).cuda()).isnan().sum() == 1
+
+
+def test_two_streams_at_once(gpu):
+    cases = [(text(n, R, n).cuda(), torch.randn(n, D).cuda().to(BF16), R) for n, R, D in ((9000, 3000, 136), (7001, 500, 640))]
+    want = [runtime.embed_bwd(dy, ids, R, 0.5) for ids, dy, R in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for i, (case, st) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(st):
+                got.append((i, runtime.embed_bwd(case[1], case[0], case[2], 0.5)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i, x in got)
+
+
+def test_two_graphs(gpu):
+    """Captured lookups and gradients share nothing: replayed in turn with new ids, against eager calls."""
+    table, graphs = torch.randn(700, 72).cuda(), []
+    side = torch.cuda.Stream()
+    for n in (300, 9000):
+        ids, dy = text(n, 700, n).cuda(), torch.randn(n, 72).cuda()
+
+        def both(ids=ids, dy=dy):
+            return runtime.embed_fwd(table, ids, 3.0), runtime.embed_bwd(dy, ids, 700, 3.0)
+
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            both()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = both()
+        graphs.append((graph, ids, both, held))
+    for seed in (3, 4, 5):
+        for _, ids, _, _ in graphs:
+            ids.copy_(text(len(ids), 900, seed) - 50)
+        for graph, *_ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, _, both, held in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(held, both()))

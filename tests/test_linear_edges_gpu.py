@@ -325,3 +325,36 @@ def test_beyond_32_bits(gpu):
         if n == "g":
             a, b = a[:, 1:], b[:, 1:]              # the forgetting one's is 0 but for what cancels
         assert float(((a - b).abs() - tol * size - half * b.abs()).max()) <= 0, n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["fp32", "bf16"])
+def test_packed_with_a_decay_per_head(gpu, dtype):
+    """Parts of packed sequences, shared heads, V in more than one block; dg sums over all."""
+    edges, T, Hk, H, K, V = [0, 1, 300, 300, 1030], 1030, 1, 2, 20, 136
+    spans = list(zip(edges, edges[1:]))
+    x = inputs(1, T, Hk, H, K, V, dtype, seed=8, N=len(spans), head_g=True)
+    leaf = [x[n].clone().requires_grad_() for n in NAMES]
+    out, send = runtime.linear_attention(*leaf, cu_seqlens=torch.tensor(edges, dtype=torch.int32, device="cuda"))
+    forward_close(x, out, send, parts=spans)
+    dout, dsend = torch.randn_like(out), torch.randn_like(send)
+    got = torch.autograd.grad((out, send), leaf, (dout, dsend))
+
+    def packed(q, k, v, g, s0):
+        res = [ref(q[:, a:e], k[:, a:e], v[:, a:e], g, s0[i:i + 1]) for i, (a, e) in enumerate(spans)]
+        return torch.cat([r[0] for r in res], 1), torch.cat([r[1] for r in res])
+
+    gradients_close(x, got, dout, dsend, packed)
+
+
+def test_states_off_16_bytes(gpu):
+    """States that begin four bytes past an aligned address equal aligned ones, bit for bit."""
+    for B, T, H, K, V in ((3, 1, 2, 64, 32), (2, 700, 2, 32, 64), (1, 40, 3, 128, 100)):
+        x = inputs(B, T, H, H, K, V, F32, seed=T)
+        off = torch.empty(x["s0"].numel() + 1, device="cuda")[1:].view(x["s0"].shape).copy_(x["s0"])
+        dout, dsend = torch.randn(B, T, H, V).cuda(), torch.randn(B, H, K, V).cuda()
+        doff = torch.empty(dsend.numel() + 1, device="cuda")[1:].view(dsend.shape).copy_(dsend)
+        plain = [x[n] for n in NAMES[:4]]
+        assert all(torch.equal(a, b) for a, b in zip(run([*plain, x["s0"]], dout, dsend), run([*plain, off], dout, doff)))
+        one = [t[:, 0] for t in plain]
+        a, b = x["s0"].clone(), off
+        assert torch.equal(runtime.linear_step(*one, a), runtime.linear_step(*one, b)) and torch.equal(a, b)
