@@ -113,12 +113,11 @@ template <typename T> __device__ __forceinline__ const T* lin_at(const LinRows& 
     return static_cast<const T*>(r.p) + b * r.st[0] + t * r.st[1] + h / r.rep * r.st[2];
 }
 
-// One recurrence. States are (K, V) in memory; `turned` says that the rows of S here are
-// V's (dq and dk).
+// One recurrence. States are (K, V) in memory; in the runs with dots (dq and dk) the rows of S
+// are V's.
 struct LinPass {
     LinRows A, B, C, X;     // X: with which y is multiplied for the decay's gradient
     int rows, cols;         // A's and C's columns
-    bool turned;
     bool vec;               // every eight elements of a row of A, B, C and X are 16-byte aligned (X's too)
     const float* begin;     // (N,H,K,V) the state at the sequence's (backward: last) first token, or null
     float* end;             // (N,H,K,V) the state after all tokens, or null

@@ -416,7 +416,6 @@ snhip_status snhip_op_linear_bwd_dev(const SnHipLinear* d, const SnHipLinearGrad
         b.vec = vec;
         b.A = A, b.B = B, b.C = C, b.X = X;
         b.rows = (int)d->V, b.cols = (int)d->K;
-        b.turned = true;
         b.begin = begin;
         b.parts = at;
         b.y_rep = (int)rep;

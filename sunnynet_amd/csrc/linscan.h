@@ -144,22 +144,17 @@ template <int PAIRS, typename F> __device__ __forceinline__ void each_product(F 
 }
 
 // Four neighbouring elements from `off`, of which the first n exist. vec: aligned, all exist.
-template <typename T> __device__ __forceinline__ void buf_load4e(__amdgpu_buffer_rsrc_t r, int off, int n, bool vec, float* x) {
+template <typename T> struct Vec4 { typedef T type __attribute__((ext_vector_type(4))); };
+template <typename T> __device__ __forceinline__ typename Vec4<T>::type buf_load4e(__amdgpu_buffer_rsrc_t r, int off, int n, bool vec) {
+    typedef typename Vec4<T>::type T4;
     if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4 v = buf_load4(r, off);
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = v[i];
-        } else {
-            typedef T T4 __attribute__((ext_vector_type(4)));
-            const T4 v = __builtin_bit_cast(T4, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
-#pragma unroll
-            for (int i = 0; i < 4; i++) x[i] = (float)v[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = (float)buf_load<T>(r, i < n ? off + i * (int)sizeof(T) : kNowhere);
+        if constexpr (sizeof(T) == 4) return buf_load4(r, off);
+        else return __builtin_bit_cast(T4, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
     }
+    T4 x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = buf_load<T>(r, i < n ? off + i * (int)sizeof(T) : kNowhere);
+    return x;
 }
 template <typename T> __device__ __forceinline__ void buf_store4e(__amdgpu_buffer_rsrc_t r, int off, int n, bool vec, f32x4 x) {
     typedef T T4 __attribute__((ext_vector_type(4)));
@@ -176,7 +171,7 @@ template <typename T> __device__ __forceinline__ void buf_store4e(__amdgpu_buffe
 __device__ __forceinline__ int lin_tile_row(int i) { return i < 1 ? 0 : i < 3 ? 1 : i < 6 ? 2 : 3; }
 
 // One part of one sequence and head, 64 NC columns: four waves of 16 NC columns each. REV:
-// backward in time. DOT: with X.y. STATE: only the part's sum of B C^T. The next chunk's
+// backward in time. DOT: with X.y, and S transposed, its rows V's (dq, dk). STATE: only the part's sum of B C^T. The next chunk's
 // tiles are fetched into registers while this one is worked on, two barriers a chunk.
 //
 // Bound by the issue of matrix and vector instructions, which do not run side by side on
@@ -221,7 +216,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
     const int r0 = row_block * kLinRows, c0 = col_block * W + wave * 16 * NC;
     f32x4 S[NC][NK];       // S[c][2 p + e][r] is row 32 p + g8 + 4 e + r of column 16 c + l16
     const int64_t kv = d.K * d.V;
-    const int rs = (a.turned ? 1 : (int)d.V) * 4, cs = (a.turned ? (int)d.V : 1) * 4;
+    const int rs = (DOT ? 1 : (int)d.V) * 4, cs = (DOT ? (int)d.V : 1) * 4;
     auto each_state = [&](auto f) {
         const int g = here(g8), j0 = c0 + here(l16);
 #pragma unroll
@@ -242,7 +237,11 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
     {
         const float* const from = STATE ? nullptr : first_run ? a.begin : a.parts;
         const __amdgpu_buffer_rsrc_t st = state_at(from, first_run ? seq : (int64_t)blockIdx.x);
-        each_state([&](f32x4& x, int r, int at) { x[r] = buf_load<float>(st, at); });
+        if (DOT && d.V % 4 == 0) {             // four rows lie next to each other: 128 -> 120 us
+            each_state([&](f32x4& x, int r, int at) { if (r == 0) x = buf_load4(st, at); });
+        } else {
+            each_state([&](f32x4& x, int r, int at) { x[r] = buf_load<float>(st, at); });
+        }
     }
     LinFetch<T, C, DP, NTH> fa, fb;
     LinFetch<T, C, W, NTH> fc;
@@ -399,23 +398,23 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
 #pragma unroll
             for (int i = 0; i < STEPS; i++) weigh(0, i);
         }
-        if (more) fetch(chunk_at(ci + 1));
+        if (more && !DOT) fetch(chunk_at(ci + 1));
         Frag<P> bf[2][2];
         auto columns_of_b = [&](int i) {       // step i: 32 rows of S, of 32 tokens
             const int b = i / (NK / 2), k2 = i % (NK / 2) * 2;
 #pragma unroll
             for (int e = 0; e < 2; e++) bf[i & 1][e] = Bt.tfrag(32 * b, 16 * k2 + 8 * (lane & 3) + 4 * e, lane);
         };
-        if (!DOT) columns_of_b(0);             // with the dots' registers a step ahead is too much
+        columns_of_b(0);             // with the dots' registers a step ahead is too much
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             if (b + 1 < NB) columns_of(b + 1);
+            else if (DOT && more) fetch(chunk_at(ci + 1));         // later: one of them would spill (134 -> 128 us)
             int m = 0;
 #pragma unroll
             for (int k = 0; k < NK / 2; k++) {
                 const int i = b * (NK / 2) + k;
-                if (DOT) columns_of_b(i);
-                else if (i + 1 < NB * NK / 2) columns_of_b(i + 1);
+                if (i + 1 < NB * NK / 2) columns_of_b(i + 1);
                 if (b == 0)
 #pragma unroll
                     for (int c = 0; c < NC; c++) S[c][2 * k] *= decay, S[c][2 * k + 1] *= decay;
@@ -443,6 +442,17 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
             }
         }
         const int j4 = wave * 16 * NC + (lane >> 4) * 4;       // this lane's first column in C
+        typename Vec4<T>::type xv[DOT ? NT : 1][NC];
+        if constexpr (DOT) {
+            const __amdgpu_buffer_rsrc_t r = rows_window(xp + t0 * a.X.st[1], a.X.st[1], n, cols);
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const int j = j4 + 16 * c;
+                    xv[t][c] = buf_load4e<T>(r, j < cols ? ((16 * t + l16) * (int)a.X.st[1] + j) * E : kNowhere, cols - j, a.vec);
+                }
+        }
         Frag<P> own[DOT ? NT : 1][NC];         // C of the token itself, whose share is added after the dots
         if constexpr (DOT) {
 #pragma unroll
@@ -456,17 +466,6 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
         barrier_lds();
         if (more) store();                     // only P is read from here on
         __builtin_amdgcn_sched_barrier(0);
-        float xv[DOT ? NT : 1][NC][4];
-        if constexpr (DOT) {
-            const __amdgpu_buffer_rsrc_t r = rows_window(xp + t0 * a.X.st[1], a.X.st[1], n, cols);
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-#pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const int j = j4 + 16 * c;
-                    buf_load4e<T>(r, j < cols ? ((16 * t + l16) * (int)a.X.st[1] + j) * E : kNowhere, cols - j, a.vec, xv[t][c]);
-                }
-        }
         if constexpr (!STATE) {
 #pragma unroll
             for (int jb = 0; jb < NB; jb++)
@@ -491,7 +490,7 @@ __global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinS
                     for (int c = 0; c < NC; c++)
 #pragma unroll
                         for (int r = 0; r < 4; r++) {
-                            e = fmaf(xv[t][c][r], y[t][c][r], e);
+                            e = fmaf((float)xv[t][c][r], y[t][c][r], e);
                             y[t][c][r] = fmaf(w, value_of(own[t][c], r), y[t][c][r]);
                         }
                     e += __shfl_xor(e, 16);
