@@ -37,9 +37,6 @@ constexpr int64_t kLinStride = 1 << 24;            // token strides: offsets ins
 constexpr int kLinWaves = 4;                       // of a block, and so the parts of a dot
 constexpr int kLinRows = 128;                      // contracted rows of a block: all of K, or of a block of V
 
-// Tokens of a chunk: three planes of fp32 leave no room for more than 32.
-template <typename T> struct LinChunk { static constexpr int n = sizeof(T) == 4 ? 32 : 64; };
-
 // A call's sizes, and the parts into which its sequences are cut: `part` tokens each. The
 // parts of sequence n are the slots from first(n) on.
 struct LinShape {

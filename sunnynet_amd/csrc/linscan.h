@@ -171,23 +171,25 @@ template <typename T> __device__ __forceinline__ void buf_store4e(__amdgpu_buffe
 __device__ __forceinline__ int lin_tile_row(int i) { return i < 1 ? 0 : i < 3 ? 1 : i < 6 ? 2 : 3; }
 
 // One part of one sequence and head, 64 NC columns: four waves of 16 NC columns each. REV:
-// backward in time. DOT: with X.y, and S transposed, its rows V's (dq, dk). STATE: only the part's sum of B C^T. The next chunk's
-// tiles are fetched into registers while this one is worked on, two barriers a chunk.
+// backward in time. DOT: with X.y, and S transposed, its rows V's (dq, dk). STATE: only the
+// part's sum of B C^T. The next chunk's tiles are fetched into registers while this one is
+// worked on, two barriers a chunk.
 //
 // Bound by the issue of matrix and vector instructions, which do not run side by side on
 // this card (a SIMD with four waves takes 246 ns for 32 v_mfma_f32_16x16x32, 149 for 128
 // v_sub_f32, and 390 for both): a wave and chunk of 64 bf16 tokens and 128 x 32 of S is 240
 // matrix and about 1,200 vector instructions, half of them splitting S and C times its weight
-// into planes. 5.6 us a chunk and CU, with one block on it or with two. 8 x 2048 tokens, 16
-// heads of 128 in bf16, in 512 parts: 102 us for the output, 101 for dv, 133 and 125 for dq
-// and dk with their dots, 47 for the parts' sums; of each, 13 are the start and the state's
-// reading. A chunk of 64 takes S apart half as often as one of 32; 16-bit types have the LDS
-// for it. Two column tiles a wave halve the LDS reads and P's share (8 waves of 16 columns:
-// 155 us).
+// into planes. 8 x 2048 tokens, 16 heads of 128 in bf16, in 512 parts: 102 us for the output
+// and for dv, 120 for dq and for dk with their dots, 47 for the parts' sums; of each, 13 are
+// the start and the state's reading. A chunk of 64 takes S apart half as often as one of 32,
+// but has to leave LDS for a second block on the CU, without which every wait stands (fp16,
+// 8 x 2048 tokens: 237 us with 64, 189 with 32; fp32, chunks of 32, held to the registers of
+// two blocks: 318 -> 270). Two column tiles a wave halve the LDS reads and P's share (8 waves
+// of 16 columns: 155 us).
 template <typename T, int DP, int NC, bool REV, bool DOT, bool STATE>
-__global__ __launch_bounds__(256, ElemPlanes<T>::n == 1 ? 2 : 1) void k_lin(LinShape d, LinPass a) {
-    constexpr int P = ElemPlanes<T>::n, C = LinChunk<T>::n, NB = C / 32, NT = C / 16, NK = DP / 16, NW = kLinWaves, W = 64 * NC, PAIRS = P == 1 ? 3 : P == 2 ? 5 : 6,
-                  NTH = 256, E = (int)sizeof(T);
+__global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
+    constexpr int P = ElemPlanes<T>::n, C = P == 1 || (P == 2 && (STATE || (DP == 64 && NC == 1))) ? 64 : 32, NB = C / 32, NT = C / 16,
+                  NK = DP / 16, NW = kLinWaves, W = 64 * NC, PAIRS = P == 1 ? 3 : P == 2 ? 5 : 6, NTH = 256, E = (int)sizeof(T);
     typedef SwTile<P, C, DP> Rows;
     typedef SwTile<P, C, W> Cols;
     typedef SwTile<3, C, C> Mat;
