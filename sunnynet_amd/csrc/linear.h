@@ -67,7 +67,7 @@ __device__ __forceinline__ LinSeq lin_seq(const LinShape& d, int64_t n) {
         s.row = s.t0 = a;
         s.b = 0;
         s.len = (int)(e > a ? e - a : 0);
-        s.slot = a / d.part + n;
+        s.slot = (unsigned)a / (unsigned)d.part + n;
     } else {
         s.row = n * d.T;
         s.t0 = 0;
@@ -77,24 +77,25 @@ __device__ __forceinline__ LinSeq lin_seq(const LinShape& d, int64_t n) {
     }
     return s;
 }
-// The sequence and part of a slot. False for a slot that is not used; an empty sequence
-// has one part of no tokens.
-__device__ __forceinline__ bool lin_part_of(const LinShape& d, int64_t slot, LinSeq* s, int64_t* seq, int* part) {
-    int64_t n;
+// The sequence and part of a slot, for a whole wave. False for a slot that is not used; an
+// empty sequence has one part of no tokens. The lanes look at 64 sequences a step (by halves
+// a step is a load's latency for each bit of N).
+__device__ __forceinline__ bool lin_part_of(const LinShape& d, unsigned slot, LinSeq* s, int64_t* seq, int* part) {
+    unsigned n = 0;                            // the last sequence that begins at or before the slot
     if (d.cu) {
-        int64_t lo = 0, hi = d.N - 1;          // the last sequence that begins at or before the slot
-        while (lo < hi) {
-            const int64_t mid = (lo + hi + 1) / 2;
-            if (lin_edge(d, mid) / d.part + mid <= slot) lo = mid;
-            else hi = mid - 1;
+        for (unsigned left = (unsigned)d.N; left > 1;) {
+            const unsigned step = (left + 63) / 64, i = (threadIdx.x & 63) * step;
+            const bool before = i < left && (unsigned)lin_edge(d, n + i) / (unsigned)d.part + n + i <= slot;
+            const unsigned some = __popcll(__ballot(before)), to = some ? (some - 1) * step : 0;
+            n += to;
+            left = step < left - to ? step : left - to;
         }
-        n = lo;
     } else {
-        n = slot / d.per_seq;
+        n = slot / (unsigned)d.per_seq;
     }
     *s = lin_seq(d, n);
     *seq = n;
-    const int64_t p = slot - s->slot;
+    const int64_t p = (int64_t)slot - s->slot;
     *part = (int)p;
     return p == 0 || (p > 0 && p * d.part < s->len);
 }

@@ -192,13 +192,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_lin_add(const flo
     for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += gridDim.x * (int64_t)256) {
         if (d.cu) {                            // rows of no sequence were not written
             const int64_t t = i / per;
-            int64_t lo = 0, hi = d.N - 1;
-            while (lo < hi) {
-                const int64_t mid = (lo + hi + 1) / 2;
-                if (lin_edge(d, mid) <= t) lo = mid;
-                else hi = mid - 1;
-            }
-            if (t < lin_edge(d, lo) || t >= lin_edge(d, lo + 1)) continue;
+            if (t < lin_edge(d, 0) || t >= lin_edge(d, d.N)) continue;
         }
         float v = 0.f;
         for (int c = 0; c < count; c++) v += x[c * n + i];
