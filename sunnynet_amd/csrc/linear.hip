@@ -98,14 +98,23 @@ __global__ __launch_bounds__(256) void k_lin_join(LinShape d, float* all, const 
     F run = {};
     if (begin) run = reinterpret_cast<const F*>(begin)[(seq * d.H + h) * kv + i];
     auto slot = [&](int p) { return (s.slot + (REV ? np - 1 - p : p)) * d.H + h; };
-    F own = {};
-    if (np > 1) own = parts[slot(0) * kv + i];
-    for (int p = 0; p + 1 < np; p++) {
-        F next = {};
-        if (p + 2 < np) next = parts[slot(p + 1) * kv + i];
-        run = run * decay[slot(p)] + own;
-        parts[slot(p + 1) * kv + i] = run;
-        own = next;
+    constexpr int U = 8;                       // steps whose reads are on their way at once
+    F own[U + 1] = {};
+    if (np > 1) own[0] = parts[slot(0) * kv + i];
+    for (int p0 = 0; p0 + 1 < np; p0 += U) {
+        float a[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (p0 + u + 1 < np) a[u] = decay[slot(p0 + u)];
+            if (p0 + u + 2 < np) own[u + 1] = parts[slot(p0 + u + 1) * kv + i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (p0 + u + 1 >= np) continue;
+            run = run * a[u] + own[u];
+            parts[slot(p0 + u + 1) * kv + i] = run;
+        }
+        own[0] = own[U];
     }
 }
 
@@ -207,16 +216,20 @@ bool lin_in_range(const SnHipLinear& d) {
            d.dtype >= SNHIP_F32 && d.dtype <= SNHIP_F16;
 }
 
-// Blocks that fill the card (two a CU), and the fewest tokens worth a part: 3 x 333 tokens of 5
-// heads, all kernels of a training pass, 100 us with 64, 133 with 128, 210 with 256.
-constexpr int64_t kLinBlocks = 512, kLinPart = 64;
+// Blocks that fill the card: two a CU, or three where K and V are at most 64 (16 x 1024 tokens
+// of 16 heads of 64 in bf16: 66 us and 61), and not one more: a few blocks in a second round
+// take as long as all (16384 tokens of 12 heads of 128 in 516 and in 444 blocks: 138 us and
+// 118). And the fewest tokens worth a part: 3 x 333 tokens of 5 heads, all kernels of a
+// training pass, 100 us with 64, 133 with 128, 210 with 256.
+constexpr int64_t kLinBlocks = 512, kLinSmall = 768, kLinPart = 64;
 
 void lin_shape(const SnHipLinear& d, LinShape* s) {
     const int64_t tokens = d.B * d.T;
     // Blocks of 64 columns where even the shortest parts leave CUs idle: 16 us less of those 100.
     s->narrow = tokens * d.H * ((d.V + 127) / 128) / kLinPart < 256;
     const int64_t blocks = d.H * (s->narrow ? (d.V + 63) / 64 : (d.V + 127) / 128);
-    int64_t part = tokens * blocks / kLinBlocks;
+    const int64_t fit = (d.K <= 64 && d.V <= 64 ? kLinSmall : kLinBlocks) / (blocks * d.B), parts = fit < 1 ? 1 : fit;
+    int64_t part = (d.T + parts - 1) / parts;
     part = ((part < kLinPart ? kLinPart : part) + 63) / 64 * 64;
     if (part > d.T) part = (d.T + 63) / 64 * 64;
     s->g = d.g;

@@ -188,7 +188,7 @@ __device__ __forceinline__ int lin_tile_row(int i) { return i < 1 ? 0 : i < 3 ? 
 // of 16 columns: 155 us).
 template <typename T, int DP, int NC, bool REV, bool DOT, bool STATE>
 __global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
-    constexpr int P = ElemPlanes<T>::n, C = P == 1 || (P == 2 && (STATE || (DP == 64 && NC == 1))) ? 64 : 32, NB = C / 32, NT = C / 16,
+    constexpr int P = ElemPlanes<T>::n, C = P == 1 || (P == 2 && STATE) ? 64 : 32, NB = C / 32, NT = C / 16,
                   NK = DP / 16, NW = kLinWaves, W = 64 * NC, PAIRS = P == 1 ? 3 : P == 2 ? 5 : 6, NTH = 256, E = (int)sizeof(T);
     typedef SwTile<P, C, DP> Rows;
     typedef SwTile<P, C, W> Cols;
