@@ -109,7 +109,8 @@ snhip_status snhip_op_delta_bwd_dev(const SnHipDelta* d, const SnHipDeltaGrad* g
  * Layouts, types, sequences, non-finite values and ranges as for the gated delta rule, but:
  * g is (B,T,H), or with head_g (H): one decay for all tokens of a head; H K and H V are
  * below 2^23; chunks are of up to 64 tokens and their number is not bounded; no call has
- * to have a workspace unless snhip_op_linear_parts_floats says so. */
+ * to have a workspace unless snhip_op_linear_parts_floats says so; and tokens of no
+ * sequence are 0 in every output. */
 typedef struct SnHipLinear {
     const void* q;
     const void* k;

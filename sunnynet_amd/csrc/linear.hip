@@ -209,6 +209,35 @@ template <typename T> __global__ __launch_bounds__(256) void k_lin_add(const flo
     }
 }
 
+// Clears the rows of no sequence, before the first edge and from the last on, of up to four
+// arrays. A launch of 2 us, where clearing whole arrays first took 4 to 5 each.
+struct LinClear {
+    struct { char* p; int64_t row; } at[4];    // bytes of a row, an even number
+};
+__global__ __launch_bounds__(256) void k_lin_clear(LinShape d, LinClear c) {
+    const int64_t first = lin_edge(d, 0), last = lin_edge(d, d.N), i0 = blockIdx.x * (int64_t)256 + threadIdx.x, n = gridDim.x * (int64_t)256;
+    char* const p = c.at[blockIdx.y].p;
+    const int64_t row = c.at[blockIdx.y].row;
+    auto clear = [&](char* a, char* e) {
+        char* const a16 = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(a) + 15) & ~(uintptr_t)15);
+        char* const e16 = reinterpret_cast<char*>(reinterpret_cast<uintptr_t>(e) & ~(uintptr_t)15);
+        if (a16 >= e16) {
+            for (char* x = a + 2 * i0; x < e; x += 2 * n) *reinterpret_cast<short*>(x) = 0;
+            return;
+        }
+        for (char* x = a + 2 * i0; x < a16; x += 2 * n) *reinterpret_cast<short*>(x) = 0;
+        for (char* x = a16 + 16 * i0; x < e16; x += 16 * n) *reinterpret_cast<u32x4*>(x) = u32x4{};
+        for (char* x = e16 + 2 * i0; x < e; x += 2 * n) *reinterpret_cast<short*>(x) = 0;
+    };
+    if (first > 0) clear(p, p + first * row);
+    if (last < d.T) clear(p + last * row, p + d.T * row);
+}
+snhip_status lin_clear(const LinShape& s, const LinClear& c, int arrays, hipStream_t st) {
+    k_lin_clear<<<dim3((unsigned)(s.T < 64 ? 1 : s.T / 64 < 256 ? s.T / 64 : 256), (unsigned)arrays), 256, 0, st>>>(s, c);
+    SNHIP_CHECK(hipGetLastError());
+    return SNHIP_OK;
+}
+
 bool lin_in_range(const SnHipLinear& d) {
     return d.B >= 1 && d.T >= 1 && d.N >= 1 && d.N <= 65535 && d.H >= 1 && d.H <= 65535 && d.Hk >= 1 &&
            d.H % d.Hk == 0 && d.K >= 1 && d.K <= 128 && d.V >= 1 && d.V <= 4096 && d.T <= kLinTokens / d.B &&
@@ -374,6 +403,10 @@ snhip_status snhip_op_linear_fwd_dev(const SnHipLinear* d, void* out, float* sen
     a.y = out;
     a.y_rep = 1;
     a.y_vec = lin_four(out, d->V, d->dtype);
+    if (d->cu) {
+        const snhip_status rc = lin_clear(s, {{{static_cast<char*>(out), d->H * d->V * (d->dtype == SNHIP_F32 ? 4 : 2)}}}, 1, st);
+        if (rc != SNHIP_OK) return rc;
+    }
     if (s.split) {
         snhip_status rc = lin_run_any(*d, s, a, false, 2, st);
         if (rc == SNHIP_OK) rc = lin_join(s, false, d->parts, d->s0, st);
@@ -412,7 +445,13 @@ snhip_status snhip_op_linear_bwd_dev(const SnHipLinear* d, const SnHipLinearGrad
     a.y = gr->dv;
     a.y_vec = lin_four(gr->dv, d->V, d->dtype);
     snhip_status rc = SNHIP_OK;
-    if (s.split) {
+    if (d->cu) {
+        const int64_t e = d->dtype == SNHIP_F32 ? 4 : 2;
+        rc = lin_clear(s, {{{static_cast<char*>(gr->dv), d->H * d->V * e}, {static_cast<char*>(gr->dq), d->Hk * d->K * e},
+                            {static_cast<char*>(gr->dk), d->Hk * d->K * e}, {reinterpret_cast<char*>(gr->dg), d->H * 4}}},
+                       s.head_g ? 3 : 4, st);
+    }
+    if (rc == SNHIP_OK && s.split) {
         rc = lin_run_any(*d, s, a, true, 2, st);
         if (rc == SNHIP_OK) rc = lin_join(s, true, parts, gr->dsend, st);
     }

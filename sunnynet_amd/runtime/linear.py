@@ -92,8 +92,7 @@ def linear_fwd(q, k, v, g, s0=None, *, scale=None, cu_seqlens=None, keep=False):
 def _fwd(q, k, v, g, s0, cu_seqlens, dims, scale, keep):
     B, T, N, Hk, H, K, V = dims
     scale = K ** -0.5 if scale is None else float(scale)
-    new = torch.empty if cu_seqlens is None else torch.zeros
-    out = new(B, T, H, V, dtype=v.dtype, device=q.device)
+    out = torch.empty(B, T, H, V, dtype=v.dtype, device=q.device)
     send = torch.empty(N, H, K, V, dtype=torch.float32, device=q.device)
     if B * T == 0 or N == 0:
         send.zero_() if s0 is None else send.copy_(s0)
@@ -138,10 +137,9 @@ def linear_bwd(q, k, v, g, s0, send, parts, dout, dsend=None, *, scale=None, cu_
 def _bwd(q, k, v, g, s0, cu_seqlens, dims, scale, send, parts, dout, dsend, need_ds0):
     B, T, N, Hk, H, K, V = dims
     scale = K ** -0.5 if scale is None else float(scale)
-    new = torch.empty if cu_seqlens is None else torch.zeros
-    dq, dk = (new(B, T, Hk, K, dtype=q.dtype, device=q.device) for _ in range(2))
-    dv = new(B, T, H, V, dtype=q.dtype, device=q.device)
-    dg = new(g.shape, dtype=torch.float32, device=q.device)
+    dq, dk = (torch.empty(B, T, Hk, K, dtype=q.dtype, device=q.device) for _ in range(2))
+    dv = torch.empty(B, T, H, V, dtype=q.dtype, device=q.device)
+    dg = torch.empty(g.shape, dtype=torch.float32, device=q.device)
     ds0 = torch.empty(N, H, K, V, dtype=torch.float32, device=q.device) if need_ds0 else None
     if B * T == 0 or N == 0:
         dg.zero_()

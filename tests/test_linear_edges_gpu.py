@@ -358,3 +358,29 @@ def test_states_off_16_bytes(gpu):
         one = [t[:, 0] for t in plain]
         a, b = x["s0"].clone(), off
         assert torch.equal(runtime.linear_step(*one, a), runtime.linear_step(*one, b)) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("head_g", [False, True], ids=["token_g", "head_g"])
+@pytest.mark.parametrize("edges", [[3, 10, 90], [0, 1], [7, 7], [0, 0, 700], [150, 150, 151, 699]], ids=str)
+def test_tokens_of_no_sequence_are_cleared(gpu, monkeypatch, edges, head_g, dtype):
+    """Whatever the outputs' memory held before; rows of odd sizes. Against the call without
+    those tokens, whose sums differ by twice their tolerance, and each is rounded once more:
+    finfo(T).eps / 2 of its value beside close's own."""
+    T, Hk, H, K, V = 700, 1, 3, 5, 7
+    x = inputs(1, T, Hk, H, K, V, dtype, seed=T, N=len(edges) - 1, head_g=head_g)
+    cu = torch.tensor(edges, dtype=torch.int32, device="cuda")
+    dout, dsend = torch.randn(1, T, H, V).cuda().to(dtype), torch.randn(len(edges) - 1, H, K, V).cuda()
+    live = torch.zeros(T, dtype=torch.bool, device="cuda")
+    live[edges[0]:edges[-1]] = True
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(77))
+    out, send, *grads = run([x[n] for n in NAMES], dout, dsend, cu_seqlens=cu)
+    for t in (out, *grads[:3], *([] if head_g else grads[3:4])):
+        assert not t[0, ~live].any()
+    part = {n: t if n == "s0" or t.dim() == 1 else t[:, live] for n, t in x.items()}
+    if live.any():
+        near = run([part[n] for n in NAMES], dout[:, live], dsend, cu_seqlens=cu - edges[0])
+        for a, b in zip((out, *grads[:3]), (near[0], *near[2:5])):
+            close(a[:, live], b.double().cpu(), dtype,
+                  16 * (7 + 64) * 2.0 ** -24 + torch.finfo(dtype).eps / 2 * (dtype != F32), "a shifted call")
