@@ -143,6 +143,11 @@ template <int PAIRS, typename F> __device__ __forceinline__ void each_product(F 
             if (s - i >= 0 && s - i < P) f(i, s - i);
 }
 
+// Spreads `steps` steps evenly over `all` products, also where the numbers do not divide: whether
+// one is due after product m, and which. Each is, once, in order.
+constexpr bool lin_due(int m, int all, int steps) { return (m + 1) * steps / all > m * steps / all; }
+constexpr int lin_step_at(int m, int all, int steps) { return m * steps / all; }
+
 // Four neighbouring elements from `off`, of which the first n exist. vec: aligned, all exist.
 template <typename T> struct Vec4 { typedef T type __attribute__((ext_vector_type(4))); };
 template <typename T> __device__ __forceinline__ typename Vec4<T>::type buf_load4e(__amdgpu_buffer_rsrc_t r, int off, int n, bool vec) {
@@ -385,10 +390,12 @@ __global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
 #pragma unroll
                         for (int c = 0; c < NC; c++) {
                             y[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[p & 1][c].p[i], af[p & 1][t].p[j], y[t][c], 0, 0, 0);
-                            constexpr int each = PAIRS * NT * NC / STEPS;
-                            if (m % each == each - 1) {
-                                if (p + 1 < DP / 32) planes_of(p + 1, m / each);
-                                else weigh(0, m / each);
+                            constexpr int all = PAIRS * NT * NC;
+                            static_assert(all >= STEPS);
+                            if (lin_due(m, all, STEPS)) {
+                                const int made = lin_step_at(m, all, STEPS);
+                                if (p + 1 < DP / 32) planes_of(p + 1, made);
+                                else weigh(0, made);
                                 __builtin_amdgcn_sched_barrier(0);
                             }
                             m++;
@@ -427,14 +434,16 @@ __global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
                         for (int c = 0; c < NC; c++) {
                             f32x4& x = S[c][2 * k + e];
                             x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[i & 1][e].p[pi], u[b & 1][c].p[pj], x, 0, 0, 0);
-                            constexpr int all = PAIRS * NK * NC, each = all / STEPS;
-                            if (m % each == each - 1) {
-                                if (b + 1 < NB) weigh(b + 1, m / each);
+                            constexpr int all = PAIRS * NK * NC;
+                            static_assert(all >= STEPS && NT <= STEPS);
+                            if (lin_due(m, all, STEPS)) {
+                                const int made = lin_step_at(m, all, STEPS);
+                                if (b + 1 < NB) weigh(b + 1, made);
                                 else if constexpr (!STATE)
-                                    if (m / each < NT) {
-                                        const float r = s.row[16 * (m / each) + l16];
+                                    if (made < NT) {
+                                        const float r = s.row[16 * made + l16];
 #pragma unroll
-                                        for (int q = 0; q < NC; q++) y[m / each][q] *= r;
+                                        for (int q = 0; q < NC; q++) y[made][q] *= r;
                                     }
                                 __builtin_amdgcn_sched_barrier(0);
                             }
