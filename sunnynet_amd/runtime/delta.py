@@ -120,7 +120,10 @@ def _check_state(s, shape, name):
 
 
 def _rows(t):
-    """t with its last axis contiguous; the others may have any stride below MAX_STRIDE."""
+    """t with its last axis contiguous; the others may have any stride below MAX_STRIDE. The
+    stride of a single token's axis, which nothing uses, is 0 where it is not."""
+    if t.dim() == 4 and t.shape[1] == 1 and t.stride(1) >= MAX_STRIDE:     # contiguous to torch: never copied
+        t = t.as_strided(t.shape, (t.stride(0), 0, *t.stride()[2:]))
     if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 4 or t.stride(1) < MAX_STRIDE):
         return t
     return t.contiguous()
