@@ -12,7 +12,7 @@ from operator import attrgetter
 import torch
 
 from .. import _native
-from .delta import DTYPES
+from .delta import DTYPES, refuse_tangents
 
 __all__ = ["clip_grad_norm", "grad_norm"]
 
@@ -74,8 +74,10 @@ def grad_norm(grads):
     """The norm of all elements of the gradients (contiguous float32, bfloat16 or float16
     tensors of one GPU, each of its own type) -> float32 scalar on the device. Squares are
     summed in 64 bits in a fixed order: the same calls give the same bits. Not
-    differentiable."""
-    return _run(list(grads), 0.0, None)
+    differentiable; forward-mode derivatives are refused."""
+    grads = list(grads)
+    refuse_tangents("grad_norm", *grads)
+    return _run(grads, 0.0, None)
 
 
 @torch.no_grad()
@@ -84,13 +86,15 @@ def clip_grad_norm(grads, max_norm, *, out=None):
     place, or into the tensors of ``out`` (like the gradients), and returns the norm before,
     a float32 scalar on the device. Where nothing is to clip, gradients in place are not
     touched. A norm that is infinite makes finite values 0, one that is NaN makes all NaN.
-    Two gradients that share memory are refused. Not differentiable."""
+    Two gradients that share memory are refused. Not differentiable; forward-mode
+    derivatives are refused."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative")
     grads = list(grads)
     if out is not None:
         out = list(out)
+    refuse_tangents("clip_grad_norm", *grads, *(out or ()))
     if any(t is not None and t.requires_grad and t.is_leaf for t in (grads if out is None else out)):
         raise RuntimeError("a leaf that requires a gradient cannot be written in place")
     norm = _run(grads, max_norm, grads if out is None else out)
