@@ -195,6 +195,11 @@ template <typename T, int DP, int NC, bool REV, bool DOT, bool STATE>
 __global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
     constexpr int P = ElemPlanes<T>::n, C = P == 1 || (P == 2 && STATE) ? 64 : 32, NB = C / 32, NT = C / 16,
                   NK = DP / 16, NW = kLinWaves, W = 64 * NC, PAIRS = P == 1 ? 3 : P == 2 ? 5 : 6, NTH = 256, E = (int)sizeof(T);
+    // With five or six partial products they are summed before S takes them up, by one rounding
+    // with the decay. Each added to S by itself left 17 2^-24 (rms, fp32) after 128 chunks
+    // without a decay, this 3.7, for 1 % of the time. bf16's three, in chunks twice as long,
+    // leave 6.6 there; their sums would spill.
+    constexpr bool APART = P > 1;
     typedef SwTile<P, C, DP> Rows;
     typedef SwTile<P, C, W> Cols;
     typedef SwTile<3, C, C> Mat;
@@ -424,15 +429,20 @@ __global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
             for (int k = 0; k < NK / 2; k++) {
                 const int i = b * (NK / 2) + k;
                 if (i + 1 < NB * NK / 2) columns_of_b(i + 1);
-                if (b == 0)
+                f32x4 sum[2][NC];
 #pragma unroll
-                    for (int c = 0; c < NC; c++) S[c][2 * k] *= decay, S[c][2 * k + 1] *= decay;
+                for (int e = 0; e < 2; e++)
+#pragma unroll
+                    for (int c = 0; c < NC; c++) {
+                        if (APART && b == 0) sum[e][c] = {0, 0, 0, 0};
+                        else if (b == 0) S[c][2 * k + e] *= decay;
+                    }
                 each_product<PAIRS>([&](int pj, int pi) {          // u's plane pj, B's pi
 #pragma unroll
                     for (int e = 0; e < 2; e++)
 #pragma unroll
                         for (int c = 0; c < NC; c++) {
-                            f32x4& x = S[c][2 * k + e];
+                            f32x4& x = APART && b == 0 ? sum[e][c] : S[c][2 * k + e];
                             x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bf[i & 1][e].p[pi], u[b & 1][c].p[pj], x, 0, 0, 0);
                             constexpr int all = PAIRS * NK * NC;
                             static_assert(all >= STEPS && NT <= STEPS);
@@ -450,6 +460,16 @@ __global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
                             m++;
                         }
                 });
+                if (APART && b == 0)
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+#pragma unroll
+                        for (int c = 0; c < NC; c++) {
+                            f32x4& x = S[c][2 * k + e];
+#pragma unroll
+                            for (int r = 0; r < 4; r++) x[r] = fmaf(x[r], decay, sum[e][c][r]);
+                            asm volatile("" : "+v"(x));        // here, not at the chunk's end with all sums held (spills)
+                        }
             }
         }
         const int j4 = wave * 16 * NC + (lane >> 4) * 4;       // this lane's first column in C
