@@ -196,7 +196,8 @@ snhip_status snhip_op_embed_bwd_dev(const void* dy, const void* ids, int32_t wid
  * y[i] is x[i] or lies apart from every x and other y (overlaps are refused; y NULL: the
  * norm alone). Squares are summed in 64 bits in a fixed order, the factor is fp32 and a
  * product is rounded once. Where the factor is 1, tensors in place are not touched. A norm
- * that is infinite makes finite values 0 and others NaN, one that is NaN makes all NaN.
+ * that is infinite (some value is) makes finite values 0 and others NaN, one that is NaN
+ * makes all NaN. max_norm may be infinite: then only a norm of NaN changes values.
  * norm: one fp32 on the device. ws: snhip_op_clip_doubles doubles, on the device.
  * 0 <= n[i] < 2^36, count < 2^20. */
 typedef struct SnHipClip {

@@ -120,7 +120,8 @@ __global__ __launch_bounds__(256) void k_clip_norm(const double* partial, int64_
 }
 
 __global__ __launch_bounds__(256) void k_clip_scale(ClipTable t, const double* partial, int64_t partials, double max_norm, float* norm) {
-    const double n = clip_norm(partial, partials), f = max_norm / (n + 1e-6);
+    // a bound without end scales nothing, beside an infinite value neither
+    const double n = clip_norm(partial, partials), f = isinf(max_norm) && isinf(n) ? 1. : max_norm / (n + 1e-6);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const float factor = f >= 1. ? 1.f : (float)f;         // NaN stays
     clip_pieces<true>(t, [&](int i, int64_t piece) {

@@ -85,9 +85,9 @@ def clip_grad_norm(grads, max_norm, *, out=None):
     """Multiplies the gradients (see grad_norm) by min(1, max_norm / (norm + 1e-6)), in
     place, or into the tensors of ``out`` (like the gradients), and returns the norm before,
     a float32 scalar on the device. Where nothing is to clip, gradients in place are not
-    touched. A norm that is infinite makes finite values 0, one that is NaN makes all NaN.
-    Two gradients that share memory are refused. Not differentiable; forward-mode
-    derivatives are refused."""
+    touched. A norm that is infinite (some value is) makes finite values 0, one that is NaN
+    makes all NaN. An infinite ``max_norm`` clips nothing. Two gradients that share memory
+    are refused. Not differentiable; forward-mode derivatives are refused."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative")
