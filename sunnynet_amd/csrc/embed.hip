@@ -18,11 +18,10 @@
 // runs of one id in fp32 and writes the rows that lie inside it; runs that go on in a
 // neighbour's tokens are left as partial sums, which k_embed_join adds in order. Rows that
 // no token names are cleared by blocks of their own beside these.
-// Rows of up to half a wave's columns share a wave (524288 tokens of 64 in bf16: 200 us
-// without, 129 so), and a wave joins a group's run by itself unless it is long (204 -> 95 us there
-// for ids that are all alike often).
-// 32768 tokens of text, a table of 32000 x 1024 in bf16: two passes of 4 us to count and 8 (the
-// latency of their steps), sums 25, joins 10; up to 4096 tokens one block sorts alone.
+// Rows of up to half a wave's columns share a wave, and a wave joins a group's run by itself
+// unless it is long (524288 tokens of text, 64 columns in bf16: 208 us without either, 90 so).
+// 32768 tokens of text, a table of 32000 x 1024 in bf16: two passes of 3.5 us to count and 7.7 (the
+// latency of their steps), sums 30, joins 10; up to 4096 tokens one block sorts alone.
 #include <type_traits>
 
 #include "common.h"

@@ -120,8 +120,8 @@ __global__ __launch_bounds__(256) void k_lin_join(LinShape d, float* all, const 
 
 // The decay's gradient over one part and head: e_t = q_t.dq_t - k_t.dk_t summed from the
 // part's last token back, from <S, R> at its end. Sums in 64 bits. dg: (B,T,H), or the
-// part's total in `sums` (slots, H). Bound by the two states that it reads: 23 us for 8 x 4
-// parts, 16 heads of 128 x 128 (2.9 TB/s).
+// part's total in `sums` (slots, H). Waits for its reads, the two states before any token: 22 us
+// for 8 x 4 parts, 16 heads of 128 x 128 (3.4 TB/s; its waves wait 77 % of their time).
 __global__ __launch_bounds__(256) void k_lin_dg(LinShape d, const float* dots, int waves, const float* s_parts, const float* r_parts,
                                                 const float* send, const float* dsend, float* dg, double* sums) {
     __shared__ double sw[4];
@@ -247,8 +247,8 @@ bool lin_in_range(const SnHipLinear& d) {
 
 // Blocks that fill the card: two a CU, or three where K and V are at most 64 (16 x 1024 tokens
 // of 16 heads of 64 in bf16: 66 us and 61), and not one more: a few blocks in a second round
-// take as long as all (16384 tokens of 12 heads of 128 in 516 and in 444 blocks: 138 us and
-// 118). And the fewest tokens worth a part: 3 x 333 tokens of 5 heads, all kernels of a
+// take as long as all (the output of 16384 tokens of 12 heads of 128, bf16: 96 us in 516
+// blocks, 77 in 444). And the fewest tokens worth a part: 3 x 333 tokens of 5 heads, all kernels of a
 // training pass, 100 us with 64, 133 with 128, 210 with 256.
 constexpr int64_t kLinBlocks = 512, kLinSmall = 768, kLinPart = 64;
 

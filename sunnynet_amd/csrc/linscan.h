@@ -180,13 +180,15 @@ __device__ __forceinline__ int lin_tile_row(int i) { return i < 1 ? 0 : i < 3 ? 
 // part's sum of B C^T. The next chunk's tiles are fetched into registers while this one is
 // worked on, two barriers a chunk.
 //
-// Bound by the issue of matrix and vector instructions, which do not run side by side on
-// this card (a SIMD with four waves takes 246 ns for 32 v_mfma_f32_16x16x32, 149 for 128
-// v_sub_f32, and 390 for both): a wave and chunk of 64 bf16 tokens and 128 x 32 of S is 240
-// matrix and about 1,200 vector instructions, half of them splitting S and C times its weight
-// into planes. 8 x 2048 tokens, 16 heads of 128 in bf16, in 512 parts: 102 us for the output
-// and for dv, 120 for dq and for dk with their dots, 47 for the parts' sums; of each, 13 are
-// the start and the state's reading. A chunk of 64 takes S apart half as often as one of 32,
+// Bound first by the issue of matrix and vector instructions, which do not run side by side on
+// this card (two waves on a SIMD take 65 ns each for 8 v_mfma_f32_16x16x32, 49 for 40
+// v_sub_f32, and 124 for both in turn): a wave and chunk of 64 bf16 tokens and 128 x 32 of S is
+// 240 matrix and about 1,280 vector instructions, half of them splitting S and C times its
+// weight into planes. 8 x 2048 tokens, 16 heads of 128 in bf16, in 512 parts: 102 us for the
+// output and for dv, 120 for dq and for dk with their dots, 47 for the parts' sums. Of the
+// output's 102, 61 are that issue, about 22 waits for LDS, barriers and the fetch (a quarter of
+// the waves' time by the counters), the rest starts and ends. Its 314 MB would take 62 by
+// themselves. A chunk of 64 takes S apart half as often as one of 32,
 // but has to leave LDS for a second block on the CU, without which every wait stands (fp16,
 // 8 x 2048 tokens: 237 us with 64, 189 with 32; fp32, chunks of 32, held to the registers of
 // two blocks: 318 -> 270). Two column tiles a wave halve the LDS reads and P's share (8 waves
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(256, 2) void k_lin(LinShape d, LinPass a) {
                   NK = DP / 16, NW = kLinWaves, W = 64 * NC, PAIRS = P == 1 ? 3 : P == 2 ? 5 : 6, NTH = 256, E = (int)sizeof(T);
     // With five or six partial products they are summed before S takes them up, by one rounding
     // with the decay. Each added to S by itself left 17 2^-24 (rms, fp32) after 128 chunks
-    // without a decay, this 3.7, for 1 % of the time. bf16's three, in chunks twice as long,
+    // without a decay, this 3.7, for 1 to 2 % of the time. bf16's three, in chunks twice as long,
     // leave 6.6 there; their sums would spill.
     constexpr bool APART = P > 1;
     typedef SwTile<P, C, DP> Rows;
